@@ -203,7 +203,13 @@ def _prepare_lora(case, seed):
     offsets = np.cumsum(ranks) - ranks
     of_token = np.repeat(_adapter_of_requests(case), _tokens_of_requests(case))
     order = np.argsort(of_token, kind="stable")
+    # the batch's plan: tiles of up to 64 tokens of one adapter, as positions in `order`
     ids, first = np.unique(of_token[order], return_index=True)
+    lens = np.diff(np.append(first, T))
+    n = -(-lens // 64)
+    start = np.repeat(first, n) + 64 * (np.arange(n.sum()) - np.repeat(np.cumsum(n) - n, n))
+    count = np.minimum(64, np.repeat(first + lens, n) - start)
+    tiles = np.stack([start, count, np.repeat(ids, n), start * 0], 1)
     i32 = lambda v: torch.from_numpy(np.ascontiguousarray(v).astype(np.int32)).to(dev)  # noqa: E731
     alpha = torch.rand(case["adapters"], generator=g, device=dev) + 0.5
     return {
@@ -213,8 +219,7 @@ def _prepare_lora(case, seed):
         "b": (torch.randn((R, N), generator=g, device=dev) * 0.1).to(dt),
         "base": torch.randn((T, N), generator=g, device=dev),
         "scales": alpha, "ranks": i32(ranks), "offsets": i32(offsets),
-        "of_token": i32(of_token), "order": i32(order), "seg_adapter": i32(ids),
-        "seg_start": i32(np.append(first, T)),
+        "max_rank": int(ranks.max()), "of_token": i32(of_token), "order": i32(order), "tiles": i32(tiles),
     }
 
 
@@ -301,8 +306,8 @@ def _own_lora(s):
     from microserve_b200.lora import LoraPlan, LoraProjection, lora_add
 
     proj = LoraProjection(a=s["a"], b=s["b"], offsets=s["offsets"], ranks=s["ranks"], scales=s["scales"],
-                          slices=s["slices"], interleaved=s["kind"] == "swiglu")
-    plan = LoraPlan(order=s["order"], seg_start=s["seg_start"], seg_adapter=s["seg_adapter"])
+                          max_rank=s["max_rank"], slices=s["slices"], interleaved=s["kind"] == "swiglu")
+    plan = LoraPlan(order=s["order"], tiles=s["tiles"])
     return lora_add(s["x"], s["base"], proj, plan, swiglu=s["kind"] == "swiglu", out_dtype=s["out"])
 
 
