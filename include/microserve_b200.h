@@ -105,6 +105,71 @@ MS_API int ms_sample(const float* logits, int64_t row_stride, int n_rows, int vo
               int32_t* tokens, float* probs, ms_row_stats* stats,
               int32_t* scatter_dst, const int32_t* scatter_idx, void* stream);
 
+/* ---- per-request controls on logits -------------------------------------- */
+/* What each request has said, in slots (one row per request that counts):
+ *   counts: (n_slots, vocab) int32, generated tokens;
+ *   seen:   (n_slots, ceil(vocab / 32)) words, bit v % 32 of word v / 32 set
+ *           when token v is in the prompt or was generated.
+ * Zero before use.  No reference counterpart (the reference samples from
+ * the model's logits as they are), like everything in this section. */
+
+/* Count sequence i's tokens into slot slots[i] (< 0: skipped): its row
+ * starts at tokens + row_start[i] (NULL: i * row_stride) and holds
+ * min(lens[i] + len_add, max_len) tokens (lens NULL: 0).  The first
+ * n_prompt[i] (NULL: 0) only set the seen bit.  With ms_spec_accept's
+ * outputs: tokens = out_tokens, row_stride = max_len = gamma + 1, lens =
+ * out_num_accepted, len_add = 1.  Slots may repeat. */
+MS_API int ms_token_counts_append(int32_t* counts, uint32_t* seen, int n_slots, int vocab,
+                                  const int32_t* slots, int n_seqs, const int32_t* tokens,
+                                  const int64_t* row_start, int64_t row_stride,
+                                  const int32_t* lens, int len_add, int max_len,
+                                  const int32_t* n_prompt, void* stream);
+
+/* Zero the counts and seen bits of slots[0, n_seqs) (< 0: skipped). */
+MS_API int ms_token_counts_reset(int32_t* counts, uint32_t* seen, int n_slots, int vocab,
+                                 const int32_t* slots, int n_seqs, void* stream);
+
+/* Controls of n_requests requests; device arrays, each group nullable. */
+typedef struct {
+  /* penalties: slots[b] < 0 leaves request b unpenalised; penalties[3b..]
+   * = repetition (> 0), presence, frequency */
+  const int32_t* slots;
+  const float* penalties;
+  const int32_t* counts;
+  const uint32_t* seen;
+  int32_t n_slots;
+  /* proposals a request has drafted in this round, position-major:
+   * proposal j of request b at proposals[j * n_requests + b] (at most 64).
+   * Row i of a request sees the first first_proposal + i of them as said. */
+  int32_t n_proposals;
+  const int32_t* proposals;
+  int32_t first_proposal;
+  /* sparse biases: request b's entries are [bias_start[b], bias_start[b+1])
+   * of the n_bias entries, token ids strictly ascending */
+  int32_t n_bias;
+  const int32_t* bias_start;
+  const int32_t* bias_ids;
+  const float* bias_values;
+  /* masks: (n_masks, ceil(vocab / 32)) words, a set bit allows the token;
+   * mask_rows[row] < 0 leaves the row unmasked */
+  const int32_t* mask_rows;
+  const uint32_t* masks;
+  int32_t n_masks;
+  int32_t reserved_;
+} ms_logit_controls;
+
+/* out = the controlled logits of n_requests * rows_per_request rows (row
+ * b * rows_per_request + i is row i of request b): repetition penalty on
+ * tokens in the prompt or generated, minus frequency * count and presence on
+ * generated tokens, plus bias, and -inf where the row's mask forbids the
+ * token (a row whose mask allows nothing is all -inf).  In place when out ==
+ * logits: only the changed logits are then read and written.  Otherwise the
+ * two must not overlap.  A bad slot, token, mask row or bias order sets the
+ * device error word and is skipped. */
+MS_API int ms_apply_logit_controls(const float* logits, int64_t row_stride, float* out,
+                                   int64_t out_stride, int n_requests, int rows_per_request,
+                                   int vocab, const ms_logit_controls* controls, void* stream);
+
 /* Fused accept / resample / bonus for B requests with gamma proposals each
  * (reference speculative.py:44-86 verify_proposals, applied as in
  * speculative.py:191-202).  Target side: (B*(gamma+1)) rows of logits,
@@ -301,6 +366,55 @@ MS_API int ms_forward_static_scratch(const ms_model* model,
                                      const int32_t* logit_rows,
                                      int n_logit_rows, float* logits,
                                      int64_t logits_row_stride, void* stream);
+
+/* ---- low-rank adapters ------------------------------------------------------ */
+/* Adapters of many requests beside a shared projection.  No reference
+ * counterpart.  Adapter i has rank ranks[i] (at most max_rank, and at most
+ * MS_LORA_MAX_RANK) and occupies rows [offsets[i], offsets[i] + ranks[i]) of
+ * total_rank.  Of a projection with n_slices fused outputs (q | k | v:
+ * 3, gate | up: 2, else 1), with the model's dtype for both:
+ *   a: (n_slices * total_rank, K); adapter i's rows start at n_slices *
+ *      offsets[i], slice by slice (ranks[i] rows each);
+ *   b: (total_rank, N), the transpose of the usual (N, rank): row offsets[i]
+ *      + r holds rank r of every output column. */
+#define MS_LORA_TILE 64
+#define MS_LORA_MAX_RANK 256
+typedef struct {
+  int32_t n_adapters;
+  int32_t total_rank;
+  int32_t max_rank;
+  int32_t reserved_;
+  const int32_t* offsets; /* device [n_adapters] */
+  const int32_t* ranks;
+  const float* scales; /* usually alpha / rank */
+} ms_lora_adapters;
+
+/* Which tokens of a batch use which adapter: `order` lists the n_tokens
+ * tokens grouped by adapter; tile i covers positions [tiles[4i], +
+ * tiles[4i+1]) of it (at most MS_LORA_TILE), all of adapter tiles[4i+2] (-1:
+ * none); tiles[4i+3] is unused.  Every token in one tile.  16-byte aligned. */
+typedef struct {
+  int32_t n_tokens;
+  int32_t n_tiles;
+  const int32_t* order;
+  const int32_t* tiles;
+} ms_lora_plan;
+
+/* out = base + scale * B (A x) per token (x in `dtype`, base float32, out in
+ * out_dtype), column n with the A of its slice: slice_cols (host,
+ * n_slices entries) gives the column counts, or interleaved != 0: two slices
+ * alternating every 8 columns, as w_gate_up.  swiglu: out (N/2 columns) =
+ * silu(gate) * up of those.  out may be base (float32, no SwiGLU): then tokens
+ * without an adapter are not touched; otherwise the two must not overlap.
+ * Tokens of no tile are left as they were.  A bad tile, token or adapter
+ * sets the device error word and is skipped. */
+MS_API size_t ms_lora_workspace_size(const ms_lora_adapters* adapters, const ms_lora_plan* plan,
+                                     int K, int n_slices);
+MS_API int ms_lora_add(const void* x, int64_t x_stride, const float* base, int64_t base_stride,
+                       void* out, int64_t out_stride, const void* a, const void* b, int K, int N,
+                       int n_slices, const int32_t* slice_cols, int interleaved, int swiglu,
+                       const ms_lora_adapters* adapters, const ms_lora_plan* plan, int dtype,
+                       int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- building blocks, exported for tests and for callers that compose
  *      their own forward ---------------------------------------------- */

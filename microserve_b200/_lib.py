@@ -8,6 +8,7 @@ device raises immediately.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
@@ -109,6 +110,48 @@ class MsBatch(ctypes.Structure):
     ]
 
 
+class MsLogitControls(ctypes.Structure):
+    _fields_ = [
+        ("slots", c_void_p),
+        ("penalties", c_void_p),
+        ("counts", c_void_p),
+        ("seen", c_void_p),
+        ("n_slots", c_int32),
+        ("n_proposals", c_int32),
+        ("proposals", c_void_p),
+        ("first_proposal", c_int32),
+        ("n_bias", c_int32),
+        ("bias_start", c_void_p),
+        ("bias_ids", c_void_p),
+        ("bias_values", c_void_p),
+        ("mask_rows", c_void_p),
+        ("masks", c_void_p),
+        ("n_masks", c_int32),
+        ("reserved_", c_int32),
+    ]
+
+
+class MsLoraAdapters(ctypes.Structure):
+    _fields_ = [
+        ("n_adapters", c_int32),
+        ("total_rank", c_int32),
+        ("max_rank", c_int32),
+        ("reserved_", c_int32),
+        ("offsets", c_void_p),
+        ("ranks", c_void_p),
+        ("scales", c_void_p),
+    ]
+
+
+class MsLoraPlan(ctypes.Structure):
+    _fields_ = [
+        ("n_tokens", c_int32),
+        ("n_tiles", c_int32),
+        ("order", c_void_p),
+        ("tiles", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ms_version": (c_int, []),
@@ -139,6 +182,17 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
          c_void_p],
     ),
+    "ms_token_counts_append": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+         c_int, c_int, c_void_p, c_void_p],
+    ),
+    "ms_token_counts_reset": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "ms_apply_logit_controls": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, POINTER(MsLogitControls),
+         c_void_p],
+    ),
     "ms_host_blocks_needed": (c_int64, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                                         c_void_p]),
     "ms_host_append": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64,
@@ -166,6 +220,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ms_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int64, c_int,
                         c_int, c_int, c_void_p]),
     "ms_gemm_set_policy": (c_int, [c_int]),
+    "ms_lora_workspace_size": (c_size_t, [POINTER(MsLoraAdapters), POINTER(MsLoraPlan), c_int, c_int]),
+    "ms_lora_add": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int,
+         c_int, c_void_p, c_int, c_int, POINTER(MsLoraAdapters), POINTER(MsLoraPlan), c_int, c_int,
+         c_void_p, c_size_t, c_void_p],
+    ),
     "ms_attention_scratch_size": (c_size_t, [POINTER(MsKVCache), c_int, POINTER(MsBatch)]),
     "ms_paged_attention": (c_int, [c_void_p, POINTER(MsKVCache), c_int, POINTER(MsBatch), c_int,
                                    c_void_p, c_void_p]),
@@ -218,6 +279,14 @@ def require_cuda(device: torch.device | str) -> torch.device:
         raise RuntimeError("microserve_b200 needs a CUDA device and none is available")
     load()
     return dev
+
+
+def on_device(device: torch.device):
+    """A context in which launches go to ``device`` (kernels are launched on the
+    current device, whichever device their stream belongs to)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def stream_ptr(device: torch.device | None = None) -> int:

@@ -98,6 +98,10 @@ enum DeviceError : int {
   kErrBlock = 2,     // block id outside the pool
   kErrToken = 3,     // token id outside the vocabulary
   kErrPosition = 4,  // position beyond the RoPE table
+  // 5: a kernel's bounded wait ran out (gemm_tc.cu, attention_tma.cu)
+  kErrMask = 6,      // mask row outside the masks
+  kErrOrder = 7,     // a list that has to be ascending (bias ids, offsets) is not
+  kErrAdapter = 8,   // adapter id, rank or segment outside the adapters' arrays
 };
 __device__ __forceinline__ void raise_device_error(int* err, int code) {
   atomicCAS(err, 0, code);

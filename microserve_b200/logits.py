@@ -1,0 +1,238 @@
+"""What a request sets for its own logits before a draw: penalties for repeated
+tokens, per-token biases and grammar masks.
+
+``apply_logit_controls`` computes, for row ``i`` of request ``b`` (a row that
+sees the request's first ``first_proposal + i`` proposals of a speculative
+round as already said) and token ``v`` with raw logit ``x``::
+
+    c = times v was generated;  s = v is in the prompt or was generated
+    y = (x / repetition if x > 0 else x * repetition) if s else x
+    y = y - frequency * c - (presence if c > 0 else 0)
+    y = y + bias[v]
+    y = y if the row's mask allows v else -inf
+
+in float32, one kernel (``ms_apply_logit_controls``) for the whole batch.  What each
+request has said lives on the device (:class:`TokenCounts`) and is updated from
+the drawn tokens there, so a speculative round never waits for the host.
+The reference samples from unmodified logits; none of this has a counterpart
+there.  :class:`RequestControls` is the host side the engine and the
+speculative decoder use.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Sequence
+from dataclasses import dataclass
+from typing import TYPE_CHECKING
+
+import numpy as np
+import torch
+
+from . import _lib
+from .batching import HostStaging, pack_int32
+
+if TYPE_CHECKING:
+    from .scheduler import Request
+
+MAX_PROPOSALS = 64
+
+
+def mask_words(vocab_size: int) -> int:
+    """32-bit words of one mask or seen row."""
+    return (vocab_size + 31) // 32
+
+
+def pack_masks(allowed: np.ndarray) -> np.ndarray:
+    """``(n, vocab)`` truth values (True: allowed) as ``(n, words)`` int32 words,
+    token ``v`` at bit ``v % 32`` of word ``v // 32``."""
+    allowed = np.asarray(allowed, dtype=bool)
+    n, vocab = allowed.shape
+    full = np.zeros((n, mask_words(vocab) * 32), dtype=np.uint8)
+    full[:, :vocab] = allowed
+    return np.packbits(full, axis=1, bitorder="little").view("<u4").view(np.int32)
+
+
+def _check(t: torch.Tensor | None, name: str, dtype: torch.dtype, device: torch.device,
+           shape: tuple[int | None, ...]) -> int | None:
+    """The data pointer of an optional argument after checking it."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.dim() != len(shape) \
+            or any(w is not None and w != h for w, h in zip(shape, t.shape)):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}; "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+@dataclass
+class TokenCounts:
+    """What the requests have said, one slot each: ``counts`` (slots, vocab)
+    int32, how often each token was generated; ``seen`` (slots, words) int32
+    bit words, set for tokens in the prompt or generated."""
+
+    counts: torch.Tensor
+    seen: torch.Tensor
+
+    @classmethod
+    def empty(cls, n_slots: int, vocab_size: int, device: str | torch.device = "cuda") -> TokenCounts:
+        dev = _lib.require_cuda(device)
+        if n_slots < 1 or vocab_size < 1:
+            raise ValueError("n_slots and vocab_size must be at least 1")
+        return cls(torch.zeros((n_slots, vocab_size), dtype=torch.int32, device=dev),
+                   torch.zeros((n_slots, mask_words(vocab_size)), dtype=torch.int32, device=dev))
+
+    @property
+    def n_slots(self) -> int:
+        return self.counts.shape[0]
+
+    @property
+    def vocab_size(self) -> int:
+        return self.counts.shape[1]
+
+    def pointers(self, device: torch.device) -> tuple[int | None, int | None]:
+        n, v = self.counts.shape
+        return (_check(self.counts, "counts", torch.int32, device, (n, v)),
+                _check(self.seen, "seen", torch.int32, device, (n, mask_words(v))))
+
+    def reset(self, slots: torch.Tensor) -> None:
+        """Forget everything in ``slots`` (int32, device; negative: skipped)."""
+        dev = self.counts.device
+        c, s = self.pointers(dev)
+        p = _check(slots, "slots", torch.int32, dev, (None,))
+        with _lib.on_device(dev):
+            _lib.call("ms_token_counts_reset", c, s, self.n_slots, self.vocab_size, p,
+                      slots.numel(), _lib.stream_ptr(dev))
+
+    def append(self, slots: torch.Tensor, tokens: torch.Tensor, lens: torch.Tensor | None = None,
+               len_add: int = 0, row_start: torch.Tensor | None = None, max_len: int | None = None,
+               n_prompt: torch.Tensor | None = None) -> None:
+        """Count sequence ``i``'s tokens into slot ``slots[i]``.
+
+        Without ``row_start``, ``tokens`` is (n, width) int32 and row ``i``'s
+        first ``lens[i] + len_add`` tokens count (all of them without
+        ``lens``).  With it (int64), ``tokens`` is flat, sequence ``i`` starts at
+        ``row_start[i]`` and ``max_len`` bounds every length; each sequence must
+        lie inside ``tokens``.  The first ``n_prompt[i]`` tokens are prompt:
+        they only become seen."""
+        dev = self.counts.device
+        c, s = self.pointers(dev)
+        n = slots.numel()
+        ps = _check(slots, "slots", torch.int32, dev, (None,))
+        pl = _check(lens, "lens", torch.int32, dev, (n,))
+        pp = _check(n_prompt, "n_prompt", torch.int32, dev, (n,))
+        pr = _check(row_start, "row_start", torch.int64, dev, (n,))
+        if row_start is None:
+            pt = _check(tokens, "tokens", torch.int32, dev, (n, None))
+            stride = width = tokens.shape[1]
+        else:
+            pt = _check(tokens, "tokens", torch.int32, dev, (None,))
+            if max_len is None or lens is None:
+                raise ValueError("flat tokens need lens and max_len")
+            stride, width = 0, max_len
+        if lens is None:
+            len_add = width
+        if n == 0 or width == 0:
+            return
+        with _lib.on_device(dev):
+            _lib.call("ms_token_counts_append", c, s, self.n_slots, self.vocab_size, ps, n, pt, pr,
+                      stride, pl, len_add, width, pp, _lib.stream_ptr(dev))
+
+
+@dataclass
+class LogitControls:
+    """The controls of a batch's requests, as device tensors (None: not used).
+
+    ``slots`` (B,) int32, the requests' rows in a :class:`TokenCounts` (negative: no
+    penalties) and ``penalties`` (B, 3) float32: repetition, presence,
+    frequency.  ``bias_start`` (B + 1,), ``bias_ids`` int32 and ``bias_values``
+    float32: request ``b``'s biases are entries ``bias_start[b]`` up to
+    ``bias_start[b + 1]``, ids ascending.  ``masks`` (n, words) int32 bit words (see
+    :func:`pack_masks`) and ``mask_rows`` (rows,) int32: each row's mask
+    (negative: none)."""
+
+    slots: torch.Tensor | None = None
+    penalties: torch.Tensor | None = None
+    bias_start: torch.Tensor | None = None
+    bias_ids: torch.Tensor | None = None
+    bias_values: torch.Tensor | None = None
+    masks: torch.Tensor | None = None
+    mask_rows: torch.Tensor | None = None
+
+
+def apply_logit_controls(
+    logits: torch.Tensor,
+    controls: LogitControls,
+    counts: TokenCounts | None = None,
+    *,
+    rows_per_request: int = 1,
+    proposals: torch.Tensor | None = None,
+    first_proposal: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The controlled logits of ``(B * rows_per_request, vocab)`` float32 rows.
+
+    ``proposals`` (gamma, B) int32 are a speculative round's draft tokens: row
+    ``i`` of a request treats its first ``first_proposal + i`` as generated.
+    ``out`` may be ``logits`` itself (only the changed logits are then touched)
+    or a tensor that does not overlap it; by default a new one is returned.
+    Masked tokens become ``-inf``; a row whose mask allows nothing is all
+    ``-inf``.  Rows may be strided; a row's logits must be contiguous."""
+    dev = _lib.require_cuda(logits.device)
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise ValueError("logits must be a float32 (rows, vocab) tensor with contiguous rows")
+    rows, vocab = logits.shape
+    if rows_per_request < 1 or rows % rows_per_request:
+        raise ValueError(f"{rows} rows are not a multiple of rows_per_request={rows_per_request}")
+    B = rows // rows_per_request
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
+    elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != dev \
+            or out.stride(1) != 1:
+        raise ValueError("out must be a float32 tensor of the logits' shape with contiguous rows")
+    if rows == 0 or vocab == 0:
+        return out
+    c = controls
+    words = mask_words(vocab)
+    s = _lib.MsLogitControls()
+    if c.slots is not None:
+        if counts is None or c.penalties is None:
+            raise ValueError("penalties need slots, penalties and token counts")
+        if counts.vocab_size != vocab:
+            raise ValueError(f"token counts are for a vocabulary of {counts.vocab_size}, not {vocab}")
+        s.slots = _check(c.slots, "slots", torch.int32, dev, (B,))
+        s.penalties = _check(c.penalties, "penalties", torch.float32, dev, (B, 3))
+        s.counts, s.seen = counts.pointers(dev)
+        s.n_slots = counts.n_slots
+        if proposals is not None:
+            s.proposals = _check(proposals, "proposals", torch.int32, dev, (None, B))
+            s.n_proposals = proposals.shape[0]
+            s.first_proposal = first_proposal
+            if not 0 <= first_proposal <= s.n_proposals - rows_per_request + 1 \
+                    or s.n_proposals > MAX_PROPOSALS:
+                raise ValueError(f"rows see {first_proposal} to {first_proposal + rows_per_request - 1} "
+                                 f"proposals of {s.n_proposals} (at most {MAX_PROPOSALS})")
+            if s.n_proposals == 0:
+                s.proposals = None
+    elif c.penalties is not None:
+        raise ValueError("penalties need slots, penalties and token counts")
+    if c.bias_start is not None:
+        if c.bias_ids is None or c.bias_values is None:
+            raise ValueError("bias_start needs bias_ids and bias_values")
+        n = c.bias_ids.numel()
+        s.bias_start = _check(c.bias_start, "bias_start", torch.int32, dev, (B + 1,))
+        s.bias_ids = _check(c.bias_ids, "bias_ids", torch.int32, dev, (n,))
+        s.bias_values = _check(c.bias_values, "bias_values", torch.float32, dev, (n,))
+        s.n_bias = n
+    if c.mask_rows is not None:
+        if c.masks is None:
+            raise ValueError("mask_rows needs masks")
+        s.mask_rows = _check(c.mask_rows, "mask_rows", torch.int32, dev, (rows,))
+        s.masks = _check(c.masks, "masks", torch.int32, dev, (None, words))
+        s.n_masks = c.masks.shape[0]
+        if s.n_masks == 0:
+            s.mask_rows = None
+    with _lib.on_device(dev):
+        _lib.call("ms_apply_logit_controls", logits.data_ptr(), logits.stride(0), out.data_ptr(),
+                  out.stride(0), B, rows_per_request, vocab, ctypes.byref(s), _lib.stream_ptr(dev))
+    return out
