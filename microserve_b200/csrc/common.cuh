@@ -76,6 +76,22 @@ struct ProfScope {
   int slot;
 };
 
+// Lets `kernel` take up to `bytes` of dynamic shared memory on the current
+// device; `granted` (one per kernel) remembers the devices, a bit each.
+template <typename F>
+int grant_dynamic_smem(F kernel, int bytes, std::atomic<uint64_t>& granted) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == cudaSuccess && dev < 64 && (granted.load(std::memory_order_relaxed) & bit)) return MS_OK;
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess)
+    return fail(MS_ERR_CUDA, "shared memory of %d bytes: %s", bytes, cudaGetErrorString(e));
+  granted.fetch_or(bit, std::memory_order_relaxed);
+  return MS_OK;
+}
+
 #define MS_REQUIRE(cond, ...)                              \
   do {                                                     \
     if (!(cond)) return ::ms::fail(MS_ERR_INVALID, __VA_ARGS__); \

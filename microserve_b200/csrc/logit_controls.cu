@@ -18,9 +18,8 @@ namespace ms {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;
-constexpr int kSlice = kThreads * 4 * kUnroll;  // tokens per CTA
-constexpr int kMaxProposals = 64;               // the draft lanes of one round
+constexpr int kSlice = 4096;       // tokens per CTA
+constexpr int kMaxProposals = 64;  // the draft lanes of one round
 
 struct ControlArgs {
   const float* in;
@@ -42,201 +41,357 @@ __device__ __forceinline__ float penalise(float x, const Penalty& p, int count) 
   return count > 0 ? __fsub_rn(y, p.pres) : y;
 }
 
-// One CTA: kSlice tokens of rows_per_cta rows of one request.
-template <bool VEC, bool INPLACE>
-__global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a) {
-  pdl_enter();
-  __shared__ int s_prop[kMaxProposals];  // proposals inside this slice: id - first token
-  __shared__ int s_when[kMaxProposals];  // and their positions
-  __shared__ int s_nprop;
-  __shared__ int s_bias_lo, s_bias_hi;
-  __shared__ float s_bias[kSlice];
+// The edits of one request in one slice of the vocabulary, gathered once per
+// CTA and applied to each of its rows: few tokens are touched (the seen ones,
+// the round's proposals, the biased ones), so they are listed and shared out
+// over the threads instead of being looked for at every logit of every row.
+struct Slice {
+  // proposals inside the slice: offset and position in the round
+  int prop[kMaxProposals];
+  int when[kMaxProposals];
+  int n_prop;
+  int bias_lo, bias_hi;  // the bias entries to look at
+  int n_list;
+  // mask words of the row at hand and of the next one
+  uint32_t mask[2][kSlice / 32];
+  // touched tokens: offset | seen << 12 | count << 13 (kCountCap: look it up)
+  uint32_t list[kSlice];
+};
+static_assert(kSlice == 4096, "12 bits of offset");
+constexpr uint32_t kCountCap = (1u << 19) - 1;
+
+__device__ __forceinline__ int valid_slot(const ControlArgs& a, int b) {
+  const int slot = a.c.slots ? a.c.slots[b] : -1;
+  if (slot < a.c.n_slots) return max(slot, -1);
+  if (threadIdx.x == 0) raise_device_error(a.err, kErrSlot);
+  return -1;
+}
+
+// Word `threadIdx.x` of the row's mask in the slice (all ones: no mask).
+__device__ __forceinline__ uint32_t mask_word(const ControlArgs& a, int64_t row, int t0, bool& masked) {
+  int m = a.c.mask_rows ? a.c.mask_rows[row] : -1;
+  if (m >= a.c.n_masks) {
+    if (threadIdx.x == 0) raise_device_error(a.err, kErrMask);
+    m = -1;
+  }
+  masked = m >= 0;
+  const int w = (t0 >> 5) + threadIdx.x;
+  return masked && threadIdx.x < kSlice / 32 && w < a.words
+             ? __ldg(a.c.masks + (int64_t)m * a.words + w)
+             : 0xffffffffu;
+}
+
+// Gathers the slice's edits and the first row's mask; block-wide, ends with a barrier.
+__device__ void load_slice(const ControlArgs& a, int b, int slot, int64_t row0, int t0, int n_here,
+                           Slice& sl, bool& masked) {
   const ms_logit_controls& c = a.c;
   const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * kSlice;
-  const int b = blockIdx.y;
-  const int r0 = blockIdx.z * a.rows_per_cta;
-  const int r1 = min(a.rows, r0 + a.rows_per_cta);
-  const int n_here = min(kSlice, a.vocab - t0);
-
-  int slot = c.slots ? c.slots[b] : -1;
-  if (slot >= c.n_slots) {
-    if (tid == 0) raise_device_error(a.err, kErrSlot);
-    slot = -1;
+  if (tid == 0) sl.n_prop = sl.n_list = 0;
+  uint32_t seen = 0;
+  const int w = (t0 >> 5) + tid;
+  if (slot >= 0 && tid < kSlice / 32 && w < a.words) {
+    seen = __ldg(c.seen + (int64_t)slot * a.words + w);
+    const int left = n_here - 32 * tid;  // bits past the vocabulary mean nothing
+    if (left < 32) seen &= left > 0 ? (1u << left) - 1u : 0u;
   }
-  if (slot < 0) slot = -1;
-  Penalty p{1.f, 0.f, 0.f};
-  if (slot >= 0) p = Penalty{c.penalties[3 * b], c.penalties[3 * b + 1], c.penalties[3 * b + 2]};
-
-  // What of the proposals and the bias list falls into this slice.
-  if (tid == 0) s_nprop = 0;
-  if (tid < 2 && c.bias_start) {
-    int lo = c.bias_start[b], hi = c.bias_start[b + 1];
-    if (lo < 0 || hi < lo || hi > c.n_bias) {
-      raise_device_error(a.err, kErrOrder);
-      lo = hi = 0;
-    }
-    // first entry at or past the slice's first / one-past-last token
-    const int want = tid == 0 ? t0 : t0 + n_here;
-    const bool edge = tid == 0 ? blockIdx.x == 0 : blockIdx.x + 1 == gridDim.x;
-    if (!edge) {
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (c.bias_ids[mid] < want) lo = mid + 1; else hi = mid;
+  const uint32_t first_mask = mask_word(a, row0, t0, masked);
+  if (tid < kSlice / 32) sl.mask[0][tid] = first_mask;
+  // threads 64 and 65 cut the request's bias list to the slice; the outer
+  // slices also take (and report) ids outside the vocabulary
+  if (tid == 64 || tid == 65) {
+    int lo = 0, hi = 0;
+    if (c.bias_start) {
+      lo = c.bias_start[b];
+      hi = c.bias_start[b + 1];
+      if (lo < 0 || hi < lo || hi > c.n_bias) {
+        raise_device_error(a.err, kErrOrder);
+        lo = hi = 0;
       }
-    } else if (tid == 1) {
-      lo = hi;  // the last slice also takes (and reports) ids past the vocabulary
+      const int want = tid == 64 ? t0 : t0 + n_here;
+      if (tid == 64 ? blockIdx.x > 0 : blockIdx.x + 1 < gridDim.x) {
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (c.bias_ids[mid] < want) lo = mid + 1; else hi = mid;
+        }
+      } else if (tid == 65) {
+        lo = hi;
+      }
     }
-    (tid == 0 ? s_bias_lo : s_bias_hi) = lo;
+    (tid == 64 ? sl.bias_lo : sl.bias_hi) = lo;
   }
   __syncthreads();
+  int at = seen ? atomicAdd(&sl.n_list, __popc(seen)) : 0;
+  for (uint32_t m = seen; m; m &= m - 1)
+    sl.list[at++] = (uint32_t)(32 * tid + __ffs(m) - 1) | 1u << 12;
   if (slot >= 0 && c.proposals && tid < c.n_proposals) {
     const int v = c.proposals[(int64_t)tid * a.n_requests + b];
     if (v < 0 || v >= a.vocab) {
       raise_device_error(a.err, kErrToken);
     } else if (v >= t0 && v < t0 + n_here) {
-      const int k = atomicAdd(&s_nprop, 1);
-      s_prop[k] = v - t0;
-      s_when[k] = tid;
+      const int k = atomicAdd(&sl.n_prop, 1);
+      sl.prop[k] = v - t0;
+      sl.when[k] = tid;
     }
   }
-  const int blo = c.bias_start ? s_bias_lo : 0, bhi = c.bias_start ? s_bias_hi : 0;
-  const bool biased = bhi > blo;
-  if (biased) {
-    for (int i = tid; i < n_here; i += kThreads) s_bias[i] = 0.f;
+  __syncthreads();
+  if (tid < sl.n_prop) {  // list the proposals that no other entry stands for
+    const int o = sl.prop[tid];
+    bool fresh = !(__ldg(c.seen + (int64_t)slot * a.words + ((t0 + o) >> 5)) >> (o & 31) & 1u);
+    for (int j = 0; j < sl.n_prop; ++j)
+      fresh &= !(sl.prop[j] == o && sl.when[j] < sl.when[tid]);
+    if (fresh) sl.list[atomicAdd(&sl.n_list, 1)] = (uint32_t)o;
+  }
+  if (c.proposals) __syncthreads();
+  for (int e = tid; e < sl.n_list; e += kThreads) {
+    const uint32_t entry = sl.list[e];
+    const uint32_t n = (uint32_t)c.counts[(int64_t)slot * a.vocab + t0 + (entry & (kSlice - 1))];
+    sl.list[e] = entry | min(n, kCountCap) << 13;
+  }
+  __syncthreads();
+}
+
+// Applies the edits to one row's slice x (shared or global memory; token o of
+// the slice at x[o], `mis` floats past a 16-byte boundary): penalties, biases,
+// then the mask.  Block-wide; the caller's barrier follows.
+template <bool SHARED>
+__device__ __forceinline__ void edit_row(const ControlArgs& a, const Slice& sl, int b, int slot,
+                                         const Penalty& p, int visible, int t0, int n_here,
+                                         const uint32_t* mask, bool masked, float* x, int mis) {
+  const ms_logit_controls& c = a.c;
+  const int tid = threadIdx.x;
+  for (int e = tid; e < sl.n_list; e += kThreads) {
+    const uint32_t entry = sl.list[e];
+    const int o = entry & (kSlice - 1);
+    bool said = entry >> 12 & 1u;
+    int n = (int)(entry >> 13);
+    if (n == (int)kCountCap) n = c.counts[(int64_t)slot * a.vocab + t0 + o];
+    for (int j = 0; j < sl.n_prop; ++j) {
+      const bool hit = sl.prop[j] == o && sl.when[j] < visible;
+      said |= hit;
+      n += hit;
+    }
+    if (said) x[o] = penalise(x[o], p, n);
+  }
+  if (sl.bias_hi > sl.bias_lo) {
     __syncthreads();
     const int first = c.bias_start[b];
-    for (int e = blo + tid; e < bhi; e += kThreads) {
+    for (int e = sl.bias_lo + tid; e < sl.bias_hi; e += kThreads) {
       const int v = c.bias_ids[e];
       if (v < 0 || v >= a.vocab)
         raise_device_error(a.err, kErrToken);
       else if (e > first && c.bias_ids[e - 1] >= v)
         raise_device_error(a.err, kErrOrder);  // not ascending: the entry is skipped
       else if (v >= t0 && v < t0 + n_here)
-        s_bias[v - t0] = c.bias_values[e];
+        x[v - t0] = __fadd_rn(x[v - t0], c.bias_values[e]);
     }
   }
-  __syncthreads();
-  const int nprop = s_nprop;
-
-  // Token group u of this thread: VEC: 4 tokens at 4 * (u * kThreads + tid);
-  // else single tokens at (4 u + k) * kThreads + tid, so a warp's 32 tokens
-  // are one bit word.
-  auto token = [&](int u, int k) {
-    return VEC ? 4 * (u * kThreads + tid) + k : (4 * u + k) * kThreads + tid;
-  };
-  auto bits_of = [&](const uint32_t* words, int u) -> uint32_t {
-    if constexpr (VEC) {
-      const int o = token(u, 0);
-      return o < n_here ? (__ldg(words + ((t0 + o) >> 5)) >> (o & 31)) & 15u : 0u;
+  if (!masked) return;
+  if (sl.n_list > 0 || sl.bias_hi > sl.bias_lo) __syncthreads();
+  // groups of 4 tokens on 16-byte boundaries
+  for (int o = 4 * tid - mis; o < n_here; o += 4 * kThreads) {
+    uint32_t ok;
+    if (o >= 0) {
+      const int sh = o & 31;
+      ok = mask[o >> 5] >> sh;
+      if (sh > 28 && o + 32 - sh < n_here) ok |= mask[(o >> 5) + 1] << (32 - sh);
     } else {
-      uint32_t r = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int o = token(u, k);
-        if (o < n_here) r |= ((__ldg(words + ((t0 + o) >> 5)) >> (o & 31)) & 1u) << k;
-      }
-      return r;
+      ok = mask[0] << -o;
     }
-  };
-  uint32_t seen[kUnroll];
+    const int lo = max(0, -o), hi = min(4, n_here - o);  // its tokens inside the slice
+    const uint32_t in = (1u << hi) - (1u << lo);
+    const uint32_t no = ~ok & in;
+    if (no == 15u) {
+      *reinterpret_cast<float4*>(x + o) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    } else if (SHARED && no && in == 15u) {
+      float4 q = *reinterpret_cast<float4*>(x + o);
+      if (no & 1u) q.x = -INFINITY;
+      if (no & 2u) q.y = -INFINITY;
+      if (no & 4u) q.z = -INFINITY;
+      if (no & 8u) q.w = -INFINITY;
+      *reinterpret_cast<float4*>(x + o) = q;
+    } else if (no) {
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    seen[u] = slot >= 0 ? bits_of(c.seen + (int64_t)slot * a.words, u) : 0u;
-  const int32_t* count_row = slot >= 0 ? c.counts + (int64_t)slot * a.vocab + t0 : nullptr;
+      for (int k = 0; k < 4; ++k)
+        if (no >> k & 1u) x[o + k] = -INFINITY;
+    }
+  }
+}
 
-  for (int r = r0; r < r1; ++r) {
-    const int64_t row = (int64_t)b * a.rows + r;
-    const float* xin = a.in + row * a.in_stride + t0;
-    float* yout = a.out + row * a.out_stride + t0;
-    int mrow = c.mask_rows ? c.mask_rows[row] : -1;
-    if (mrow >= c.n_masks) {
-      if (tid == 0) raise_device_error(a.err, kErrMask);
-      mrow = -1;
+// ---- out of place, through shared memory ------------------------------------
+// A CTA takes kSlice tokens of one request's rows.  Each row's slice comes in
+// by one bulk copy, is edited in shared memory and goes out by one bulk copy,
+// in a ring of rows.  The kernel moves 8 bytes per logit and is bound by HBM.
+// A row that does not start on 16 bytes keeps its misalignment in shared
+// memory; its up to 3 first and last logits are copied one by one.
+constexpr int kRing = 2;
+constexpr int kRowFloats = kSlice + 4;
+constexpr long long kWaitCycles = 1ll << 32;  // ~2.2 s
+constexpr int kErrTimeout = 5;
+
+__device__ __forceinline__ uint32_t s_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity, int* err) {
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (clock64() - t0 > kWaitCycles) {
+      atomicCAS(err, 0, kErrTimeout);
+      return false;
     }
-    const uint32_t* mask = mrow >= 0 ? c.masks + (int64_t)mrow * a.words : nullptr;
-    const int visible = c.first_proposal + r;  // proposals this row sees
-    float v[kUnroll][4];
-    if constexpr (!INPLACE) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if constexpr (VEC) {
-          const int o = token(u, 0);
-          float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (o < n_here) q = __ldcs(reinterpret_cast<const float4*>(xin + o));
-          v[u][0] = q.x, v[u][1] = q.y, v[u][2] = q.z, v[u][3] = q.w;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int o = token(u, k);
-            v[u][k] = o < n_here ? __ldcs(xin + o) : 0.f;
-          }
-        }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a, int ring) {
+  extern __shared__ __align__(16) float smem[];  // [ring][kRowFloats]
+  __shared__ Slice sl;
+  __shared__ __align__(8) uint64_t bars[kRing];
+  const ms_logit_controls& c = a.c;
+  const int tid = threadIdx.x;
+  const int t0 = blockIdx.x * kSlice;
+  const int b = blockIdx.y;
+  const int r0 = blockIdx.z * a.rows_per_cta;
+  const int n_rows = min(a.rows - r0, a.rows_per_cta);
+  const int n_here = min(kSlice, a.vocab - t0);
+  const int64_t row0 = (int64_t)b * a.rows + r0;
+
+  // Row it: misalignment (in floats), loose first logits, bulk-copied logits.
+  struct Cut {
+    int mis, head, body;
+  };
+  auto cut = [&](int it) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a.in + (row0 + it) * a.in_stride + t0);
+    Cut q;
+    q.mis = (int)(p >> 2) & 3;
+    q.head = min((4 - q.mis) & 3, n_here);
+    q.body = (n_here - q.head) & ~3;
+    return q;
+  };
+  auto issue = [&](int it) {  // thread 0
+    const Cut q = cut(it);
+    const uint32_t bar = s_addr(&bars[it % ring]);
+    const uint32_t bytes = 4u * q.body;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+    if (bytes)
+      bulk_load(s_addr(smem + (it % ring) * kRowFloats + q.mis + q.head),
+                a.in + (row0 + it) * a.in_stride + t0 + q.head, bytes, bar);
+  };
+  const int ahead = ring > 1 ? ring - 1 : 1;  // rows in flight
+  if (tid == 0) {
+    for (int k = 0; k < ring; ++k)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s_addr(&bars[k])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  pdl_enter();
+  if (tid == 0)
+    for (int it = 0; it < min(ahead, n_rows); ++it) issue(it);
+  const int slot = valid_slot(a, b);
+  Penalty p{1.f, 0.f, 0.f};
+  if (slot >= 0) p = Penalty{c.penalties[3 * b], c.penalties[3 * b + 1], c.penalties[3 * b + 2]};
+  bool masked;
+  load_slice(a, b, slot, row0, t0, n_here, sl, masked);
+
+  for (int it = 0; it < n_rows; ++it) {
+    float* buf = smem + (it % ring) * kRowFloats;
+    const Cut q = cut(it);
+    const float* xin = a.in + (row0 + it) * a.in_stride + t0;
+    float* yout = a.out + (row0 + it) * a.out_stride + t0;
+    const int tail0 = q.head + q.body;
+    const bool loose = q.head > 0 || tail0 < n_here;
+    if (tid < q.head) buf[q.mis + tid] = xin[tid];
+    if (tid >= 32 && tail0 + tid - 32 < n_here) buf[q.mis + tail0 + tid - 32] = xin[tail0 + tid - 32];
+    bool next_masked = false;
+    uint32_t next_mask = 0;
+    if (it + 1 < n_rows) next_mask = mask_word(a, row0 + it + 1, t0, next_masked);
+    const bool ok = wait_full(s_addr(&bars[it % ring]), (it / ring) & 1, a.err);
+    if (loose) __syncthreads();
+    float* x = buf + q.mis;
+    edit_row<true>(a, sl, b, slot, p, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
+                   masked, x, q.mis);
+    if (tid < kSlice / 32) sl.mask[(it + 1) & 1][tid] = next_mask;
+    masked = next_masked;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    // all threads agree to stop when a copy did not arrive in time
+    if (__syncthreads_or(!ok)) {
+      if (tid == 0)  // no copy may arrive after the block has gone
+        for (int k = it; k < min(it + ahead, n_rows); ++k)
+          wait_full(s_addr(&bars[k % ring]), (k / ring) & 1, a.err);
+      break;
+    }
+    if (tid < q.head) yout[tid] = x[tid];
+    if (tid >= 32 && tail0 + tid - 32 < n_here) yout[tail0 + tid - 32] = x[tail0 + tid - 32];
+    if (tid == 0) {
+      if (q.body) bulk_store(yout + q.head, s_addr(x + q.head), 4u * q.body);
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      if (it + ahead < n_rows) {
+        // the row `ahead` from here takes the buffer of the row before this one
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        issue(it + ahead);
       }
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (token(u, 0) >= n_here) break;
-      uint32_t said = seen[u];
-      for (int j = 0; j < nprop; ++j) {
-        if (s_when[j] >= visible) continue;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (s_prop[j] == token(u, k)) said |= 1u << k;
-      }
-      const uint32_t ok = mask ? bits_of(mask, u) : 15u;
-      uint32_t touched = said;
-      if (biased) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int o = token(u, k);
-          if (o < n_here && s_bias[o] != 0.f) touched |= 1u << k;
-        }
-      }
-      if (touched & ok) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (!((touched & ok) >> k & 1u)) continue;
-          const int o = token(u, k);
-          float y = INPLACE ? xin[o] : v[u][k];
-          if (said >> k & 1u) {
-            int n = count_row[o];
-            for (int j = 0; j < nprop; ++j) n += s_prop[j] == o && s_when[j] < visible;
-            y = penalise(y, p, n);
-          }
-          if (biased && s_bias[o] != 0.f) y = __fadd_rn(y, s_bias[o]);
-          v[u][k] = y;
-          if (INPLACE) yout[o] = y;
-        }
-      }
-      if (ok != 15u) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (ok >> k & 1u) continue;
-          v[u][k] = -INFINITY;
-          if (INPLACE && (!VEC || ok != 0u) && token(u, k) < n_here) yout[token(u, k)] = -INFINITY;
-        }
-        if (INPLACE && VEC && ok == 0u)
-          *reinterpret_cast<float4*>(yout + token(u, 0)) =
-              make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      }
+    if (loose) __syncthreads();  // its loose logits are out before the buffer is filled again
+  }
+  if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// ---- in place, or with input and output rows aligned differently ---------------
+// In place only what a control touches is read and written; else the slice is
+// copied first and then edited where it is.
+__global__ void __launch_bounds__(kThreads) logit_controls_direct_kernel(ControlArgs a) {
+  pdl_enter();
+  __shared__ Slice sl;
+  const ms_logit_controls& c = a.c;
+  const int tid = threadIdx.x;
+  const int t0 = blockIdx.x * kSlice;
+  const int b = blockIdx.y;
+  const int r0 = blockIdx.z * a.rows_per_cta;
+  const int n_rows = min(a.rows - r0, a.rows_per_cta);
+  const int n_here = min(kSlice, a.vocab - t0);
+  const int64_t row0 = (int64_t)b * a.rows + r0;
+  const int slot = valid_slot(a, b);
+  Penalty p{1.f, 0.f, 0.f};
+  if (slot >= 0) p = Penalty{c.penalties[3 * b], c.penalties[3 * b + 1], c.penalties[3 * b + 2]};
+  bool masked;
+  load_slice(a, b, slot, row0, t0, n_here, sl, masked);
+  for (int it = 0; it < n_rows; ++it) {
+    float* x = a.out + (row0 + it) * a.out_stride + t0;
+    if (a.in != a.out) {
+      const float* xin = a.in + (row0 + it) * a.in_stride + t0;
+#pragma unroll 8
+      for (int o = tid; o < n_here; o += kThreads) x[o] = xin[o];
+      __syncthreads();
     }
-    if constexpr (!INPLACE) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if constexpr (VEC) {
-          const int o = token(u, 0);
-          if (o < n_here)
-            __stcs(reinterpret_cast<float4*>(yout + o),
-                   make_float4(v[u][0], v[u][1], v[u][2], v[u][3]));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int o = token(u, k);
-            if (o < n_here) __stcs(yout + o, v[u][k]);
-          }
-        }
-      }
+    bool next_masked = false;
+    uint32_t next_mask = 0;
+    if (it + 1 < n_rows) next_mask = mask_word(a, row0 + it + 1, t0, next_masked);
+    edit_row<false>(a, sl, b, slot, p, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
+                    masked, x, (int)(reinterpret_cast<uintptr_t>(x) >> 2) & 3);
+    if (it + 1 < n_rows) {
+      if (tid < kSlice / 32) sl.mask[(it + 1) & 1][tid] = next_mask;
+      masked = next_masked;
+      __syncthreads();
     }
   }
 }
@@ -355,19 +510,19 @@ extern "C" int ms_apply_logit_controls(const float* logits, int64_t row_stride, 
   const int slices = ceil_div(vocab, kSlice);
   a.rows_per_cta = rows_per_request;
   const dim3 grid(slices, n_requests, ceil_div(rows_per_request, a.rows_per_cta));
-  const bool vec = vocab % 4 == 0 && row_stride % 4 == 0 && out_stride % 4 == 0 &&
-                   ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const uintptr_t pi = reinterpret_cast<uintptr_t>(logits), po = reinterpret_cast<uintptr_t>(out);
   cudaStream_t s = as_stream(stream);
   ProfScope prof(kClsSample, s);
-  if (vec && in_place)
-    launch_pdl(logit_controls_kernel<true, true>, grid, kThreads, 0, s, a);
-  else if (vec)
-    launch_pdl(logit_controls_kernel<true, false>, grid, kThreads, 0, s, a);
-  else if (in_place)
-    launch_pdl(logit_controls_kernel<false, true>, grid, kThreads, 0, s, a);
-  else
-    launch_pdl(logit_controls_kernel<false, false>, grid, kThreads, 0, s, a);
-  return check_launch("logit_controls_kernel");
+  // every row of the input and of the output equally far from 16 bytes
+  if (!in_place && ((pi ^ po) & 15) == 0 && (row_stride - out_stride) % 4 == 0) {
+    const int ring = a.rows_per_cta < kRing ? a.rows_per_cta : kRing;
+    static std::atomic<uint64_t> granted{0};  // with the static part past the default 48 KB
+    MS_TRY(grant_dynamic_smem(logit_controls_kernel, kRing * kRowFloats * 4, granted));
+    launch_pdl(logit_controls_kernel, grid, kThreads, ring * kRowFloats * 4, s, a, ring);
+    return check_launch("logit_controls_kernel");
+  }
+  launch_pdl(logit_controls_direct_kernel, grid, kThreads, 0, s, a);
+  return check_launch("logit_controls_direct_kernel");
 }
 
 extern "C" int ms_token_counts_append(int32_t* counts, uint32_t* seen, int n_slots, int vocab,

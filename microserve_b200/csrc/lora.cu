@@ -431,26 +431,12 @@ int shrink_split(int n_tiles, int K, int n_slices, int max_rank) {
   return split;
 }
 
-// Lets `kernel` take up to `most` bytes of dynamic shared memory on the
-// current device; `granted` remembers the devices (a bit each).
-template <typename F>
-int grant_smem(F kernel, int most, std::atomic<uint64_t>& granted) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (e == cudaSuccess && dev < 64 && (granted.load(std::memory_order_relaxed) & bit)) return MS_OK;
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-  if (e != cudaSuccess) return fail(MS_ERR_CUDA, "lora: shared memory: %s", cudaGetErrorString(e));
-  granted.fetch_or(bit, std::memory_order_relaxed);
-  return MS_OK;
-}
 constexpr int kMostSmem = 226 * 1024;
 
 template <int EPI>
 int launch_expand(const ExpandArgs& p, int smem, cudaStream_t s) {
   static std::atomic<uint64_t> granted{0};
-  if (smem > 48 * 1024) MS_TRY(grant_smem(lora_expand_kernel<EPI>, kMostSmem, granted));
+  if (smem > 48 * 1024) MS_TRY(grant_dynamic_smem(lora_expand_kernel<EPI>, kMostSmem, granted));
   const dim3 grid(ceil_div(p.N, kExpCols), p.plan.n_tiles);
   launch_pdl(lora_expand_kernel<EPI>, grid, kExpWarps * 32, smem, s, p);
   return check_launch("lora_expand_kernel");
@@ -460,7 +446,7 @@ template <int MT>
 int launch_shrink(const ShrinkArgs& p, int row_blocks, cudaStream_t s) {
   const int smem = kShrinkWarps * 16 * MT * kShrinkTokens * 4;
   static std::atomic<uint64_t> granted{0};
-  if (smem > 48 * 1024) MS_TRY(grant_smem(lora_shrink_kernel<MT>, smem, granted));
+  if (smem > 48 * 1024) MS_TRY(grant_dynamic_smem(lora_shrink_kernel<MT>, smem, granted));
   const dim3 grid(p.plan.n_tiles * (kTile / kShrinkTokens), row_blocks, p.k_split);
   launch_pdl(lora_shrink_kernel<MT>, grid, kShrinkWarps * 32, smem, s, p);
   return check_launch("lora_shrink_kernel");
