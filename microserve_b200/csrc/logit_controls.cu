@@ -45,6 +45,7 @@ __device__ __forceinline__ float penalise(float x, const Penalty& p, int count) 
 // CTA and applied to each of its rows: few tokens are touched (the seen ones,
 // the round's proposals, the biased ones), so they are listed and shared out
 // over the threads instead of being looked for at every logit of every row.
+// A thread keeps its first entry and that token's count in registers.
 struct Slice {
   // proposals inside the slice: offset and position in the round
   int prop[kMaxProposals];
@@ -54,11 +55,10 @@ struct Slice {
   int n_list;
   // mask words of the row at hand and of the next one
   uint32_t mask[2][kSlice / 32];
-  // touched tokens: offset | seen << 12 | count << 13 (kCountCap: look it up)
-  uint32_t list[kSlice];
+  // touched tokens: offset | seen << 12
+  uint16_t list[kSlice];
 };
 static_assert(kSlice == 4096, "12 bits of offset");
-constexpr uint32_t kCountCap = (1u << 19) - 1;
 
 __device__ __forceinline__ int valid_slot(const ControlArgs& a, int b) {
   const int slot = a.c.slots ? a.c.slots[b] : -1;
@@ -79,6 +79,20 @@ __device__ __forceinline__ uint32_t mask_word(const ControlArgs& a, int64_t row,
   return masked && threadIdx.x < kSlice / 32 && w < a.words
              ? __ldg(a.c.masks + (int64_t)m * a.words + w)
              : 0xffffffffu;
+}
+
+struct Entry {
+  int o;      // offset in the slice (-1: none)
+  bool seen;  // else listed for a proposal only
+  int count;
+};
+
+__device__ __forceinline__ Entry list_entry(const ControlArgs& a, const Slice& sl, int slot, int t0,
+                                            int e) {
+  if (e >= sl.n_list) return Entry{-1, false, 0};
+  const int v = sl.list[e];
+  const int o = v & (kSlice - 1);
+  return Entry{o, (v >> 12) != 0, a.c.counts[(int64_t)slot * a.vocab + t0 + o]};
 }
 
 // Gathers the slice's edits and the first row's mask; block-wide, ends with a barrier.
@@ -122,7 +136,7 @@ __device__ void load_slice(const ControlArgs& a, int b, int slot, int64_t row0, 
   __syncthreads();
   int at = seen ? atomicAdd(&sl.n_list, __popc(seen)) : 0;
   for (uint32_t m = seen; m; m &= m - 1)
-    sl.list[at++] = (uint32_t)(32 * tid + __ffs(m) - 1) | 1u << 12;
+    sl.list[at++] = (uint16_t)((32 * tid + __ffs(m) - 1) | 1 << 12);
   if (slot >= 0 && c.proposals && tid < c.n_proposals) {
     const int v = c.proposals[(int64_t)tid * a.n_requests + b];
     if (v < 0 || v >= a.vocab) {
@@ -139,15 +153,9 @@ __device__ void load_slice(const ControlArgs& a, int b, int slot, int64_t row0, 
     bool fresh = !(__ldg(c.seen + (int64_t)slot * a.words + ((t0 + o) >> 5)) >> (o & 31) & 1u);
     for (int j = 0; j < sl.n_prop; ++j)
       fresh &= !(sl.prop[j] == o && sl.when[j] < sl.when[tid]);
-    if (fresh) sl.list[atomicAdd(&sl.n_list, 1)] = (uint32_t)o;
+    if (fresh) sl.list[atomicAdd(&sl.n_list, 1)] = (uint16_t)o;
   }
   if (c.proposals) __syncthreads();
-  for (int e = tid; e < sl.n_list; e += kThreads) {
-    const uint32_t entry = sl.list[e];
-    const uint32_t n = (uint32_t)c.counts[(int64_t)slot * a.vocab + t0 + (entry & (kSlice - 1))];
-    sl.list[e] = entry | min(n, kCountCap) << 13;
-  }
-  __syncthreads();
 }
 
 // Applies the edits to one row's slice x (shared or global memory; token o of
@@ -155,27 +163,23 @@ __device__ void load_slice(const ControlArgs& a, int b, int slot, int64_t row0, 
 // then the mask.  Block-wide; the caller's barrier follows.
 template <bool SHARED>
 __device__ __forceinline__ void edit_row(const ControlArgs& a, const Slice& sl, int b, int slot,
-                                         const Penalty& p, int visible, int t0, int n_here,
+                                         const Penalty& p, const Entry& own, int visible, int t0, int n_here,
                                          const uint32_t* mask, bool masked, float* x, int mis) {
   const ms_logit_controls& c = a.c;
   const int tid = threadIdx.x;
-  for (int e = tid; e < sl.n_list; e += kThreads) {
-    const uint32_t entry = sl.list[e];
-    const int o = entry & (kSlice - 1);
-    bool said = entry >> 12 & 1u;
-    int n = (int)(entry >> 13);
-    if (n == (int)kCountCap) n = c.counts[(int64_t)slot * a.vocab + t0 + o];
+  for (int e = tid; e < sl.n_list; e += blockDim.x) {
+    Entry t = e == tid ? own : list_entry(a, sl, slot, t0, e);
     for (int j = 0; j < sl.n_prop; ++j) {
-      const bool hit = sl.prop[j] == o && sl.when[j] < visible;
-      said |= hit;
-      n += hit;
+      const bool hit = sl.prop[j] == t.o && sl.when[j] < visible;
+      t.seen |= hit;
+      t.count += hit;
     }
-    if (said) x[o] = penalise(x[o], p, n);
+    if (t.seen) x[t.o] = penalise(x[t.o], p, t.count);
   }
   if (sl.bias_hi > sl.bias_lo) {
     __syncthreads();
     const int first = c.bias_start[b];
-    for (int e = sl.bias_lo + tid; e < sl.bias_hi; e += kThreads) {
+    for (int e = sl.bias_lo + tid; e < sl.bias_hi; e += blockDim.x) {
       const int v = c.bias_ids[e];
       if (v < 0 || v >= a.vocab)
         raise_device_error(a.err, kErrToken);
@@ -188,7 +192,7 @@ __device__ __forceinline__ void edit_row(const ControlArgs& a, const Slice& sl, 
   if (!masked) return;
   if (sl.n_list > 0 || sl.bias_hi > sl.bias_lo) __syncthreads();
   // groups of 4 tokens on 16-byte boundaries
-  for (int o = 4 * tid - mis; o < n_here; o += 4 * kThreads) {
+  for (int o = 4 * tid - mis; o < n_here; o += 4 * blockDim.x) {
     uint32_t ok;
     if (o >= 0) {
       const int sh = o & 31;
@@ -312,6 +316,7 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
   if (slot >= 0) p = Penalty{c.penalties[3 * b], c.penalties[3 * b + 1], c.penalties[3 * b + 2]};
   bool masked;
   load_slice(a, b, slot, row0, t0, n_here, sl, masked);
+  const Entry own = list_entry(a, sl, slot, t0, tid);
 
   for (int it = 0; it < n_rows; ++it) {
     float* buf = smem + (it % ring) * kRowFloats;
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
     const bool ok = wait_full(s_addr(&bars[it % ring]), (it / ring) & 1, a.err);
     if (loose) __syncthreads();
     float* x = buf + q.mis;
-    edit_row<true>(a, sl, b, slot, p, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
+    edit_row<true>(a, sl, b, slot, p, own, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
                    masked, x, q.mis);
     if (tid < kSlice / 32) sl.mask[(it + 1) & 1][tid] = next_mask;
     masked = next_masked;
@@ -358,8 +363,11 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
 
 // ---- in place, or with input and output rows aligned differently ---------------
 // In place only what a control touches is read and written; else the slice is
-// copied first and then edited where it is.
-__global__ void __launch_bounds__(kThreads) logit_controls_direct_kernel(ControlArgs a) {
+// copied first and then edited where it is.  128 threads a CTA: its work is
+// a chain of short dependent reads, so more CTAs per SM beat more threads
+// (grammar masks over 256 x 128256: 28.6 us, 33.9 with 256).
+constexpr int kDirectThreads = 128;
+__global__ void __launch_bounds__(kDirectThreads) logit_controls_direct_kernel(ControlArgs a) {
   pdl_enter();
   __shared__ Slice sl;
   const ms_logit_controls& c = a.c;
@@ -375,18 +383,19 @@ __global__ void __launch_bounds__(kThreads) logit_controls_direct_kernel(Control
   if (slot >= 0) p = Penalty{c.penalties[3 * b], c.penalties[3 * b + 1], c.penalties[3 * b + 2]};
   bool masked;
   load_slice(a, b, slot, row0, t0, n_here, sl, masked);
+  const Entry own = list_entry(a, sl, slot, t0, tid);
   for (int it = 0; it < n_rows; ++it) {
     float* x = a.out + (row0 + it) * a.out_stride + t0;
     if (a.in != a.out) {
       const float* xin = a.in + (row0 + it) * a.in_stride + t0;
 #pragma unroll 8
-      for (int o = tid; o < n_here; o += kThreads) x[o] = xin[o];
+      for (int o = tid; o < n_here; o += kDirectThreads) x[o] = xin[o];
       __syncthreads();
     }
     bool next_masked = false;
     uint32_t next_mask = 0;
     if (it + 1 < n_rows) next_mask = mask_word(a, row0 + it + 1, t0, next_masked);
-    edit_row<false>(a, sl, b, slot, p, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
+    edit_row<false>(a, sl, b, slot, p, own, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
                     masked, x, (int)(reinterpret_cast<uintptr_t>(x) >> 2) & 3);
     if (it + 1 < n_rows) {
       if (tid < kSlice / 32) sl.mask[(it + 1) & 1][tid] = next_mask;
@@ -521,7 +530,7 @@ extern "C" int ms_apply_logit_controls(const float* logits, int64_t row_stride, 
     launch_pdl(logit_controls_kernel, grid, kThreads, ring * kRowFloats * 4, s, a, ring);
     return check_launch("logit_controls_kernel");
   }
-  launch_pdl(logit_controls_direct_kernel, grid, kThreads, 0, s, a);
+  launch_pdl(logit_controls_direct_kernel, grid, kDirectThreads, 0, s, a);
   return check_launch("logit_controls_direct_kernel");
 }
 
