@@ -406,10 +406,11 @@ typedef struct {
  * alternating every 8 columns, as w_gate_up.  swiglu: out (N/2 columns) =
  * silu(gate) * up of those.  out may be base (float32, no SwiGLU): then tokens
  * without an adapter are not touched; otherwise the two must not overlap.
- * Tokens of no tile are left as they were.  A bad tile, token or adapter
+ * The workspace is 16-byte aligned scratch of this call alone.  Tokens of no
+ * tile are left as they were.  A bad tile, token or adapter
  * sets the device error word and is skipped. */
 MS_API size_t ms_lora_workspace_size(const ms_lora_adapters* adapters, const ms_lora_plan* plan,
-                                     int K, int n_slices);
+                                     int n_slices);
 MS_API int ms_lora_add(const void* x, int64_t x_stride, const float* base, int64_t base_stride,
                        void* out, int64_t out_stride, const void* a, const void* b, int K, int N,
                        int n_slices, const int32_t* slice_cols, int interleaved, int swiglu,

@@ -220,7 +220,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ms_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int64, c_int,
                         c_int, c_int, c_void_p]),
     "ms_gemm_set_policy": (c_int, [c_int]),
-    "ms_lora_workspace_size": (c_size_t, [POINTER(MsLoraAdapters), POINTER(MsLoraPlan), c_int, c_int]),
+    "ms_lora_workspace_size": (c_size_t, [POINTER(MsLoraAdapters), POINTER(MsLoraPlan), c_int]),
     "ms_lora_add": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int,

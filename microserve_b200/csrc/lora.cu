@@ -1,21 +1,23 @@
 // Low-rank adapters of many requests at once beside a shared projection:
-//   s_j[t]   = A_{a(t), j} x[t]                        (first product, rank r)
-//   y[t, n]  = base[t, n] + scale_a * sum_r B_{a(t)}[r, n] s_{j(n)}[t, r]
+//   s_j[t]   = scale_a A_{a(t), j} x[t]                (first product, rank r)
+//   y[t, n]  = base[t, n] + sum_r B_{a(t)}[r, n] s_{j(n)}[t, r]
 // for every token t of the batch, where a(t) is the token's adapter, j(n) the
 // fused slice of column n (q | k | v, gate | up) and base the projection's
 // float32 output.  Optionally y goes through the SwiGLU of the interleaved
 // gate/up columns and out in the model's type.
 //
 // The plan lists tiles of up to 64 tokens that share an adapter (adapter -1:
-// none).  Two launches: lora_shrink computes s (float32, K split over CTAs as
-// needed, the parts summed by the reader in a fixed order, so results do not
-// depend on timing), lora_expand adds B s to the base.
+// none).  Two launches: lora_shrink computes s (k shared out over the CTAs of
+// a cluster when there are few tiles, the parts summed in a fixed order, so
+// results do not depend on timing), lora_expand adds B s to the base.
 //
-// s stays float32 between the launches; the bf16 second product takes it as
-// hi + lo, both bf16 (hi = s rounded, lo = the rest rounded: s to about
-// 2^-17), because a single bf16 s would put 2^-9 of the adapter's part into
-// a float32 output.
+// s is a float32 sum.  The second product takes it in bf16 terms (s rounded,
+// then what is left rounded, ...) whose sum is s: one term would put 2^-9 of
+// the adapter's part into the result.  Two (2^-17 and better) for a bf16
+// result, three (2^-25) for a float32 one.
 #include <cmath>
+
+#include <cooperative_groups.h>
 
 #include "lora.cuh"
 
@@ -24,6 +26,7 @@ namespace {
 
 constexpr int kTile = MS_LORA_TILE;  // most tokens of a tile
 constexpr int kMaxRank = MS_LORA_MAX_RANK;
+constexpr int kMaxTiles = 65535 / (kTile / 16);  // the second product's grid
 
 struct Tile {
   int start, count, adapter, rank, offset;
@@ -90,8 +93,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
                : "memory");
 }
-__device__ __forceinline__ void cp_wait_all() {
-  asm volatile("cp.async.wait_all;" ::: "memory");
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // ---- first product, bf16 ------------------------------------------------------
@@ -100,7 +105,10 @@ __device__ __forceinline__ void cp_wait_all() {
 // global memory: the sum over k may take its terms in any order, so lane
 // (g, t) of a fragment takes the 16 bytes k0 + 8t .. 8t+7 of its row for two
 // MMAs at once, instead of the four separate pairs of the nominal layout.
-// A CTA takes 16 * MT rank rows x 32 tokens; its 8 warps share out k.
+// A CTA takes 16 * MT rank rows x 32 tokens; its 8 warps and the CTAs of its
+// cluster share out k, and the parts meet in (distributed) shared memory.
+// Each slice's rank rows are padded to a multiple of 16 (`rank_p`), with
+// zeros in s.
 constexpr int kShrinkWarps = 8;
 constexpr int kShrinkNT = 4;
 constexpr int kShrinkTokens = 8 * kShrinkNT;
@@ -109,24 +117,42 @@ struct ShrinkArgs {
   const __nv_bfloat16* x;
   int64_t x_stride;
   const __nv_bfloat16* a;
-  int K, ns, width, k_split, k_per;  // k_per: k values per split, a multiple of 32
+  int K, ns, k_per;  // k_per: k values per CTA of a cluster, a multiple of 32
+  int terms;
+  int64_t s_stride;  // row stride of s (elements)
   ms_lora_adapters ad;
   ms_lora_plan plan;
-  float* s;  // (k_split, n_tokens, width)
+  __nv_bfloat16* s;  // row per position: [slice][term][rank_p]
   int* err;
 };
 
+__device__ __forceinline__ int pad16(int r) { return (r + 15) & ~15; }
+
+// v as `terms` bf16 terms at dst[0], dst[step], ...
+__device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int terms, float v) {
+  for (int k = 0; k < terms; ++k) {
+    const __nv_bfloat16 h = __float2bfloat16_rn(v);
+    dst[k * step] = h;
+    v -= __bfloat162float(h);
+  }
+}
+
 template <int MT>
-__global__ void __launch_bounds__(kShrinkWarps * 32) lora_shrink_kernel(ShrinkArgs p) {
+__global__ void __launch_bounds__(kShrinkWarps * 32, MT > 2 ? 1 : 2) lora_shrink_kernel(ShrinkArgs p) {
   pdl_enter();
-  extern __shared__ __align__(16) float s_red[];  // [warps][16 MT][kShrinkTokens]
+  extern __shared__ __align__(16) float s_red[];  // [warps][kShrinkTokens][16 MT]
   constexpr int kHalves = kTile / kShrinkTokens;
+  constexpr int kOuts = kShrinkTokens * 16 * MT;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int splits = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
   Tile tile;
   if (!load_tile(p.plan, p.ad, blockIdx.x / kHalves, tile, p.err)) return;
   const int first = (blockIdx.x % kHalves) * kShrinkTokens;  // of this CTA's tokens in the tile
-  const int rows = p.ns * tile.rank, m0 = blockIdx.y * 16 * MT;
+  const int rank_p = pad16(tile.rank);
+  const int rows = p.ns * rank_p, m0 = blockIdx.y * 16 * MT;
   const int count = min(tile.count - first, kShrinkTokens);
-  if (count <= 0 || m0 >= rows) return;
+  if (count <= 0 || m0 >= rows) return;  // the whole cluster alike
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   const __nv_bfloat16* xr[kShrinkNT];
@@ -140,14 +166,15 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_shrink_kernel(ShrinkAr
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = min(m0 + 16 * m + 8 * h + g, rows - 1);
-      ar[m][h] = p.a + ((int64_t)p.ns * tile.offset + row) * p.K + 8 * t;
+      const int mp = min(m0 + 16 * m, rows - 16) + 8 * h + g;
+      const int j = mp / rank_p, r = min(mp - j * rank_p, tile.rank - 1);
+      ar[m][h] = p.a + ((int64_t)p.ns * tile.offset + j * tile.rank + r) * p.K + 8 * t;
     }
   float acc[MT][kShrinkNT][4] = {};
-  const int k_end = min(p.K, (int)(blockIdx.z + 1) * p.k_per);
+  const int k_end = min(p.K, (split + 1) * p.k_per);
   const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll 2
-  for (int k0 = blockIdx.z * p.k_per + 32 * warp; k0 < k_end; k0 += 32 * kShrinkWarps) {
+  for (int k0 = split * p.k_per + 32 * warp; k0 < k_end; k0 += 32 * kShrinkWarps) {
     const bool in = k0 + 8 * t < k_end;
     uint4 xv[kShrinkNT], av[MT][2];
 #pragma unroll
@@ -176,29 +203,47 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_shrink_kernel(ShrinkAr
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = 16 * m + g + 8 * (e >> 1), col = 8 * n + 2 * t + (e & 1);
-        s_red[(warp * kShrinkTokens + col) * (16 * MT) + row] = acc[m][n][e];
+        s_red[warp * kOuts + col * 16 * MT + row] = acc[m][n][e];
       }
   __syncthreads();
-  float* out = p.s + ((int64_t)blockIdx.z * p.plan.n_tokens + tile.start + first) * p.width;
-  const int here = min(16 * MT, rows - m0);
-  for (int i = threadIdx.x; i < count * 16 * MT; i += kShrinkWarps * 32) {
-    const int col = i / (16 * MT), row = i % (16 * MT);
-    if (row >= here) continue;
+  const int todo = count * 16 * MT;
+  for (int i = threadIdx.x; i < todo; i += kShrinkWarps * 32) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kShrinkWarps; ++w) v += s_red[(w * kShrinkTokens) * (16 * MT) + i];
-    out[(int64_t)col * p.width + m0 + row] = v;
+    for (int w = 0; w < kShrinkWarps; ++w) v += s_red[w * kOuts + i];
+    s_red[i] = v;  // only this thread reads or writes column i of the parts
   }
+  if (splits > 1) cluster.sync();
+  // each CTA of the cluster finishes a share of the outputs, the parts in cluster order
+  const float scale = p.ad.scales[tile.adapter];
+  for (int i = split * kShrinkWarps * 32 + threadIdx.x; i < todo; i += splits * kShrinkWarps * 32) {
+    float v = 0.f;
+    if (splits > 1) {
+      for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(s_red, k)[i];
+    } else {
+      v = s_red[i];
+    }
+    const int col = i / (16 * MT), mp = m0 + i % (16 * MT);
+    if (mp >= rows) continue;
+    const int j = mp / rank_p, r = mp - j * rank_p;
+    __nv_bfloat16* dst = p.s + (tile.start + first + col) * p.s_stride + j * p.terms * rank_p + r;
+    store_terms(dst, rank_p, p.terms, r < tile.rank ? v * scale : 0.f);
+  }
+  if (splits > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
 
 // ---- second product, bf16 -----------------------------------------------------
-// A CTA of 4 warps: up to 64 tokens of a tile x 128 columns (32 per warp).
-// mma m16n8k16 with tokens as M, columns as N, the rank as K: s (hi, lo) and
-// the adapter's B rows in shared memory, the base read into registers while
-// the MMAs run.
+// A CTA keeps the s rows of `tm` tokens of a tile in shared memory and goes
+// through its share of the columns.  Each of its 4 warps works on its own:
+// 32 columns at a time, whose base values and adapter rows come in by
+// cp.async one step ahead into the warp's own buffers, so no barrier stands
+// in the loop.  mma m16n8k16 with tokens as M, columns as N, the rank as K;
+// the sums start from the base and leave through the warp's buffer in whole
+// 32-byte sectors.
 constexpr int kExpWarps = 4;
-constexpr int kExpCols = 32 * kExpWarps;
-constexpr int kBLd = kExpCols + 8;  // padded row (elements): conflict-free ldmatrix
+constexpr int kGroup = 32;             // columns per step of a warp
+constexpr int kBaseLd = kGroup + 8;    // floats per base row: conflict-free 8-byte reads
+constexpr int kBLd = kGroup + 8;       // bf16 per adapter row: conflict-free ldmatrix
 
 struct ExpandArgs {
   const float* base;
@@ -206,13 +251,17 @@ struct ExpandArgs {
   void* out;
   int64_t out_stride;
   const __nv_bfloat16* b;
-  int N, ns, width, k_split;
+  int N, ns, terms;
   int slice_end[3];
   int interleaved, in_place, after_shrink;
-  int tm;  // tokens per pass (16, 32 or 64)
+  int tm, stages;  // tokens per CTA (16, 32 or 64), steps in a warp's ring (1 or 2)
+  int rank_pm;     // padded largest rank: buffer sizes
+  int64_t s_stride;
   ms_lora_adapters ad;
   ms_lora_plan plan;
-  const float* s;
+  const __nv_bfloat16* s;
+  const float* s_any;  // any-shape kernels: float32 s, one row per position
+  int width_any;
   int* err;
 };
 
@@ -230,140 +279,175 @@ __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __ex
 
 template <int EPI>
 __global__ void __launch_bounds__(kExpWarps * 32) lora_expand_kernel(ExpandArgs p) {
+  constexpr int TERMS = EPI == kLoraF32 ? 3 : 2;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int s_tok[kTile];
-  Tile tile;
   // The plan and the adapters are read before the launch wait when
   // lora_shrink runs directly before: it does not write them, and everything
   // before it has completed once its blocks allow this kernel to start.
   if (!p.after_shrink) pdl_enter();
-  const bool ok = load_tile(p.plan, p.ad, blockIdx.y, tile, p.err);
-  const int n0 = blockIdx.x * kExpCols;
+  Tile tile;
+  const int per = kTile / p.tm;
+  const bool ok = load_tile(p.plan, p.ad, blockIdx.y / per, tile, p.err);
+  const int first = (blockIdx.y % per) * p.tm;
+  const int here = min(tile.count - first, p.tm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int rank_p = (tile.rank + 15) & ~15;
-  const int j0 = p.interleaved ? 0 : slice_of(p, n0);
-  const int j1 = p.interleaved ? 1 : slice_of(p, min(n0 + kExpCols, p.N) - 1);
-  const int s_ld = (j1 - j0 + 1) * rank_p + 8;
-  __nv_bfloat16* s_b = reinterpret_cast<__nv_bfloat16*>(smem);  // [rank_p][kBLd]
-  __nv_bfloat16* s_hi = s_b + rank_p * kBLd;                    // [tm][s_ld]
-  __nv_bfloat16* s_lo = s_hi + p.tm * s_ld;
-  const bool work = ok && tile.count > 0 && !(p.in_place && tile.rank == 0);
-  if (work) {
-    for (int i = threadIdx.x; i < rank_p * (kExpCols / 8); i += kExpWarps * 32) {
-      const int r = i / (kExpCols / 8), c = 8 * (i % (kExpCols / 8));
-      const bool in = r < tile.rank && n0 + c < p.N;
-      cp_async16(s_addr(s_b + r * kBLd + c),
-                 p.b + (in ? ((int64_t)tile.offset + r) * p.N + n0 + c : 0), in);
+  const int rank_p = pad16(tile.rank);
+  const int s_row = p.ns * TERMS * rank_p, s_ld = s_row + 8;
+  // s rows, then each warp's ring of (base rows, adapter rows)
+  const int s_bytes = p.tm * (p.ns * TERMS * p.rank_pm + 8) * 2;
+  const int base_bytes = p.tm * kBaseLd * 4, stage_bytes = base_bytes + p.rank_pm * kBLd * 2;
+  __nv_bfloat16* s_s = reinterpret_cast<__nv_bfloat16*>(smem);
+  unsigned char* ring = smem + s_bytes + warp * p.stages * stage_bytes;
+  const bool work = ok && here > 0 && !(p.in_place && tile.rank == 0);
+  const int step = kExpWarps * gridDim.x * kGroup;
+  const int c_first = (blockIdx.x * kExpWarps + warp) * kGroup;
+
+  if (work && threadIdx.x < here)
+    s_tok[threadIdx.x] = token_at(p.plan, tile.start + first + threadIdx.x, p.err);
+  // columns c .. c+31 into ring slot `slot`
+  auto load_b = [&](int c, int slot) {
+    __nv_bfloat16* s_b = reinterpret_cast<__nv_bfloat16*>(ring + slot * stage_bytes + base_bytes);
+    for (int i = lane; i < rank_p * 4; i += 32) {
+      const int r = i >> 2, q = 8 * (i & 3);
+      const bool in = r < tile.rank && c + q < p.N;
+      cp_async16(s_addr(s_b + r * kBLd + q),
+                 p.b + (in ? ((int64_t)tile.offset + r) * p.N + c + q : 0), in);
     }
-    if (threadIdx.x < kTile)
-      s_tok[threadIdx.x] =
-          threadIdx.x < tile.count ? token_at(p.plan, tile.start + threadIdx.x, p.err) : -1;
-  }
+  };
+  auto load_base = [&](int c, int slot) {
+    float* s_base = reinterpret_cast<float*>(ring + slot * stage_bytes);
+    for (int i = lane; i < here * 8; i += 32) {
+      const int row = i >> 3, q = 4 * (i & 7);
+      const int tok = s_tok[row];
+      const bool in = tok >= 0 && c + q < p.N;
+      cp_async16(s_addr(s_base + row * kBaseLd + q),
+                 p.base + (in ? tok * p.base_stride + c + q : 0), in);
+    }
+  };
+  __syncthreads();  // s_tok
+  if (work && c_first < p.N) load_b(c_first, 0);
   if (p.after_shrink) pdl_enter();
   if (!work) return;
-  const float scale = tile.rank > 0 ? p.ad.scales[tile.adapter] : 0.f;
-  const int64_t split_stride = (int64_t)p.plan.n_tokens * p.width;
-  for (int p0 = 0; p0 < tile.count; p0 += p.tm) {
-    const int here = min(p.tm, tile.count - p0);
-    const int rows_p = (here + 15) & ~15;
-    __syncthreads();  // the previous pass has read s
-    const int cols = (j1 - j0 + 1) * rank_p;
-    for (int i = threadIdx.x; i < rows_p * cols; i += kExpWarps * 32) {
-      const int row = i / cols, c = i - row * cols;
-      const int j = c / rank_p, r = c - j * rank_p;
-      float v = 0.f;
-      if (row < here && r < tile.rank) {
-        const float* src = p.s + ((int64_t)tile.start + p0 + row) * p.width +
-                           (j0 + j) * tile.rank + r;
-        for (int k = 0; k < p.k_split; ++k) v += src[k * split_stride];
-        v *= scale;
+  for (int i = threadIdx.x; i < here * (s_row / 8); i += kExpWarps * 32) {
+    const int row = i / (s_row / 8), q = 8 * (i - row * (s_row / 8));
+    cp_async16(s_addr(s_s + row * s_ld + q), p.s + (tile.start + first + row) * p.s_stride + q, true);
+  }
+  if (c_first < p.N) load_base(c_first, 0);
+  cp_commit();
+  cp_wait<0>();
+  __syncthreads();  // s
+
+  int slot = 0;
+  for (int c = c_first; c < p.N; c += step) {
+    const int next = p.stages > 1 ? slot ^ 1 : 0;
+    if (p.stages > 1) {
+      if (c + step < p.N) {
+        load_b(c + step, next);
+        load_base(c + step, next);
       }
-      const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-      s_hi[row * s_ld + c] = hi;
-      s_lo[row * s_ld + c] = __float2bfloat16_rn(v - __bfloat162float(hi));
+      cp_commit();
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
     }
-    cp_wait_all();
-    __syncthreads();
-    const int wc = n0 + 32 * warp;  // this warp's first column
-    if (wc >= p.N) continue;
-    for (int m = 0; m < rows_p; m += 16) {
-      int64_t row_at[2];
-      bool has[2];
+    __syncwarp();
+    float* s_base = reinterpret_cast<float*>(ring + slot * stage_bytes);
+    const __nv_bfloat16* s_b =
+        reinterpret_cast<const __nv_bfloat16*>(ring + slot * stage_bytes + base_bytes);
+    int lo[4], hi[4];  // first and last slice of each 8 columns
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int tok = m + g + 8 * h < here ? s_tok[p0 + m + g + 8 * h] : -1;
-        has[h] = tok >= 0;
-        row_at[h] = max(tok, 0);
-      }
+    for (int n = 0; n < 4; ++n) {
+      lo[n] = slice_of(p, min(c + 8 * n, p.N - 1));
+      hi[n] = slice_of(p, min(c + 8 * n + 7, p.N - 1));
+    }
+    const int j_lo = lo[0], j_hi = p.interleaved ? 1 : hi[3];
+    for (int m = 0; m < here; m += 16) {
       float acc[4][4];
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int c = wc + 8 * n + 2 * t;
-          float2 v = make_float2(0.f, 0.f);
-          if (has[h] && c < p.N)
-            v = *reinterpret_cast<const float2*>(p.base + row_at[h] * p.base_stride + c);
+          const float2 v = *reinterpret_cast<const float2*>(s_base + (m + g + 8 * h) * kBaseLd + 8 * n + 2 * t);
           acc[n][2 * h] = v.x;
           acc[n][2 * h + 1] = v.y;
         }
-      int slice[4];
+      for (int k = 0; k < rank_p; k += 16) {
+        uint32_t b01[4], b23[4];
+        const __nv_bfloat16* bp = s_b + (k + (lane & 15)) * kBLd + 8 * (lane >> 4);
+        ldsm4_t(b01, s_addr(bp));
+        ldsm4_t(b23, s_addr(bp + 16));
+        for (int j = j_lo; j <= j_hi; ++j) {
+          uint32_t a[TERMS][4];
+          const __nv_bfloat16* sp = s_s + (m + (lane & 15)) * s_ld + j * TERMS * rank_p + k + 8 * (lane >> 4);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) slice[n] = slice_of(p, min(wc + 8 * n, p.N - 1));
-      for (int j = slice[0]; j <= max(slice[1], slice[3]); ++j) {
-        for (int k = 0; k < rank_p; k += 16) {
-          uint32_t hi[4], lo[4], b01[4], b23[4];
-          const int srow = (m + (lane & 15)) * s_ld + (j - j0) * rank_p + k + 8 * (lane >> 4);
-          ldsm4(hi, s_addr(s_hi + srow));
-          ldsm4(lo, s_addr(s_lo + srow));
-          const int brow = (k + (lane & 15)) * kBLd + 32 * warp + 8 * (lane >> 4);
-          ldsm4_t(b01, s_addr(s_b + brow));
-          ldsm4_t(b23, s_addr(s_b + brow + 16));
+          for (int e = 0; e < TERMS; ++e) ldsm4(a[e], s_addr(sp + e * rank_p));
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            if (slice[n] != j) continue;
-            const uint32_t w0 = n < 2 ? b01[2 * n] : b23[2 * n - 4];
-            const uint32_t w1 = n < 2 ? b01[2 * n + 1] : b23[2 * n - 3];
-            mma_bf16(acc[n], lo[0], lo[1], lo[2], lo[3], w0, w1);
-            mma_bf16(acc[n], hi[0], hi[1], hi[2], hi[3], w0, w1);
+            if (j < lo[n] || j > hi[n]) continue;
+            uint32_t w0 = n < 2 ? b01[2 * n] : b23[2 * n - 4];
+            uint32_t w1 = n < 2 ? b01[2 * n + 1] : b23[2 * n - 3];
+            if (lo[n] != hi[n] && slice_of(p, c + 8 * n + g) != j) w0 = w1 = 0u;  // another slice's column
+#pragma unroll
+            for (int e = TERMS - 1; e >= 0; --e)  // the small terms first
+              mma_bf16(acc[n], a[e][0], a[e][1], a[e][2], a[e][3], w0, w1);
           }
         }
       }
+      // out through the rows of s_base, which every lane has read
+      __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!has[h]) continue;
+        float* row = s_base + (m + g + 8 * h) * kBaseLd;
         if constexpr (EPI == kLoraSwiGLU) {
-          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + row_at[h] * p.out_stride;
 #pragma unroll
-          for (int n = 0; n < 4; n += 2) {
-            const int c = (wc + 8 * n) / 2 + 2 * t;  // 8 outputs per 16 columns
-            if (wc + 8 * n < p.N)
-              *reinterpret_cast<__nv_bfloat162*>(o + c) =
-                  __floats2bfloat162_rn(silu(acc[n][2 * h]) * acc[n + 1][2 * h],
-                                        silu(acc[n][2 * h + 1]) * acc[n + 1][2 * h + 1]);
-          }
+          for (int n = 0; n < 4; n += 2)
+            reinterpret_cast<__nv_bfloat162*>(row)[2 * n + t] =
+                __floats2bfloat162_rn(silu(acc[n][2 * h]) * acc[n + 1][2 * h],
+                                      silu(acc[n][2 * h + 1]) * acc[n + 1][2 * h + 1]);
         } else {
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const int c = wc + 8 * n + 2 * t;
-            if (c >= p.N) continue;
             const float2 v = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
             if constexpr (EPI == kLoraF32)
-              *reinterpret_cast<float2*>(static_cast<float*>(p.out) + row_at[h] * p.out_stride + c) = v;
+              reinterpret_cast<float2*>(row)[4 * n + t] = v;
             else
-              *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) +
-                                                 row_at[h] * p.out_stride + c) =
-                  __floats2bfloat162_rn(v.x, v.y);
+              reinterpret_cast<__nv_bfloat162*>(row)[4 * n + t] = __floats2bfloat162_rn(v.x, v.y);
           }
         }
       }
+      __syncwarp();
+      constexpr int kChunks = EPI == kLoraF32 ? 8 : EPI == kLoraBf16 ? 4 : 2;  // of 16 bytes per row
+      constexpr int kPer = EPI == kLoraF32 ? 4 : 8;                            // outputs per chunk
+      const int c_out = EPI == kLoraSwiGLU ? c / 2 : c, n_out = EPI == kLoraSwiGLU ? p.N / 2 : p.N;
+#pragma unroll
+      for (int i = lane; i < 16 * kChunks; i += 32) {
+        const int row = i / kChunks, q = i % kChunks;
+        if (m + row >= here || c_out + q * kPer >= n_out) continue;
+        const int tok = s_tok[m + row];
+        if (tok < 0) continue;
+        const int64_t at = tok * p.out_stride + c_out + q * kPer;
+        const float4 v = reinterpret_cast<const float4*>(s_base + (m + row) * kBaseLd)[q];
+        if constexpr (EPI == kLoraF32)
+          *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+        else
+          *reinterpret_cast<float4*>(static_cast<__nv_bfloat16*>(p.out) + at) = v;
+      }
     }
+    __syncwarp();  // the slot's rows are out before it is filled again
+    if (p.stages == 1 && c + step < p.N) {
+      load_b(c + step, 0);
+      load_base(c + step, 0);
+      cp_commit();
+    }
+    slot = next;
   }
 }
 
 // ---- any type, size and alignment ----------------------------------------------
-// The float32 models and shapes the tensor-core kernels do not take: one warp
-// per (token, rank row) dot product, one thread per output.
+// The float32 models and shapes the tensor-core kernels do not take: a CTA per
+// token; one warp per dot product of the first product, one thread per output
+// of the second.
 template <typename T>
 __global__ void lora_shrink_any_kernel(const T* __restrict__ x, int64_t x_stride,
                                        const T* __restrict__ a, int K, int ns, int width,
@@ -372,106 +456,130 @@ __global__ void lora_shrink_any_kernel(const T* __restrict__ x, int64_t x_stride
   pdl_enter();
   Tile tile;
   if (!load_tile(plan, ad, blockIdx.x, tile, err)) return;
+  const int q = blockIdx.y;
+  if (q >= tile.count) return;
+  const int tok = token_at(plan, tile.start + q, err);
   const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  const int rows = ns * tile.rank, work = tile.count * rows;
-  for (int i = blockIdx.y * nw + (threadIdx.x >> 5); i < work; i += gridDim.y * nw) {
-    const int q = i / rows, m = i - q * rows;
-    const int tok = token_at(plan, tile.start + q, err);
-    const T* xr = x + (int64_t)max(tok, 0) * x_stride;
+  const T* xr = x + (int64_t)max(tok, 0) * x_stride;
+  for (int m = threadIdx.x >> 5; m < ns * tile.rank; m += nw) {
     const T* ar = a + ((int64_t)ns * tile.offset + m) * K;
     float v = 0.f;
     for (int k = lane; k < K; k += 32) v = fmaf(to_f(xr[k]), to_f(ar[k]), v);
     v = warp_sum(v);
-    if (lane == 0) s[((int64_t)tile.start + q) * width + m] = v;
+    if (lane == 0) s[((int64_t)tile.start + q) * width + m] = v * ad.scales[tile.adapter];
   }
 }
 
 template <typename T, typename TO>
-__global__ void lora_expand_any_kernel(const float* base, int64_t base_stride, TO* out,
-                                       int64_t out_stride, const T* __restrict__ b, int swiglu,
-                                       ExpandArgs p) {
+__global__ void lora_expand_any_kernel(const T* __restrict__ b, TO* out, int swiglu, ExpandArgs p) {
   pdl_enter();
+  extern __shared__ __align__(16) float s_row[];  // the token's s
   Tile tile;
   if (!load_tile(p.plan, p.ad, blockIdx.x, tile, p.err)) return;
-  if (p.in_place && tile.rank == 0) return;
-  const float scale = tile.rank > 0 ? p.ad.scales[tile.adapter] : 0.f;
-  const int outs = swiglu ? p.N / 2 : p.N;
-  for (int64_t i = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; i < (int64_t)tile.count * outs;
-       i += (int64_t)gridDim.y * blockDim.x) {
-    const int q = (int)(i / outs), o = (int)(i - (int64_t)q * outs);
-    const int tok = token_at(p.plan, tile.start + q, p.err);
-    if (tok < 0) continue;
-    const float* sr = p.s + ((int64_t)tile.start + q) * p.width;
-    auto column = [&](int n) {
-      const float* sj = sr + slice_of(p, n) * tile.rank;
-      float v = 0.f;
-      for (int r = 0; r < tile.rank; ++r)
-        v = fmaf(sj[r], to_f(b[((int64_t)tile.offset + r) * p.N + n]), v);
-      return fmaf(scale, v, base[(int64_t)tok * base_stride + n]);
-    };
-    float y;
-    if (swiglu) {
-      const int n = (o >> 3) * 16 + (o & 7);
-      const float gate = column(n);
-      y = gate / (1.f + expf(-gate)) * column(n + 8);
-    } else {
-      y = column(o);
-    }
-    out[(int64_t)tok * out_stride + o] = from_f<TO>(y);
+  const int q = blockIdx.y;
+  if (q >= tile.count || (p.in_place && tile.rank == 0)) return;
+  const int tok = token_at(p.plan, tile.start + q, p.err);
+  for (int i = threadIdx.x; i < p.ns * tile.rank; i += blockDim.x)
+    s_row[i] = p.s_any[((int64_t)tile.start + q) * p.width_any + i];
+  __syncthreads();
+  const int o = blockIdx.z * blockDim.x + threadIdx.x;
+  if (tok < 0 || o >= (swiglu ? p.N / 2 : p.N)) return;
+  auto column = [&](int n) {
+    const float* sj = s_row + slice_of(p, n) * tile.rank;
+    const T* bn = b + (int64_t)tile.offset * p.N + n;
+    float v = 0.f;
+    for (int r = 0; r < tile.rank; ++r) v = fmaf(sj[r], to_f(bn[(int64_t)r * p.N]), v);
+    return p.base[tok * p.base_stride + n] + v;
+  };
+  float y;
+  if (swiglu) {
+    const int n = (o >> 3) * 16 + (o & 7);
+    const float gate = column(n);
+    y = gate / (1.f + expf(-gate)) * column(n + 8);
+  } else {
+    y = column(o);
   }
-}
-
-// Number of parts k is cut into: enough CTAs for the GPU, at least 256 k values per CTA.
-int shrink_split(int n_tiles, int K, int n_slices, int max_rank) {
-  const int rows = n_slices * max_rank;
-  const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int64_t ctas = (int64_t)n_tiles * ceil_div(rows, 16 * mt);
-  int split = 1;
-  while (split < 16 && ctas * split < 2 * 148 && K / (2 * split) >= 256) split *= 2;
-  return split;
+  out[tok * p.out_stride + o] = from_f<TO>(y);
 }
 
 constexpr int kMostSmem = 226 * 1024;
 
+// CTAs of a cluster that share out k: enough CTAs for the GPU, at least 256 k
+// values for each.
+int shrink_split(int n_tiles, int K, int rows, int mt) {
+  const int64_t ctas = (int64_t)n_tiles * ceil_div(rows, 16 * mt);
+  int split = 1;
+  while (split < 8 && ctas * split < 2 * 148 && K / (2 * split) >= 256) split *= 2;
+  return split;
+}
+
 template <int EPI>
-int launch_expand(const ExpandArgs& p, int smem, cudaStream_t s) {
+int launch_expand(ExpandArgs p, cudaStream_t s) {
   static std::atomic<uint64_t> granted{0};
-  if (smem > 48 * 1024) MS_TRY(grant_dynamic_smem(lora_expand_kernel<EPI>, kMostSmem, granted));
-  const dim3 grid(ceil_div(p.N, kExpCols), p.plan.n_tiles);
-  launch_pdl(lora_expand_kernel<EPI>, grid, kExpWarps * 32, smem, s, p);
+  MS_TRY(grant_dynamic_smem(lora_expand_kernel<EPI>, kMostSmem, granted));
+  // Tokens per CTA by the tiles' mean size; fewer, and a ring of one, where
+  // large ranks need the shared memory.
+  const int terms = EPI == kLoraF32 ? 3 : 2;
+  const int mean = p.plan.n_tokens / p.plan.n_tiles;
+  p.tm = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+  p.stages = 2;
+  auto smem = [&]() {
+    return p.tm * (p.ns * terms * p.rank_pm + 8) * 2 +
+           kExpWarps * p.stages * (p.tm * kBaseLd * 4 + p.rank_pm * kBLd * 2);
+  };
+  while (p.tm > 16 && smem() > 110 * 1024) p.tm /= 2;
+  if (smem() > kMostSmem) p.stages = 1;
+  const int tiles = p.plan.n_tiles * (kTile / p.tm), groups = ceil_div(p.N, kGroup * kExpWarps);
+  // about 8 CTAs per SM in all, so that a warp's steps follow one another
+  const int gx = max(1, min(groups, ceil_div(8 * 148, tiles)));
+  launch_pdl(lora_expand_kernel<EPI>, dim3(gx, tiles), kExpWarps * 32, smem(), s, p);
   return check_launch("lora_expand_kernel");
 }
 
 template <int MT>
-int launch_shrink(const ShrinkArgs& p, int row_blocks, cudaStream_t s) {
+int launch_shrink(ShrinkArgs p, int rows, cudaStream_t s) {
   const int smem = kShrinkWarps * 16 * MT * kShrinkTokens * 4;
   static std::atomic<uint64_t> granted{0};
   if (smem > 48 * 1024) MS_TRY(grant_dynamic_smem(lora_shrink_kernel<MT>, smem, granted));
-  const dim3 grid(p.plan.n_tiles * (kTile / kShrinkTokens), row_blocks, p.k_split);
-  launch_pdl(lora_shrink_kernel<MT>, grid, kShrinkWarps * 32, smem, s, p);
+  const int split = shrink_split(p.plan.n_tiles, p.K, rows, MT);
+  p.k_per = ceil_div(ceil_div(p.K, split), 32) * 32;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.plan.n_tiles * (kTile / kShrinkTokens), ceil_div(rows, 16 * MT), split);
+  cfg.blockDim = kShrinkWarps * 32;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {1, 1, (unsigned)split};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  (void)cudaLaunchKernelEx(&cfg, lora_shrink_kernel<MT>, p);
   return check_launch("lora_shrink_kernel");
 }
 
 template <typename T, typename TO>
 int launch_any(const LoraCall& c, const ExpandArgs& e, cudaStream_t s) {
-  const int per = c.n_slices * e.ad.max_rank;
-  const dim3 g1(e.plan.n_tiles, min(64, max(1, ceil_div(kTile * per, 64))));
-  launch_pdl(lora_shrink_any_kernel<T>, g1, 256, 0, s, static_cast<const T*>(c.x), c.x_stride,
-             static_cast<const T*>(c.a), c.K, c.n_slices, e.width, e.ad, e.plan,
-             const_cast<float*>(e.s), e.err);
-  MS_TRY(check_launch("lora_shrink_any_kernel"));
+  if (e.ad.max_rank > 0) {
+    launch_pdl(lora_shrink_any_kernel<T>, dim3(e.plan.n_tiles, kTile), 256, 0, s,
+               static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.a), c.K, c.n_slices,
+               e.width_any, e.ad, e.plan, const_cast<float*>(e.s_any), e.err);
+    MS_TRY(check_launch("lora_shrink_any_kernel"));
+  }
   const int outs = c.swiglu ? c.N / 2 : c.N;
-  const dim3 g2(e.plan.n_tiles, (int)min((int64_t)256, ((int64_t)kTile * outs + 1023) / 1024));
-  launch_pdl(lora_expand_any_kernel<T, TO>, g2, 256, 0, s, c.base, c.base_stride,
-             static_cast<TO*>(c.out), c.out_stride, static_cast<const T*>(c.b), c.swiglu ? 1 : 0, e);
+  launch_pdl(lora_expand_any_kernel<T, TO>, dim3(e.plan.n_tiles, kTile, ceil_div(outs, 128)), 128,
+             c.n_slices * e.ad.max_rank * 4, s, static_cast<const T*>(c.b), static_cast<TO*>(c.out),
+             c.swiglu ? 1 : 0, e);
   return check_launch("lora_expand_any_kernel");
 }
 
 }  // namespace
 
-size_t lora_workspace_size(int n_tokens, int n_tiles, int K, int n_slices, int max_rank) {
-  if (n_tokens <= 0 || n_tiles <= 0 || K <= 0 || n_slices <= 0 || max_rank <= 0) return 0;
-  return (size_t)shrink_split(n_tiles, K, n_slices, max_rank) * n_tokens * n_slices * max_rank * 4;
+// s: three bf16 terms of the padded rank per token and slice, or float32.
+size_t lora_workspace_size(int n_tokens, int n_slices, int max_rank) {
+  if (n_tokens <= 0 || n_slices <= 0 || max_rank <= 0) return 0;
+  return (size_t)n_tokens * n_slices * ((max_rank + 15) & ~15) * 6;
 }
 
 int validate_lora(const ms_lora_adapters* ad, const ms_lora_plan* plan) {
@@ -481,7 +589,7 @@ int validate_lora(const ms_lora_adapters* ad, const ms_lora_plan* plan) {
   MS_REQUIRE(ad->n_adapters == 0 || (ad->offsets && ad->ranks && ad->scales),
              "lora: null adapter arrays");
   MS_REQUIRE(plan->n_tokens >= 0 && plan->n_tiles >= 0, "lora: bad plan sizes");
-  MS_REQUIRE(plan->n_tiles <= 65535, "lora: more than 65535 tiles");
+  MS_REQUIRE(plan->n_tiles <= kMaxTiles, "lora: more than %d tiles", kMaxTiles);
   MS_REQUIRE(plan->n_tiles == 0 || (plan->order && plan->tiles), "lora: null plan arrays");
   MS_REQUIRE((reinterpret_cast<uintptr_t>(plan->tiles) & 15) == 0, "lora: tiles not 16-byte aligned");
   return MS_OK;
@@ -490,10 +598,12 @@ int validate_lora(const ms_lora_adapters* ad, const ms_lora_plan* plan) {
 int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& plan,
              void* workspace, size_t workspace_bytes, cudaStream_t s) {
   if (plan.n_tiles == 0 || plan.n_tokens == 0) return MS_OK;
-  const bool in_place = static_cast<const void*>(c.base) == c.out;
-  const size_t need = lora_workspace_size(plan.n_tokens, plan.n_tiles, c.K, c.n_slices, ad.max_rank);
+  const size_t need = lora_workspace_size(plan.n_tokens, c.n_slices, ad.max_rank);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr))
     return fail(MS_ERR_INVALID, "lora: workspace too small (%zu < %zu)", workspace_bytes, need);
+  auto aligned = [](const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  MS_REQUIRE(aligned(workspace, 16), "lora: workspace not 16-byte aligned");
+  const bool out_f32 = c.out_dtype == MS_DTYPE_F32;
   ExpandArgs e{};
   e.base = c.base;
   e.base_stride = c.base_stride;
@@ -502,27 +612,28 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
   e.b = static_cast<const __nv_bfloat16*>(c.b);
   e.N = c.N;
   e.ns = c.n_slices;
-  e.width = c.n_slices * ad.max_rank;
-  e.k_split = 1;
+  e.terms = out_f32 ? 3 : 2;
   for (int k = 0; k < 3; ++k) e.slice_end[k] = c.slice_end[k];
   e.interleaved = c.interleaved;
-  e.in_place = in_place;
+  e.in_place = static_cast<const void*>(c.base) == c.out;
+  e.rank_pm = (ad.max_rank + 15) & ~15;
+  e.s_stride = (int64_t)c.n_slices * e.terms * e.rank_pm;
   e.ad = ad;
   e.plan = plan;
-  e.s = static_cast<float*>(workspace);
+  e.s = static_cast<const __nv_bfloat16*>(workspace);
+  e.s_any = static_cast<const float*>(workspace);
+  e.width_any = c.n_slices * ad.max_rank;
   e.err = device_error_word();
-  auto aligned = [](const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
-  bool slices8 = true;
-  for (int k = 0; k + 1 < c.n_slices && !c.interleaved; ++k) slices8 &= c.slice_end[k] % 8 == 0;
-  const bool tensor =
-      c.dtype == MS_DTYPE_BF16 && c.K % 8 == 0 && c.x_stride % 8 == 0 && c.N % 8 == 0 && slices8 &&
-      aligned(c.x, 16) && aligned(c.a, 16) && aligned(c.b, 16) && aligned(c.base, 8) &&
-      c.base_stride % 2 == 0 && aligned(c.out, 8) && c.out_stride % 2 == 0 &&
-      !(c.swiglu && c.out_dtype != MS_DTYPE_BF16);
+  // 16-byte loads and stores of x, A, B, the base and the result
+  const bool tensor = c.dtype == MS_DTYPE_BF16 && c.K % 8 == 0 && c.x_stride % 8 == 0 &&
+                      c.N % (c.swiglu ? 16 : 8) == 0 && aligned(c.x, 16) && aligned(c.a, 16) &&
+                      aligned(c.b, 16) && aligned(c.base, 16) && c.base_stride % 4 == 0 &&
+                      aligned(c.out, 16) && c.out_stride % (out_f32 ? 4 : 8) == 0 &&
+                      !(c.swiglu && out_f32);
   if (!tensor) {
-    if (c.dtype == MS_DTYPE_F32 && c.out_dtype == MS_DTYPE_F32) return launch_any<float, float>(c, e, s);
+    if (c.dtype == MS_DTYPE_F32 && out_f32) return launch_any<float, float>(c, e, s);
     if (c.dtype == MS_DTYPE_F32) return launch_any<float, __nv_bfloat16>(c, e, s);
-    if (c.out_dtype == MS_DTYPE_F32) return launch_any<__nv_bfloat16, float>(c, e, s);
+    if (out_f32) return launch_any<__nv_bfloat16, float>(c, e, s);
     return launch_any<__nv_bfloat16, __nv_bfloat16>(c, e, s);
   }
   if (ad.max_rank > 0) {
@@ -532,31 +643,21 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
     p.a = static_cast<const __nv_bfloat16*>(c.a);
     p.K = c.K;
     p.ns = c.n_slices;
-    p.width = e.width;
-    p.k_split = shrink_split(plan.n_tiles, c.K, c.n_slices, ad.max_rank);
-    p.k_per = ceil_div(ceil_div(c.K, p.k_split), 32) * 32;
+    p.terms = e.terms;
+    p.s_stride = e.s_stride;
     p.ad = ad;
     p.plan = plan;
-    p.s = static_cast<float*>(workspace);
+    p.s = static_cast<__nv_bfloat16*>(workspace);
     p.err = e.err;
-    e.k_split = p.k_split;
     e.after_shrink = 1;
-    const int rows = e.width;
+    const int rows = c.n_slices * e.rank_pm;
     if (rows <= 16)
-      MS_TRY(launch_shrink<1>(p, 1, s));
-    else if (rows <= 32)
-      MS_TRY(launch_shrink<2>(p, 1, s));
+      MS_TRY(launch_shrink<1>(p, rows, s));
     else
-      MS_TRY(launch_shrink<4>(p, ceil_div(rows, 64), s));
+      MS_TRY(launch_shrink<2>(p, rows, s));
   }
-  const int rank_p = (ad.max_rank + 15) & ~15;
-  const int s_ld = c.n_slices * rank_p + 8;
-  e.tm = 64;
-  auto smem = [&]() { return rank_p * kBLd * 2 + e.tm * s_ld * 4; };
-  while (e.tm > 16 && smem() > 100 * 1024) e.tm /= 2;
-  if (c.swiglu) return launch_expand<kLoraSwiGLU>(e, smem(), s);
-  if (c.out_dtype == MS_DTYPE_F32) return launch_expand<kLoraF32>(e, smem(), s);
-  return launch_expand<kLoraBf16>(e, smem(), s);
+  if (c.swiglu) return launch_expand<kLoraSwiGLU>(e, s);
+  return out_f32 ? launch_expand<kLoraF32>(e, s) : launch_expand<kLoraBf16>(e, s);
 }
 
 }  // namespace ms
@@ -564,9 +665,9 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
 using namespace ms;
 
 extern "C" size_t ms_lora_workspace_size(const ms_lora_adapters* adapters,
-                                         const ms_lora_plan* plan, int K, int n_slices) {
+                                         const ms_lora_plan* plan, int n_slices) {
   if (adapters == nullptr || plan == nullptr) return 0;
-  return lora_workspace_size(plan->n_tokens, plan->n_tiles, K, n_slices, adapters->max_rank);
+  return lora_workspace_size(plan->n_tokens, n_slices, adapters->max_rank);
 }
 
 extern "C" int ms_lora_add(const void* x, int64_t x_stride, const float* base, int64_t base_stride,

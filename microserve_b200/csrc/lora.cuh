@@ -21,7 +21,7 @@ struct LoraCall {
   int dtype, out_dtype;
 };
 
-size_t lora_workspace_size(int n_tokens, int n_tiles, int K, int n_slices, int max_rank);
+size_t lora_workspace_size(int n_tokens, int n_slices, int max_rank);
 int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& plan,
              void* workspace, size_t workspace_bytes, cudaStream_t s);
 int validate_lora(const ms_lora_adapters* ad, const ms_lora_plan* plan);

@@ -138,7 +138,7 @@ def lora_add(
         return out
     with _lib.on_device(dev):
         lib = _lib.load()
-        need = lib.ms_lora_workspace_size(ctypes.byref(ad), ctypes.byref(pl), K, ns)
+        need = lib.ms_lora_workspace_size(ctypes.byref(ad), ctypes.byref(pl), ns)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         cols = (ctypes.c_int32 * ns)(*proj.slices)
         _lib.call("ms_lora_add", x.data_ptr(), max(x.stride(0), K), base.data_ptr(),
