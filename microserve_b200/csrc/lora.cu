@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kTile = MS_LORA_TILE;  // most tokens of a tile
 constexpr int kMaxRank = MS_LORA_MAX_RANK;
-constexpr int kMaxTiles = 65535 / (kTile / 16);  // the second product's grid
+constexpr int kMaxTiles = 65535;  // the second product's grid
 
 struct Tile {
   int start, count, adapter, rank, offset;
@@ -105,13 +105,11 @@ __device__ __forceinline__ void cp_wait() {
 // global memory: the sum over k may take its terms in any order, so lane
 // (g, t) of a fragment takes the 16 bytes k0 + 8t .. 8t+7 of its row for two
 // MMAs at once, instead of the four separate pairs of the nominal layout.
-// A CTA takes 16 * MT rank rows x 32 tokens; its 8 warps and the CTAs of its
+// A CTA takes 16 * MT rank rows, 8 * NT tokens at a time; its 8 warps and the CTAs of its
 // cluster share out k, and the parts meet in (distributed) shared memory.
 // Each slice's rank rows are padded to a multiple of 16 (`rank_p`), with
 // zeros in s.
 constexpr int kShrinkWarps = 8;
-constexpr int kShrinkNT = 4;
-constexpr int kShrinkTokens = 8 * kShrinkNT;
 
 struct ShrinkArgs {
   const __nv_bfloat16* x;
@@ -137,30 +135,22 @@ __device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int te
   }
 }
 
-template <int MT>
-__global__ void __launch_bounds__(kShrinkWarps * 32, MT > 2 ? 1 : 2) lora_shrink_kernel(ShrinkArgs p) {
+template <int MT, int NT>
+__global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(ShrinkArgs p) {
   pdl_enter();
+  constexpr int kShrinkTokens = 8 * NT;
   extern __shared__ __align__(16) float s_red[];  // [warps][kShrinkTokens][16 MT]
-  constexpr int kHalves = kTile / kShrinkTokens;
   constexpr int kOuts = kShrinkTokens * 16 * MT;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int splits = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
   Tile tile;
-  if (!load_tile(p.plan, p.ad, blockIdx.x / kHalves, tile, p.err)) return;
-  const int first = (blockIdx.x % kHalves) * kShrinkTokens;  // of this CTA's tokens in the tile
+  if (!load_tile(p.plan, p.ad, blockIdx.x, tile, p.err)) return;
   const int rank_p = pad16(tile.rank);
   const int rows = p.ns * rank_p, m0 = blockIdx.y * 16 * MT;
-  const int count = min(tile.count - first, kShrinkTokens);
-  if (count <= 0 || m0 >= rows) return;  // the whole cluster alike
+  if (m0 >= rows) return;  // the whole cluster alike
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-  const __nv_bfloat16* xr[kShrinkNT];
-#pragma unroll
-  for (int n = 0; n < kShrinkNT; ++n) {
-    const int tok = token_at(p.plan, tile.start + first + min(8 * n + g, count - 1), p.err);
-    xr[n] = p.x + (int64_t)max(tok, 0) * p.x_stride + 8 * t;
-  }
   const __nv_bfloat16* ar[MT][2];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -170,80 +160,86 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, MT > 2 ? 1 : 2) lora_shrink
       const int j = mp / rank_p, r = min(mp - j * rank_p, tile.rank - 1);
       ar[m][h] = p.a + ((int64_t)p.ns * tile.offset + j * tile.rank + r) * p.K + 8 * t;
     }
-  float acc[MT][kShrinkNT][4] = {};
   const int k_end = min(p.K, (split + 1) * p.k_per);
   const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
-  for (int k0 = split * p.k_per + 32 * warp; k0 < k_end; k0 += 32 * kShrinkWarps) {
-    const bool in = k0 + 8 * t < k_end;
-    uint4 xv[kShrinkNT], av[MT][2];
+  for (int first = 0; first < tile.count; first += kShrinkTokens) {
+    const int count = min(tile.count - first, kShrinkTokens);
+    const __nv_bfloat16* xr[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int tok = token_at(p.plan, tile.start + first + min(8 * n + g, count - 1), p.err);
+      xr[n] = p.x + (int64_t)max(tok, 0) * p.x_stride + 8 * t;
+    }
+    float acc[MT][NT][4] = {};
+#pragma unroll (MT + NT <= 3 ? 4 : 2)
+    for (int k0 = split * p.k_per + 32 * warp; k0 < k_end; k0 += 32 * kShrinkWarps) {
+      const bool in = k0 + 8 * t < k_end;
+      uint4 xv[NT], av[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          av[m][h] = in ? __ldg(reinterpret_cast<const uint4*>(ar[m][h] + k0)) : zero;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        xv[n] = in && 8 * n < count ? __ldg(reinterpret_cast<const uint4*>(xr[n] + k0)) : zero;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (8 * n >= count) break;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma_bf16(acc[m][n], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv[n].x, xv[n].y);
+          mma_bf16(acc[m][n], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv[n].z, xv[n].w);
+        }
+      }
+    }
+    // the warps' parts, summed in warp order
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        av[m][h] = in ? __ldg(reinterpret_cast<const uint4*>(ar[m][h] + k0)) : zero;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int n = 0; n < kShrinkNT; ++n)
-      xv[n] = in && 8 * n < count ? __ldg(reinterpret_cast<const uint4*>(xr[n] + k0)) : zero;
+        for (int e = 0; e < 4; ++e) {
+          const int row = 16 * m + g + 8 * (e >> 1), col = 8 * n + 2 * t + (e & 1);
+          s_red[warp * kOuts + col * 16 * MT + row] = acc[m][n][e];
+        }
+    __syncthreads();
+    const int todo = count * 16 * MT;
+    for (int i = threadIdx.x; i < todo; i += kShrinkWarps * 32) {
+      float v = 0.f;
 #pragma unroll
-    for (int n = 0; n < kShrinkNT; ++n) {
-      if (8 * n >= count) break;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        mma_bf16(acc[m][n], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv[n].x, xv[n].y);
-        mma_bf16(acc[m][n], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv[n].z, xv[n].w);
-      }
+      for (int w = 0; w < kShrinkWarps; ++w) v += s_red[w * kOuts + i];
+      s_red[i] = v;  // only this thread reads or writes column i of the parts
     }
-  }
-  // the warps' parts, summed in warp order
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < kShrinkNT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = 16 * m + g + 8 * (e >> 1), col = 8 * n + 2 * t + (e & 1);
-        s_red[warp * kOuts + col * 16 * MT + row] = acc[m][n][e];
+    if (splits > 1) cluster.sync();
+    // each CTA of the cluster finishes a share of the outputs, the parts in cluster order
+    const float scale = p.ad.scales[tile.adapter];
+    for (int i = split * kShrinkWarps * 32 + threadIdx.x; i < todo; i += splits * kShrinkWarps * 32) {
+      float v = 0.f;
+      if (splits > 1) {
+        for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(s_red, k)[i];
+      } else {
+        v = s_red[i];
       }
-  __syncthreads();
-  const int todo = count * 16 * MT;
-  for (int i = threadIdx.x; i < todo; i += kShrinkWarps * 32) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kShrinkWarps; ++w) v += s_red[w * kOuts + i];
-    s_red[i] = v;  // only this thread reads or writes column i of the parts
-  }
-  if (splits > 1) cluster.sync();
-  // each CTA of the cluster finishes a share of the outputs, the parts in cluster order
-  const float scale = p.ad.scales[tile.adapter];
-  for (int i = split * kShrinkWarps * 32 + threadIdx.x; i < todo; i += splits * kShrinkWarps * 32) {
-    float v = 0.f;
-    if (splits > 1) {
-      for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(s_red, k)[i];
-    } else {
-      v = s_red[i];
+      const int col = i / (16 * MT), mp = m0 + i % (16 * MT);
+      if (mp >= rows) continue;
+      const int j = mp / rank_p, r = mp - j * rank_p;
+      __nv_bfloat16* dst = p.s + (tile.start + first + col) * p.s_stride + j * p.terms * rank_p + r;
+      store_terms(dst, rank_p, p.terms, r < tile.rank ? v * scale : 0.f);
     }
-    const int col = i / (16 * MT), mp = m0 + i % (16 * MT);
-    if (mp >= rows) continue;
-    const int j = mp / rank_p, r = mp - j * rank_p;
-    __nv_bfloat16* dst = p.s + (tile.start + first + col) * p.s_stride + j * p.terms * rank_p + r;
-    store_terms(dst, rank_p, p.terms, r < tile.rank ? v * scale : 0.f);
+    // no CTA leaves, or starts on s_red again, while another reads its part
+    if (splits > 1) cluster.sync(); else __syncthreads();
   }
-  if (splits > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
 
 // ---- second product, bf16 -----------------------------------------------------
-// A CTA keeps the s rows of `tm` tokens of a tile in shared memory and goes
-// through its share of the columns.  Each of its 4 warps works on its own:
-// 32 columns at a time, whose base values and adapter rows come in by
-// cp.async one step ahead into the warp's own buffers, so no barrier stands
-// in the loop.  mma m16n8k16 with tokens as M, columns as N, the rank as K;
-// the sums start from the base and leave through the warp's buffer in whole
-// 32-byte sectors.
-constexpr int kExpWarps = 4;
-constexpr int kGroup = 32;             // columns per step of a warp
-constexpr int kBaseLd = kGroup + 8;    // floats per base row: conflict-free 8-byte reads
-constexpr int kBLd = kGroup + 8;       // bf16 per adapter row: conflict-free ldmatrix
+// A CTA keeps the s rows of up to 16 WM tokens of a tile in shared memory and
+// goes through its share of the columns, 32 WN at a step: their base values
+// and adapter rows come in by cp.async, up to two steps ahead.  mma m16n8k16
+// with tokens as M, columns as N, the rank as K; warp (m, n) of the WM x WN
+// has 16 tokens and 32 columns.  The sums start from the base and leave
+// through its buffer, in whole 32-byte sectors.
+constexpr int kPad = 8;  // elements after each shared-memory row: conflict-free fragment reads
 
 struct ExpandArgs {
   const float* base;
@@ -254,7 +250,7 @@ struct ExpandArgs {
   int N, ns, terms;
   int slice_end[3];
   int interleaved, in_place, after_shrink;
-  int tm, stages;  // tokens per CTA (16, 32 or 64), steps in a warp's ring (1 or 2)
+  int stages;  // steps in the ring (2 to 4)
   int rank_pm;     // padded largest rank: buffer sizes
   int64_t s_stride;
   ms_lora_adapters ad;
@@ -277,9 +273,63 @@ enum LoraEpilogue { kLoraF32, kLoraBf16, kLoraSwiGLU };
 
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
-template <int EPI>
-__global__ void __launch_bounds__(kExpWarps * 32) lora_expand_kernel(ExpandArgs p) {
+// Which slice a warp's 32 columns take their s from.
+enum SliceMode { kOneSlice, kInterleaved, kMixed };
+
+// acc += s B for one warp: sa, sb the shared addresses of this lane's ldmatrix
+// rows (first rank step), term and slice offsets in bytes.
+template <int TERMS, int MODE>
+__device__ __forceinline__ void expand_mma(float (&acc)[4][4], uint32_t sa, uint32_t sb, int rank_p,
+                                           uint32_t b_step, const ExpandArgs& p, int c, int j0,
+                                           int j1) {
+  const uint32_t term = 2u * rank_p, slice = TERMS * term;
+  const int g = (threadIdx.x & 31) >> 2;
+#pragma unroll 2
+  for (int k = 0; k < rank_p; k += 16, sa += 32, sb += b_step) {
+    uint32_t b[8];  // n-tile n: b[2n], b[2n + 1]
+    {
+      uint32_t b01[4], b23[4];
+      ldsm4_t(b01, sb);
+      ldsm4_t(b23, sb + 32);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = b01[e], b[4 + e] = b23[e];
+    }
+    if constexpr (MODE == kMixed) {
+      for (int j = j0; j <= j1; ++j) {
+        uint32_t a[TERMS][4];
+#pragma unroll
+        for (int e = 0; e < TERMS; ++e) ldsm4(a[e], sa + j * slice + e * term);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const bool mine = slice_of(p, c + 8 * n + g) == j;  // this lane's column
+          const uint32_t w0 = mine ? b[2 * n] : 0u, w1 = mine ? b[2 * n + 1] : 0u;
+#pragma unroll
+          for (int e = TERMS - 1; e >= 0; --e)
+            mma_bf16(acc[n], a[e][0], a[e][1], a[e][2], a[e][3], w0, w1);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < (MODE == kInterleaved ? 2 : 1); ++h) {
+        uint32_t a[TERMS][4];
+        const uint32_t at = sa + (MODE == kInterleaved ? h : j0) * slice;
+#pragma unroll
+        for (int e = 0; e < TERMS; ++e) ldsm4(a[e], at + e * term);
+#pragma unroll
+        for (int e = TERMS - 1; e >= 0; --e)  // the small terms first
+#pragma unroll
+          for (int n = h; n < 4; n += MODE == kInterleaved ? 2 : 1)
+            mma_bf16(acc[n], a[e][0], a[e][1], a[e][2], a[e][3], b[2 * n], b[2 * n + 1]);
+      }
+    }
+  }
+}
+
+template <int EPI, int WM, int WN>
+__global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p) {
   constexpr int TERMS = EPI == kLoraF32 ? 3 : 2;
+  constexpr int kTm = 16 * WM, kCols = 32 * WN, kThreads = 32 * WM * WN;
+  constexpr int kBaseLd = kCols + kPad, kBLd = kCols + kPad;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int s_tok[kTile];
   // The plan and the adapters are read before the launch wait when
@@ -287,118 +337,104 @@ __global__ void __launch_bounds__(kExpWarps * 32) lora_expand_kernel(ExpandArgs 
   // before it has completed once its blocks allow this kernel to start.
   if (!p.after_shrink) pdl_enter();
   Tile tile;
-  const int per = kTile / p.tm;
-  const bool ok = load_tile(p.plan, p.ad, blockIdx.y / per, tile, p.err);
-  const int first = (blockIdx.y % per) * p.tm;
-  const int here = min(tile.count - first, p.tm);
+  const bool ok = load_tile(p.plan, p.ad, blockIdx.y, tile, p.err);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int wm = warp % WM, wn = warp / WM;
   const int rank_p = pad16(tile.rank);
-  const int s_row = p.ns * TERMS * rank_p, s_ld = s_row + 8;
-  // s rows, then each warp's ring of (base rows, adapter rows)
-  const int s_bytes = p.tm * (p.ns * TERMS * p.rank_pm + 8) * 2;
-  const int base_bytes = p.tm * kBaseLd * 4, stage_bytes = base_bytes + p.rank_pm * kBLd * 2;
+  const int s_row = p.ns * TERMS * rank_p, s_ld = s_row + kPad;
+  // s rows, then the ring of (base rows, adapter rows)
+  const int s_bytes = kTm * (p.ns * TERMS * p.rank_pm + kPad) * 2;
+  constexpr int kBaseBytes = kTm * kBaseLd * 4;
+  const int stage_bytes = kBaseBytes + p.rank_pm * kBLd * 2;
   __nv_bfloat16* s_s = reinterpret_cast<__nv_bfloat16*>(smem);
-  unsigned char* ring = smem + s_bytes + warp * p.stages * stage_bytes;
-  const bool work = ok && here > 0 && !(p.in_place && tile.rank == 0);
-  const int step = kExpWarps * gridDim.x * kGroup;
-  const int c_first = (blockIdx.x * kExpWarps + warp) * kGroup;
+  unsigned char* ring = smem + s_bytes;
+  const bool work = ok && tile.count > 0 && !(p.in_place && tile.rank == 0);
+  const int step = kCols * gridDim.x, c_first = kCols * blockIdx.x;
 
-  if (work && threadIdx.x < here)
-    s_tok[threadIdx.x] = token_at(p.plan, tile.start + first + threadIdx.x, p.err);
-  // columns c .. c+31 into ring slot `slot`
+  if (work)
+    for (int i = threadIdx.x; i < tile.count; i += kThreads)
+      s_tok[i] = token_at(p.plan, tile.start + i, p.err);
+  __syncthreads();
+  // adapter rows / base rows of columns c .. c + kCols - 1 into ring slot `slot`
   auto load_b = [&](int c, int slot) {
-    __nv_bfloat16* s_b = reinterpret_cast<__nv_bfloat16*>(ring + slot * stage_bytes + base_bytes);
-    for (int i = lane; i < rank_p * 4; i += 32) {
-      const int r = i >> 2, q = 8 * (i & 3);
+    __nv_bfloat16* s_b = reinterpret_cast<__nv_bfloat16*>(ring + slot * stage_bytes + kBaseBytes);
+    for (int i = threadIdx.x; i < rank_p * (kCols / 8); i += kThreads) {
+      const int r = i / (kCols / 8), q = 8 * (i % (kCols / 8));
       const bool in = r < tile.rank && c + q < p.N;
       cp_async16(s_addr(s_b + r * kBLd + q),
                  p.b + (in ? ((int64_t)tile.offset + r) * p.N + c + q : 0), in);
     }
   };
-  auto load_base = [&](int c, int slot) {
+  auto load_base = [&](int c, int slot, int first, int here) {
     float* s_base = reinterpret_cast<float*>(ring + slot * stage_bytes);
-    for (int i = lane; i < here * 8; i += 32) {
-      const int row = i >> 3, q = 4 * (i & 7);
-      const int tok = s_tok[row];
+    for (int i = threadIdx.x; i < here * (kCols / 4); i += kThreads) {
+      const int row = i / (kCols / 4), q = 4 * (i % (kCols / 4));
+      const int tok = s_tok[first + row];
       const bool in = tok >= 0 && c + q < p.N;
       cp_async16(s_addr(s_base + row * kBaseLd + q),
                  p.base + (in ? tok * p.base_stride + c + q : 0), in);
     }
   };
-  __syncthreads();  // s_tok
-  if (work && c_first < p.N) load_b(c_first, 0);
+  if (work && p.after_shrink) load_b(c_first, 0);
   if (p.after_shrink) pdl_enter();
   if (!work) return;
-  for (int i = threadIdx.x; i < here * (s_row / 8); i += kExpWarps * 32) {
-    const int row = i / (s_row / 8), q = 8 * (i - row * (s_row / 8));
-    cp_async16(s_addr(s_s + row * s_ld + q), p.s + (tile.start + first + row) * p.s_stride + q, true);
-  }
-  if (c_first < p.N) load_base(c_first, 0);
-  cp_commit();
-  cp_wait<0>();
-  __syncthreads();  // s
 
-  int slot = 0;
-  for (int c = c_first; c < p.N; c += step) {
-    const int next = p.stages > 1 ? slot ^ 1 : 0;
-    if (p.stages > 1) {
-      if (c + step < p.N) {
-        load_b(c + step, next);
-        load_base(c + step, next);
+  for (int first = 0; first < tile.count; first += kTm) {
+    const int here = min(tile.count - first, kTm);
+    if (first > 0) __syncthreads();  // the last pass is done with s and the ring
+    for (int i = threadIdx.x; i < here * (s_row / 8); i += kThreads) {
+      const int row = i / (s_row / 8), q = 8 * (i - row * (s_row / 8));
+      cp_async16(s_addr(s_s + row * s_ld + q), p.s + (tile.start + first + row) * p.s_stride + q, true);
+    }
+    for (int k = 0; k + 1 < p.stages; ++k) {
+      if (c_first + k * step < p.N) {
+        if (first > 0 || k > 0 || !p.after_shrink) load_b(c_first + k * step, k);
+        load_base(c_first + k * step, k, first, here);
       }
       cp_commit();
-      cp_wait<1>();
-    } else {
-      cp_wait<0>();
     }
-    __syncwarp();
-    float* s_base = reinterpret_cast<float*>(ring + slot * stage_bytes);
-    const __nv_bfloat16* s_b =
-        reinterpret_cast<const __nv_bfloat16*>(ring + slot * stage_bytes + base_bytes);
-    int lo[4], hi[4];  // first and last slice of each 8 columns
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      lo[n] = slice_of(p, min(c + 8 * n, p.N - 1));
-      hi[n] = slice_of(p, min(c + 8 * n + 7, p.N - 1));
-    }
-    const int j_lo = lo[0], j_hi = p.interleaved ? 1 : hi[3];
-    for (int m = 0; m < here; m += 16) {
+    int slot = 0;
+    for (int c0 = c_first; c0 < p.N; c0 += step) {
+      if (p.stages > 3) cp_wait<2>(); else if (p.stages > 2) cp_wait<1>(); else cp_wait<0>();
+      __syncthreads();  // this step's data is there, the last step's slot is free
+      const int ahead = p.stages - 1, cn = c0 + ahead * step;
+      if (cn < p.N) {
+        const int free = slot == 0 ? p.stages - 1 : slot - 1;
+        load_b(cn, free);
+        load_base(cn, free, first, here);
+      }
+      cp_commit();
+      const int c = c0 + 32 * wn, m = 16 * wm;
+      float* s_base = reinterpret_cast<float*>(ring + slot * stage_bytes) + m * kBaseLd + 32 * wn;
+      const __nv_bfloat16* s_b =
+          reinterpret_cast<const __nv_bfloat16*>(ring + slot * stage_bytes + kBaseBytes) + 32 * wn;
+      slot = slot + 1 == p.stages ? 0 : slot + 1;
+      if (m >= here || c >= p.N) continue;
       float acc[4][4];
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float2 v = *reinterpret_cast<const float2*>(s_base + (m + g + 8 * h) * kBaseLd + 8 * n + 2 * t);
+          const float2 v = *reinterpret_cast<const float2*>(s_base + (g + 8 * h) * kBaseLd + 8 * n + 2 * t);
           acc[n][2 * h] = v.x;
           acc[n][2 * h + 1] = v.y;
         }
-      for (int k = 0; k < rank_p; k += 16) {
-        uint32_t b01[4], b23[4];
-        const __nv_bfloat16* bp = s_b + (k + (lane & 15)) * kBLd + 8 * (lane >> 4);
-        ldsm4_t(b01, s_addr(bp));
-        ldsm4_t(b23, s_addr(bp + 16));
-        for (int j = j_lo; j <= j_hi; ++j) {
-          uint32_t a[TERMS][4];
-          const __nv_bfloat16* sp = s_s + (m + (lane & 15)) * s_ld + j * TERMS * rank_p + k + 8 * (lane >> 4);
-#pragma unroll
-          for (int e = 0; e < TERMS; ++e) ldsm4(a[e], s_addr(sp + e * rank_p));
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            if (j < lo[n] || j > hi[n]) continue;
-            uint32_t w0 = n < 2 ? b01[2 * n] : b23[2 * n - 4];
-            uint32_t w1 = n < 2 ? b01[2 * n + 1] : b23[2 * n - 3];
-            if (lo[n] != hi[n] && slice_of(p, c + 8 * n + g) != j) w0 = w1 = 0u;  // another slice's column
-#pragma unroll
-            for (int e = TERMS - 1; e >= 0; --e)  // the small terms first
-              mma_bf16(acc[n], a[e][0], a[e][1], a[e][2], a[e][3], w0, w1);
-          }
-        }
+      const uint32_t sa = s_addr(s_s + (m + (lane & 15)) * s_ld + 8 * (lane >> 4));
+      const uint32_t sb = s_addr(s_b + (lane & 15) * kBLd + 8 * (lane >> 4));
+      if (p.interleaved) {
+        expand_mma<TERMS, kInterleaved>(acc, sa, sb, rank_p, 32 * kBLd, p, c, 0, 1);
+      } else {
+        const int j0 = slice_of(p, c), j1 = slice_of(p, min(c + 31, p.N - 1));
+        if (j0 == j1)
+          expand_mma<TERMS, kOneSlice>(acc, sa, sb, rank_p, 32 * kBLd, p, c, j0, j0);
+        else
+          expand_mma<TERMS, kMixed>(acc, sa, sb, rank_p, 32 * kBLd, p, c, j0, j1);
       }
-      // out through the rows of s_base, which every lane has read
+      // out through this warp's part of the base rows, which all its lanes have read
       __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float* row = s_base + (m + g + 8 * h) * kBaseLd;
+        float* row = s_base + (g + 8 * h) * kBaseLd;
         if constexpr (EPI == kLoraSwiGLU) {
 #pragma unroll
           for (int n = 0; n < 4; n += 2)
@@ -424,23 +460,16 @@ __global__ void __launch_bounds__(kExpWarps * 32) lora_expand_kernel(ExpandArgs 
       for (int i = lane; i < 16 * kChunks; i += 32) {
         const int row = i / kChunks, q = i % kChunks;
         if (m + row >= here || c_out + q * kPer >= n_out) continue;
-        const int tok = s_tok[m + row];
+        const int tok = s_tok[first + m + row];
         if (tok < 0) continue;
         const int64_t at = tok * p.out_stride + c_out + q * kPer;
-        const float4 v = reinterpret_cast<const float4*>(s_base + (m + row) * kBaseLd)[q];
+        const float4 v = reinterpret_cast<const float4*>(s_base + row * kBaseLd)[q];
         if constexpr (EPI == kLoraF32)
           *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
         else
           *reinterpret_cast<float4*>(static_cast<__nv_bfloat16*>(p.out) + at) = v;
       }
     }
-    __syncwarp();  // the slot's rows are out before it is filled again
-    if (p.stages == 1 && c + step < p.N) {
-      load_b(c + step, 0);
-      load_base(c + step, 0);
-      cp_commit();
-    }
-    slot = next;
   }
 }
 
@@ -513,38 +542,47 @@ int shrink_split(int n_tiles, int K, int rows, int mt) {
   return split;
 }
 
-template <int EPI>
+template <int EPI, int WM, int WN>
 int launch_expand(ExpandArgs p, cudaStream_t s) {
-  static std::atomic<uint64_t> granted{0};
-  MS_TRY(grant_dynamic_smem(lora_expand_kernel<EPI>, kMostSmem, granted));
-  // Tokens per CTA by the tiles' mean size; fewer, and a ring of one, where
-  // large ranks need the shared memory.
-  const int terms = EPI == kLoraF32 ? 3 : 2;
-  const int mean = p.plan.n_tokens / p.plan.n_tiles;
-  p.tm = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
-  p.stages = 2;
+  constexpr int terms = EPI == kLoraF32 ? 3 : 2, cols = 32 * WN;
   auto smem = [&]() {
-    return p.tm * (p.ns * terms * p.rank_pm + 8) * 2 +
-           kExpWarps * p.stages * (p.tm * kBaseLd * 4 + p.rank_pm * kBLd * 2);
+    return 16 * WM * (p.ns * terms * p.rank_pm + kPad) * 2 +
+           p.stages * (cols + kPad) * (16 * WM * 4 + p.rank_pm * 2);
   };
-  while (p.tm > 16 && smem() > 110 * 1024) p.tm /= 2;
-  if (smem() > kMostSmem) p.stages = 1;
-  const int tiles = p.plan.n_tiles * (kTile / p.tm), groups = ceil_div(p.N, kGroup * kExpWarps);
-  // about 8 CTAs per SM in all, so that a warp's steps follow one another
-  const int gx = max(1, min(groups, ceil_div(8 * 148, tiles)));
-  launch_pdl(lora_expand_kernel<EPI>, dim3(gx, tiles), kExpWarps * 32, smem(), s, p);
+  // As deep a ring as two CTAs per SM allow, or one where two do not fit
+  p.stages = 2;
+  const int room = smem() > 112 * 1024 ? kMostSmem : 112 * 1024;
+  while (p.stages < 4 && (++p.stages, smem() > room)) {
+    --p.stages;
+    break;
+  }
+  if constexpr (WM * WN > 2)
+    if (smem() > kMostSmem) return launch_expand<EPI, 1, 2>(p, s);  // ranks of 128 and more
+  static std::atomic<uint64_t> granted{0};
+  MS_TRY(grant_dynamic_smem(lora_expand_kernel<EPI, WM, WN>, kMostSmem, granted));
+  // about three rounds of CTAs over the GPU, so that each has several steps
+  const int resident = max(1, min(64 / (WM * WN), 227 * 1024 / (smem() + 1024)));
+  const int gx = max(1, min(ceil_div(p.N, cols), ceil_div(3 * 148 * resident, p.plan.n_tiles)));
+  launch_pdl(lora_expand_kernel<EPI, WM, WN>, dim3(gx, p.plan.n_tiles), 32 * WM * WN, smem(), s, p);
   return check_launch("lora_expand_kernel");
 }
 
-template <int MT>
+// Tokens per CTA by the tiles' mean size.
+template <int EPI>
+int dispatch_expand(const ExpandArgs& p, cudaStream_t s) {
+  const int mean = p.plan.n_tokens / p.plan.n_tiles;
+  if (mean <= 16) return launch_expand<EPI, 1, 4>(p, s);
+  if (mean <= 32) return launch_expand<EPI, 2, 4>(p, s);
+  return launch_expand<EPI, 4, 2>(p, s);
+}
+
+template <int MT, int NT>
 int launch_shrink(ShrinkArgs p, int rows, cudaStream_t s) {
-  const int smem = kShrinkWarps * 16 * MT * kShrinkTokens * 4;
-  static std::atomic<uint64_t> granted{0};
-  if (smem > 48 * 1024) MS_TRY(grant_dynamic_smem(lora_shrink_kernel<MT>, smem, granted));
+  const int smem = kShrinkWarps * 16 * MT * 8 * NT * 4;
   const int split = shrink_split(p.plan.n_tiles, p.K, rows, MT);
   p.k_per = ceil_div(ceil_div(p.K, split), 32) * 32;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.plan.n_tiles * (kTile / kShrinkTokens), ceil_div(rows, 16 * MT), split);
+  cfg.gridDim = dim3(p.plan.n_tiles, ceil_div(rows, 16 * MT), split);
   cfg.blockDim = kShrinkWarps * 32;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -555,8 +593,13 @@ int launch_shrink(ShrinkArgs p, int rows, cudaStream_t s) {
   attr[1].val.clusterDim = {1, 1, (unsigned)split};
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  (void)cudaLaunchKernelEx(&cfg, lora_shrink_kernel<MT>, p);
+  (void)cudaLaunchKernelEx(&cfg, lora_shrink_kernel<MT, NT>, p);
   return check_launch("lora_shrink_kernel");
+}
+
+template <int NT>
+int dispatch_shrink(const ShrinkArgs& p, int rows, cudaStream_t s) {
+  return rows <= 16 ? launch_shrink<1, NT>(p, rows, s) : launch_shrink<2, NT>(p, rows, s);
 }
 
 template <typename T, typename TO>
@@ -650,14 +693,17 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
     p.s = static_cast<__nv_bfloat16*>(workspace);
     p.err = e.err;
     e.after_shrink = 1;
-    const int rows = c.n_slices * e.rank_pm;
-    if (rows <= 16)
-      MS_TRY(launch_shrink<1>(p, rows, s));
+    // tokens at a time by the tiles' mean size
+    const int rows = c.n_slices * e.rank_pm, mean = plan.n_tokens / plan.n_tiles;
+    if (mean <= 8)
+      MS_TRY(dispatch_shrink<1>(p, rows, s));
+    else if (mean <= 16)
+      MS_TRY(dispatch_shrink<2>(p, rows, s));
     else
-      MS_TRY(launch_shrink<2>(p, rows, s));
+      MS_TRY(dispatch_shrink<4>(p, rows, s));
   }
-  if (c.swiglu) return launch_expand<kLoraSwiGLU>(e, s);
-  return out_f32 ? launch_expand<kLoraF32>(e, s) : launch_expand<kLoraBf16>(e, s);
+  if (c.swiglu) return dispatch_expand<kLoraSwiGLU>(e, s);
+  return out_f32 ? dispatch_expand<kLoraF32>(e, s) : dispatch_expand<kLoraBf16>(e, s);
 }
 
 }  // namespace ms
