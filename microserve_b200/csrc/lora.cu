@@ -330,6 +330,8 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
   constexpr int TERMS = EPI == kLoraF32 ? 3 : 2;
   constexpr int kTm = 16 * WM, kCols = 32 * WN, kThreads = 32 * WM * WN;
   constexpr int kBaseLd = kCols + kPad, kBLd = kCols + kPad;
+  constexpr int kBRows = kThreads / (kCols / 8), kBaseRows = kThreads / (kCols / 4);  // rows a pass of loads
+  static_assert(kBaseRows >= 1, "a row of loads fits the block");
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int s_tok[kTile];
   // The plan and the adapters are read before the launch wait when
@@ -358,21 +360,26 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
   // adapter rows / base rows of columns c .. c + kCols - 1 into ring slot `slot`
   auto load_b = [&](int c, int slot) {
     __nv_bfloat16* s_b = reinterpret_cast<__nv_bfloat16*>(ring + slot * stage_bytes + kBaseBytes);
-    for (int i = threadIdx.x; i < rank_p * (kCols / 8); i += kThreads) {
-      const int r = i / (kCols / 8), q = 8 * (i % (kCols / 8));
-      const bool in = r < tile.rank && c + q < p.N;
-      cp_async16(s_addr(s_b + r * kBLd + q),
-                 p.b + (in ? ((int64_t)tile.offset + r) * p.N + c + q : 0), in);
+    const int q = 8 * (threadIdx.x % (kCols / 8)), r0 = threadIdx.x / (kCols / 8);
+    const bool in = c + q < p.N;
+    const __nv_bfloat16* src = p.b + ((int64_t)tile.offset + r0) * p.N + (in ? c + q : 0);
+    uint32_t dst = s_addr(s_b + r0 * kBLd + q);
+    for (int r = r0; r < rank_p; r += kBRows) {
+      const bool row = r < tile.rank;
+      cp_async16(dst, row ? src : p.b, row && in);
+      src += (int64_t)kBRows * p.N;
+      dst += kBRows * kBLd * 2;
     }
   };
   auto load_base = [&](int c, int slot, int first, int here) {
     float* s_base = reinterpret_cast<float*>(ring + slot * stage_bytes);
-    for (int i = threadIdx.x; i < here * (kCols / 4); i += kThreads) {
-      const int row = i / (kCols / 4), q = 4 * (i % (kCols / 4));
-      const int tok = s_tok[first + row];
-      const bool in = tok >= 0 && c + q < p.N;
-      cp_async16(s_addr(s_base + row * kBaseLd + q),
-                 p.base + (in ? tok * p.base_stride + c + q : 0), in);
+    const int q = 4 * (threadIdx.x % (kCols / 4)), r0 = threadIdx.x / (kCols / 4);
+    const bool in = c + q < p.N;
+    uint32_t dst = s_addr(s_base + r0 * kBaseLd + q);
+    for (int r = r0; r < here; r += kBaseRows) {
+      const int tok = s_tok[first + r];
+      cp_async16(dst, in && tok >= 0 ? p.base + tok * p.base_stride + c + q : p.base, in && tok >= 0);
+      dst += kBaseRows * kBaseLd * 4;
     }
   };
   if (work && p.after_shrink) load_b(c_first, 0);
@@ -573,7 +580,7 @@ int dispatch_expand(const ExpandArgs& p, cudaStream_t s) {
   const int mean = p.plan.n_tokens / p.plan.n_tiles;
   if (mean <= 16) return launch_expand<EPI, 1, 4>(p, s);
   if (mean <= 32) return launch_expand<EPI, 2, 4>(p, s);
-  return launch_expand<EPI, 4, 2>(p, s);
+  return launch_expand<EPI, 4, 4>(p, s);
 }
 
 template <int MT, int NT>
