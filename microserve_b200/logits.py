@@ -36,6 +36,7 @@ if TYPE_CHECKING:
     from .scheduler import Request
 
 MAX_PROPOSALS = 64
+_check = _lib.check_tensor
 
 
 def mask_words(vocab_size: int) -> int:
@@ -51,18 +52,6 @@ def pack_masks(allowed: np.ndarray) -> np.ndarray:
     full = np.zeros((n, mask_words(vocab) * 32), dtype=np.uint8)
     full[:, :vocab] = allowed
     return np.packbits(full, axis=1, bitorder="little").view("<u4").view(np.int32)
-
-
-def _check(t: torch.Tensor | None, name: str, dtype: torch.dtype, device: torch.device,
-           shape: tuple[int | None, ...]) -> int | None:
-    """The data pointer of an optional argument after checking it."""
-    if t is None:
-        return None
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.dim() != len(shape) \
-            or any(w is not None and w != h for w, h in zip(shape, t.shape)):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}; "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
 
 
 @dataclass
@@ -90,19 +79,19 @@ class TokenCounts:
     def vocab_size(self) -> int:
         return self.counts.shape[1]
 
-    def pointers(self, device: torch.device) -> tuple[int | None, int | None]:
+    def pointers(self, index: int) -> tuple[int | None, int | None]:
+        """Data pointers of counts and seen, checked to lie on CUDA device ``index``."""
         n, v = self.counts.shape
-        return (_check(self.counts, "counts", torch.int32, device, (n, v)),
-                _check(self.seen, "seen", torch.int32, device, (n, mask_words(v))))
+        return (_check(self.counts, "counts", torch.int32, index, (n, v)),
+                _check(self.seen, "seen", torch.int32, index, (n, mask_words(v))))
 
     def reset(self, slots: torch.Tensor) -> None:
         """Forget everything in ``slots`` (int32, device; negative: skipped)."""
-        dev = self.counts.device
+        dev = _lib.cuda_index(self.counts)
         c, s = self.pointers(dev)
-        p = _check(slots, "slots", torch.int32, dev, (None,))
-        with _lib.on_device(dev):
-            _lib.call("ms_token_counts_reset", c, s, self.n_slots, self.vocab_size, p,
-                      slots.numel(), _lib.stream_ptr(dev))
+        p = _check(slots, "slots", torch.int32, dev, (slots.numel(),))
+        _lib.launch_on(dev, "ms_token_counts_reset", c, s, self.n_slots, self.vocab_size, p,
+                       slots.numel())
 
     def append(self, slots: torch.Tensor, tokens: torch.Tensor, lens: torch.Tensor | None = None,
                len_add: int = 0, row_start: torch.Tensor | None = None, max_len: int | None = None,
@@ -115,18 +104,19 @@ class TokenCounts:
         ``row_start[i]`` and ``max_len`` bounds every length; each sequence must
         lie inside ``tokens``.  The first ``n_prompt[i]`` tokens are prompt:
         they only become seen."""
-        dev = self.counts.device
+        dev = _lib.cuda_index(self.counts)
         c, s = self.pointers(dev)
         n = slots.numel()
-        ps = _check(slots, "slots", torch.int32, dev, (None,))
-        pl = _check(lens, "lens", torch.int32, dev, (n,))
-        pp = _check(n_prompt, "n_prompt", torch.int32, dev, (n,))
-        pr = _check(row_start, "row_start", torch.int64, dev, (n,))
+        ps = _check(slots, "slots", torch.int32, dev, (n,))
+        pl = None if lens is None else _check(lens, "lens", torch.int32, dev, (n,))
+        pp = None if n_prompt is None else _check(n_prompt, "n_prompt", torch.int32, dev, (n,))
+        pr = None
         if row_start is None:
-            pt = _check(tokens, "tokens", torch.int32, dev, (n, None))
-            stride = width = tokens.shape[1]
+            stride = width = tokens.shape[-1]
+            pt = _check(tokens, "tokens", torch.int32, dev, (n, width))
         else:
-            pt = _check(tokens, "tokens", torch.int32, dev, (None,))
+            pr = _check(row_start, "row_start", torch.int64, dev, (n,))
+            pt = _check(tokens, "tokens", torch.int32, dev, (tokens.numel(),))
             if max_len is None or lens is None:
                 raise ValueError("flat tokens need lens and max_len")
             stride, width = 0, max_len
@@ -134,9 +124,8 @@ class TokenCounts:
             len_add = width
         if n == 0 or width == 0:
             return
-        with _lib.on_device(dev):
-            _lib.call("ms_token_counts_append", c, s, self.n_slots, self.vocab_size, ps, n, pt, pr,
-                      stride, pl, len_add, width, pp, _lib.stream_ptr(dev))
+        _lib.launch_on(dev, "ms_token_counts_append", c, s, self.n_slots, self.vocab_size, ps, n,
+                       pt, pr, stride, pl, len_add, width, pp)
 
 
 @dataclass
@@ -178,61 +167,61 @@ def apply_logit_controls(
     or a tensor that does not overlap it; by default a new one is returned.
     Masked tokens become ``-inf``; a row whose mask allows nothing is all
     ``-inf``.  Rows may be strided; a row's logits must be contiguous."""
-    dev = _lib.require_cuda(logits.device)
-    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+    dev = _lib.cuda_index(logits)
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or logits.stride(1) != 1:
         raise ValueError("logits must be a float32 (rows, vocab) tensor with contiguous rows")
     rows, vocab = logits.shape
     if rows_per_request < 1 or rows % rows_per_request:
         raise ValueError(f"{rows} rows are not a multiple of rows_per_request={rows_per_request}")
     B = rows // rows_per_request
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
-    elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != dev \
-            or out.stride(1) != 1:
+        out = torch.empty((rows, vocab), dtype=torch.float32, device=logits.device)
+    elif out is not logits and (out.shape != logits.shape or out.dtype is not torch.float32
+                                or out.get_device() != dev or out.stride(1) != 1):
         raise ValueError("out must be a float32 tensor of the logits' shape with contiguous rows")
     if rows == 0 or vocab == 0:
         return out
     c = controls
-    words = mask_words(vocab)
-    s = _lib.MsLogitControls()
+    i32, f32 = torch.int32, torch.float32
+    slots = penalties = p_counts = p_seen = props = starts = ids = values = mask_rows = masks = None
+    n_slots = n_props = n_bias = n_masks = 0
     if c.slots is not None:
         if counts is None or c.penalties is None:
             raise ValueError("penalties need slots, penalties and token counts")
-        if counts.vocab_size != vocab:
+        if counts.counts.shape[1] != vocab:
             raise ValueError(f"token counts are for a vocabulary of {counts.vocab_size}, not {vocab}")
-        s.slots = _check(c.slots, "slots", torch.int32, dev, (B,))
-        s.penalties = _check(c.penalties, "penalties", torch.float32, dev, (B, 3))
-        s.counts, s.seen = counts.pointers(dev)
-        s.n_slots = counts.n_slots
+        slots = _check(c.slots, "slots", i32, dev, (B,))
+        penalties = _check(c.penalties, "penalties", f32, dev, (B, 3))
+        p_counts, p_seen = counts.pointers(dev)
+        n_slots = counts.n_slots
         if proposals is not None:
-            s.proposals = _check(proposals, "proposals", torch.int32, dev, (None, B))
-            s.n_proposals = proposals.shape[0]
-            s.first_proposal = first_proposal
-            if not 0 <= first_proposal <= s.n_proposals - rows_per_request + 1 \
-                    or s.n_proposals > MAX_PROPOSALS:
+            n_props = proposals.shape[0]
+            props = _check(proposals, "proposals", i32, dev, (n_props, B))
+            if not 0 <= first_proposal <= n_props - rows_per_request + 1 or n_props > MAX_PROPOSALS:
                 raise ValueError(f"rows see {first_proposal} to {first_proposal + rows_per_request - 1} "
-                                 f"proposals of {s.n_proposals} (at most {MAX_PROPOSALS})")
-            if s.n_proposals == 0:
-                s.proposals = None
+                                 f"proposals of {n_props} (at most {MAX_PROPOSALS})")
+            if n_props == 0:
+                props = None
     elif c.penalties is not None:
         raise ValueError("penalties need slots, penalties and token counts")
     if c.bias_start is not None:
         if c.bias_ids is None or c.bias_values is None:
             raise ValueError("bias_start needs bias_ids and bias_values")
-        n = c.bias_ids.numel()
-        s.bias_start = _check(c.bias_start, "bias_start", torch.int32, dev, (B + 1,))
-        s.bias_ids = _check(c.bias_ids, "bias_ids", torch.int32, dev, (n,))
-        s.bias_values = _check(c.bias_values, "bias_values", torch.float32, dev, (n,))
-        s.n_bias = n
+        n_bias = c.bias_ids.numel()
+        starts = _check(c.bias_start, "bias_start", i32, dev, (B + 1,))
+        ids = _check(c.bias_ids, "bias_ids", i32, dev, (n_bias,))
+        values = _check(c.bias_values, "bias_values", f32, dev, (n_bias,))
     if c.mask_rows is not None:
         if c.masks is None:
             raise ValueError("mask_rows needs masks")
-        s.mask_rows = _check(c.mask_rows, "mask_rows", torch.int32, dev, (rows,))
-        s.masks = _check(c.masks, "masks", torch.int32, dev, (None, words))
-        s.n_masks = c.masks.shape[0]
-        if s.n_masks == 0:
-            s.mask_rows = None
-    with _lib.on_device(dev):
-        _lib.call("ms_apply_logit_controls", logits.data_ptr(), logits.stride(0), out.data_ptr(),
-                  out.stride(0), B, rows_per_request, vocab, ctypes.byref(s), _lib.stream_ptr(dev))
+        mask_rows = _check(c.mask_rows, "mask_rows", i32, dev, (rows,))
+        n_masks = c.masks.shape[0]
+        masks = _check(c.masks, "masks", i32, dev, (n_masks, mask_words(vocab)))
+        if n_masks == 0:
+            mask_rows = None
+    s = _lib.MsLogitControls(slots, penalties, p_counts, p_seen, n_slots, n_props, props,
+                             first_proposal if props else 0, n_bias, starts, ids, values, mask_rows,
+                             masks, n_masks, 0)
+    _lib.launch_on(dev, "ms_apply_logit_controls", logits.data_ptr(), logits.stride(0),
+                   out.data_ptr(), out.stride(0), B, rows_per_request, vocab, ctypes.byref(s))
     return out

@@ -23,10 +23,11 @@ import numpy as np
 import torch
 
 from . import _lib
-from .logits import _check
 
 TILE = 64  # tokens of a plan's tile (MS_LORA_TILE)
 MAX_RANK = 256  # MS_LORA_MAX_RANK
+_check = _lib.check_tensor
+_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
 @dataclass
@@ -96,54 +97,56 @@ def lora_add(
     interleaved projection instead.  ``out`` (float32 or bfloat16) defaults to a
     new tensor of ``out_dtype``; it may be ``base`` itself (no SwiGLU): tokens
     without an adapter are then not touched."""
-    dev = _lib.require_cuda(x.device)
+    dev = _lib.cuda_index(x)
     T, K = x.shape
-    if base.dim() != 2 or base.shape[0] != T or base.dtype != torch.float32 or base.device != dev:
-        raise ValueError(f"base must be a float32 ({T}, N) tensor on {dev}")
+    if base.dim() != 2 or base.shape[0] != T or base.dtype is not torch.float32 \
+            or base.get_device() != dev:
+        raise ValueError(f"base must be a float32 ({T}, N) tensor on cuda:{dev}")
     N = base.shape[1]
-    if (T > 1 and (x.stride(0) < K or base.stride(0) < N)) or x.stride(1) != 1 or base.stride(1) != 1:
+    x_ld, x_inner = x.stride()
+    base_ld, base_inner = base.stride()
+    if (T > 1 and (x_ld < K or base_ld < N)) or x_inner != 1 or base_inner != 1:
         raise ValueError("x and base need contiguous, non-overlapping rows")
-    codes = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
-    if x.dtype not in codes:
-        raise ValueError(f"x must be float32 or bfloat16, got {x.dtype}")
-    ns = len(proj.slices)
-    if not 1 <= ns <= 4 or sum(proj.slices) != N or min(proj.slices) < 1:
-        raise ValueError(f"slices {list(proj.slices)} do not make up {N} columns")
-    if proj.interleaved and (ns != 2 or N % 16 or proj.slices[0] != proj.slices[1]):
+    dtype = x.dtype
+    if dtype not in _CODES:
+        raise ValueError(f"x must be float32 or bfloat16, got {dtype}")
+    slices = proj.slices
+    ns = len(slices)
+    if not 1 <= ns <= 4 or sum(slices) != N or min(slices) < 1:
+        raise ValueError(f"slices {list(slices)} do not make up {N} columns")
+    if proj.interleaved and (ns != 2 or N % 16 or slices[0] != slices[1]):
         raise ValueError("interleaved columns are two equal slices alternating every 8 columns")
     if swiglu and not proj.interleaved:
         raise ValueError("SwiGLU needs interleaved gate/up columns")
     if not 0 <= proj.max_rank <= MAX_RANK:
         raise ValueError(f"max_rank {proj.max_rank} is not in 0..{MAX_RANK}")
     R = proj.b.shape[0]
-    pa = _check(proj.a, "a", x.dtype, dev, (ns * R, K))
-    pb = _check(proj.b, "b", x.dtype, dev, (R, N))
+    pa = _check(proj.a, "a", dtype, dev, (ns * R, K))
+    pb = _check(proj.b, "b", dtype, dev, (R, N))
     n = proj.ranks.numel()
-    ad = _lib.MsLoraAdapters(n, R, proj.max_rank, 0,
-                             _check(proj.offsets, "offsets", torch.int32, dev, (n,)),
-                             _check(proj.ranks, "ranks", torch.int32, dev, (n,)),
+    i32 = torch.int32
+    ad = _lib.MsLoraAdapters(n, R, proj.max_rank, 0, _check(proj.offsets, "offsets", i32, dev, (n,)),
+                             _check(proj.ranks, "ranks", i32, dev, (n,)),
                              _check(proj.scales, "scales", torch.float32, dev, (n,)))
-    pl = _lib.MsLoraPlan(T, plan.tiles.shape[0],
-                         _check(plan.order, "order", torch.int32, dev, (T,)),
-                         _check(plan.tiles, "tiles", torch.int32, dev, (None, 4)))
+    n_tiles = plan.tiles.shape[0]
+    pl = _lib.MsLoraPlan(T, n_tiles, _check(plan.order, "order", i32, dev, (T,)),
+                         _check(plan.tiles, "tiles", i32, dev, (n_tiles, 4)))
     width = N // 2 if swiglu else N
     if out is None:
-        out = torch.empty((T, width), dtype=out_dtype, device=dev)
-    elif out.shape != (T, width) or out.device != dev or out.stride(1) != 1 \
+        out = torch.empty((T, width), dtype=out_dtype, device=x.device)
+    elif out.shape != (T, width) or out.get_device() != dev or out.stride(1) != 1 \
             or (T > 1 and out.stride(0) < width):
-        raise ValueError(f"out must be a ({T}, {width}) tensor on {dev} with contiguous rows")
-    if out.dtype not in codes:
+        raise ValueError(f"out must be a ({T}, {width}) tensor on cuda:{dev} with contiguous rows")
+    if out.dtype not in _CODES:
         raise ValueError(f"out must be float32 or bfloat16, got {out.dtype}")
     if T == 0:
         return out
-    with _lib.on_device(dev):
-        lib = _lib.load()
-        need = lib.ms_lora_workspace_size(ctypes.byref(ad), ctypes.byref(pl), ns)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        cols = (ctypes.c_int32 * ns)(*proj.slices)
-        _lib.call("ms_lora_add", x.data_ptr(), max(x.stride(0), K), base.data_ptr(),
-                  max(base.stride(0), N), out.data_ptr(), max(out.stride(0), width), pa, pb, K, N, ns,
-                  ctypes.cast(cols, ctypes.c_void_p), int(proj.interleaved), int(swiglu),
-                  ctypes.byref(ad), ctypes.byref(pl), codes[x.dtype], codes[out.dtype],
-                  ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
+    # ms_lora_workspace_size: s as up to three bf16 terms of the padded rank
+    need = T * ns * ((proj.max_rank + 15) // 16 * 16) * 6
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
+    cols = (ctypes.c_int32 * ns)(*slices)
+    _lib.launch_on(dev, "ms_lora_add", x.data_ptr(), max(x_ld, K), base.data_ptr(),
+                   max(base_ld, N), out.data_ptr(), max(out.stride(0), width), pa, pb, K, N, ns,
+                   ctypes.addressof(cols), int(proj.interleaved), int(swiglu), ctypes.byref(ad),
+                   ctypes.byref(pl), _CODES[dtype], _CODES[out.dtype], ws.data_ptr(), ws.numel())
     return out
