@@ -140,7 +140,8 @@ typedef struct {
   int32_t n_slots;
   /* proposals a request has drafted in this round, position-major:
    * proposal j of request b at proposals[j * n_requests + b] (at most 64).
-   * Row i of a request sees the first first_proposal + i of them as said. */
+   * Row i of a request sees the first first_proposal + i of them as said;
+   * those that no row sees are not read. */
   int32_t n_proposals;
   const int32_t* proposals;
   int32_t first_proposal;
@@ -416,6 +417,34 @@ MS_API int ms_lora_add(const void* x, int64_t x_stride, const float* base, int64
                        int n_slices, const int32_t* slice_cols, int interleaved, int swiglu,
                        const ms_lora_adapters* adapters, const ms_lora_plan* plan, int dtype,
                        int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The adapters of a whole model: per projection, host arrays [n_layers] of
+ * device pointers (an array may be null, or an entry: no adapter there).
+ * qkv and gate_up are laid out as the model's w_qkv (3 slices) and
+ * w_gate_up (interleaved). */
+typedef struct {
+  ms_lora_adapters adapters;
+  const void* const* a_qkv;
+  const void* const* b_qkv;
+  const void* const* a_o;
+  const void* const* b_o;
+  const void* const* a_gate_up;
+  const void* const* b_gate_up;
+  const void* const* a_down;
+  const void* const* b_down;
+} ms_lora_model;
+
+/* ms_forward for a batch whose tokens use adapters: plan covers the batch's
+ * n_tokens tokens (flat order).  lora == NULL or a plan of no tiles is ms_forward.
+ * The shared projections keep their GEMMs; qkv and gate/up leave them in
+ * float32 and meet the adapters' part before their one rounding. */
+MS_API size_t ms_forward_lora_workspace_size(const ms_model* model, const ms_lora_model* lora,
+                                             int max_tokens, int max_logit_rows);
+MS_API int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache, const ms_batch* batch,
+                           const ms_lora_model* lora, const ms_lora_plan* plan,
+                           const int32_t* logit_rows, int n_logit_rows, float* logits,
+                           int64_t logits_row_stride, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 /* ---- building blocks, exported for tests and for callers that compose
  *      their own forward ---------------------------------------------- */

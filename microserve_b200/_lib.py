@@ -151,6 +151,20 @@ class MsLoraPlan(ctypes.Structure):
     ]
 
 
+class MsLoraModel(ctypes.Structure):
+    _fields_ = [
+        ("adapters", MsLoraAdapters),
+        ("a_qkv", POINTER(c_void_p)),
+        ("b_qkv", POINTER(c_void_p)),
+        ("a_o", POINTER(c_void_p)),
+        ("b_o", POINTER(c_void_p)),
+        ("a_gate_up", POINTER(c_void_p)),
+        ("b_gate_up", POINTER(c_void_p)),
+        ("a_down", POINTER(c_void_p)),
+        ("b_down", POINTER(c_void_p)),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ms_version": (c_int, []),
@@ -213,6 +227,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [POINTER(MsModel), POINTER(MsKVCache), POINTER(MsBatch), c_void_p, c_int, c_void_p,
          c_int64, c_void_p],
+    ),
+    "ms_forward_lora_workspace_size": (
+        c_size_t, [POINTER(MsModel), POINTER(MsLoraModel), c_int, c_int]),
+    "ms_forward_lora": (
+        c_int,
+        [POINTER(MsModel), POINTER(MsKVCache), POINTER(MsBatch), POINTER(MsLoraModel),
+         POINTER(MsLoraPlan), c_void_p, c_int, c_void_p, c_int64, c_void_p, c_size_t, c_void_p],
     ),
     "ms_rmsnorm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int,
                            c_void_p]),

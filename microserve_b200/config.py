@@ -2,12 +2,13 @@
 
 Reference: src/microserve/config.py.  The same names, defaults and
 validation, so that an ``EngineConfig`` written for MicroServe loads here
-unchanged.  Two additions for the B200 path:
+unchanged.  Additions for the B200 path:
 
 * ``ModelConfig.n_kv_heads`` -- grouped-query attention (``None`` = one KV
   head per query head, the reference's multi-head attention);
 * ``ModelConfig.dtype`` -- weight/activation dtype of the device model
-  (``"float32"`` or ``"bfloat16"``); the KV cache must use the same dtype.
+  (``"float32"`` or ``"bfloat16"``); the KV cache must use the same dtype;
+* ``SamplingConfig``'s penalties, biases and allowed tokens.
 
 ``EngineConfig.device`` defaults to ``"cuda"``: there is no CPU compute path.
 """
@@ -15,9 +16,12 @@ unchanged.  Two additions for the B200 path:
 from __future__ import annotations
 
 import json
+from collections.abc import Callable
 from dataclasses import asdict, dataclass, field, fields
 from pathlib import Path
 from typing import Any
+
+import numpy as np
 
 _DTYPES = ("float32", "bfloat16")
 
@@ -139,10 +143,32 @@ class SamplingConfig:
     max_new_tokens: int = 32
     seed: int | None = None
     stop_token: int | None = None
+    # Additions: controls on the request's logits before each draw (see
+    # logits.py).  Tokens of the prompt or generated so far have positive
+    # logits divided and negative ones multiplied by ``repetition_penalty``;
+    # generated tokens lose ``frequency_penalty`` per occurrence and
+    # ``presence_penalty`` once; ``logit_bias`` adds to single tokens;
+    # ``allowed_tokens`` maps the tokens generated so far to the tokens allowed
+    # next: a bool array over the vocabulary, or None for all of them.
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: dict[int, float] | None = None
+    allowed_tokens: Callable[[list[int]], np.ndarray | None] | None = None
 
     @property
     def greedy(self) -> bool:
         return self.temperature == 0.0
+
+    @property
+    def penalised(self) -> bool:
+        return (self.repetition_penalty != 1.0 or self.presence_penalty != 0.0
+                or self.frequency_penalty != 0.0)
+
+    @property
+    def controlled(self) -> bool:
+        """Whether anything changes this request's logits before a draw."""
+        return self.penalised or bool(self.logit_bias) or self.allowed_tokens is not None
 
 
 @dataclass

@@ -4,8 +4,12 @@
 //                     -> norm -> gate/up GEMM+SwiGLU -> down GEMM+res -> norm]
 //   -> final norm on the requested rows -> tied lm_head GEMM (float32 logits)
 // The residual stream stays float32; GEMM inputs are in the model dtype.
+// Tokens with a low-rank adapter: the qkv and gate/up GEMMs store float32, the
+// adapters' part is added (with the SwiGLU, or before RoPE + KV write) and the
+// sum rounded once; after the O and down GEMMs it is added to the residual.
 #include "common.cuh"
 #include "gemm.cuh"
+#include "lora.cuh"
 #include "model_kernels.cuh"
 
 namespace ms {
@@ -21,10 +25,14 @@ struct Workspace {
   void* h;       // (T, d_ff)
   void* xl;      // (R, d) final-normed logit rows
   int32_t* order;  // (T) attention schedule order of the sequences
+  float* y;        // (T, max(qkv width, 2 d_ff)) float32 projection (with adapters)
+  void* lora;      // the adapters' scratch
+  size_t lora_bytes;
   size_t bytes;
 };
 
-Workspace carve(const ms_model& m, int T, int R, unsigned char* base) {
+// `lora_rank` > 0: also what the adapters need, for ranks up to it.
+Workspace carve(const ms_model& m, int T, int R, unsigned char* base, int lora_rank = 0) {
   const size_t es = m.dtype == MS_DTYPE_BF16 ? 2 : 4;
   const size_t qkv_w = (size_t)(m.n_heads + 2 * m.n_kv_heads) * m.d_head;
   Workspace w{};
@@ -41,6 +49,12 @@ Workspace carve(const ms_model& m, int T, int R, unsigned char* base) {
   w.h = take((size_t)T * m.d_ff * es);
   w.xl = take((size_t)(R > 0 ? R : 1) * m.d_model * es);
   w.order = reinterpret_cast<int32_t*>(take((size_t)(T > 0 ? T : 1) * 4));
+  if (lora_rank > 0) {
+    const size_t wide = qkv_w > (size_t)2 * m.d_ff ? qkv_w : (size_t)2 * m.d_ff;
+    w.y = reinterpret_cast<float*>(take((size_t)T * wide * 4));
+    w.lora_bytes = lora_workspace_size(T, 3, lora_rank);
+    w.lora = take(w.lora_bytes);
+  }
   w.bytes = off;
   return w;
 }
@@ -71,10 +85,25 @@ extern "C" size_t ms_forward_workspace_size(const ms_model* model, int max_token
   return carve(*model, max_tokens, max_logit_rows, nullptr).bytes;
 }
 
+extern "C" size_t ms_forward_lora_workspace_size(const ms_model* model, const ms_lora_model* lora,
+                                                 int max_tokens, int max_logit_rows) {
+  if (model == nullptr || max_tokens < 0) return 0;
+  return carve(*model, max_tokens, max_logit_rows, nullptr, lora ? lora->adapters.max_rank : 0).bytes;
+}
+
 extern "C" int ms_forward(const ms_model* model, const ms_kv_cache* cache, const ms_batch* batch,
                           const int32_t* logit_rows, int n_logit_rows, float* logits,
                           int64_t logits_row_stride, void* workspace, size_t workspace_bytes,
                           void* stream) {
+  return ms_forward_lora(model, cache, batch, nullptr, nullptr, logit_rows, n_logit_rows, logits,
+                         logits_row_stride, workspace, workspace_bytes, stream);
+}
+
+extern "C" int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache,
+                               const ms_batch* batch, const ms_lora_model* lora,
+                               const ms_lora_plan* plan, const int32_t* logit_rows,
+                               int n_logit_rows, float* logits, int64_t logits_row_stride,
+                               void* workspace, size_t workspace_bytes, void* stream) {
   MS_TRY(validate_model(model));
   MS_TRY(validate_cache(cache, 0));
   MS_REQUIRE(batch != nullptr, "ms_forward: null batch");
@@ -92,7 +121,15 @@ extern "C" int ms_forward(const ms_model* model, const ms_kv_cache* cache, const
   const int T = bt.n_tokens;
   const int R = logit_rows ? n_logit_rows : T;
   MS_REQUIRE(R >= 0 && (R == 0 || logits), "ms_forward: logits output missing");
-  const Workspace w = carve(m, T, R, static_cast<unsigned char*>(workspace));
+  const bool adapted = lora != nullptr && plan != nullptr && plan->n_tiles > 0 &&
+                       lora->adapters.max_rank > 0;
+  if (adapted) {
+    MS_TRY(validate_lora(&lora->adapters, plan));
+    MS_REQUIRE(plan->n_tokens == T, "ms_forward_lora: the plan has %d tokens, the batch %d",
+               plan->n_tokens, T);
+  }
+  const Workspace w = carve(m, T, R, static_cast<unsigned char*>(workspace),
+                            adapted ? lora->adapters.max_rank : 0);
   MS_REQUIRE(workspace != nullptr && workspace_bytes >= w.bytes,
              "ms_forward: workspace too small (%zu < %zu)", workspace_bytes, w.bytes);
   cudaStream_t s = as_stream(stream);
@@ -102,6 +139,30 @@ extern "C" int ms_forward(const ms_model* model, const ms_kv_cache* cache, const
   // workspace past the carve is scratch for the attention's split-KV partials
   void* attn_scratch = static_cast<unsigned char*>(workspace) + w.bytes;
   const size_t attn_scratch_bytes = workspace_bytes - w.bytes;
+
+  // The adapters' part of one projection, if the layer has any: a, b its entries.
+  auto entry = [&](const void* const* arr, int l) { return adapted && arr ? arr[l] : nullptr; };
+  auto add_adapters = [&](const void* a, const void* b, const void* x, int K, const float* base,
+                          int N, void* out, int out_dtype, int n_slices, bool gate_up) {
+    LoraCall c{};
+    c.x = x;
+    c.x_stride = K;
+    c.base = base;
+    c.base_stride = N;
+    c.out = out;
+    c.out_stride = gate_up ? N / 2 : N;
+    c.a = a;
+    c.b = b;
+    c.K = K;
+    c.N = N;
+    c.n_slices = n_slices;
+    c.slice_end[0] = hq * dh;
+    c.slice_end[1] = (hq + hkv) * dh;
+    c.interleaved = c.swiglu = gate_up;
+    c.dtype = dt;
+    c.out_dtype = out_dtype;
+    return lora_add(c, lora->adapters, *plan, w.lora, w.lora_bytes, s);
+  };
 
   // Longest sequences first in every layer's attention grid (one sort per pass).
   const int32_t* order = nullptr;
@@ -114,8 +175,12 @@ extern "C" int ms_forward(const ms_model* model, const ms_kv_cache* cache, const
   for (int l = 0; l < m.n_layers; ++l) {
     // q, k, v projection with RoPE and the cache write in the GEMM's epilogue
     // (bf16 tensor-core shapes), else the projection and then rope_kv_write.
+    const void* qkv_a = entry(lora ? lora->a_qkv : nullptr, l);
+    const void* o_a = entry(lora ? lora->a_o : nullptr, l);
+    const void* gate_up_a = entry(lora ? lora->a_gate_up : nullptr, l);
+    const void* down_a = entry(lora ? lora->a_down : nullptr, l);
     int rc = MS_ERR_UNSUPPORTED;
-    if (dt == MS_DTYPE_BF16) {
+    if (dt == MS_DTYPE_BF16 && !qkv_a) {
       const RopeKv rk{bt.positions, bt.slot_mapping, m.rope_cos, m.rope_sin, m.max_seq_len, hq,
                       hkv, dh, c.block_size, c.num_blocks,
                       static_cast<__nv_bfloat16*>(c.k_pool[l]),
@@ -123,8 +188,14 @@ extern "C" int ms_forward(const ms_model* model, const ms_kv_cache* cache, const
       rc = gemm_qkv_rope(w.xn, m.w_qkv[l], w.qkv, T, qkv_w, d, rk, s, true);
     }
     if (rc == MS_ERR_UNSUPPORTED) {
-      MS_TRY(gemm_dispatch(w.xn, m.w_qkv[l], w.qkv, nullptr, T, qkv_w, d, 0, dt, dt, kEpiStore, s,
-                           true));
+      if (qkv_a) {
+        MS_TRY(gemm_dispatch(w.xn, m.w_qkv[l], w.y, nullptr, T, qkv_w, d, 0, dt, MS_DTYPE_F32,
+                             kEpiStore, s, true));
+        MS_TRY(add_adapters(qkv_a, lora->b_qkv[l], w.xn, d, w.y, qkv_w, w.qkv, dt, 3, false));
+      } else {
+        MS_TRY(gemm_dispatch(w.xn, m.w_qkv[l], w.qkv, nullptr, T, qkv_w, d, 0, dt, dt, kEpiStore,
+                             s, true));
+      }
       MS_TRY(rope_kv_write(w.qkv, bt.positions, bt.slot_mapping, m.rope_cos, m.rope_sin,
                            m.max_seq_len, T, hq, hkv, dh, c, l, dt, s));
     } else {
@@ -135,11 +206,21 @@ extern "C" int ms_forward(const ms_model* model, const ms_kv_cache* cache, const
                            s, order));
     MS_TRY(gemm_dispatch(w.attn, m.w_o[l], w.x, w.x, T, d, hq * dh, 0, dt, MS_DTYPE_F32,
                          kEpiResidual, s, true));
+    if (o_a)
+      MS_TRY(add_adapters(o_a, lora->b_o[l], w.attn, hq * dh, w.x, d, w.x, MS_DTYPE_F32, 1, false));
     MS_TRY(rmsnorm(w.x, m.ffn_norm[l], w.xn, nullptr, T, d, m.norm_eps, dt, s, true));
-    MS_TRY(gemm_dispatch(w.xn, m.w_gate_up[l], w.h, nullptr, T, 2 * m.d_ff, d, 0, dt, dt,
-                         kEpiSwiGLU, s, true));
+    if (gate_up_a) {
+      MS_TRY(gemm_dispatch(w.xn, m.w_gate_up[l], w.y, nullptr, T, 2 * m.d_ff, d, 0, dt,
+                           MS_DTYPE_F32, kEpiStore, s, true));
+      MS_TRY(add_adapters(gate_up_a, lora->b_gate_up[l], w.xn, d, w.y, 2 * m.d_ff, w.h, dt, 2, true));
+    } else {
+      MS_TRY(gemm_dispatch(w.xn, m.w_gate_up[l], w.h, nullptr, T, 2 * m.d_ff, d, 0, dt, dt,
+                           kEpiSwiGLU, s, true));
+    }
     MS_TRY(gemm_dispatch(w.h, m.w_down[l], w.x, w.x, T, d, m.d_ff, 0, dt, MS_DTYPE_F32,
                          kEpiResidual, s, true));
+    if (down_a)
+      MS_TRY(add_adapters(down_a, lora->b_down[l], w.h, m.d_ff, w.x, d, w.x, MS_DTYPE_F32, 1, false));
     if (l + 1 < m.n_layers)
       MS_TRY(rmsnorm(w.x, m.attn_norm[l + 1], w.xn, nullptr, T, d, m.norm_eps, dt, s, true));
   }

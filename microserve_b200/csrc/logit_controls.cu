@@ -137,7 +137,8 @@ __device__ void load_slice(const ControlArgs& a, int b, int slot, int64_t row0, 
   int at = seen ? atomicAdd(&sl.n_list, __popc(seen)) : 0;
   for (uint32_t m = seen; m; m &= m - 1)
     sl.list[at++] = (uint16_t)((32 * tid + __ffs(m) - 1) | 1 << 12);
-  if (slot >= 0 && c.proposals && tid < c.n_proposals) {
+  // those that the last row sees; the others may not have been drawn yet
+  if (slot >= 0 && c.proposals && tid < c.first_proposal + a.rows - 1) {
     const int v = c.proposals[(int64_t)tid * a.n_requests + b];
     if (v < 0 || v >= a.vocab) {
       raise_device_error(a.err, kErrToken);

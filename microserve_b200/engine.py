@@ -21,6 +21,12 @@ draws on the device, and reads the tokens back in one copy; the speculative
 round is ``SpeculativeDecoder.step`` (three uploads, one read-back).
 ``_commit`` then applies the stop rules to each request's tokens in one
 slice (``Request.extend_until_stop``).
+
+A request may bring logit controls (``SamplingConfig`` penalties, biases and
+allowed tokens) and the name of a low-rank adapter loaded beside the model
+(``add_request(adapter=...)``); both work inside the shared batch.  While a
+scheduled request restricts its tokens (``allowed_tokens`` asks the host between
+tokens), the iteration is an ordinary pass.
 """
 
 from __future__ import annotations
@@ -38,6 +44,8 @@ from . import _lib
 from .batching import HostStaging, batch_from_host, host_batch_arrays, pack_int32
 from .cache import OutOfCacheMemory, PagedKVCache
 from .config import CacheConfig, EngineConfig, SamplingConfig
+from .logits import RequestControls, apply_logit_controls
+from .lora import LoraPlan
 from .model import PagedBatch, Transformer
 from .sampling import make_params, validate
 from .scheduler import Request, RequestStatus, Scheduler, SchedulerOutput
@@ -123,6 +131,7 @@ class LLMEngine:
         self.cache = PagedKVCache(model.cfg, self._cache_cfg, self.device)
         self.stats = EngineStats()
         self._generators: dict[int, torch.Generator] = {}
+        self._adapter_of: dict[int, str] = {}  # unfinished requests with an adapter
         self._meta_upload = HostStaging(self.device)
         self._param_upload = HostStaging(self.device)
         self._q_start = np.zeros(1, dtype=np.int32)  # the last built pass's row offsets
@@ -136,6 +145,10 @@ class LLMEngine:
                                            cache_cfg=self._cache_cfg,
                                            gamma=self.config.speculative.gamma,
                                            device=self.device)
+        # one set of token counts, whichever kind of pass draws
+        self.controls = (self.spec.controls if self.spec is not None
+                         else RequestControls(model.cfg.vocab_size, self.device))
+        self._lora_upload = HostStaging(self.device)
         self.scheduler = self._new_scheduler()
 
     def _new_scheduler(self) -> Scheduler:
@@ -151,12 +164,15 @@ class LLMEngine:
         sampling: SamplingConfig | None = None,
         request_id: int | None = None,
         arrival_time: float | None = None,
+        adapter: str | None = None,
     ) -> Request:
-        """Queue a request given token ids (or text, with a tokenizer).
+        """Queue a request given token ids (or text, with a tokenizer), to be served with the
+        model's weights plus ``adapter``, one of ``model.adapters``.
 
         Raises ``ValueError`` for an empty prompt, text without a tokenizer,
-        invalid sampling settings, a prompt plus budget beyond
-        ``max_seq_len``, or a request the whole pool could never hold."""
+        invalid sampling settings, an adapter that is not loaded, a prompt
+        plus budget beyond ``max_seq_len``, or a request the whole pool could
+        never hold."""
         if isinstance(prompt_ids, str):
             if self.tokenizer is None:
                 raise ValueError("text prompts need a tokenizer")
@@ -166,6 +182,10 @@ class LLMEngine:
             raise ValueError("prompt must contain at least one token")
         sampling = sampling if sampling is not None else SamplingConfig()
         validate(sampling)
+        self.controls.check(sampling)
+        if adapter is not None and (self.model.adapters is None
+                                    or adapter not in self.model.adapters):
+            raise ValueError(f"no adapter {adapter!r} is loaded")
         # the id is taken before the length checks, so a refused request
         # consumes one as in the reference (later seeds depend on it)
         rid = request_id if request_id is not None else self.scheduler.next_request_id()
@@ -179,7 +199,20 @@ class LLMEngine:
         seed = sampling.seed if sampling.seed is not None else self.config.seed + rid
         self._generators[rid] = torch.Generator().manual_seed(seed)
         arrived = arrival_time if arrival_time is not None else self.clock()
-        return self.scheduler.add(Request(rid, ids, sampling, arrival_time=arrived))
+        request = self.scheduler.add(Request(rid, ids, sampling, arrival_time=arrived,
+                                             adapter=adapter))
+        if adapter is not None:
+            assert self.model.adapters is not None
+            self.model.adapters.acquire(adapter)
+            self._adapter_of[rid] = adapter
+        return request
+
+    def _release(self, request_id: int) -> None:
+        """A finished request lets go of its token counts and its adapter."""
+        self.controls.free(request_id)
+        adapter = self._adapter_of.pop(request_id, None)
+        if adapter is not None and self.model.adapters is not None:
+            self.model.adapters.release(adapter)
 
     @property
     def has_unfinished(self) -> bool:
@@ -212,8 +245,10 @@ class LLMEngine:
 
     def _round_fits(self, plan: SchedulerOutput) -> bool:
         """A speculative round needs every request decoding (one uncomputed
-        token) and room for gamma + 1 tokens per request."""
-        if self.spec is None:
+        token), room for gamma + 1 tokens per request, and no request whose
+        allowed tokens the host has to name one token at a time."""
+        if self.spec is None or any(r.sampling.allowed_tokens is not None
+                                    for r in plan.scheduled):
             return False
         width = self.config.speculative.gamma + 1
         return all(not r.is_prefill and self.cache.can_append(r.request_id, width)
@@ -232,6 +267,7 @@ class LLMEngine:
                 self.scheduler.finish(request, now)
                 if self.spec is not None:
                     self.spec.free(request.request_id)
+                self._release(request.request_id)
                 done.append(self.make_output(request))
         self.stats.record_step(len(batch), self.cache.utilization)
         return done
@@ -242,11 +278,15 @@ class LLMEngine:
         whose tokens are now all computed (reference engine.py:204-220).  A
         request whose prefill continues in a later chunk draws nothing and
         keeps its round counter, so its stream equals the unchunked one."""
+        # asked for before anything changes: a refused mask leaves the step undone
+        drawing = [r for r in batch if self.scheduler.step_len(r) == r.num_uncomputed]
+        masks = self.controls.masks_of(drawing)
         meta = self.build_batch(batch)
+        lora = self._lora_plan(batch)
         done = [i for i, r in enumerate(batch) if r.num_uncomputed == 0]
         out: list[list[int]] = [[] for _ in batch]
         if not done:
-            self.model.forward_paged(meta, self.cache, logit_rows=self._no_rows)  # K/V only
+            self.model.forward_paged(meta, self.cache, logit_rows=self._no_rows, lora=lora)  # K/V only
             return out
         fin = [batch[i] for i in done]
         last_rows = (self._q_start[1:] - 1).astype(np.int32)[done]
@@ -256,17 +296,35 @@ class LLMEngine:
         dev = self._param_upload.upload(blob)
         (p_off, _), (r_off, r_len) = spans
         rows = dev[r_off : r_off + r_len]
-        logits = self.model.forward_paged(meta, self.cache, logit_rows=rows)
+        logits = self.model.forward_paged(meta, self.cache, logit_rows=rows, lora=lora)
+        controls = self.controls.prepare(fin, masks)
+        if controls is not None:
+            apply_logit_controls(logits, controls, self.controls.counts, out=logits)
         V = self.model.cfg.vocab_size
         drawn = torch.empty(len(fin), dtype=torch.int32, device=self.device)
         _lib.call("ms_sample", logits.data_ptr(), V, len(fin), V, dev[p_off:].data_ptr(), None,
                   _lib.LANE_SAMPLE, drawn.data_ptr(), None, None, None, None,
                   _lib.stream_ptr(self.device))
+        if controls is not None:
+            self.controls.drew(controls, drawn.view(-1, 1))
+            self.controls.confirm(fin, [1] * len(fin))
         for r in fin:
             r.rng_step += 1
         for i, t in zip(done, drawn.cpu().tolist(), strict=True):
             out[i] = [t]
         return out
+
+    def _lora_plan(self, batch: list[Request]) -> LoraPlan | None:
+        """The adapters of the pass that ``build_batch`` has just laid out (None: no request has one)."""
+        if all(r.adapter is None for r in batch):
+            return None
+        assert self.model.adapters is not None
+        ids = self.model.adapters.ids_of_tokens((r.adapter for r in batch), np.diff(self._q_start))
+        order, tiles = LoraPlan.host_arrays(ids)
+        blob, spans = pack_int32([tiles, order])  # the tiles on 16 bytes
+        dev = self._lora_upload.upload(blob)
+        (t0, tn), (o0, on) = spans
+        return LoraPlan(dev[o0 : o0 + on], dev[t0 : t0 + tn].view(-1, 4))
 
     def build_batch(self, batch: list[Request]) -> PagedBatch:
         """Reserve cache slots for every request's uncomputed tokens and upload
@@ -326,9 +384,10 @@ class LLMEngine:
         self,
         prompts: Sequence[str] | Sequence[Sequence[int]],
         sampling: SamplingConfig | None = None,
+        adapter: str | None = None,
     ) -> list[RequestOutput]:
         """Queue every prompt, run to completion, return outputs in prompt order."""
-        order = [self.add_request(p, sampling).request_id for p in prompts]
+        order = [self.add_request(p, sampling, adapter=adapter).request_id for p in prompts]
         by_id = {o.request_id: o for o in self.run()}
         return [by_id[i] for i in order]
 
@@ -337,6 +396,9 @@ class LLMEngine:
         self.cache.reset()
         if self.spec is not None:
             self.spec.reset()
+        for rid in list(self._adapter_of):
+            self._release(rid)
+        self.controls.reset()
         self.scheduler = self._new_scheduler()
         self.stats = EngineStats()
         self._generators.clear()

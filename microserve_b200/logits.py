@@ -33,6 +33,7 @@ from . import _lib
 from .batching import HostStaging, pack_int32
 
 if TYPE_CHECKING:
+    from .config import SamplingConfig
     from .scheduler import Request
 
 MAX_PROPOSALS = 64
@@ -225,3 +226,163 @@ def apply_logit_controls(
     _lib.launch_on(dev, "ms_apply_logit_controls", logits.data_ptr(), logits.stride(0),
                    out.data_ptr(), out.stride(0), B, rows_per_request, vocab, ctypes.byref(s))
     return out
+
+
+class RequestControls:
+    """The controls of live requests, kept between steps (host side of the engine and of the
+    speculative decoder).
+
+    Each request with penalties holds a slot of a :class:`TokenCounts`, from its
+    first step until :meth:`free`; the slots grow by doubling.  ``prepare``
+    brings a batch's controls to the device; after its draws, ``drew`` counts
+    the new tokens there, and ``confirm`` tells the host how many they were.  A
+    request whose token lists do not have the length that was counted (its
+    first step, or a caller that changed them) is counted afresh.
+    """
+
+    def __init__(self, vocab_size: int, device: torch.device) -> None:
+        self.vocab_size = vocab_size
+        self.device = device
+        self.counts: TokenCounts | None = None
+        self.version = 0  # of the uploaded controls: each prepare replaces them
+        self._slot: dict[int, int] = {}
+        self._counted: dict[int, int] = {}  # tokens counted, prompt included
+        self._free: list[int] = []
+        self._upload = HostStaging(device)
+        self._recount_upload = HostStaging(device)
+
+    def check(self, sampling: SamplingConfig) -> None:
+        """Raise ``ValueError`` for biases of no token, or that are no number or +inf."""
+        if sampling.logit_bias:
+            self._check_bias(np.array(list(sampling.logit_bias)),
+                             np.array(list(sampling.logit_bias.values()), np.float32))
+
+    def _check_bias(self, ids: np.ndarray, values: np.ndarray) -> None:
+        if ids.dtype.kind not in "iu" or ids.min() < 0 or ids.max() >= self.vocab_size:
+            raise ValueError("logit_bias names a token outside the vocabulary")
+        if not np.all(values < np.inf):
+            raise ValueError("logit_bias values must be numbers below +inf")  # -inf bans a token
+
+    @staticmethod
+    def wanted(requests: Sequence[Request]) -> bool:
+        return any(r.sampling.controlled for r in requests)
+
+    def masks_of(self, requests: Sequence[Request]) -> dict[int, np.ndarray]:
+        """The allowed tokens of the requests that restrict them, by index.  Raises ``ValueError``
+        for an array of the wrong shape or one that allows nothing."""
+        out: dict[int, np.ndarray] = {}
+        for i, r in enumerate(requests):
+            if r.sampling.allowed_tokens is None:
+                continue
+            got = r.sampling.allowed_tokens(list(r.output_ids))
+            if got is None:
+                continue
+            allowed = np.asarray(got)
+            if allowed.shape != (self.vocab_size,) or allowed.dtype != np.bool_:
+                raise ValueError(f"request {r.request_id}: allowed_tokens must give a bool array of "
+                                 f"{self.vocab_size} entries")
+            if not allowed.any():
+                raise ValueError(f"request {r.request_id}: allowed_tokens allows no token")
+            out[i] = allowed
+        return out
+
+    # -- token counts ------------------------------------------------------------
+    def _grow(self, n: int) -> None:
+        old = self.counts
+        have = 0 if old is None else old.n_slots
+        if len(self._free) >= n:
+            return
+        want = max(have + n - len(self._free), 2 * have)
+        new = TokenCounts.empty(want, self.vocab_size, self.device)
+        if old is not None:
+            new.counts[:have].copy_(old.counts)
+            new.seen[:have].copy_(old.seen)
+        self._free += range(have, want)
+        self.counts = new
+
+    def _recount(self, requests: list[Request]) -> None:
+        """Count the requests' tokens from the start."""
+        slots = np.array([self._slot[r.request_id] for r in requests], np.int32)
+        lens = np.array([r.num_tokens for r in requests], np.int32)
+        prompts = np.array([len(r.prompt_ids) for r in requests], np.int32)
+        start = (np.cumsum(lens, dtype=np.int64) - lens).view(np.int32)
+        tokens = np.fromiter((t for r in requests for t in r.all_ids), np.int32, int(lens.sum()))
+        blob, spans = pack_int32([start, slots, lens, prompts, tokens])
+        dev = self._recount_upload.upload(blob)
+        st, sl, ln, pr, tk = (dev[o : o + n] for o, n in spans)
+        assert self.counts is not None
+        self.counts.reset(sl)
+        self.counts.append(sl, tk, ln, row_start=st.view(torch.int64), max_len=int(lens.max()),
+                           n_prompt=pr)
+        for r in requests:
+            self._counted[r.request_id] = r.num_tokens
+
+    def prepare(self, requests: Sequence[Request],
+                masks: dict[int, np.ndarray] | None = None) -> LogitControls | None:
+        """The batch's controls on the device (None: nothing to control), with ``masks`` (one
+        row per request, from :meth:`masks_of`)."""
+        if not self.wanted(requests):
+            return None
+        self.version += 1
+        B = len(requests)
+        parts: dict[str, np.ndarray] = {}
+        if any(r.sampling.logit_bias for r in requests):
+            lists = [sorted((r.sampling.logit_bias or {}).items()) for r in requests]
+            ids = np.array([v for x in lists for v, _ in x])
+            values = np.array([b for x in lists for _, b in x], np.float32)
+            self._check_bias(ids, values)
+            parts["bias_start"] = np.cumsum([0] + [len(x) for x in lists]).astype(np.int32)
+            parts["bias_ids"] = ids.astype(np.int32)
+            parts["bias_values"] = values.view(np.int32)
+        pen = [r for r in requests if r.sampling.penalised]
+        if pen:
+            new = [r for r in pen if r.request_id not in self._slot]
+            self._grow(len(new))
+            for r in new:
+                self._slot[r.request_id] = self._free.pop()
+            stale = [r for r in pen if self._counted.get(r.request_id) != r.num_tokens]
+            if stale:
+                self._recount(stale)
+        if masks:
+            parts["masks"] = pack_masks(np.stack([masks[i] for i in sorted(masks)]))
+            rows = np.full(B, -1, np.int32)
+            rows[sorted(masks)] = np.arange(len(masks))
+            parts["mask_rows"] = rows
+        if pen:
+            parts["slots"] = np.array([self._slot[r.request_id] if r.sampling.penalised else -1
+                                       for r in requests], np.int32)
+            p = np.array([(s.repetition_penalty, s.presence_penalty, s.frequency_penalty)
+                          for s in (r.sampling for r in requests)], np.float32)
+            parts["penalties"] = p.view(np.int32)
+        if not parts:  # allowed_tokens alone, and every one of them allowed everything
+            return None
+        blob, spans = pack_int32(list(parts.values()))
+        dev = self._upload.upload(blob)
+        t = {k: dev[o : o + n].view(parts[k].shape) for k, (o, n) in zip(parts, spans)}
+        for k in ("penalties", "bias_values"):
+            if k in t:
+                t[k] = t[k].view(torch.float32)
+        return LogitControls(**t)
+
+    def drew(self, controls: LogitControls | None, tokens: torch.Tensor,
+             lens: torch.Tensor | None = None, len_add: int = 0) -> None:
+        """Count the drawn tokens, (B, width) with ``lens + len_add`` valid ones per request."""
+        if controls is not None and controls.slots is not None:
+            assert self.counts is not None
+            self.counts.append(controls.slots, tokens, lens, len_add)
+
+    def confirm(self, requests: Sequence[Request], drawn: Sequence[int]) -> None:
+        """The batch's requests are getting ``drawn`` new tokens each."""
+        for r, n in zip(requests, drawn, strict=True):
+            if r.request_id in self._counted:
+                self._counted[r.request_id] += int(n)
+
+    def free(self, request_id: int) -> None:
+        slot = self._slot.pop(request_id, None)
+        self._counted.pop(request_id, None)
+        if slot is not None:
+            self._free.append(slot)
+
+    def reset(self) -> None:
+        for rid in list(self._slot):
+            self.free(rid)

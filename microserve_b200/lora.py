@@ -16,13 +16,17 @@ read in whole lines.  ``n_slices`` is the number of projections fused into one
 from __future__ import annotations
 
 import ctypes
-from collections.abc import Sequence
+from collections.abc import Iterable, Mapping, Sequence
 from dataclasses import dataclass
+from typing import TYPE_CHECKING
 
 import numpy as np
 import torch
 
 from . import _lib
+
+if TYPE_CHECKING:
+    from .model import Transformer
 
 TILE = 64  # tokens of a plan's tile (MS_LORA_TILE)
 MAX_RANK = 256  # MS_LORA_MAX_RANK
@@ -79,6 +83,13 @@ class LoraPlan:
         dev = torch.device(device)
         return cls(torch.from_numpy(order).to(dev), torch.from_numpy(tiles).to(dev))
 
+    def c_struct(self, n_tokens: int, device: torch.device) -> _lib.MsLoraPlan:
+        index = torch.cuda.current_device() if device.index is None else device.index
+        n = self.tiles.shape[0]
+        return _lib.MsLoraPlan(
+            n_tokens, n, _check(self.order, "order", torch.int32, index, (n_tokens,)),
+            _check(self.tiles, "tiles", torch.int32, index, (n, 4)))
+
 
 def lora_add(
     x: torch.Tensor,
@@ -128,9 +139,7 @@ def lora_add(
     ad = _lib.MsLoraAdapters(n, R, proj.max_rank, 0, _check(proj.offsets, "offsets", i32, dev, (n,)),
                              _check(proj.ranks, "ranks", i32, dev, (n,)),
                              _check(proj.scales, "scales", torch.float32, dev, (n,)))
-    n_tiles = plan.tiles.shape[0]
-    pl = _lib.MsLoraPlan(T, n_tiles, _check(plan.order, "order", i32, dev, (T,)),
-                         _check(plan.tiles, "tiles", i32, dev, (n_tiles, 4)))
+    pl = plan.c_struct(T, x.device)
     width = N // 2 if swiglu else N
     if out is None:
         out = torch.empty((T, width), dtype=out_dtype, device=x.device)
@@ -150,3 +159,215 @@ def lora_add(
                    ctypes.addressof(cols), int(proj.interleaved), int(swiglu), ctypes.byref(ad),
                    ctypes.byref(pl), _CODES[dtype], _CODES[out.dtype], ws.data_ptr(), ws.numel())
     return out
+
+
+# fused projection -> (its parts' state-dict names, interleaved)
+_PROJECTIONS: dict[str, tuple[tuple[str, ...], bool]] = {
+    "qkv": (("attn.q_proj", "attn.k_proj", "attn.v_proj"), False),
+    "o": (("attn.o_proj",), False),
+    "gate_up": (("ffn.gate_proj", "ffn.up_proj"), True),
+    "down": (("ffn.down_proj",), False),
+}
+
+
+class LoraAdapters:
+    """The adapters loaded beside a :class:`Transformer`, by name.
+
+    ``load`` takes a state dict with, for any of the model's projections,
+    ``blocks.{i}.attn.q_proj.lora_A.weight`` (rank, in) and ``...lora_B.weight``
+    (out, rank), all of one rank; projections it does not name get nothing.
+    Adapters share one rank axis per projection, grown by doubling; ``unload``
+    frees an adapter's part of it and is refused while requests hold the
+    adapter (``acquire`` / ``release``, kept by the engine).  Loading writes the
+    weights on the current stream: call it from the stream that runs the model.
+    """
+
+    def __init__(self, model: Transformer, rank_capacity: int = 64) -> None:
+        if rank_capacity < 1:
+            raise ValueError("rank_capacity must be at least 1")
+        self.cfg, self.device, self.dtype = model.cfg, model.device, model.dtype
+        c = model.cfg
+        d, ff = c.d_model, c.ffn_hidden
+        q, kv = c.n_heads * c.d_head, c.kv_heads * c.d_head
+        # (inputs, column counts of the fused parts)
+        self._shape = {"qkv": (d, (q, kv, kv)), "o": (q, (d,)), "gate_up": (d, (ff, ff)),
+                       "down": (ff, (d,))}
+        self._capacity = rank_capacity
+        self._a: dict[str, list[torch.Tensor]] = {}
+        self._b: dict[str, list[torch.Tensor]] = {}
+        for name in self._shape:
+            self._a[name], self._b[name] = self._pools(name, rank_capacity)
+        self._ids: dict[str, int] = {}
+        self._offset: list[int] = []  # per id; rank 0: a free id
+        self._rank: list[int] = []
+        self._scale: list[float] = []
+        self._users: dict[str, int] = {}
+        self._uses: list[set[str]] = []  # the projections each id changes
+        self._c: _lib.MsLoraModel | None = None
+        model.adapters = self
+
+    def _pools(self, name: str, capacity: int) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
+        k, cols = self._shape[name]
+        z = lambda rows, width: torch.zeros((rows, width), dtype=self.dtype,  # noqa: E731
+                                            device=self.device)
+        n = range(self.cfg.n_layers)
+        return ([z(len(cols) * capacity, k) for _ in n], [z(capacity, sum(cols)) for _ in n])
+
+    # -- loading ----------------------------------------------------------------
+    @property
+    def names(self) -> list[str]:
+        return list(self._ids)
+
+    def __contains__(self, name: object) -> bool:
+        return name in self._ids
+
+    def _reserve(self, rank: int) -> int:
+        """The first gap of ``rank`` rows in the rank axis, growing it if there is none."""
+        used = sorted((o, r) for o, r in zip(self._offset, self._rank) if r)
+        at = 0
+        for o, r in used:
+            if o - at >= rank:
+                return at
+            at = o + r
+        if at + rank > self._capacity:
+            capacity = max(2 * self._capacity, at + rank)
+            for name in self._shape:
+                ns = len(self._shape[name][1])
+                for pool, new, per in zip((self._a[name], self._b[name]),
+                                          self._pools(name, capacity), (ns, 1)):
+                    for i, (old, fresh) in enumerate(zip(pool, new)):
+                        fresh[: per * self._capacity].copy_(old)
+                        pool[i] = fresh
+            self._capacity = capacity
+        return at
+
+    def load(self, name: str, state: Mapping[str, torch.Tensor], alpha: float | None = None) -> int:
+        """Add adapter ``name``; its part is scaled by ``alpha / rank`` (1 without ``alpha``).
+        Returns its id.  Nothing changes when the state dict is refused."""
+        if name in self._ids:
+            raise ValueError(f"adapter {name!r} is already loaded")
+        parts: dict[tuple[int, str], tuple[torch.Tensor, torch.Tensor]] = {}
+        left, rank = set(state), None
+        for i in range(self.cfg.n_layers):
+            for proj, (names, _) in _PROJECTIONS.items():
+                k, cols = self._shape[proj]
+                for part, n in zip(names, cols):
+                    key = f"blocks.{i}.{part}.lora_"
+                    ka, kb = key + "A.weight", key + "B.weight"
+                    if ka not in state and kb not in state:
+                        continue
+                    if ka not in state or kb not in state:
+                        raise ValueError(f"adapter {name!r}: {key}A and {key}B go together")
+                    a, b = (torch.as_tensor(state[x]) for x in (ka, kb))
+                    r = a.shape[0] if a.dim() == 2 else 0
+                    if rank is None:
+                        rank = r
+                    if a.shape != (r, k) or b.shape != (n, r) or r != rank:
+                        raise ValueError(f"adapter {name!r}: {key}A {tuple(a.shape)}, {key}B "
+                                         f"{tuple(b.shape)} do not fit ({rank}, {k}), ({n}, {rank})")
+                    parts[i, part] = (a, b)
+                    left -= {ka, kb}
+        if left:
+            raise ValueError(f"adapter {name!r}: unknown weights {sorted(left)[:3]}")
+        if rank is None or not 1 <= rank <= MAX_RANK:
+            raise ValueError(f"adapter {name!r}: rank {rank} is not in 1..{MAX_RANK}")
+        scale = 1.0 if alpha is None else float(alpha) / rank
+        if not np.isfinite(scale):
+            raise ValueError(f"adapter {name!r}: alpha {alpha}")
+        at = self._reserve(rank)
+        for i in range(self.cfg.n_layers):
+            for proj, (names, interleaved) in _PROJECTIONS.items():
+                k, cols = self._shape[proj]
+                ns = len(cols)
+                pa = self._a[proj][i][ns * at : ns * (at + rank)]
+                pb = self._b[proj][i][at : at + rank]
+                for j, part in enumerate(names):
+                    col0 = sum(cols[:j])
+                    dst = pb.view(rank, -1, ns, 8)[:, :, j] if interleaved else \
+                        pb[:, col0 : col0 + cols[j]]
+                    got = parts.get((i, part))
+                    if got is None:
+                        pa[j * rank : (j + 1) * rank].zero_()
+                        dst.zero_()
+                    else:
+                        pa[j * rank : (j + 1) * rank].copy_(got[0])
+                        dst.copy_(got[1].t().reshape(dst.shape))
+        free = [i for i, r in enumerate(self._rank) if r == 0]
+        if free:
+            i = free[0]
+        else:
+            i = len(self._rank)
+            self._offset.append(0)
+            self._rank.append(0)
+            self._scale.append(0.0)
+            self._uses.append(set())
+        self._uses[i] = {p for p, (names, _) in _PROJECTIONS.items()
+                         if any((layer, n) in parts for layer in range(self.cfg.n_layers)
+                                for n in names)}
+        self._offset[i], self._rank[i], self._scale[i] = at, rank, scale
+        self._ids[name] = i
+        self._users[name] = 0
+        self._c = None
+        return i
+
+    def unload(self, name: str) -> None:
+        """Forget an adapter that no request holds."""
+        if name not in self._ids:
+            raise ValueError(f"no adapter {name!r}")
+        if self._users[name]:
+            raise ValueError(f"adapter {name!r} is held by {self._users[name]} requests")
+        del self._users[name]
+        self._rank[self._ids.pop(name)] = 0
+        self._c = None
+
+    def acquire(self, name: str) -> None:
+        if name not in self._ids:
+            raise ValueError(f"no adapter {name!r} is loaded")
+        self._users[name] += 1
+
+    def release(self, name: str) -> None:
+        self._users[name] -= 1
+
+    # -- use ----------------------------------------------------------------------
+    def id_of(self, name: str | None) -> int:
+        """The id of an adapter (-1 for None)."""
+        if name is None:
+            return -1
+        if name not in self._ids:
+            raise ValueError(f"no adapter {name!r} is loaded")
+        return self._ids[name]
+
+    def ids_of_tokens(self, names: Iterable[str | None], lens: Sequence[int] | np.ndarray
+                      ) -> np.ndarray:
+        """Each token's adapter id, for sequences of ``lens`` tokens."""
+        ids = np.fromiter((self.id_of(n) for n in names), np.int64)
+        return np.repeat(ids, lens)
+
+    def plan(self, names: Iterable[str | None], lens: Sequence[int] | np.ndarray) -> LoraPlan:
+        """The plan of a batch whose sequence ``i`` has ``lens[i]`` tokens and adapter ``names[i]``."""
+        return LoraPlan.build(self.ids_of_tokens(names, lens), self.device)
+
+    def projection(self, name: str, layer: int) -> LoraProjection:
+        """One layer's ``"qkv"``, ``"o"``, ``"gate_up"`` or ``"down"`` for :func:`lora_add`."""
+        self.c_struct()
+        return LoraProjection(
+            a=self._a[name][layer], b=self._b[name][layer], offsets=self._d_offsets,
+            ranks=self._d_ranks, scales=self._d_scales, max_rank=max(self._rank, default=0),
+            slices=self._shape[name][1], interleaved=_PROJECTIONS[name][1])
+
+    def c_struct(self) -> _lib.MsLoraModel:
+        if self._c is None:
+            t = lambda v, d: torch.tensor(v, dtype=d).to(self.device)  # noqa: E731
+            self._d_offsets, self._d_ranks = t(self._offset, torch.int32), t(self._rank, torch.int32)
+            self._d_scales = t(self._scale, torch.float32)
+            head = _lib.MsLoraAdapters(len(self._rank), self._capacity, max(self._rank, default=0), 0,
+                                       self._d_offsets.data_ptr(), self._d_ranks.data_ptr(),
+                                       self._d_scales.data_ptr())
+            # a projection that no loaded adapter changes costs nothing
+            used = set().union(*(u for u, r in zip(self._uses, self._rank) if r))
+            self._arrays = [_lib.pointer_array(pool[name]) if name in used else None
+                            for name in self._shape for pool in (self._a, self._b)]
+            ptr = ctypes.POINTER(ctypes.c_void_p)
+            cast = lambda x: ptr() if x is None else ctypes.cast(x, ptr)  # noqa: E731
+            self._c = _lib.MsLoraModel(head, *map(cast, self._arrays))
+        return self._c

@@ -22,7 +22,7 @@ import ctypes
 import math
 from dataclasses import dataclass
 from pathlib import Path
-from typing import Any
+from typing import TYPE_CHECKING, Any
 
 import numpy as np
 import torch
@@ -30,6 +30,9 @@ import torch
 from . import _lib
 from .cache import PagedKVCache
 from .config import ModelConfig
+
+if TYPE_CHECKING:
+    from .lora import LoraAdapters, LoraPlan
 
 
 @dataclass
@@ -155,6 +158,7 @@ class Transformer:
         self.cfg = cfg
         self.dtype_code = _lib.DTYPE_CODES[cfg.dtype]
         self.dtype = _lib.TORCH_DTYPES[self.dtype_code]
+        self.adapters: LoraAdapters | None = None  # set by LoraAdapters(model)
         self._ws: torch.Tensor | None = None
         self._empty_rows: torch.Tensor | None = None
         if init:
@@ -300,11 +304,14 @@ class Transformer:
             self._empty_rows = torch.zeros(1, dtype=torch.int32, device=self.device)
         return self._empty_rows
 
-    def workspace(self, n_tokens: int, n_rows: int, attn_scratch: int = 0) -> torch.Tensor:
-        """Grow-only device workspace: ms_forward's carve plus ``attn_scratch``
-        bytes for the attention's split-KV partials."""
-        need = int(_lib.load().ms_forward_workspace_size(ctypes.byref(self._c_model), n_tokens,
-                                                           n_rows))
+    def workspace(self, n_tokens: int, n_rows: int, attn_scratch: int = 0,
+                  lora: _lib.MsLoraModel | None = None) -> torch.Tensor:
+        """Grow-only device workspace: the forward's carve (with the adapters' part for a
+        batch that uses them) plus ``attn_scratch`` bytes for the attention's split-KV
+        partials."""
+        need = int(_lib.load().ms_forward_lora_workspace_size(
+            ctypes.byref(self._c_model), None if lora is None else ctypes.byref(lora), n_tokens,
+            n_rows))
         need += attn_scratch
         if self._ws is None or self._ws.numel() < need:
             self._ws = torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
@@ -317,8 +324,12 @@ class Transformer:
         logit_rows: torch.Tensor | None = None,
         out: torch.Tensor | None = None,
         out_row_stride: int = 0,
+        lora: LoraPlan | None = None,
     ) -> torch.Tensor:
         """Paged forward; returns float32 logits ``(rows, vocab)``.
+
+        ``lora`` says which of :attr:`adapters` each token of the batch uses
+        (``adapters.plan``); None: the shared weights alone.
 
         ``logit_rows`` (int32, device) selects which flat token rows get
         logits (default: all, as the reference).  ``out`` may be a
@@ -339,6 +350,17 @@ class Transformer:
         cc = cache.c_struct()
         scratch = int(_lib.load().ms_attention_scratch_size(ctypes.byref(cc), self.cfg.n_heads,
                                                             ctypes.byref(cb)))
+        if lora is not None:
+            if self.adapters is None:
+                raise ValueError("the model has no adapters loaded")
+            cl, cp = self.adapters.c_struct(), lora.c_struct(batch.n_tokens, self.device)
+            ws = self.workspace(batch.n_tokens, n_rows, scratch, cl)
+            _lib.call(
+                "ms_forward_lora", ctypes.byref(self._c_model), ctypes.byref(cc),
+                ctypes.byref(cb), ctypes.byref(cl), ctypes.byref(cp), rows_ptr, n_rows, out_ptr,
+                out_row_stride, ws.data_ptr(), ws.numel(), _lib.stream_ptr(self.device),
+            )
+            return out
         ws = self.workspace(batch.n_tokens, n_rows, scratch)
         _lib.call(
             "ms_forward", ctypes.byref(self._c_model), ctypes.byref(cache.c_struct()),

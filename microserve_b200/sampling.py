@@ -16,6 +16,8 @@ uniforms, plus a chi-square test against the reference itself.
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import torch
 
@@ -45,6 +47,10 @@ def validate(cfg: SamplingConfig) -> None:
         raise ValueError("top_k must be positive")
     if cfg.top_p is not None and not 0.0 < cfg.top_p <= 1.0:
         raise ValueError("top_p must be in (0, 1]")
+    if not (0.0 < cfg.repetition_penalty < math.inf):
+        raise ValueError("repetition_penalty must be positive and finite")
+    if not (math.isfinite(cfg.presence_penalty) and math.isfinite(cfg.frequency_penalty)):
+        raise ValueError("presence_penalty and frequency_penalty must be finite")
 
 
 def params_to_device(params: np.ndarray, device: torch.device) -> torch.Tensor:

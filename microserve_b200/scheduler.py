@@ -74,6 +74,7 @@ class Request:
     num_draft_proposed: int = 0
     num_draft_accepted: int = 0
     rng_step: int = 0
+    adapter: str | None = None  # the low-rank adapter its tokens use (an addition)
 
     # -- tokens ------------------------------------------------------------
     @property

@@ -37,6 +37,8 @@ from . import _lib
 from .batching import HostStaging, batch_from_host, pack_int32
 from .cache import OutOfCacheMemory, PagedKVCache
 from .config import CacheConfig, SamplingConfig
+from .logits import LogitControls, RequestControls, apply_logit_controls
+from .lora import LoraPlan
 from .model import PagedBatch, Transformer
 from .sampling import generator_seed_and_step, make_params, validate
 from .scheduler import Request
@@ -201,6 +203,8 @@ class _RoundPlan:
     dev_blob_v: torch.Tensor | None = None
     v_slot: int = 0  # which of the decoder's two verify-blob buffers holds it
     target_cache: PagedKVCache | None = None
+    controls: LogitControls | None = None  # the requests' logit controls on the device
+    lora_spans: tuple[int, int] | None = None  # (order, tiles) parts of the verify blob
 
 
 @dataclass
@@ -220,6 +224,8 @@ class _Lookahead:
     params: torch.Tensor  # the next round's sampling parameters (device)
     idsv: torch.Tensor  # the next round's verify token ids (device)
     events: tuple[torch.cuda.Event, torch.cuda.Event] | None
+    controls: LogitControls | None = None
+    controls_version: int = 0  # the upload that `controls` views
     # filled once the round's results are read
     n_tok: np.ndarray = field(default_factory=_empty)  # token counts with the round's tokens
     last: list[int] = field(default_factory=list)  # last tokens then
@@ -244,7 +250,15 @@ class SpeculativeDecoder:
     seeds and target cache state); otherwise they are ignored and the round
     is planned on the host.  Draws are a function of (seed, round counter,
     lane), so the token streams are the same either way.  The target cache,
-    which the scheduler's admission reads, is never touched ahead of time."""
+    which the scheduler's admission reads, is never touched ahead of time.
+
+    Logit controls (penalties and biases of ``SamplingConfig``) apply to the
+    draft's and the target's logits alike: row i of a verify pass sees the
+    proposals before it as generated, and the tokens a round emits are counted
+    on the device right after the accept kernel, before a chained round's draft
+    passes.  ``allowed_tokens`` needs the host between tokens and is refused here
+    (the engine serves such requests with ordinary passes).  A request's
+    adapter applies to the target; the draft proposes with its shared weights."""
 
     def __init__(
         self,
@@ -297,6 +311,7 @@ class SpeculativeDecoder:
         self._pending: _Lookahead | None = None
         self._scat: torch.Tensor | None = None
         self._scat_key: tuple[int, int] | None = None
+        self.controls = RequestControls(target.cfg.vocab_size, self.device)
         self.lookahead_hits = 0
         self.lookahead_misses = 0
 
@@ -315,6 +330,12 @@ class SpeculativeDecoder:
         configs = list({id(r.sampling): r.sampling for r in requests}.values())
         for cfg in configs:
             validate(cfg)
+            if cfg.allowed_tokens is not None:
+                raise ValueError("allowed_tokens cannot be combined with a speculative round")
+        for r in requests:
+            if r.adapter is not None and (self.target.adapters is None
+                                          or r.adapter not in self.target.adapters):
+                raise ValueError(f"request {r.request_id}: no adapter {r.adapter!r} is loaded")
         launches0 = _lib.launch_count()
         ahead, self._pending = self._pending, None
         plan = None
@@ -325,7 +346,9 @@ class SpeculativeDecoder:
             else:
                 self.lookahead_misses += 1
         if plan is None:
+            controls = self.controls.prepare(requests)
             plan = self._plan(requests, target_cache, generators, configs)
+            plan.controls = controls
             ev = self._round_start_events()
             self._launch_draft(plan)
         chain = self.lookahead and self._no_request_can_stop(requests)
@@ -347,6 +370,8 @@ class SpeculativeDecoder:
         tokens = res[: B * (G + 1)].reshape(B, G + 1)
         nacc = res[B * (G + 1) : B * (G + 2)].astype(np.int64)
         results = self._finish(requests, target_cache, plan, tokens, nacc)
+        if plan.controls is not None:
+            self.controls.confirm(requests, nacc + 1)
         if self._pending is not None:
             la = self._pending
             la.n_tok = plan.n_tok + nacc + 1
@@ -404,6 +429,7 @@ class SpeculativeDecoder:
                                 context_lens=ctx[(j - 1) * B : j * B], q_lens=ones,
                                 q_start=unit_qs, max_q=1, n_tokens=B, max_context=max_ctx + j)
                 self.draft.forward_paged(bj, dc, out=out, out_row_stride=V)
+            self._control(plan.controls, out, 1, j)
             _lib.call("ms_sample", out.data_ptr(), V, B, V, params.data_ptr(), None,
                       _lib.LANE_DRAFT + j, buf.proposals[j].data_ptr(), None,
                       buf.dstats[j].data_ptr(), idsv.data_ptr(), scat[j].data_ptr(), stream)
@@ -412,7 +438,8 @@ class SpeculativeDecoder:
             ids=tuple(plan.ids), requests=plan.requests, gens=plan.gens, configs=plan.configs,
             samplings=[r.sampling for r in plan.requests],
             seeds=[g.initial_seed() for g in plan.gens], target_cache=plan.target_cache,
-            max_ctx=max_ctx, params=params, idsv=idsv, events=ev)
+            max_ctx=max_ctx, params=params, idsv=idsv, events=ev, controls=plan.controls,
+            controls_version=self.controls.version)
 
     def _chain_buffers(self, B: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Device buffers of the chained round: its metadata, its sampling
@@ -465,13 +492,24 @@ class SpeculativeDecoder:
         plan.qv, plan.segv, plan.withinv = qv, segv, withinv
         plan.kv_draft = int(n_tok.sum()) * G + B * (G - 1) * G // 2
         plan.dev_params, plan.dev_idsv = ahead.params, ahead.idsv
+        plan.controls = ahead.controls
         return plan
+
+    def _control(self, controls: LogitControls | None, logits: torch.Tensor, rows: int,
+                 said: int) -> None:
+        """Apply the requests' controls in place to ``rows`` rows each, the first of which
+        sees ``said`` of the round's proposals."""
+        if controls is not None:
+            apply_logit_controls(logits, controls, self.controls.counts, rows_per_request=rows,
+                                 proposals=self._buf.proposals, first_proposal=said, out=logits)
 
     def _lookahead_holds(self, ahead: _Lookahead, requests: list[Request],
                          target_cache: PagedKVCache,
                          generators: dict[int, torch.Generator]) -> bool:
         """Did the caller do what the lookahead assumed?"""
         if target_cache is not ahead.target_cache or len(requests) != len(ahead.ids):
+            return False
+        if ahead.controls is not None and self.controls.version != ahead.controls_version:
             return False
         for i, r in enumerate(requests):
             if r.request_id != ahead.ids[i] or r.sampling is not ahead.samplings[i]:
@@ -681,6 +719,14 @@ class SpeculativeDecoder:
             parts.append(np.concatenate([plan.n_tok.astype(np.int32), last.astype(np.int32),
                                          dtab.reshape(-1)]))
             plan.chain_span, plan.chain_dw = len(parts) - 1, dw
+        if any(r.adapter is not None for r in plan.requests):
+            assert self.target.adapters is not None  # checked in step
+            ids = self.target.adapters.ids_of_tokens((r.adapter for r in plan.requests), npre + G)
+            order, tiles = LoraPlan.host_arrays(ids)
+            # the tiles start on 16 bytes of the blob: pad the order before them
+            at = sum(int(np.asarray(p).size) for p in parts) + order.size
+            plan.lora_spans = (len(parts), len(parts) + 1)
+            parts += [np.concatenate([order, np.zeros(-at % 4, np.int32)]), tiles]
         blob, spans = pack_int32([np.ascontiguousarray(p).astype(np.int32, copy=False) for p in parts])
         plan.blob_v, plan.spans_v, plan.tw = blob, spans, tw
         plan.ctxv, plan.kv_verify = int(ctxv.max()), int(ctxv.sum())
@@ -731,6 +777,7 @@ class SpeculativeDecoder:
             out = buf.dlogits[j]
             if bj is not None:
                 self.draft.forward_paged(bj, self.draft_cache, out=out, out_row_stride=V)
+            self._control(plan.controls, out, 1, j)
             _lib.call(
                 "ms_sample", out.data_ptr(), V, B, V, params.data_ptr(), None, _lib.LANE_DRAFT + j,
                 buf.proposals[j].data_ptr(), None, buf.dstats[j].data_ptr(),
@@ -776,16 +823,23 @@ class SpeculativeDecoder:
         if self.verify_events is not None:
             vev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
             vev[0].record()
+        lora = None
+        if plan.lora_spans is not None:
+            order, tiles = (w[i] for i in plan.lora_spans)
+            lora = LoraPlan(order[: plan.Tv], tiles.view(-1, 4))
         self.target.forward_paged(bv, target_cache, logit_rows=rowsv, out=buf.vlogits,
-                                  out_row_stride=V)
+                                  out_row_stride=V, lora=lora)
         if vev is not None and self.verify_events is not None:
             vev[1].record()
             self.verify_events.append(vev)
+        self._control(plan.controls, buf.vlogits, G + 1, 0)
         _lib.call(
             "ms_spec_accept", buf.vlogits.data_ptr(), V, buf.dlogits.data_ptr(), V,
             buf.dstats.data_ptr(), 0, buf.proposals.data_ptr(), plan.dev_params.data_ptr(), B,
             G, V, buf.out.data_ptr(), buf.out[B * (G + 1) :].data_ptr(), stream,
         )
+        self.controls.drew(plan.controls, buf.out[: B * (G + 1)].view(B, G + 1),
+                           buf.out[B * (G + 1) : B * (G + 2)], 1)
         self._release_blob_v(plan)
         if ev is not None and self.round_events is not None:
             ev[1].record()
@@ -838,6 +892,7 @@ class SpeculativeDecoder:
         self._pending = None
         self._row_cache = None
         self.draft_cache.reset()
+        self.controls.reset()
         self.num_proposed = 0
         self.num_accepted = 0
 
@@ -868,3 +923,4 @@ class SpeculativeDecoder:
         finally:
             cache.free(seq_id)
             self.draft_cache.free(seq_id)
+            self.controls.free(seq_id)

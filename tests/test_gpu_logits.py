@@ -305,6 +305,18 @@ def test_bad_metadata_sets_the_error_word_and_is_skipped() -> None:
         assert_controlled(got[0], want, mag)
 
 
+def test_proposals_not_drawn_yet_are_not_read() -> None:
+    """A draft pass hands over the round's whole buffer; what no row sees may hold anything."""
+    from microserve_b200 import _lib
+
+    c = Case(3, 2, 4100, seed=13, gamma=4, first=1)
+    c.dprops[2:] = -12345
+    got = c.run(torch.from_numpy(c.x).to(DEV)).cpu().numpy()
+    want, mag = c.want()
+    assert_controlled(got, want, mag)
+    assert _lib.device_error() == 0
+
+
 def test_replayed_graph_and_other_stream_read_current_values() -> None:
     c = Case(3, 3, 5001, seed=21, gamma=2)
     x = torch.from_numpy(c.x).to(DEV)
