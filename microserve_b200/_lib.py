@@ -203,8 +203,8 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ms_token_counts_reset": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
     "ms_apply_logit_controls": (
         c_int,
-        [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, POINTER(MsLogitControls),
-         c_void_p],
+        # the structures of this and ms_lora_add may also come as packed bytes
+        [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p],
     ),
     "ms_host_blocks_needed": (c_int64, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                                         c_void_p]),
@@ -244,8 +244,8 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ms_lora_add": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int,
-         c_int, c_void_p, c_int, c_int, POINTER(MsLoraAdapters), POINTER(MsLoraPlan), c_int, c_int,
-         c_void_p, c_size_t, c_void_p],
+         c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_size_t,
+         c_void_p],
     ),
     "ms_attention_scratch_size": (c_size_t, [POINTER(MsKVCache), c_int, POINTER(MsBatch)]),
     "ms_paged_attention": (c_int, [c_void_p, POINTER(MsKVCache), c_int, POINTER(MsBatch), c_int,

@@ -16,6 +16,7 @@ read in whole lines.  ``n_slices`` is the number of projections fused into one
 from __future__ import annotations
 
 import ctypes
+import struct
 from collections.abc import Iterable, Mapping, Sequence
 from dataclasses import dataclass
 from typing import TYPE_CHECKING
@@ -31,6 +32,10 @@ if TYPE_CHECKING:
 TILE = 64  # tokens of a plan's tile (MS_LORA_TILE)
 MAX_RANK = 256  # MS_LORA_MAX_RANK
 _check = _lib.check_tensor
+# the C structures as bytes (a third of the time ctypes structures take to fill)
+_PACK_ADAPTERS = struct.Struct("=iiiiQQQ").pack
+_PACK_PLAN = struct.Struct("=iiQQ").pack
+_PACK_COLUMNS = [struct.Struct(f"={k}i").pack for k in range(5)]
 _CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
@@ -136,13 +141,17 @@ def lora_add(
     pb = _check(proj.b, "b", dtype, dev, (R, N))
     n = proj.ranks.numel()
     i32 = torch.int32
-    ad = _lib.MsLoraAdapters(n, R, proj.max_rank, 0, _check(proj.offsets, "offsets", i32, dev, (n,)),
-                             _check(proj.ranks, "ranks", i32, dev, (n,)),
-                             _check(proj.scales, "scales", torch.float32, dev, (n,)))
-    pl = plan.c_struct(T, x.device)
+    n_tiles = plan.tiles.shape[0]
+    ad = _PACK_ADAPTERS(n, R, proj.max_rank, 0, _check(proj.offsets, "offsets", i32, dev, (n,)),
+                        _check(proj.ranks, "ranks", i32, dev, (n,)),
+                        _check(proj.scales, "scales", torch.float32, dev, (n,)))
+    pl = _PACK_PLAN(T, n_tiles, _check(plan.order, "order", i32, dev, (T,)),
+                    _check(plan.tiles, "tiles", i32, dev, (n_tiles, 4)))
     width = N // 2 if swiglu else N
     if out is None:
-        out = torch.empty((T, width), dtype=out_dtype, device=x.device)
+        # (empty_like costs half of what empty does)
+        out = torch.empty_like(base) if out_dtype is torch.float32 and width == N \
+            and base.is_contiguous() else torch.empty((T, width), dtype=out_dtype, device=x.device)
     elif out.shape != (T, width) or out.get_device() != dev or out.stride(1) != 1 \
             or (T > 1 and out.stride(0) < width):
         raise ValueError(f"out must be a ({T}, {width}) tensor on cuda:{dev} with contiguous rows")
@@ -153,11 +162,10 @@ def lora_add(
     # ms_lora_workspace_size: s as up to three bf16 terms of the padded rank
     need = T * ns * ((proj.max_rank + 15) // 16 * 16) * 6
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
-    cols = (ctypes.c_int32 * ns)(*slices)
+    cols = _PACK_COLUMNS[ns](*slices)
     _lib.launch_on(dev, "ms_lora_add", x.data_ptr(), max(x_ld, K), base.data_ptr(),
                    max(base_ld, N), out.data_ptr(), max(out.stride(0), width), pa, pb, K, N, ns,
-                   ctypes.addressof(cols), int(proj.interleaved), int(swiglu), ctypes.byref(ad),
-                   ctypes.byref(pl), _CODES[dtype], _CODES[out.dtype], ws.data_ptr(), ws.numel())
+                   cols, int(proj.interleaved), int(swiglu), ad, pl, _CODES[dtype], _CODES[out.dtype], ws.data_ptr(), ws.numel())
     return out
 
 
