@@ -232,6 +232,118 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
   }
 }
 
+// The same for larger tiles: 64 tokens x RB rank rows per CTA, both operands
+// through shared memory (each is read RB / 16 and 4 times), k in steps of 64
+// behind a ring of cp.async.  Warp (m, n) of the 4 x 2 has 16 tokens and RB / 2
+// rank rows.
+constexpr int kBigK = 64;
+constexpr int kBigLd = kBigK + 8;  // padded row (elements): conflict-free ldmatrix
+constexpr int kBigStages = 4;
+
+template <int RB>
+__global__ void __launch_bounds__(256, 2) lora_shrink_tile_kernel(ShrinkArgs p) {
+  pdl_enter();
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int kStage = (kTile + RB) * kBigLd;  // elements
+  constexpr int kOutLd = RB + 4;                 // floats per token of the parts
+  static_assert(kTile * kOutLd * 4 <= kBigStages * kStage * 2, "the parts fit the ring");
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int splits = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
+  Tile tile;
+  if (!load_tile(p.plan, p.ad, blockIdx.x, tile, p.err)) return;
+  const int rank_p = pad16(tile.rank), rows = p.ns * rank_p, m0 = blockIdx.y * RB;
+  if (tile.count == 0 || m0 >= rows) return;  // the whole cluster alike
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int wm = warp & 3, wn = warp >> 2;
+  __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(smem);
+
+  // This thread's loads of a step: 16 bytes at k offset kq of rows r0, r0 + 32, ...
+  constexpr int kLoads = (kTile + RB) / 32;
+  const int kq = 8 * (threadIdx.x & 7), r0 = threadIdx.x >> 3;
+  const __nv_bfloat16* src[kLoads];
+  bool have[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = r0 + 32 * i;
+    src[i] = p.a;
+    if (r < kTile) {
+      const int tok = r < tile.count ? token_at(p.plan, tile.start + r, p.err) : -1;
+      have[i] = tok >= 0;
+      if (have[i]) src[i] = p.x + (int64_t)tok * p.x_stride + kq;
+    } else {
+      const int mp = m0 + r - kTile, j = mp / rank_p, q = mp - j * rank_p;
+      have[i] = mp < rows && q < tile.rank;
+      if (have[i]) src[i] = p.a + ((int64_t)p.ns * tile.offset + j * tile.rank + q) * p.K + kq;
+    }
+  }
+  const int k_begin = split * p.k_per, k_end = min(p.K, k_begin + p.k_per);
+  const int steps = k_end > k_begin ? (k_end - k_begin + kBigK - 1) / kBigK : 0;
+  auto load = [&](int step) {
+    if (step < steps) {
+      const int k = k_begin + step * kBigK;
+      const uint32_t dst = s_addr(ring + (step % kBigStages) * kStage + r0 * kBigLd + kq);
+      const bool in = k + kq < k_end;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        cp_async16(dst + 32 * i * kBigLd * 2, have[i] && in ? src[i] + k : p.a, have[i] && in);
+    }
+    cp_commit();
+  };
+  for (int i = 0; i < kBigStages - 1; ++i) load(i);
+  constexpr int NT = RB / 16;  // 8-row tiles per warp
+  float acc[NT][4] = {};
+  const bool active = 16 * wm < tile.count && m0 + wn * (RB / 2) < rows;
+  for (int step = 0; step < steps; ++step) {
+    cp_wait<kBigStages - 2>();
+    __syncthreads();  // this step's data is there, the last step's slot is free
+    load(step + kBigStages - 1);
+    if (!active) continue;
+    const __nv_bfloat16* xs = ring + (step % kBigStages) * kStage;
+    const uint32_t xa = s_addr(xs + (16 * wm + (lane & 15)) * kBigLd + 8 * (lane >> 4));
+    const uint32_t aa = s_addr(xs + (kTile + wn * (RB / 2) + (lane & 7) + 8 * (lane >> 4)) * kBigLd +
+                               8 * ((lane >> 3) & 1));
+#pragma unroll
+    for (int k = 0; k < kBigK; k += 16) {
+      uint32_t xf[4];
+      ldsm4(xf, xa + 2 * k);
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t af[4];  // rank rows 8n .. 8n+15: b0, b1 of n, then of n + 1
+        ldsm4(af, aa + n * 8 * kBigLd * 2 + 2 * k);
+        mma_bf16(acc[n], xf[0], xf[1], xf[2], xf[3], af[0], af[1]);
+        mma_bf16(acc[n + 1], xf[0], xf[1], xf[2], xf[3], af[2], af[3]);
+      }
+    }
+  }
+  cp_wait<0>();
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(smem);  // [token][kOutLd]
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      part[(16 * wm + g + 8 * (e >> 1)) * kOutLd + wn * (RB / 2) + 8 * n + 2 * t + (e & 1)] = acc[n][e];
+  if (splits > 1) cluster.sync(); else __syncthreads();
+  // each CTA of the cluster finishes a share of the outputs, the parts in cluster order
+  const float scale = tile.rank > 0 ? p.ad.scales[tile.adapter] : 0.f;
+  const int here = min(RB, rows - m0);
+  for (int i = split * 256 + threadIdx.x; i < tile.count * RB; i += splits * 256) {
+    const int col = i / RB, row = i % RB;
+    if (row >= here) continue;
+    float v = 0.f;
+    if (splits > 1) {
+      for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(part, k)[col * kOutLd + row];
+    } else {
+      v = part[col * kOutLd + row];
+    }
+    const int mp = m0 + row, j = mp / rank_p, r = mp - j * rank_p;
+    store_terms(p.s + (tile.start + col) * p.s_stride + j * p.terms * rank_p + r, rank_p, p.terms,
+                v * scale);
+  }
+  if (splits > 1) cluster.sync();  // no CTA leaves while another reads its part
+}
+
 // ---- second product, bf16 -----------------------------------------------------
 // A CTA keeps the s rows of up to 16 WM tokens of a tile in shared memory and
 // goes through its share of the columns, 32 WN at a step: their base values
@@ -567,9 +679,19 @@ int launch_expand(ExpandArgs p, cudaStream_t s) {
     if (smem() > kMostSmem) return launch_expand<EPI, 1, 2>(p, s);  // ranks of 128 and more
   static std::atomic<uint64_t> granted{0};
   MS_TRY(grant_dynamic_smem(lora_expand_kernel<EPI, WM, WN>, kMostSmem, granted));
-  // about three rounds of CTAs over the GPU, so that each has several steps
-  const int resident = max(1, min(64 / (WM * WN), 227 * 1024 / (smem() + 1024)));
-  const int gx = max(1, min(ceil_div(p.N, cols), ceil_div(3 * 148 * resident, p.plan.n_tiles)));
+  // CTAs per tile: the number whose rounds over the GPU take the fewest steps,
+  // a CTA's start counted as three
+  const int resident = max(1, min(64 / (WM * WN), 227 * 1024 / (smem() + 1536)));
+  const int slots = 148 * resident, steps = ceil_div(p.N, cols);
+  int gx = 1;
+  int64_t best = INT64_MAX;
+  for (int n = 1; n <= min(steps, 64); ++n) {
+    const int64_t cost = (int64_t)ceil_div(p.plan.n_tiles * n, slots) * (ceil_div(steps, n) + 3);
+    if (cost < best) {
+      best = cost;
+      gx = n;
+    }
+  }
   launch_pdl(lora_expand_kernel<EPI, WM, WN>, dim3(gx, p.plan.n_tiles), 32 * WM * WN, smem(), s, p);
   return check_launch("lora_expand_kernel");
 }
@@ -583,14 +705,12 @@ int dispatch_expand(const ExpandArgs& p, cudaStream_t s) {
   return launch_expand<EPI, 4, 4>(p, s);
 }
 
-template <int MT, int NT>
-int launch_shrink(ShrinkArgs p, int rows, cudaStream_t s) {
-  const int smem = kShrinkWarps * 16 * MT * 8 * NT * 4;
-  const int split = shrink_split(p.plan.n_tiles, p.K, rows, MT);
-  p.k_per = ceil_div(ceil_div(p.K, split), 32) * 32;
+// Clusters of `split` CTAs along z.
+int launch_cluster(void (*kernel)(ShrinkArgs), dim3 grid, int threads, int smem, int split,
+                   cudaStream_t s, const ShrinkArgs& p) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.plan.n_tiles, ceil_div(rows, 16 * MT), split);
-  cfg.blockDim = kShrinkWarps * 32;
+  cfg.gridDim = grid;
+  cfg.blockDim = threads;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2]{};
@@ -600,8 +720,32 @@ int launch_shrink(ShrinkArgs p, int rows, cudaStream_t s) {
   attr[1].val.clusterDim = {1, 1, (unsigned)split};
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  (void)cudaLaunchKernelEx(&cfg, lora_shrink_kernel<MT, NT>, p);
-  return check_launch("lora_shrink_kernel");
+  (void)cudaLaunchKernelEx(&cfg, kernel, p);
+  return check_launch("lora_shrink");
+}
+
+template <int MT, int NT>
+int launch_shrink(ShrinkArgs p, int rows, cudaStream_t s) {
+  const int smem = kShrinkWarps * 16 * MT * 8 * NT * 4;
+  const int split = shrink_split(p.plan.n_tiles, p.K, rows, MT);
+  p.k_per = ceil_div(ceil_div(p.K, split), 32) * 32;
+  return launch_cluster(lora_shrink_kernel<MT, NT>,
+                        dim3(p.plan.n_tiles, ceil_div(rows, 16 * MT), split), kShrinkWarps * 32,
+                        smem, split, s, p);
+}
+
+template <int RB>
+int launch_shrink_tile(ShrinkArgs p, int rows, cudaStream_t s) {
+  const int smem = kBigStages * (kTile + RB) * kBigLd * 2;
+  static std::atomic<uint64_t> granted{0};
+  MS_TRY(grant_dynamic_smem(lora_shrink_tile_kernel<RB>, smem, granted));
+  const int blocks = ceil_div(rows, RB);
+  int split = 1;
+  while (split < 8 && (int64_t)p.plan.n_tiles * blocks * split < 2 * 148 && p.K / (2 * split) >= 256)
+    split *= 2;
+  p.k_per = ceil_div(ceil_div(p.K, split), kBigK) * kBigK;
+  return launch_cluster(lora_shrink_tile_kernel<RB>, dim3(p.plan.n_tiles, blocks, split), 256, smem,
+                        split, s, p);
 }
 
 template <int NT>
@@ -706,8 +850,10 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
       MS_TRY(dispatch_shrink<1>(p, rows, s));
     else if (mean <= 16)
       MS_TRY(dispatch_shrink<2>(p, rows, s));
+    else if (rows <= 64)
+      MS_TRY(launch_shrink_tile<64>(p, rows, s));
     else
-      MS_TRY(dispatch_shrink<4>(p, rows, s));
+      MS_TRY(launch_shrink_tile<128>(p, rows, s));
   }
   if (c.swiglu) return dispatch_expand<kLoraSwiGLU>(e, s);
   return out_f32 ? dispatch_expand<kLoraF32>(e, s) : dispatch_expand<kLoraBf16>(e, s);
