@@ -19,85 +19,10 @@
 
 #include <cooperative_groups.h>
 
-#include "lora.cuh"
+#include "lora_device.cuh"
 
 namespace ms {
 namespace {
-
-constexpr int kTile = MS_LORA_TILE;  // most tokens of a tile
-constexpr int kMaxRank = MS_LORA_MAX_RANK;
-constexpr int kMaxTiles = 65535;  // the second product's grid
-
-struct Tile {
-  int start, count, adapter, rank, offset;
-};
-
-// Tile `i` of the plan with its adapter's rank and offset, every index checked:
-// false (and the device error word) when one is out of range.
-__device__ __forceinline__ bool load_tile(const ms_lora_plan& p, const ms_lora_adapters& ad, int i,
-                                          Tile& t, int* err) {
-  const int4 q = reinterpret_cast<const int4*>(p.tiles)[i];
-  t.start = q.x;
-  t.count = q.y;
-  t.adapter = q.z;
-  t.rank = 0;
-  t.offset = 0;
-  bool ok = t.start >= 0 && t.count >= 0 && t.count <= kTile && t.start <= p.n_tokens - t.count &&
-            t.adapter < ad.n_adapters;
-  if (ok && t.adapter >= 0) {
-    t.rank = ad.ranks[t.adapter];
-    t.offset = ad.offsets[t.adapter];
-    ok = t.rank >= 0 && t.rank <= ad.max_rank && t.offset >= 0 &&
-         t.offset <= ad.total_rank - t.rank;
-  }
-  if (!ok) {
-    if (threadIdx.x == 0) raise_device_error(err, kErrAdapter);
-    t.count = 0;
-  }
-  return ok;
-}
-
-// The token (row of x and out) at sorted position `pos`, or -1 (and the error word).
-__device__ __forceinline__ int token_at(const ms_lora_plan& p, int pos, int* err) {
-  const int t = p.order[pos];
-  if (t >= 0 && t < p.n_tokens) return t;
-  raise_device_error(err, kErrAdapter);
-  return -1;
-}
-
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t s_addr(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
-               : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 // ---- first product, bf16 ------------------------------------------------------
 // mma m16n8k16 with the rank rows of A as M and the tokens as N (8 of them:
@@ -123,8 +48,6 @@ struct ShrinkArgs {
   __nv_bfloat16* s;  // row per position: [slice][term][rank_p]
   int* err;
 };
-
-__device__ __forceinline__ int pad16(int r) { return (r + 15) & ~15; }
 
 // v as `terms` bf16 terms at dst[0], dst[step], ...
 __device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int terms, float v) {
@@ -352,38 +275,6 @@ __global__ void __launch_bounds__(256, 2) lora_shrink_tile_kernel(ShrinkArgs p) 
 // has 16 tokens and 32 columns.  The sums start from the base and leave
 // through its buffer, in whole 32-byte sectors.
 constexpr int kPad = 8;  // elements after each shared-memory row: conflict-free fragment reads
-
-struct ExpandArgs {
-  const float* base;
-  int64_t base_stride;
-  void* out;
-  int64_t out_stride;
-  const __nv_bfloat16* b;
-  int N, ns, terms;
-  int slice_end[3];
-  int interleaved, in_place, after_shrink;
-  int stages;  // steps in the ring (2 to 4)
-  int rank_pm;     // padded largest rank: buffer sizes
-  int64_t s_stride;
-  ms_lora_adapters ad;
-  ms_lora_plan plan;
-  const __nv_bfloat16* s;
-  const float* s_any;  // any-shape kernels: float32 s, one row per position
-  int width_any;
-  int* err;
-};
-
-__device__ __forceinline__ int slice_of(const ExpandArgs& p, int n) {
-  if (p.interleaved) return (n >> 3) & 1;
-  int j = 0;
-#pragma unroll
-  for (int k = 0; k < 3; ++k) j += k < p.ns - 1 && n >= p.slice_end[k];
-  return j;
-}
-
-enum LoraEpilogue { kLoraF32, kLoraBf16, kLoraSwiGLU };
-
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
 // Which slice a warp's 32 columns take their s from.
 enum SliceMode { kOneSlice, kInterleaved, kMixed };
@@ -696,10 +587,15 @@ int launch_expand(ExpandArgs p, cudaStream_t s) {
   return check_launch("lora_expand_kernel");
 }
 
-// Tokens per CTA by the tiles' mean size.
+// Tokens per CTA by the tiles' mean size; tcgen05 above kTcTokens.
+constexpr int kTcTokens = 48;
 template <int EPI>
 int dispatch_expand(const ExpandArgs& p, cudaStream_t s) {
   const int mean = p.plan.n_tokens / p.plan.n_tiles;
+  if (mean > kTcTokens) {
+    const int rc = lora_expand_tc(p, EPI, s);
+    if (rc != MS_ERR_UNSUPPORTED) return rc;
+  }
   if (mean <= 16) return launch_expand<EPI, 1, 4>(p, s);
   if (mean <= 32) return launch_expand<EPI, 2, 4>(p, s);
   return launch_expand<EPI, 4, 4>(p, s);

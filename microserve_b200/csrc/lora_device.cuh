@@ -1,0 +1,126 @@
+// What the adapter kernels share (lora.cu, lora_tc.cu): the plan's tiles, the
+// second product's arguments and epilogues, and small PTX helpers.
+#pragma once
+#include "lora.cuh"
+
+namespace ms {
+
+enum LoraEpilogue { kLoraF32, kLoraBf16, kLoraSwiGLU };
+
+struct ExpandArgs {
+  const float* base;
+  int64_t base_stride;
+  void* out;
+  int64_t out_stride;
+  const __nv_bfloat16* b;
+  int N, ns, terms;
+  int slice_end[3];
+  int interleaved, in_place, after_shrink;
+  int stages;  // steps in the ring (2 to 4)
+  int rank_pm;     // padded largest rank: buffer sizes
+  int64_t s_stride;
+  ms_lora_adapters ad;
+  ms_lora_plan plan;
+  const __nv_bfloat16* s;
+  const float* s_any;  // any-shape kernels: float32 s, one row per position
+  int width_any;
+  int* err;
+};
+
+namespace {
+
+constexpr int kTile = MS_LORA_TILE;  // most tokens of a tile
+constexpr int kMaxRank = MS_LORA_MAX_RANK;
+constexpr int kMaxTiles = 65535;  // the second product's grid
+
+struct Tile {
+  int start, count, adapter, rank, offset;
+};
+
+// Tile `i` of the plan with its adapter's rank and offset, every index checked:
+// false (and the device error word) when one is out of range.
+__device__ __forceinline__ bool load_tile(const ms_lora_plan& p, const ms_lora_adapters& ad, int i,
+                                          Tile& t, int* err) {
+  const int4 q = reinterpret_cast<const int4*>(p.tiles)[i];
+  t.start = q.x;
+  t.count = q.y;
+  t.adapter = q.z;
+  t.rank = 0;
+  t.offset = 0;
+  bool ok = t.start >= 0 && t.count >= 0 && t.count <= kTile && t.start <= p.n_tokens - t.count &&
+            t.adapter < ad.n_adapters;
+  if (ok && t.adapter >= 0) {
+    t.rank = ad.ranks[t.adapter];
+    t.offset = ad.offsets[t.adapter];
+    ok = t.rank >= 0 && t.rank <= ad.max_rank && t.offset >= 0 &&
+         t.offset <= ad.total_rank - t.rank;
+  }
+  if (!ok) {
+    if (threadIdx.x == 0) raise_device_error(err, kErrAdapter);
+    t.count = 0;
+  }
+  return ok;
+}
+
+// The token (row of x and out) at sorted position `pos`, or -1 (and the error word).
+__device__ __forceinline__ int token_at(const ms_lora_plan& p, int pos, int* err) {
+  const int t = p.order[pos];
+  if (t >= 0 && t < p.n_tokens) return t;
+  raise_device_error(err, kErrAdapter);
+  return -1;
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t s_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ int pad16(int r) { return (r + 15) & ~15; }
+
+__device__ __forceinline__ int slice_of(const ExpandArgs& p, int n) {
+  if (p.interleaved) return (n >> 3) & 1;
+  int j = 0;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) j += k < p.ns - 1 && n >= p.slice_end[k];
+  return j;
+}
+
+
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+
+}  // namespace
+
+// The second product on tcgen05 (lora_tc.cu), for tiles of many tokens:
+// MS_ERR_UNSUPPORTED when the shape does not apply.
+int lora_expand_tc(const ExpandArgs& p, int epilogue, cudaStream_t s);
+
+}  // namespace ms

@@ -107,6 +107,16 @@ CASES = {
     "gaps": dict(of=mixed(60, 3), ranks=[16, 5, 33], K=128, slices=[96, 32], dtype="bfloat16", gaps=True),
     "odd_k": dict(of=mixed(30, 2), ranks=[3, 20], K=67, slices=[50], dtype="bfloat16"),
     "odd_n": dict(of=mixed(30, 2), ranks=[3, 20], K=64, slices=[33, 18], dtype="bfloat16"),
+    # long runs of one adapter: pairs of tiles, odd runs, a short last tile
+    "prompts": dict(of=[0] * 300 + [-1] * 70 + [1] * 129 + [2] * 64 + [3] * 127, ranks=[16, 64, 8, 33], K=256,
+                    slices=[384], dtype="bfloat16"),
+    "prompts_interrupted": dict(of=([0] * 50 + [1] * 60) * 6, ranks=[128, 72], K=200, slices=[200], dtype="bfloat16"),
+    "prompts_qkv": dict(of=[0] * 200 + [1] * 150, ranks=[40, 16], K=512, slices=[512, 64, 64], dtype="bfloat16"),
+    "prompts_slice_edges": dict(of=[0] * 130 + [1] * 70 + [-1] * 40, ranks=[24, 64], K=128, slices=[203, 150, 47],
+                                dtype="bfloat16"),
+    "prompts_narrow_slices": dict(of=[0] * 130, ranks=[24], K=128, slices=[30, 40, 58], dtype="bfloat16"),
+    "prompts_none": dict(of=[-1] * 200 + [0] * 64, ranks=[16], K=64, slices=[136], dtype="bfloat16"),
+    "prompts_rank_256": dict(of=[0] * 140, ranks=[256], K=72, slices=[264], dtype="bfloat16"),
     "f32": dict(of=mixed(61, 3), ranks=[4, 5, 12], K=128, slices=[128, 128, 128], dtype="float32"),
     "f32_odd": dict(of=mixed(13, 2), ranks=[7, 1], K=33, slices=[29], dtype="float32"),
 }
@@ -134,6 +144,8 @@ def test_adapters_match_the_restatement(name: str) -> None:
 @pytest.mark.parametrize("dtype,of,ranks,K,N", [
     ("bfloat16", mixed(80, 5), [8, 16, 32, 64, 3], 2048, 1408),
     ("bfloat16", [1] * 130, [16, 128], 264, 176),
+    ("bfloat16", [0] * 300 + [1] * 200 + [-1] * 90 + [2] * 65, [128, 64, 20], 512, 1152),
+    ("bfloat16", [-1] * 129 + [0] * 64, [8], 64, 144),
     ("bfloat16", [0, -1, 0], [16], 72, 16),
     ("float32", mixed(61, 3), [4, 5, 12], 128, 704),
     ("bfloat16", mixed(20, 2), [4, 9], 65, 48),
