@@ -115,7 +115,14 @@ __device__ __forceinline__ int slice_of(const ExpandArgs& p, int n) {
 }
 
 
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+// x / (1 + e^-x) with the fast exponential and reciprocal instructions (the
+// result is rounded to bf16): one multiplication where a division would also
+// scale for denominators past 2^126, which give 0 either way.
+__device__ __forceinline__ float silu(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
+  return x * r;
+}
 
 }  // namespace
 

@@ -3,20 +3,23 @@
 // with the epilogues of lora.cu.  A CTA takes up to 128 tokens of one adapter
 // (two neighbouring tiles of the plan) and goes through its share of the
 // columns, 128 at a step:
-//   warps 0-2   load: s once (K-major, the bf16 terms side by side along k),
-//               then each step's adapter rows, by cp.async into the 128-byte
-//               swizzle that the MMA reads;
-//   warp 3      allocates TMEM; lane 0 issues tcgen05.mma M128 N128 K16.  The
-//               adapter rows are (rank, column) in memory, so B is MN-major.
-//               With two slices in the 128 columns (gate | up alternate every
-//               8) both s are multiplied with all of them, into two
-//               accumulators, of which the epilogue takes the columns it needs;
-//   warps 4-11  epilogue: TMEM lane quarter warp % 4, columns by half.  The base
-//               comes in and the result goes out in whole 128-byte row segments
-//               through a 4 KB exchange per warp, as in gemm_tc.cu.
-// The 4 accumulators (two steps x two slices) fill the 512 TMEM columns, so one
-// CTA runs per SM.  The kernel moves 4 bytes in per column and token and 1 to 4
-// out, and is bound by HBM.
+//   warps 0-2   load each step's adapter rows by cp.async, a ring slot per warp, into
+//               the 128-byte swizzle that the MMA reads;
+//   warp 3      allocates TMEM; lane 0 issues tcgen05.mma with s (bf16 terms side
+//               by side along k) as A in TMEM, copied there once, so that the
+//               MMAs read only B from shared memory.  The adapter rows are (rank,
+//               column) in memory, so B is MN-major.  Gate | up columns
+//               (alternating every 8) are parted by the load into two blocks of
+//               64, one accumulator each; columns where one slice ends and
+//               another begins take two passes, the other slice's columns zero;
+//   warps 4-19  epilogue: TMEM lane quarter warp % 4, 32 of the columns each; a
+//               thread has one row.  Each warp brings its own base in by cp.async,
+//               two steps ahead (16 warps keep more copies in flight than a few
+//               loading ones: 3 warps moved 30 KB per us), and sends the result
+//               out in 32- to 64-byte row segments through a 2 KB exchange.
+// TMEM: two accumulators of 128 columns, then s (up to 256).  One CTA per SM.
+// The kernel moves 4 bytes in per column and token and 1 to 4 out, and is
+// bound by HBM; shared memory sees the base twice and little else.
 #include "lora_device.cuh"
 
 namespace ms {
@@ -24,12 +27,13 @@ namespace {
 
 constexpr int kRows = 128;          // tokens per CTA
 constexpr int kChunk = 128;         // columns per step
-constexpr int kPanel = kRows * 128; // bytes of a 64-wide k panel of s
-constexpr int kLoadThreads = 96;
-constexpr int kEpiWarps = 8;
+constexpr int kSAt = 2 * kChunk;    // TMEM column of s
+constexpr int kLoadThreads = 96;  // (three warps: the fourth of their group issues the MMAs)
+constexpr int kEpiWarps = 16;
 constexpr int kThreads = kLoadThreads + 32 + 32 * kEpiWarps;
-constexpr int kExchange = 32 * 128;
-constexpr int kMaxStages = 4;
+constexpr int kSegment = 32 * 128;                    // base of 32 rows x 32 columns
+constexpr int kEpiBytes = 2 * kSegment + 32 * 64;     // two of them, and the exchange, per warp
+constexpr int kStages = 2;          // passes in the ring, a loading warp each
 constexpr int kBarBytes = 256;
 constexpr int kMostBytes = 226 * 1024;
 constexpr long long kWaitCycles = 1ll << 32;  // ~2.2 s
@@ -64,9 +68,9 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop, int* err) {
   return __all_sync(0xffffffffu, bar_wait(bar, parity, stop, err));
 }
-// 128-byte swizzle descriptors.  K-major (s): 8-row groups 1024 bytes apart.
-// MN-major (adapter rows): 64 columns per 128-byte row, groups of 8 k rows 1024
-// bytes apart (stride offset), blocks of 64 columns `lead` bytes apart.
+// Descriptor of adapter rows, MN-major with the 128-byte swizzle: 64 columns per
+// 128-byte row, groups of 8 k rows 1024 bytes apart (stride offset), blocks of
+// 64 columns `lead` bytes apart.
 __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
   uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);
   d |= (uint64_t)(lead >> 4) << 16;
@@ -75,26 +79,37 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
   d |= (uint64_t)2 << 61;
   return d;
 }
-// f32 accumulator, bf16 operands, A K-major, B MN-major, M 128, N 128.
-constexpr uint32_t kInstr = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
-                            ((uint32_t)(kChunk >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+// f32 accumulator, bf16 operands, A (in TMEM) K-major, B MN-major, M 128.
+__device__ __forceinline__ uint32_t instr(int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kRows >> 4) << 24);
+}
+__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                     uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(kInstr), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                : "memory");
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint4& a, const uint4& b) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+               "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -135,22 +150,10 @@ __device__ int tiles_before(const ms_lora_plan& p, int i, int start, int adapter
   }
 }
 
-// Stage counts and bytes for a rank: 0 stages when the shared memory does not do.
-struct Layout {
-  int panels;  // k panels of s per slice
-  int stages, bytes;
-};
-template <int TERMS>
-__host__ __device__ __forceinline__ Layout layout(int ns, int rank_pm) {
-  Layout l;
-  l.panels = (TERMS * rank_pm + 63) / 64;
-  const int fixed = 1024 + kBarBytes + kEpiWarps * kExchange + ns * l.panels * kPanel;
-  const int stage = rank_pm * kChunk * 2;
-  l.stages = stage > 0 ? (kMostBytes - fixed) / stage : 0;
-  if (l.stages > kMaxStages) l.stages = kMaxStages;
-  if (l.stages < 2) l.stages = 0;
-  l.bytes = fixed + l.stages * stage;
-  return l;
+// Shared memory for a rank; 0 when it or TMEM do not do.
+int ring_bytes(int terms, int ns, int rank_pm) {
+  const int bytes = 1024 + kBarBytes + kEpiWarps * kEpiBytes + kStages * rank_pm * kChunk * 2;
+  return bytes <= kMostBytes && ns * terms * rank_pm / 2 <= 512 - kSAt ? bytes : 0;
 }
 
 template <int EPI>
@@ -160,11 +163,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   __shared__ int s_tok[kRows];
   const uint32_t raw = s_addr(smem_raw);
   const uint32_t base = raw + ((1024u - (raw & 1023u)) & 1023u);
-  const Layout lay = layout<TERMS>(p.ns, p.rank_pm);
-  const uint32_t s_s = base, s_b = s_s + p.ns * lay.panels * kPanel;
-  const uint32_t stage_bytes = p.rank_pm * kChunk * 2;
-  const uint32_t s_x = s_b + lay.stages * stage_bytes, bars = s_x + kEpiWarps * kExchange;
-  const uint32_t full = bars, empty = full + 8 * kMaxStages, s_ready = empty + 8 * kMaxStages;
+  // adapter rows of a pass in two blocks of 64 columns; each epilogue warp's base
+  // rows and exchange
+  const uint32_t ring = base, stage_bytes = p.rank_pm * kChunk * 2;
+  const uint32_t s_x = ring + kStages * stage_bytes, bars = s_x + kEpiWarps * kEpiBytes;
+  const uint32_t full = bars, empty = full + 8 * kStages, s_ready = empty + 8 * kStages;
   const uint32_t tfull = s_ready + 8, tempty = tfull + 16, slot_addr = tempty + 16;
   unsigned char* gbars = smem_raw + (bars - raw);
   volatile uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbars + (slot_addr - bars));
@@ -197,21 +200,23 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   }
   const int rank_p = pad16(tile.rank);
   const int n_chunks = (p.N + kChunk - 1) / kChunk;
-  const int steps = (n_chunks - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
-  auto column = [&](int step) { return ((int)blockIdx.x + step * (int)gridDim.x) * kChunk; };
-  // the slices of a step's columns: first, and whether there are two
+  const int chunks = (n_chunks - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  auto column = [&](int chunk) { return ((int)blockIdx.x + chunk * (int)gridDim.x) * kChunk; };
+  // The passes of a chunk: one, or one per slice where a slice ends inside.
   auto first_slice = [&](int c) { return p.interleaved ? 0 : slice_of(p, c); };
-  auto last_slice = [&](int c) { return p.interleaved ? 1 : slice_of(p, min(c + kChunk, p.N) - 1); };
+  auto passes = [&](int c) {
+    return p.interleaved ? 1 : slice_of(p, min(c + kChunk, p.N) - 1) - slice_of(p, c) + 1;
+  };
 
   if (threadIdx.x < kRows)
     s_tok[threadIdx.x] =
         threadIdx.x < count ? token_at(p.plan, tile.start + threadIdx.x, p.err) : -1;
   if (threadIdx.x == 0) {
-    for (int k = 0; k < lay.stages; ++k) {
-      bar_init(full + 8 * k, kLoadThreads);
+    for (int k = 0; k < kStages; ++k) {
+      bar_init(full + 8 * k, 32);
       bar_init(empty + 8 * k, 1);
     }
-    bar_init(s_ready, kLoadThreads);
+    bar_init(s_ready, kEpiWarps);
     for (int k = 0; k < 2; ++k) {
       bar_init(tfull + 8 * k, 1);
       bar_init(tempty + 8 * k, kEpiWarps);
@@ -231,161 +236,216 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   const uint32_t tmem = *tmem_slot;
 
   if (warp < 3) {
-    // ---- loads.  A thread's copies of a step: 16 bytes, 8 columns, of rank rows
-    // r0, r0 + 6, ...; then a fence, so that the MMA's reads see them, and an arrive.
-    const int tid = threadIdx.x;
-    const int q = tid & 15, r0 = tid >> 4;
-    auto load_b = [&](int step) {
-      const int stage = step % lay.stages, c = column(step) + 8 * q;
-      const uint32_t block = s_b + stage * stage_bytes + (q >> 3) * (rank_p * 128);
+    // ---- loads of the adapter rows.  Each warp fills its own slot of the ring, so
+    // that a slot waiting to be free does not hold up the others.
+    const int q = lane & 15, r0 = lane >> 4;
+    auto load_b = [&](uint32_t dst, int c0, int pass) {
+      const int c = c0 + 8 * q;
+      // block and place of these 8 columns: gate | up parted, else in order
+      const int block = p.interleaved ? q & 1 : q >> 3, at = p.interleaved ? q >> 1 : q & 7;
+      const uint32_t to = dst + block * (rank_p * 128);
       const bool in = c < p.N;
+      const bool split = passes(c0) > 1;
+      const int j = first_slice(c0) + pass;
+      const bool mine = in && (!split || (slice_of(p, c) == j && slice_of(p, c + 7) == j));
+      const bool some = in && split && !mine && (slice_of(p, c) <= j && slice_of(p, c + 7) >= j);
       const __nv_bfloat16* src = p.b + ((int64_t)tile.offset + r0) * p.N + (in ? c : 0);
-      for (int r = r0; r < rank_p; r += kLoadThreads / 16, src += (int64_t)(kLoadThreads / 16) * p.N) {
-        const bool ok = in && r < tile.rank;
-        cp_async16(block + r * 128 + (((q & 7) ^ (r & 7)) << 4), ok ? src : p.b, ok);
+      constexpr int kStep = 2;
+      if (!some) {
+        const int64_t jump = (int64_t)kStep * p.N;
+        const int last = mine ? tile.rank : 0;  // rows past it: zeros
+#pragma unroll 8
+        for (int r = r0; r < rank_p; r += kStep, src += jump)
+          cp_async16(to + r * 128 + ((at ^ (r & 7)) << 4), r < last ? src : p.b, r < last);
+      } else {  // the slice ends within the 8 columns
+        for (int r = r0; r < rank_p; r += kStep, src += (int64_t)kStep * p.N) {
+          uint32_t w[4] = {0u, 0u, 0u, 0u};
+          if (r < tile.rank) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            for (int e = 0; e < 8; ++e)
+              if (slice_of(p, c + e) != j) w[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+          }
+          st4(to + r * 128 + ((at ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+        }
       }
     };
-    if (p.after_shrink) {
-      load_b(0);  // not written by lora_shrink
-      pdl_enter();
-    }
-    const int row_chunks = TERMS * rank_p / 8;  // 16-byte chunks of one slice of a row
-    for (int j = 0; j < p.ns; ++j)
-      for (int i = tid; i < kRows * row_chunks; i += kLoadThreads) {
-        const int m = i / row_chunks, k = i - m * row_chunks;
-        const uint32_t dst = s_s + (j * lay.panels + (k >> 3)) * kPanel + m * 128 + (((k & 7) ^ (m & 7)) << 4);
-        const bool ok = m < count;
-        cp_async16(dst, ok ? p.s + (tile.start + m) * p.s_stride + j * TERMS * rank_p + 8 * k : p.s, ok);
+    int step = 0;
+    bool alive = warp < kStages;
+    for (int chunk = 0; chunk < chunks && alive; ++chunk) {
+      const int c = column(chunk), n = passes(c);
+      for (int pass = 0; pass < n; ++pass, ++step) {
+        if (step % kStages != warp) continue;
+        if (step >= kStages) {
+          alive = warp_wait(empty + 8 * warp, (step / kStages - 1) & 1, stop, p.err);
+          if (!alive) break;
+        }
+        load_b(ring + warp * stage_bytes, c, pass);
+        cp_commit();
+        cp_wait<0>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        bar_arrive(full + 8 * warp);
       }
-    if (!p.after_shrink) load_b(0);
-    cp_commit();
-    const int ahead = lay.stages > 2 ? lay.stages - 2 : 1;  // steps loaded before the one handed over
-    for (int step = 1; step < ahead; ++step) {
-      if (step < steps) load_b(step);
-      cp_commit();
     }
-    for (int step = 0; step < steps; ++step) {
-      const int next = step + ahead;
-      if (next < steps) {
-        if (next >= lay.stages &&
-            !bar_wait(empty + 8 * (next % lay.stages), (next / lay.stages - 1) & 1, stop, p.err))
-          break;
-        load_b(next);
-      }
-      cp_commit();
-      if (ahead > 1) cp_wait<2>(); else cp_wait<1>();  // this step's copies have arrived
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (step == 0) bar_arrive(s_ready);
-      bar_arrive(full + 8 * (step % lay.stages));
-    }
-    cp_wait<0>();
+    if (p.after_shrink) pdl_enter();  // lora_shrink does not write the adapter rows
   } else if (warp == 3) {
     // ---- MMA
     if (p.after_shrink) pdl_enter();
     if (lane == 0 && bar_wait(s_ready, 0, stop, p.err)) {
-      for (int step = 0; step < steps; ++step) {
-        const int stage = step % lay.stages, buf = step & 1, use = step >> 1;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      int step = 0;
+      bool fine = true;
+      for (int ch = 0; ch < chunks && fine; ++ch) {
+        const int buf = ch & 1, use = ch >> 1;
         if (use >= 1 && !bar_wait(tempty + 8 * buf, (use - 1) & 1, stop, p.err)) break;
-        if (!bar_wait(full + 8 * stage, (step / lay.stages) & 1, stop, p.err)) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int c = column(step), j0 = first_slice(c), j1 = last_slice(c);
-        const uint32_t b = s_b + stage * stage_bytes;
-        for (int j = j0; j <= j1; ++j) {
-          const uint32_t d = tmem + buf * 256 + (j - j0) * kChunk;
-          const uint32_t a = s_s + j * lay.panels * kPanel;
-          uint32_t acc = 0;
-          for (int e = TERMS - 1; e >= 0; --e)  // the small terms first
-            for (int k = 0; k < rank_p; k += 16, acc = 1) {
-              const int at = e * rank_p + k;
-              umma(d, desc(a + (at >> 6) * kPanel + (at & 63) * 2, 16), desc(b + k * 128, rank_p * 128), acc);
+        const int c = column(ch), n = passes(c);
+        const uint32_t d = tmem + buf * kChunk;
+        uint32_t acc = 0;
+        for (int pass = 0; pass < n; ++pass, ++step) {
+          const int slot = step % kStages;
+          if (!(fine = bar_wait(full + 8 * slot, (step / kStages) & 1, stop, p.err))) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t lead = rank_p * 128;
+          const uint64_t b0 = desc(ring + slot * stage_bytes, lead);
+          const uint32_t term = rank_p / 2, slice = TERMS * term;  // TMEM columns
+          // all terms and rank steps of one slice into d
+          auto products = [&](uint32_t to, uint32_t a, uint64_t bj, uint32_t id) {
+            for (int e = TERMS - 1; e >= 0; --e) {  // the small terms first
+              const uint32_t ae = a + e * term;
+              if (acc)
+                umma(to, ae, bj, id, 1u);
+              else
+                umma(to, ae, bj, id, 0u);
+              acc = 1;
+#pragma unroll 4
+              for (int k = 16; k < rank_p; k += 16) umma(to, ae + k / 2, bj + k * 8, id, 1u);
             }
+          };
+          if (rank_p > 0 && p.interleaved) {
+            for (int j = 0; j < 2; ++j) {
+              acc = 0;
+              products(d + 64 * j, tmem + kSAt + j * slice, b0 + j * (lead >> 4), instr(64));
+            }
+          } else if (rank_p > 0) {
+            products(d, tmem + kSAt + (first_slice(c) + pass) * slice, b0, instr(kChunk));
+          }
+          umma_commit(empty + 8 * slot);
         }
-        umma_commit(empty + 8 * stage);
+        if (!fine) break;
         umma_commit(tfull + 8 * buf);
       }
     }
     __syncwarp();
   } else {
-    // ---- epilogue
+    // ---- epilogue: one 32-column segment of the chunk per warp
     if (p.after_shrink) pdl_enter();
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t x = s_x + (warp - 4) * kExchange;
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
+    const uint32_t base_buf = s_x + (warp - 4) * kEpiBytes, x = base_buf + 2 * kSegment;
     const int row0 = 32 * quarter;
     const int rows = max(0, min(32, count - row0));
-    constexpr int kOutCols = EPI == kLoraSwiGLU ? 16 : 32;  // outputs of a segment
-    constexpr int kOutBytes = kOutCols * (EPI == kLoraF32 ? 4 : 2);
-    const int n_out = EPI == kLoraSwiGLU ? p.N / 2 : p.N;
-    // segment u: 32 columns of the step, two per warp
-    auto load_base = [&](int c, float4 (&v)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3), tok = r < rows ? s_tok[row0 + r] : -1;
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (tok >= 0 && c + 4 * (lane & 7) < p.N)
-          v[i] = __ldcs(reinterpret_cast<const float4*>(p.base + tok * p.base_stride + c + 4 * (lane & 7)));
+    const uint32_t lanes = (uint32_t)row0 << 16;
+    {  // s into TMEM: a row's bytes are the TMEM words of its lane; shared out over `part`
+      const __nv_bfloat16* src = p.s + (tile.start + min(row0 + lane, count - 1)) * p.s_stride;
+      const int words = p.ns * TERMS * rank_p / 2;
+      for (int w = 8 * part; w < words; w += 32) {
+        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        if (row0 + lane < count) {
+          a = *reinterpret_cast<const uint4*>(src + 2 * w);
+          b = *reinterpret_cast<const uint4*>(src + 2 * w + 8);
+        }
+        tmem_st8(tmem + kSAt + w + lanes, a, b);
       }
-    };
-    float4 v0[8], v1[8];
-    if (rows > 0) {
-      load_base(column(0) + 64 * half, v0);
-      load_base(column(0) + 64 * half + 32, v1);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(s_ready);
     }
-    for (int step = 0; step < steps; ++step) {
-      const int buf = step & 1, c_step = column(step), j0 = first_slice(c_step), j1 = last_slice(c_step);
-      if (!warp_wait(tfull + 8 * buf, (step >> 1) & 1, stop, p.err)) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // 16-byte chunk k of row r in the exchange
+    auto place = [&](int r, int k) { return x + r * 64 + ((k ^ ((r >> 1) & 3)) << 4); };
+    const int n_out = EPI == kLoraSwiGLU ? p.N / 2 : p.N;
+    constexpr int kHalves = EPI == kLoraF32 ? 2 : 1;
+    constexpr int kChunks = EPI == kLoraSwiGLU ? 2 : 4;  // of 16 bytes per row
+    constexpr int kPer = EPI == kLoraF32 ? 4 : 8;        // outputs per chunk
+    // element offsets of this lane's output rows (the launch checks that they fit 32 bits)
+    uint32_t out_at[kChunks], has = 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int at = 32 * i + lane, r = at / kChunks;
+      const int tok = r < rows ? s_tok[row0 + r] : -1;
+      has |= (uint32_t)(tok >= 0) << i;
+      out_at[i] = (uint32_t)(max(tok, 0) * p.out_stride + at % kChunks * kPer);
+    }
+    // The base comes by cp.async, two chunks ahead, into this warp's own rows
+    // (16-byte chunk k of row r at k ^ (r & 7)); lane l loads chunk l & 7 of rows
+    // (l >> 3) + 4 i.
+    uint32_t base_at[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      base_at[i] = (uint32_t)(max(r < rows ? s_tok[row0 + r] : 0, 0) * p.base_stride + 4 * (lane & 7));
+    }
+    auto load_base = [&](int ch) {
+      if (ch < chunks && rows > 0) {
+        const int c = column(ch) + 32 * part;
+        const bool in = c + 4 * (lane & 7) < p.N;
+        const uint32_t to = base_buf + (ch & 1) * kSegment + (lane >> 3) * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          cp_async16(to + 512 * i + (((lane & 7) ^ ((4 * i + (lane >> 3)) & 7)) << 4),
+                     in ? p.base + (base_at[i] + c) : p.base, in);
+      }
+      cp_commit();
+    };
+    load_base(0);
+    load_base(1);
+    for (int ch = 0; ch < chunks; ++ch) {
+      const int buf = ch & 1, c = column(ch) + 32 * part;
+      float y[32];
+      // the base of this thread's row
+      cp_wait<1>();
+      __syncwarp();
       if (rows > 0) {
+        const uint32_t from = base_buf + buf * kSegment + lane * 128;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int c = c_step + 64 * half + 32 * u;
-          // the base, to the thread that has its row
+        for (int k = 0; k < 8; ++k) {
+          const uint4 v = ld4(from + ((k ^ (lane & 7)) << 4));
+          y[4 * k] = __uint_as_float(v.x);
+          y[4 * k + 1] = __uint_as_float(v.y);
+          y[4 * k + 2] = __uint_as_float(v.z);
+          y[4 * k + 3] = __uint_as_float(v.w);
+        }
+      }
+      __syncwarp();
+      load_base(ch + 2);
+      if (!warp_wait(tfull + 8 * buf, (ch >> 1) & 1, stop, p.err)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (rows > 0 && rank_p > 0) {
+        uint32_t acc[32];
+        const uint32_t d = tmem + buf * kChunk + lanes;
+        // two gate groups and two up groups, or 32 columns in order
+        tmem_ld16(d + (p.interleaved ? 16 * part : 32 * part), acc);
+        tmem_ld16(d + (p.interleaved ? 64 + 16 * part : 32 * part + 16), acc + 16);
+        tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + (lane >> 3);
-            const float4 v = u == 0 ? v0[i] : v1[i];
-            st4(x + r * 128 + (((lane & 7) ^ (r & 7)) << 4), __float_as_uint(v.x), __float_as_uint(v.y),
-                __float_as_uint(v.z), __float_as_uint(v.w));
-          }
-          uint32_t acc[32];
-          const uint32_t d = tmem + buf * 256 + 64 * half + 32 * u + ((uint32_t)row0 << 16);
-          if (rank_p > 0) {
+        for (int k = 0; k < 32; ++k)
+          y[k] += __uint_as_float(p.interleaved ? acc[(k & 7) + ((k >> 4) << 3) + ((k >> 3 & 1) << 4)] : acc[k]);
+      }
+      // the accumulators are in registers: the next MMAs may have them
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(tempty + 8 * buf);
+      if (rows > 0) {
+        // the results, rows of up to 64 bytes at a time
+        const int c_out = EPI == kLoraSwiGLU ? c / 2 : c;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tmem_ld8(d + 8 * k + (p.interleaved ? (k & 1) * kChunk : 0), acc + 8 * k);
-            tmem_wait_ld();
-            if (!p.interleaved && j1 > j0 && c < p.N && slice_of(p, min(c + 31, p.N - 1)) != j0) {
-              uint32_t other[32];  // a slice ends in or before these columns
-#pragma unroll
-              for (int k = 0; k < 4; ++k) tmem_ld8(d + kChunk + 8 * k, other + 8 * k);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (slice_of(p, c + k) != j0) acc[k] = other[k];
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) acc[k] = 0u;
-          }
-          __syncwarp();
-          float y[32];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint4 v = ld4(x + lane * 128 + ((k ^ (lane & 7)) << 4));
-            y[4 * k] = __uint_as_float(v.x) + __uint_as_float(acc[4 * k]);
-            y[4 * k + 1] = __uint_as_float(v.y) + __uint_as_float(acc[4 * k + 1]);
-            y[4 * k + 2] = __uint_as_float(v.z) + __uint_as_float(acc[4 * k + 2]);
-            y[4 * k + 3] = __uint_as_float(v.w) + __uint_as_float(acc[4 * k + 3]);
-          }
-          __syncwarp();
-          // the results of the row, 16 bytes at a time
-          constexpr int kChunks = kOutBytes / 16;
+        for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
           for (int k = 0; k < kChunks; ++k) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               if constexpr (EPI == kLoraF32) {
-                w[e] = __float_as_uint(y[4 * k + e]);
+                w[e] = __float_as_uint(y[16 * h + 4 * k + e]);
               } else if constexpr (EPI == kLoraBf16) {
                 w[e] = pack2(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]);
               } else {  // 16 k: gate, 16 k + 8: up
@@ -393,35 +453,24 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
                              silu(y[16 * k + 2 * e + 1]) * y[16 * k + 9 + 2 * e]);
               }
             }
-            st4(x + lane * 128 + ((k ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+            st4(place(lane, k), w[0], w[1], w[2], w[3]);
           }
           __syncwarp();
-          const int c_out = EPI == kLoraSwiGLU ? c / 2 : c;
-          constexpr int kPer = 16 / (EPI == kLoraF32 ? 4 : 2);
 #pragma unroll
           for (int i = 0; i < kChunks; ++i) {
             const int at = 32 * i + lane, r = at / kChunks, k = at % kChunks;
-            const int tok = r < rows ? s_tok[row0 + r] : -1;
-            if (tok >= 0 && c_out + k * kPer < n_out) {
-              const uint4 v = ld4(x + r * 128 + ((k ^ (r & 7)) << 4));
-              const int64_t o = tok * p.out_stride + c_out + k * kPer;
+            const int col = c_out + 16 * h;
+            if ((has >> i & 1u) && col + k * kPer < n_out) {
+              const uint4 q = ld4(place(r, k));
               if constexpr (EPI == kLoraF32)
-                *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + o) = v;
+                *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + (out_at[i] + col)) = q;
               else
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + o) = v;
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + (out_at[i] + col)) = q;
             }
           }
           __syncwarp();
-          // this segment's base of the next step
-          if (step + 1 < steps) {
-            const int next = column(step + 1) + 64 * half + 32 * u;
-            if (u == 0) load_base(next, v0); else load_base(next, v1);
-          }
         }
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(tempty + 8 * buf);
     }
   }
   __syncwarp();
@@ -433,12 +482,10 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
 
 template <int EPI>
 int launch(const ExpandArgs& p, cudaStream_t s) {
-  const Layout l = layout<EPI == kLoraF32 ? 3 : 2>(p.ns, p.rank_pm);
-  if (l.stages == 0) return MS_ERR_UNSUPPORTED;
+  const int bytes = ring_bytes(EPI == kLoraF32 ? 3 : 2, p.ns, p.rank_pm);
+  if (bytes == 0) return MS_ERR_UNSUPPORTED;
   static std::atomic<uint64_t> granted{0};
   MS_TRY(grant_dynamic_smem(lora_expand_tc_kernel<EPI>, kMostBytes, granted));
-  // at least half the shared memory, so that no second CTA waits for TMEM on the SM
-  const int bytes = l.bytes > 116 * 1024 ? l.bytes : 116 * 1024;
   // CTAs per pair of tiles: the number whose rounds over the GPU take the
   // fewest steps, a CTA's start counted as four
   const int pairs = (p.plan.n_tiles + 1) / 2, chunks = ceil_div(p.N, kChunk);
@@ -459,11 +506,8 @@ int launch(const ExpandArgs& p, cudaStream_t s) {
 
 int lora_expand_tc(const ExpandArgs& p, int epilogue, cudaStream_t s) {
   if (p.rank_pm == 0) return MS_ERR_UNSUPPORTED;
-  // no 128 columns with three slices
-  for (int k = 0; !p.interleaved && k + 2 < p.ns; ++k)
-    if (p.slice_end[k] / kChunk == (p.slice_end[k + 1] - 1) / kChunk &&
-        p.slice_end[k + 1] % kChunk != 0 && p.slice_end[k] % kChunk != 0)
-      return MS_ERR_UNSUPPORTED;
+  const int64_t most = p.base_stride > p.out_stride ? p.base_stride : p.out_stride;
+  if (p.plan.n_tokens * most > (int64_t)UINT32_MAX) return MS_ERR_UNSUPPORTED;  // 32-bit offsets
   if (epilogue == kLoraSwiGLU) return launch<kLoraSwiGLU>(p, s);
   return epilogue == kLoraF32 ? launch<kLoraF32>(p, s) : launch<kLoraBf16>(p, s);
 }
