@@ -159,6 +159,7 @@ int ring_bytes(int terms, int ns, int rank_pm) {
 template <int EPI>
 __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs p) {
   constexpr int TERMS = EPI == kLoraF32 ? 3 : 2;
+  const bool parted = EPI == kLoraSwiGLU || p.interleaved;  // gate | up columns
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ int s_tok[kRows];
   const uint32_t raw = s_addr(smem_raw);
@@ -203,9 +204,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   const int chunks = (n_chunks - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   auto column = [&](int chunk) { return ((int)blockIdx.x + chunk * (int)gridDim.x) * kChunk; };
   // The passes of a chunk: one, or one per slice where a slice ends inside.
-  auto first_slice = [&](int c) { return p.interleaved ? 0 : slice_of(p, c); };
+  auto first_slice = [&](int c) { return parted ? 0 : slice_of(p, c); };
   auto passes = [&](int c) {
-    return p.interleaved ? 1 : slice_of(p, min(c + kChunk, p.N) - 1) - slice_of(p, c) + 1;
+    return parted ? 1 : slice_of(p, min(c + kChunk, p.N) - 1) - slice_of(p, c) + 1;
   };
 
   if (threadIdx.x < kRows)
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
     auto load_b = [&](uint32_t dst, int c0, int pass) {
       const int c = c0 + 8 * q;
       // block and place of these 8 columns: gate | up parted, else in order
-      const int block = p.interleaved ? q & 1 : q >> 3, at = p.interleaved ? q >> 1 : q & 7;
+      const int block = parted ? q & 1 : q >> 3, at = parted ? q >> 1 : q & 7;
       const uint32_t to = dst + block * (rank_p * 128);
       const bool in = c < p.N;
       const bool split = passes(c0) > 1;
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
               for (int k = 16; k < rank_p; k += 16) umma(to, ae + k / 2, bj + k * 8, id, 1u);
             }
           };
-          if (rank_p > 0 && p.interleaved) {
+          if (rank_p > 0 && parted) {
             for (int j = 0; j < 2; ++j) {
               acc = 0;
               products(d + 64 * j, tmem + kSAt + j * slice, b0 + j * (lead >> 4), instr(64));
@@ -423,12 +424,12 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
         uint32_t acc[32];
         const uint32_t d = tmem + buf * kChunk + lanes;
         // two gate groups and two up groups, or 32 columns in order
-        tmem_ld16(d + (p.interleaved ? 16 * part : 32 * part), acc);
-        tmem_ld16(d + (p.interleaved ? 64 + 16 * part : 32 * part + 16), acc + 16);
+        tmem_ld16(d + (parted ? 16 * part : 32 * part), acc);
+        tmem_ld16(d + (parted ? 64 + 16 * part : 32 * part + 16), acc + 16);
         tmem_wait_ld();
 #pragma unroll
         for (int k = 0; k < 32; ++k)
-          y[k] += __uint_as_float(p.interleaved ? acc[(k & 7) + ((k >> 4) << 3) + ((k >> 3 & 1) << 4)] : acc[k]);
+          y[k] += __uint_as_float(parted ? acc[(k & 7) + ((k >> 4) << 3) + ((k >> 3 & 1) << 4)] : acc[k]);
       }
       // the accumulators are in registers: the next MMAs may have them
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
