@@ -22,6 +22,25 @@
 #include "lora_device.cuh"
 
 namespace ms {
+
+int launch_cluster(void (*kernel)(ShrinkArgs), dim3 grid, int threads, int smem, int split,
+                   cudaStream_t s, const ShrinkArgs& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {1, 1, (unsigned)split};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  (void)cudaLaunchKernelEx(&cfg, kernel, p);
+  return check_launch("lora_shrink");
+}
+
 namespace {
 
 // ---- first product, bf16 ------------------------------------------------------
@@ -35,28 +54,6 @@ namespace {
 // Each slice's rank rows are padded to a multiple of 16 (`rank_p`), with
 // zeros in s.
 constexpr int kShrinkWarps = 8;
-
-struct ShrinkArgs {
-  const __nv_bfloat16* x;
-  int64_t x_stride;
-  const __nv_bfloat16* a;
-  int K, ns, k_per;  // k_per: k values per CTA of a cluster, a multiple of 32
-  int terms;
-  int64_t s_stride;  // row stride of s (elements)
-  ms_lora_adapters ad;
-  ms_lora_plan plan;
-  __nv_bfloat16* s;  // row per position: [slice][term][rank_p]
-  int* err;
-};
-
-// v as `terms` bf16 terms at dst[0], dst[step], ...
-__device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int terms, float v) {
-  for (int k = 0; k < terms; ++k) {
-    const __nv_bfloat16 h = __float2bfloat16_rn(v);
-    dst[k * step] = h;
-    v -= __bfloat162float(h);
-  }
-}
 
 template <int MT, int NT>
 __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(ShrinkArgs p) {
@@ -75,12 +72,14 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   const __nv_bfloat16* ar[MT][2];
+  bool row_in[MT][2];  // the rows that pad the rank are zero
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int mp = min(m0 + 16 * m, rows - 16) + 8 * h + g;
       const int j = mp / rank_p, r = min(mp - j * rank_p, tile.rank - 1);
+      row_in[m][h] = mp - j * rank_p < tile.rank;
       ar[m][h] = p.a + ((int64_t)p.ns * tile.offset + j * tile.rank + r) * p.K + 8 * t;
     }
   const int k_end = min(p.K, (split + 1) * p.k_per);
@@ -102,7 +101,7 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          av[m][h] = in ? __ldg(reinterpret_cast<const uint4*>(ar[m][h] + k0)) : zero;
+          av[m][h] = in && row_in[m][h] ? __ldg(reinterpret_cast<const uint4*>(ar[m][h] + k0)) : zero;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
         xv[n] = in && 8 * n < count ? __ldg(reinterpret_cast<const uint4*>(xr[n] + k0)) : zero;
@@ -134,22 +133,9 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
       for (int w = 0; w < kShrinkWarps; ++w) v += s_red[w * kOuts + i];
       s_red[i] = v;  // only this thread reads or writes column i of the parts
     }
-    if (splits > 1) cluster.sync();
-    // each CTA of the cluster finishes a share of the outputs, the parts in cluster order
-    const float scale = p.ad.scales[tile.adapter];
-    for (int i = split * kShrinkWarps * 32 + threadIdx.x; i < todo; i += splits * kShrinkWarps * 32) {
-      float v = 0.f;
-      if (splits > 1) {
-        for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(s_red, k)[i];
-      } else {
-        v = s_red[i];
-      }
-      const int col = i / (16 * MT), mp = m0 + i % (16 * MT);
-      if (mp >= rows) continue;
-      const int j = mp / rank_p, r = mp - j * rank_p;
-      __nv_bfloat16* dst = p.s + (tile.start + first + col) * p.s_stride + j * p.terms * rank_p + r;
-      store_terms(dst, rank_p, p.terms, r < tile.rank ? v * scale : 0.f);
-    }
+    if (splits > 1) cluster.sync(); else __syncthreads();
+    finish_s(p, cluster, s_red, 16 * MT, tile.start + first, count, m0, min(16 * MT, rows - m0), rank_p,
+             p.ad.scales[tile.adapter]);
     // no CTA leaves, or starts on s_red again, while another reads its part
     if (splits > 1) cluster.sync(); else __syncthreads();
   }
@@ -248,22 +234,8 @@ __global__ void __launch_bounds__(256, 2) lora_shrink_tile_kernel(ShrinkArgs p) 
     for (int e = 0; e < 4; ++e)
       part[(16 * wm + g + 8 * (e >> 1)) * kOutLd + wn * (RB / 2) + 8 * n + 2 * t + (e & 1)] = acc[n][e];
   if (splits > 1) cluster.sync(); else __syncthreads();
-  // each CTA of the cluster finishes a share of the outputs, the parts in cluster order
-  const float scale = tile.rank > 0 ? p.ad.scales[tile.adapter] : 0.f;
-  const int here = min(RB, rows - m0);
-  for (int i = split * 256 + threadIdx.x; i < tile.count * RB; i += splits * 256) {
-    const int col = i / RB, row = i % RB;
-    if (row >= here) continue;
-    float v = 0.f;
-    if (splits > 1) {
-      for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(part, k)[col * kOutLd + row];
-    } else {
-      v = part[col * kOutLd + row];
-    }
-    const int mp = m0 + row, j = mp / rank_p, r = mp - j * rank_p;
-    store_terms(p.s + (tile.start + col) * p.s_stride + j * p.terms * rank_p + r, rank_p, p.terms,
-                v * scale);
-  }
+  finish_s(p, cluster, part, kOutLd, tile.start, tile.count, m0, min(RB, rows - m0), rank_p,
+           tile.rank > 0 ? p.ad.scales[tile.adapter] : 0.f);
   if (splits > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
 
@@ -601,25 +573,6 @@ int dispatch_expand(const ExpandArgs& p, cudaStream_t s) {
   return launch_expand<EPI, 4, 4>(p, s);
 }
 
-// Clusters of `split` CTAs along z.
-int launch_cluster(void (*kernel)(ShrinkArgs), dim3 grid, int threads, int smem, int split,
-                   cudaStream_t s, const ShrinkArgs& p) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = threads;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2]{};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim = {1, 1, (unsigned)split};
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  (void)cudaLaunchKernelEx(&cfg, kernel, p);
-  return check_launch("lora_shrink");
-}
-
 template <int MT, int NT>
 int launch_shrink(ShrinkArgs p, int rows, cudaStream_t s) {
   const int smem = kShrinkWarps * 16 * MT * 8 * NT * 4;
@@ -746,6 +699,8 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
       MS_TRY(dispatch_shrink<1>(p, rows, s));
     else if (mean <= 16)
       MS_TRY(dispatch_shrink<2>(p, rows, s));
+    else if (mean > kTcTokens)
+      MS_TRY(lora_shrink_tc(p, rows, s));
     else if (rows <= 64)
       MS_TRY(launch_shrink_tile<64>(p, rows, s));
     else

@@ -5,6 +5,19 @@
 
 namespace ms {
 
+struct ShrinkArgs {
+  const __nv_bfloat16* x;
+  int64_t x_stride;
+  const __nv_bfloat16* a;
+  int K, ns, k_per;  // k_per: k values per CTA of a cluster, a multiple of 32
+  int terms;
+  int64_t s_stride;  // row stride of s (elements)
+  ms_lora_adapters ad;
+  ms_lora_plan plan;
+  __nv_bfloat16* s;  // row per position: [slice][term][rank_p]
+  int* err;
+};
+
 enum LoraEpilogue { kLoraF32, kLoraBf16, kLoraSwiGLU };
 
 struct ExpandArgs {
@@ -124,10 +137,63 @@ __device__ __forceinline__ float silu(float x) {
   return x * r;
 }
 
+// Four neighbouring values as `terms` bf16 terms each, at dst, dst + step, ...
+__device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int terms, float4 v) {
+  for (int k = 0; k < terms; ++k) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    uint2 w;
+    w.x = *reinterpret_cast<const uint32_t*>(&a);
+    w.y = *reinterpret_cast<const uint32_t*>(&b);
+    *reinterpret_cast<uint2*>(dst + k * step) = w;
+    const float2 fa = __bfloat1622float2(a), fb = __bfloat1622float2(b);
+    v.x -= fa.x;
+    v.y -= fa.y;
+    v.z -= fb.x;
+    v.w -= fb.y;
+  }
+}
+
+// This CTA's share of a cluster's outputs: the parts ([token][ld] floats in each
+// CTA's shared memory) of tokens [0, count) and rank rows [m0, m0 + here), `here`
+// a multiple of 16, summed in cluster order, scaled, and stored as terms.
+template <typename Cluster>
+__device__ __forceinline__ void finish_s(const ShrinkArgs& p, const Cluster& cluster, const float* part,
+                                         int ld, int start, int count, int m0, int here, int rank_p,
+                                         float scale) {
+  const int splits = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
+  const int quads = here / 4;
+#pragma unroll 2
+  for (int o = split * blockDim.x + threadIdx.x; o < count * quads; o += splits * blockDim.x) {
+    const int col = o / quads, row = 4 * (o - col * quads);
+    const float* at = part + col * ld + row;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (splits > 1) {
+#pragma unroll 4
+      for (int k = 0; k < splits; ++k) {
+        const float4 q = *reinterpret_cast<const float4*>(cluster.map_shared_rank(at, k));
+        v.x += q.x;
+        v.y += q.y;
+        v.z += q.z;
+        v.w += q.w;
+      }
+    } else {
+      v = *reinterpret_cast<const float4*>(at);
+    }
+    const int j = (m0 + row) / rank_p, r = m0 + row - j * rank_p;
+    store_terms(p.s + (start + col) * p.s_stride + j * p.terms * rank_p + r, rank_p, p.terms,
+                make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
+  }
+}
+
 }  // namespace
 
 // The second product on tcgen05 (lora_tc.cu), for tiles of many tokens:
 // MS_ERR_UNSUPPORTED when the shape does not apply.
 int lora_expand_tc(const ExpandArgs& p, int epilogue, cudaStream_t s);
+// The first product likewise.
+int lora_shrink_tc(ShrinkArgs p, int rows, cudaStream_t s);
+// A launch of the first product in clusters of `split` CTAs along z.
+int launch_cluster(void (*kernel)(ShrinkArgs), dim3 grid, int threads, int smem, int split,
+                   cudaStream_t s, const ShrinkArgs& p);
 
 }  // namespace ms

@@ -1,4 +1,6 @@
-// The adapters' second product on tcgen05, for tiles of many tokens (prompts):
+// The adapters' products on tcgen05, for tiles of many tokens (prompts).
+//
+// The second one,
 //   y[t, n] = base[t, n] + sum_r B[r, n] s_{j(n)}[t, r],
 // with the epilogues of lora.cu.  A CTA takes up to 128 tokens of one adapter
 // (two neighbouring tiles of the plan) and goes through its share of the
@@ -20,6 +22,8 @@
 // TMEM: two accumulators of 128 columns, then s (up to 256).  One CTA per SM.
 // The kernel moves 4 bytes in per column and token and 1 to 4 out, and is
 // bound by HBM; shared memory sees the base twice and little else.
+#include <cooperative_groups.h>
+
 #include "lora_device.cuh"
 
 namespace ms {
@@ -68,7 +72,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop, int* err) {
   return __all_sync(0xffffffffu, bar_wait(bar, parity, stop, err));
 }
-// Descriptor of adapter rows, MN-major with the 128-byte swizzle: 64 columns per
+// Descriptors with the 128-byte swizzle.  K-major: rows of 64 k values, groups of
+// 8 rows 1024 bytes apart (lead 16: not used).  Adapter rows, MN-major: 64 columns per
 // 128-byte row, groups of 8 k rows 1024 bytes apart (stride offset), blocks of
 // 64 columns `lead` bytes apart.
 __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
@@ -91,6 +96,16 @@ __device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b, uint32_
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(id), "r"(accumulate)
+      : "memory");
+}
+// The same with A in shared memory.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
@@ -150,6 +165,163 @@ __device__ int tiles_before(const ms_lora_plan& p, int i, int start, int adapter
   }
 }
 
+// The tokens of tile `index` and, when it continues it, of the next one: false
+// for a bad or empty tile and for one that the tile before has taken.  The same
+// for every warp.
+__device__ bool load_pair(const ms_lora_plan& p, const ms_lora_adapters& ad, int index, Tile& tile,
+                          int& count, int* err) {
+  if (!load_tile(p, ad, index, tile, err) || tile.count == 0) return false;
+  if (tiles_before(p, index, tile.start, tile.adapter) & 1) return false;
+  count = tile.count;
+  if (count == kTile && index + 1 < p.n_tiles) {
+    const int4 q = reinterpret_cast<const int4*>(p.tiles)[index + 1];
+    if (q.z == tile.adapter && q.x == tile.start + kTile) {
+      if (q.y >= 0 && q.y <= kTile && q.x <= p.n_tokens - q.y)
+        count += q.y;
+      else if (threadIdx.x == 0)
+        raise_device_error(err, kErrAdapter);
+    }
+  }
+  return true;
+}
+
+// ---- first product ---------------------------------------------------------------
+// s of up to 128 tokens x 256 rank rows per CTA: both operands K-major, k in steps
+// of 64 through a ring of four slots, two loading warps each; k is shared out
+// over a cluster, whose parts meet in distributed shared memory, summed in
+// cluster order.  x is read once.
+constexpr int kSteps = 4;                       // ring slots
+constexpr int kStepK = 64;
+constexpr int kRankRows = 256;                  // most rank rows per CTA
+constexpr int kStepBytes = (kRows + kRankRows) * 128;
+constexpr int kPartLd = kRankRows + 4;          // floats per token of the parts
+constexpr int kShrinkBytes = 1024 + kBarBytes + kSteps * kStepBytes;
+constexpr int kShrinkThreads = 288;             // 8 loading warps, 1 for the MMAs
+static_assert(kRows * kPartLd * 4 <= kSteps * kStepBytes, "the parts fit the ring");
+
+__global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(ShrinkArgs p) {
+  pdl_enter();
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ int s_tok[kRows];
+  __shared__ int s_row[kRankRows];  // row of A, -1: padding
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int splits = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
+  const uint32_t raw = s_addr(smem_raw);
+  const uint32_t ring = raw + ((1024u - (raw & 1023u)) & 1023u), bars = ring + kSteps * kStepBytes;
+  const uint32_t full = bars, empty = full + 8 * kSteps, done = empty + 8 * kSteps, slot_addr = done + 8;
+  unsigned char* gbars = smem_raw + (bars - raw);
+  volatile uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbars + (slot_addr - bars));
+  volatile int* stop = reinterpret_cast<int*>(gbars + (slot_addr - bars) + 4);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  Tile tile;
+  int count = 0;
+  if (!load_pair(p.plan, p.ad, blockIdx.x, tile, count, p.err)) return;  // the whole cluster alike
+  const int rank_p = pad16(tile.rank), rows = p.ns * rank_p, m0 = blockIdx.y * kRankRows;
+  if (m0 >= rows) return;
+  const int here = min(kRankRows, rows - m0);  // a multiple of 16
+  for (int i = tid; i < kRows; i += kShrinkThreads)
+    s_tok[i] = i < count ? token_at(p.plan, tile.start + i, p.err) : -1;
+  for (int i = tid; i < here; i += kShrinkThreads) {
+    const int j = (m0 + i) / rank_p, r = m0 + i - j * rank_p;
+    s_row[i] = r < tile.rank ? p.ns * tile.offset + j * tile.rank + r : -1;
+  }
+  if (tid == 0) {
+    for (int k = 0; k < kSteps; ++k) {
+      bar_init(full + 8 * k, 64);
+      bar_init(empty + 8 * k, 1);
+    }
+    bar_init(done, 1);
+    *stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_addr),
+                 "r"(kRankRows));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const int k_begin = split * p.k_per, k_end = min(p.K, k_begin + p.k_per);
+  const int steps = k_end > k_begin ? (k_end - k_begin + kStepK - 1) / kStepK : 0;
+
+  if (warp < 8) {
+    // ---- loads: 16 bytes at k offset 8 i of rows r0, r0 + 8, ...
+    const int group = warp >> 1, t = tid & 63, i = t & 7, r0 = t >> 3;
+    bool alive = true;
+    for (int step = group; step < steps; step += kSteps) {
+      if (step >= kSteps) {
+        alive = warp_wait(empty + 8 * group, (step / kSteps - 1) & 1, stop, p.err);
+        if (!alive) break;
+      }
+      const int k = k_begin + step * kStepK + 8 * i;
+      const bool in = k < k_end;
+      // (row & 7 is r0 for all of a thread's rows)
+      const uint32_t to = ring + group * kStepBytes + r0 * 128 + ((i ^ r0) << 4);
+      const __nv_bfloat16* x = p.x + (in ? k : 0);
+#pragma unroll 8
+      for (int r = 0; r < kRows; r += 8) {
+        const int tok = s_tok[r + r0];
+        cp_async16(to + r * 128, x + max(tok, 0) * p.x_stride, in && tok >= 0);
+      }
+      const __nv_bfloat16* a = p.a + (in ? k : 0);
+#pragma unroll 8
+      for (int r = 0; r < here; r += 8) {
+        const int row = s_row[r + r0];
+        cp_async16(to + kRows * 128 + r * 128, a + (int64_t)max(row, 0) * p.K, in && row >= 0);
+      }
+      cp_commit();
+      cp_wait<0>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(full + 8 * group);
+    }
+    // ---- the accumulators: lane quarter warp & 3, half the columns
+    if (steps > 0) alive = alive && warp_wait(done, 0, stop, p.err);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    float* part = reinterpret_cast<float*>(smem_raw + (ring - raw));  // [token][kPartLd]
+    const int row0 = 32 * (warp & 3), c0 = (warp >> 2) * 128;
+    for (int c = c0; c < min(here, c0 + 128); c += 16) {
+      uint32_t r[16];
+      if (steps > 0) {
+        tmem_ld16(tmem + c + ((uint32_t)row0 << 16), r);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) r[e] = 0u;
+      }
+      uint4* dst = reinterpret_cast<uint4*>(part + (row0 + lane) * kPartLd + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  } else if (lane == 0) {
+    // ---- MMA
+    const uint32_t id = instr(here) & ~(1u << 16);  // B K-major as well
+    bool fine = true;
+    for (int step = 0; step < steps && fine; ++step) {
+      const int slot = step % kSteps;
+      if (!(fine = bar_wait(full + 8 * slot, (step / kSteps) & 1, stop, p.err))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t x = desc(ring + slot * kStepBytes, 16), a = desc(ring + slot * kStepBytes + kRows * 128, 16);
+#pragma unroll
+      for (int k = 0; k < kStepK / 16; ++k) umma_ss(tmem, x + 2 * k, a + 2 * k, id, step > 0 || k > 0);
+      umma_commit(empty + 8 * slot);
+    }
+    if (fine && steps > 0) umma_commit(done);
+  }
+  __syncwarp();
+  if (splits > 1) cluster.sync(); else __syncthreads();
+  finish_s(p, cluster, reinterpret_cast<const float*>(smem_raw + (ring - raw)), kPartLd, tile.start,
+           count, m0, here, rank_p, p.ad.scales[tile.adapter]);
+  if (splits > 1) cluster.sync(); else __syncthreads();  // no CTA leaves while another reads its part
+  if (warp == 8)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kRankRows));
+}
+
 // Shared memory for a rank; 0 when it or TMEM do not do.
 int ring_bytes(int terms, int ns, int rank_pm) {
   const int bytes = 1024 + kBarBytes + kEpiWarps * kEpiBytes + kStages * rank_pm * kChunk * 2;
@@ -178,23 +350,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   // The plan and the adapters are read before the launch wait (see lora.cu).
   if (!p.after_shrink) pdl_enter();
   Tile tile;
-  const int index = blockIdx.y;
-  bool work = load_tile(p.plan, p.ad, index, tile, p.err) && tile.count > 0 &&
-              !(p.in_place && tile.rank == 0);
-  int count = tile.count;
-  if (work) {
-    if (tiles_before(p.plan, index, tile.start, tile.adapter) & 1) {
-      work = false;  // the CTA of the tile before has this one
-    } else if (count == kTile && index + 1 < p.plan.n_tiles) {
-      const int4 q = reinterpret_cast<const int4*>(p.plan.tiles)[index + 1];
-      if (q.z == tile.adapter && q.x == tile.start + kTile) {
-        if (q.y >= 0 && q.y <= kTile && q.x <= p.plan.n_tokens - q.y)
-          count += q.y;
-        else if (threadIdx.x == 0)
-          raise_device_error(p.err, kErrAdapter);
-      }
-    }
-  }
+  int count = 0;
+  const bool work = load_pair(p.plan, p.ad, blockIdx.y, tile, count, p.err) &&
+                    !(p.in_place && tile.rank == 0);
   if (!work) {
     if (p.after_shrink) pdl_enter();
     return;
@@ -504,6 +662,18 @@ int launch(const ExpandArgs& p, cudaStream_t s) {
 }
 
 }  // namespace
+
+int lora_shrink_tc(ShrinkArgs p, int rows, cudaStream_t s) {
+  static std::atomic<uint64_t> granted{0};
+  MS_TRY(grant_dynamic_smem(lora_shrink_tc_kernel, kShrinkBytes, granted));
+  // as many CTAs along k as one round over the GPU takes, at least 256 k values each
+  const int blocks = ceil_div(rows, kRankRows), ctas = (p.plan.n_tiles + 1) / 2 * blocks;
+  int split = 1;
+  while (split < 8 && 2 * split * ctas <= 148 && p.K / (2 * split) >= 256) split *= 2;
+  p.k_per = ceil_div(ceil_div(p.K, split), kStepK) * kStepK;
+  return launch_cluster(lora_shrink_tc_kernel, dim3(p.plan.n_tiles, blocks, split), kShrinkThreads,
+                        kShrinkBytes, split, s, p);
+}
 
 int lora_expand_tc(const ExpandArgs& p, int epilogue, cudaStream_t s) {
   if (p.rank_pm == 0) return MS_ERR_UNSUPPORTED;
