@@ -301,7 +301,7 @@ __device__ __forceinline__ void expand_mma(float (&acc)[4][4], uint32_t sa, uint
 }
 
 template <int EPI, int WM, int WN>
-__global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p) {
+__global__ void __launch_bounds__(32 * WM * WN, WM * WN == 16 ? 2 : 1) lora_expand_kernel(ExpandArgs p) {
   constexpr int TERMS = EPI == kLoraF32 ? 3 : 2;
   constexpr int kTm = 16 * WM, kCols = 32 * WN, kThreads = 32 * WM * WN;
   constexpr int kBaseLd = kCols + kPad, kBLd = kCols + kPad;
@@ -346,16 +346,37 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
       dst += kBRows * kBLd * 2;
     }
   };
-  auto load_base = [&](int c, int slot, int first, int here) {
-    float* s_base = reinterpret_cast<float*>(ring + slot * stage_bytes);
-    const int q = 4 * (threadIdx.x % (kCols / 4)), r0 = threadIdx.x / (kCols / 4);
-    const bool in = c + q < p.N;
-    uint32_t dst = s_addr(s_base + r0 * kBaseLd + q);
-    for (int r = r0; r < here; r += kBaseRows) {
-      const int tok = s_tok[first + r];
-      cp_async16(dst, in && tok >= 0 ? p.base + tok * p.base_stride + c + q : p.base, in && tok >= 0);
-      dst += kBaseRows * kBaseLd * 4;
+  // Element offsets (lora_add checks that they fit 32 bits) of the rows that
+  // this thread loads, r0 + kBaseRows i, and of those it stores.
+  constexpr int kBaseLoads = kTm / kBaseRows;
+  constexpr int kChunks = EPI == kLoraF32 ? 8 : EPI == kLoraBf16 ? 4 : 2;  // of 16 bytes per row
+  constexpr int kPer = EPI == kLoraF32 ? 4 : 8;                            // outputs per chunk
+  constexpr int kStores = kChunks / 2;                                     // 16 rows
+  uint32_t base_at[kBaseLoads], out_at[kStores], has = 0;
+  const int base_q = 4 * (threadIdx.x % (kCols / 4)), base_r = threadIdx.x / (kCols / 4);
+  auto find_rows = [&](int first, int here) {
+    has = 0;
+#pragma unroll
+    for (int i = 0; i < kBaseLoads; ++i) {
+      const int r = base_r + kBaseRows * i, tok = r < here ? s_tok[first + r] : -1;
+      has |= (uint32_t)(tok >= 0) << i;
+      base_at[i] = (uint32_t)(max(tok, 0) * p.base_stride + base_q);
     }
+#pragma unroll
+    for (int i = 0; i < kStores; ++i) {
+      const int at = lane + 32 * i, r = 16 * wm + at / kChunks;
+      const int tok = r < here ? s_tok[first + r] : -1;
+      has |= (uint32_t)(tok >= 0) << (16 + i);
+      out_at[i] = (uint32_t)(max(tok, 0) * p.out_stride + at % kChunks * kPer);
+    }
+  };
+  auto load_base = [&](int c, int slot) {
+    const bool in = c + base_q < p.N;
+    const uint32_t dst = s_addr(reinterpret_cast<float*>(ring + slot * stage_bytes) + base_r * kBaseLd + base_q);
+#pragma unroll
+    for (int i = 0; i < kBaseLoads; ++i)
+      if (has >> i & 1u)
+        cp_async16(dst + i * kBaseRows * kBaseLd * 4, in ? p.base + (base_at[i] + c) : p.base, in);
   };
   if (work && p.after_shrink) load_b(c_first, 0);
   if (p.after_shrink) pdl_enter();
@@ -364,6 +385,7 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
   for (int first = 0; first < tile.count; first += kTm) {
     const int here = min(tile.count - first, kTm);
     if (first > 0) __syncthreads();  // the last pass is done with s and the ring
+    find_rows(first, here);
     for (int i = threadIdx.x; i < here * (s_row / 8); i += kThreads) {
       const int row = i / (s_row / 8), q = 8 * (i - row * (s_row / 8));
       cp_async16(s_addr(s_s + row * s_ld + q), p.s + (tile.start + first + row) * p.s_stride + q, true);
@@ -371,7 +393,7 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
     for (int k = 0; k + 1 < p.stages; ++k) {
       if (c_first + k * step < p.N) {
         if (first > 0 || k > 0 || !p.after_shrink) load_b(c_first + k * step, k);
-        load_base(c_first + k * step, k, first, here);
+        load_base(c_first + k * step, k);
       }
       cp_commit();
     }
@@ -383,7 +405,7 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
       if (cn < p.N) {
         const int free = slot == 0 ? p.stages - 1 : slot - 1;
         load_b(cn, free);
-        load_base(cn, free, first, here);
+        load_base(cn, free);
       }
       cp_commit();
       const int c = c0 + 32 * wn, m = 16 * wm;
@@ -392,15 +414,18 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
           reinterpret_cast<const __nv_bfloat16*>(ring + slot * stage_bytes + kBaseBytes) + 32 * wn;
       slot = slot + 1 == p.stages ? 0 : slot + 1;
       if (m >= here || c >= p.N) continue;
-      float acc[4][4];
+      const bool upper = here - m > 8;  // tokens in the upper 8 rows
+      float acc[4][4] = {};
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !upper) break;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int n = 0; n < 4; ++n) {
           const float2 v = *reinterpret_cast<const float2*>(s_base + (g + 8 * h) * kBaseLd + 8 * n + 2 * t);
           acc[n][2 * h] = v.x;
           acc[n][2 * h + 1] = v.y;
         }
+      }
       const uint32_t sa = s_addr(s_s + (m + (lane & 15)) * s_ld + 8 * (lane >> 4));
       const uint32_t sb = s_addr(s_b + (lane & 15) * kBLd + 8 * (lane >> 4));
       if (p.interleaved) {
@@ -416,6 +441,7 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
       __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !upper) break;
         float* row = s_base + (g + 8 * h) * kBaseLd;
         if constexpr (EPI == kLoraSwiGLU) {
 #pragma unroll
@@ -435,21 +461,16 @@ __global__ void __launch_bounds__(32 * WM * WN) lora_expand_kernel(ExpandArgs p)
         }
       }
       __syncwarp();
-      constexpr int kChunks = EPI == kLoraF32 ? 8 : EPI == kLoraBf16 ? 4 : 2;  // of 16 bytes per row
-      constexpr int kPer = EPI == kLoraF32 ? 4 : 8;                            // outputs per chunk
       const int c_out = EPI == kLoraSwiGLU ? c / 2 : c, n_out = EPI == kLoraSwiGLU ? p.N / 2 : p.N;
 #pragma unroll
-      for (int i = lane; i < 16 * kChunks; i += 32) {
-        const int row = i / kChunks, q = i % kChunks;
-        if (m + row >= here || c_out + q * kPer >= n_out) continue;
-        const int tok = s_tok[first + m + row];
-        if (tok < 0) continue;
-        const int64_t at = tok * p.out_stride + c_out + q * kPer;
+      for (int i = 0; i < kStores; ++i) {
+        const int at = lane + 32 * i, row = at / kChunks, q = at % kChunks;
+        if (!(has >> (16 + i) & 1u) || c_out + q * kPer >= n_out) continue;
         const float4 v = reinterpret_cast<const float4*>(s_base + row * kBaseLd)[q];
         if constexpr (EPI == kLoraF32)
-          *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+          *reinterpret_cast<float4*>(static_cast<float*>(p.out) + (out_at[i] + c_out)) = v;
         else
-          *reinterpret_cast<float4*>(static_cast<__nv_bfloat16*>(p.out) + at) = v;
+          *reinterpret_cast<float4*>(static_cast<__nv_bfloat16*>(p.out) + (out_at[i] + c_out)) = v;
       }
     }
   }
@@ -672,7 +693,10 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
                       c.N % (c.swiglu ? 16 : 8) == 0 && aligned(c.x, 16) && aligned(c.a, 16) &&
                       aligned(c.b, 16) && aligned(c.base, 16) && c.base_stride % 4 == 0 &&
                       aligned(c.out, 16) && c.out_stride % (out_f32 ? 4 : 8) == 0 &&
-                      !(c.swiglu && out_f32);
+                      !(c.swiglu && out_f32) &&
+                      // 32-bit element offsets in the second product
+                      plan.n_tokens * (c.base_stride > c.out_stride ? c.base_stride : c.out_stride) <=
+                          (int64_t)UINT32_MAX;
   if (!tensor) {
     if (c.dtype == MS_DTYPE_F32 && out_f32) return launch_any<float, float>(c, e, s);
     if (c.dtype == MS_DTYPE_F32) return launch_any<float, __nv_bfloat16>(c, e, s);

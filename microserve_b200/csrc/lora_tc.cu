@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
     constexpr int kHalves = EPI == kLoraF32 ? 2 : 1;
     constexpr int kChunks = EPI == kLoraSwiGLU ? 2 : 4;  // of 16 bytes per row
     constexpr int kPer = EPI == kLoraF32 ? 4 : 8;        // outputs per chunk
-    // element offsets of this lane's output rows (the launch checks that they fit 32 bits)
+    // element offsets of this lane's output rows (lora_add checks that they fit 32 bits)
     uint32_t out_at[kChunks], has = 0;
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
@@ -677,8 +677,6 @@ int lora_shrink_tc(ShrinkArgs p, int rows, cudaStream_t s) {
 
 int lora_expand_tc(const ExpandArgs& p, int epilogue, cudaStream_t s) {
   if (p.rank_pm == 0) return MS_ERR_UNSUPPORTED;
-  const int64_t most = p.base_stride > p.out_stride ? p.base_stride : p.out_stride;
-  if (p.plan.n_tokens * most > (int64_t)UINT32_MAX) return MS_ERR_UNSUPPORTED;  // 32-bit offsets
   if (epilogue == kLoraSwiGLU) return launch<kLoraSwiGLU>(p, s);
   return epilogue == kLoraF32 ? launch<kLoraF32>(p, s) : launch<kLoraBf16>(p, s);
 }
