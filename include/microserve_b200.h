@@ -35,6 +35,7 @@ extern "C" {
 #define MS_ERR_CUDA 2        /* a CUDA runtime call or launch failed         */
 #define MS_ERR_UNSUPPORTED 3 /* shape/dtype combination not compiled         */
 #define MS_ERR_TOO_LARGE 4   /* size beyond a documented fixed maximum       */
+#define MS_ERR_WORKSPACE 5   /* ms_lora_add: workspace missing or too small  */
 
 #define MS_DTYPE_F32 0
 #define MS_DTYPE_BF16 1
@@ -407,9 +408,11 @@ typedef struct {
  * alternating every 8 columns, as w_gate_up.  swiglu: out (N/2 columns) =
  * silu(gate) * up of those.  out may be base (float32, no SwiGLU): then tokens
  * without an adapter are not touched; otherwise the two must not overlap.
- * The workspace is 16-byte aligned scratch of this call alone.  Tokens of no
- * tile are left as they were.  A bad tile, token or adapter
- * sets the device error word and is skipped. */
+ * The workspace is 16-byte aligned scratch of this call alone.  Calls of little
+ * work take one launch that needs none (NULL, 0 bytes); MS_ERR_WORKSPACE, before
+ * anything is launched, says that a call does need it.  Tokens of no tile are
+ * left as they were.  A bad tile, token or adapter sets the device error word
+ * and is skipped. */
 MS_API size_t ms_lora_workspace_size(const ms_lora_adapters* adapters, const ms_lora_plan* plan,
                                      int n_slices);
 MS_API int ms_lora_add(const void* x, int64_t x_stride, const float* base, int64_t base_stride,

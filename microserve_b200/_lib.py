@@ -22,6 +22,7 @@ MS_ERR_INVALID = 1
 MS_ERR_CUDA = 2
 MS_ERR_UNSUPPORTED = 3
 MS_ERR_TOO_LARGE = 4
+MS_ERR_WORKSPACE = 5
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
@@ -326,15 +327,19 @@ def cuda_index(t: torch.Tensor) -> int:
     return index
 
 
-def launch_on(index: int, name: str, *args: object) -> None:
-    """``call(name, *args, stream)`` on device ``index`` and its current stream (kernels are
-    launched on the current device, whichever device their stream belongs to)."""
+def launch_status(index: int, name: str, *args: object) -> int:
+    """The status of ``name(*args, stream)`` on device ``index`` and its current stream (kernels
+    are launched on the current device, whichever device their stream belongs to)."""
     fn = getattr(_lib or load(), name)
     if index == torch._C._cuda_getDevice():
-        rc = fn(*args, raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, raw_stream(index))
+        return fn(*args, raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, raw_stream(index))
+
+
+def launch_on(index: int, name: str, *args: object) -> None:
+    """:func:`launch_status`, raising on failure."""
+    rc = launch_status(index, name, *args)
     if rc != MS_OK:
         check(name, rc)
 

@@ -239,6 +239,126 @@ __global__ void __launch_bounds__(256, 2) lora_shrink_tile_kernel(ShrinkArgs p) 
   if (splits > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
 
+// ---- both products in one launch, for a few tokens ----------------------------------
+// A call of a few tokens and a rank of at most 16 is bound by the host's launches
+// and by latency.  A cluster of 8 CTAs takes a tile: its CTAs share out k for the
+// first product (as lora_shrink_kernel, 16 rows of A, 8 tokens at a time), meet,
+// and share out the columns for the second, on the CUDA cores: a thread has 2
+// columns of 8 tokens, s stays float32.  B and the base, which the first product
+// does not wait for, are loaded before it.
+// One token at 2048 x 2048, rank 16: 20 us a call from the host and 5.4 us in a
+// replayed graph, to 28 and 6.3 us as two launches; 32 tokens of 32 adapters at
+// 4096 x 4096, 9.7 to 10.3 us in a graph.  K = 14336 costs a graph 0.7 us more than
+// two launches, and the host 8 us less.  The rule (one_launch) stops where a graph
+// would lose much: at rank 64, 9.9 to 6.8 us; at 28672 columns, 14.5 to 9.1 us.
+constexpr int kOneTokens = 8;
+constexpr int kOneRank = 16;
+constexpr int kOneSplit = 8;
+constexpr int kOneN = kOneSplit * kShrinkWarps * 64;  // 4096 columns
+
+template <typename TO>
+__global__ void __launch_bounds__(kShrinkWarps * 32) lora_one_kernel(ShrinkArgs p, ExpandArgs e) {
+  pdl_enter();
+  __shared__ float s_red[kShrinkWarps][kOneTokens][kOneRank];
+  __shared__ float s_part[kOneTokens][kOneRank];  // this CTA's share of k
+  __shared__ __align__(16) float s_sum[kOneTokens][kOneRank];
+  __shared__ int s_tok[kOneTokens];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int split = (int)cluster.block_rank();
+  Tile tile;
+  if (!load_tile(p.plan, p.ad, blockIdx.x, tile, p.err)) return;  // the whole cluster alike
+  if (tile.count == 0 || (e.in_place && tile.rank == 0)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int k_end = min(p.K, (split + 1) * p.k_per);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const float scale = tile.rank > 0 ? p.ad.scales[tile.adapter] : 0.f;
+
+  const int per = (e.N + 2 * kOneSplit - 1) / (2 * kOneSplit) * 2;  // columns of a CTA, at most 512
+  const int c = split * per + 2 * threadIdx.x;
+  const bool in = 2 * threadIdx.x < per && c < e.N;
+  __nv_bfloat162 w[kOneRank];
+  const __nv_bfloat16* b = e.b + (int64_t)tile.offset * e.N + c;
+#pragma unroll
+  for (int r = 0; r < kOneRank; ++r)
+    w[r] = in && r < tile.rank ? __ldg(reinterpret_cast<const __nv_bfloat162*>(b + r * e.N))
+                               : __nv_bfloat162{};
+
+  for (int first = 0; first < tile.count; first += kOneTokens) {
+    const int count = min(tile.count - first, kOneTokens);
+    if (threadIdx.x < kOneTokens)
+      s_tok[threadIdx.x] =
+          threadIdx.x < count ? token_at(p.plan, tile.start + first + threadIdx.x, p.err) : -1;
+    __syncthreads();
+    float2 base[kOneTokens];
+#pragma unroll
+    for (int k = 0; k < kOneTokens; ++k) {
+      const int tok = s_tok[k];
+      base[k] = in && tok >= 0 ? *reinterpret_cast<const float2*>(e.base + tok * e.base_stride + c)
+                               : make_float2(0.f, 0.f);
+    }
+    if (tile.rank > 0) {
+      const __nv_bfloat16* xr = p.x + (int64_t)max(s_tok[min(g, count - 1)], 0) * p.x_stride + 8 * t;
+      const __nv_bfloat16* ar[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        ar[h] = p.a + (int64_t)(tile.offset + min(8 * h + g, tile.rank - 1)) * p.K + 8 * t;
+      float acc[4] = {};
+#pragma unroll 2
+      for (int k0 = split * p.k_per + 32 * warp; k0 < k_end; k0 += 32 * kShrinkWarps) {
+        const bool kin = k0 + 8 * t < k_end;
+        const uint4 xv = kin ? __ldg(reinterpret_cast<const uint4*>(xr + k0)) : zero;
+        const uint4 a0 = kin && g < tile.rank ? __ldg(reinterpret_cast<const uint4*>(ar[0] + k0)) : zero;
+        const uint4 a1 = kin && 8 + g < tile.rank ? __ldg(reinterpret_cast<const uint4*>(ar[1] + k0)) : zero;
+        mma_bf16(acc, a0.x, a1.x, a0.y, a1.y, xv.x, xv.y);
+        mma_bf16(acc, a0.z, a1.z, a0.w, a1.w, xv.z, xv.w);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s_red[warp][2 * t + (q & 1)][g + 8 * (q >> 1)] = acc[q];
+      __syncthreads();
+      const int token = (threadIdx.x >> 4) & 7, row = threadIdx.x & 15;
+      if (threadIdx.x < kOneTokens * kOneRank) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < kShrinkWarps; ++k) v += s_red[k][token][row];
+        s_part[token][row] = v;
+      }
+      cluster.sync();
+      if (threadIdx.x < kOneTokens * kOneRank) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < kOneSplit; ++k) v += *cluster.map_shared_rank(&s_part[token][row], k);
+        s_sum[token][row] = row < tile.rank ? v * scale : 0.f;
+      }
+      cluster.sync();  // the parts have been read; s is complete
+    }
+#pragma unroll
+    for (int k = 0; k < kOneTokens; ++k) {
+      const int tok = s_tok[k];
+      if (!in || tok < 0) continue;
+      float x0 = 0.f, x1 = 0.f;
+      if (tile.rank > 0) {
+#pragma unroll
+        for (int r = 0; r < kOneRank; r += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(&s_sum[k][r]);
+          const float2 w0 = __bfloat1622float2(w[r]), w1 = __bfloat1622float2(w[r + 1]),
+                       w2 = __bfloat1622float2(w[r + 2]), w3 = __bfloat1622float2(w[r + 3]);
+          x0 = fmaf(s.x, w0.x, fmaf(s.y, w1.x, fmaf(s.z, w2.x, fmaf(s.w, w3.x, x0))));
+          x1 = fmaf(s.x, w0.y, fmaf(s.y, w1.y, fmaf(s.z, w2.y, fmaf(s.w, w3.y, x1))));
+        }
+      }
+      x0 += base[k].x;
+      x1 += base[k].y;
+      if constexpr (std::is_same_v<TO, float>)
+        *reinterpret_cast<float2*>(static_cast<float*>(e.out) + tok * e.out_stride + c) = make_float2(x0, x1);
+      else
+        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(e.out) + tok * e.out_stride + c) =
+            __floats2bfloat162_rn(x0, x1);
+    }
+    __syncthreads();  // s and the tokens have been read
+  }
+}
+
 // ---- second product, bf16 -----------------------------------------------------
 // A CTA keeps the s rows of up to 16 WM tokens of a tile in shared memory and
 // goes through its share of the columns, 32 WN at a step: their base values
@@ -477,61 +597,161 @@ __global__ void __launch_bounds__(32 * WM * WN, WM * WN == 16 ? 2 : 1) lora_expa
 }
 
 // ---- any type, size and alignment ----------------------------------------------
-// The float32 models and shapes the tensor-core kernels do not take: a CTA per
-// token; one warp per dot product of the first product, one thread per output
-// of the second.
-template <typename T>
-__global__ void lora_shrink_any_kernel(const T* __restrict__ x, int64_t x_stride,
-                                       const T* __restrict__ a, int K, int ns, int width,
-                                       ms_lora_adapters ad, ms_lora_plan plan,
-                                       float* __restrict__ s, int* err) {
-  pdl_enter();
-  Tile tile;
-  if (!load_tile(plan, ad, blockIdx.x, tile, err)) return;
-  const int q = blockIdx.y;
-  if (q >= tile.count) return;
-  const int tok = token_at(plan, tile.start + q, err);
-  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  const T* xr = x + (int64_t)max(tok, 0) * x_stride;
-  for (int m = threadIdx.x >> 5; m < ns * tile.rank; m += nw) {
-    const T* ar = a + ((int64_t)ns * tile.offset + m) * K;
-    float v = 0.f;
-    for (int k = lane; k < K; k += 32) v = fmaf(to_f(xr[k]), to_f(ar[k]), v);
-    v = warp_sum(v);
-    if (lane == 0) s[((int64_t)tile.start + q) * width + m] = v * ad.scales[tile.adapter];
+// The float32 models and shapes the tensor-core kernels do not take.  Second
+// product: a CTA has 8 tokens of a tile, a thread one output of each, so that an
+// element of B is read once for 8 tokens.  With K up to 256 the same CTA computes
+// its tokens' s (a warp per 4 rows of A, again for 8 tokens), which costs less than
+// another launch; above, a CTA of lora_shrink_any_kernel has 4 rows and 8 tokens,
+// its warps share out k.  Latency bounds both: in a replayed graph of float32
+// calls, one token to 256, K = 128 takes 5.6 to 7.9 us at rank 8 (6.9 to 9.9 as two
+// launches), K = 256 7.0 to 9.9 (7.2 to 11.3), K = 512 9.0 to 15.9 fused and 7.4 to
+// 9.1 as two launches; K = N = 2048 at rank 64 16 to 22 us.
+constexpr int kAnyTokens = 8;
+constexpr int kAnyThreads = 256;
+constexpr int kFusedK = 256;
+constexpr int kFusedRows = 256;
+
+// 4 rows of A times 8 tokens over this warp's k: lane l gets the sum for row
+// l / 8 and token l % 8 (a reduction that halves the values at every exchange: 31
+// shuffles for the 32 sums).
+template <typename T, typename X>
+__device__ __forceinline__ float dots_4x8(const T* a, int K, int row, int rows, X x, int k, int step) {
+  const int lane = threadIdx.x & 31;
+  const T* ar[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) ar[m] = a + (int64_t)min(row + m, rows - 1) * K;
+  float v[32] = {};
+#pragma unroll 2
+  for (int i = k + lane; i < K; i += step) {
+    float w[4], y[kAnyTokens];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) w[m] = to_f(ar[m][i]);
+#pragma unroll
+    for (int t = 0; t < kAnyTokens; ++t) y[t] = x(t, i);
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int t = 0; t < kAnyTokens; ++t) v[8 * m + t] = fmaf(y[t], w[m], v[8 * m + t]);
   }
+#pragma unroll
+  for (int h = 16; h > 0; h >>= 1)
+#pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const bool up = lane & h;
+      v[i] = (up ? v[i + h] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + h], h);
+    }
+  return v[0];
 }
 
-template <typename T, typename TO>
-__global__ void lora_expand_any_kernel(const T* __restrict__ b, TO* out, int swiglu, ExpandArgs p) {
+template <typename T>
+__global__ void __launch_bounds__(kAnyThreads)
+    lora_shrink_any_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ a, int K,
+                           int ns, int width, ms_lora_adapters ad, ms_lora_plan plan,
+                           float* __restrict__ s, int* err) {
   pdl_enter();
-  extern __shared__ __align__(16) float s_row[];  // the token's s
+  __shared__ float s_part[kAnyThreads / 32][32];
+  Tile tile;
+  if (!load_tile(plan, ad, blockIdx.x, tile, err)) return;
+  const int q0 = blockIdx.y * kAnyTokens, row = 4 * blockIdx.z, rows = ns * tile.rank;
+  if (q0 >= tile.count || row >= rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* xr[kAnyTokens];
+#pragma unroll
+  for (int t = 0; t < kAnyTokens; ++t)
+    xr[t] = x + (int64_t)max(token_at(plan, tile.start + min(q0 + t, tile.count - 1), err), 0) * x_stride;
+  s_part[warp][lane] = dots_4x8(a + (int64_t)ns * tile.offset * K, K, row, rows,
+                                [&](int t, int i) { return to_f(xr[t][i]); }, 32 * warp, kAnyThreads);
+  __syncthreads();
+  const int m = row + lane / kAnyTokens, q = q0 + lane % kAnyTokens;
+  if (warp > 0 || m >= rows || q >= tile.count) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < kAnyThreads / 32; ++k) v += s_part[k][lane];
+  s[((int64_t)tile.start + q) * width + m] = v * ad.scales[tile.adapter];
+}
+
+template <typename T, typename TO, bool FUSED>
+__global__ void __launch_bounds__(kAnyThreads)
+    lora_expand_any_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ a, int K,
+                           const T* __restrict__ b, TO* out, int swiglu, ExpandArgs p) {
+  pdl_enter();
+  extern __shared__ __align__(16) float s_any_mem[];
+  float4* s_row = reinterpret_cast<float4*>(s_any_mem);           // per rank row: the 8 tokens' s
+  float* s_x = s_any_mem + p.ns * p.ad.max_rank * kAnyTokens;     // FUSED: x, a row per token
+  __shared__ int s_tok[kAnyTokens];
   Tile tile;
   if (!load_tile(p.plan, p.ad, blockIdx.x, tile, p.err)) return;
-  const int q = blockIdx.y;
-  if (q >= tile.count || (p.in_place && tile.rank == 0)) return;
-  const int tok = token_at(p.plan, tile.start + q, p.err);
-  for (int i = threadIdx.x; i < p.ns * tile.rank; i += blockDim.x)
-    s_row[i] = p.s_any[((int64_t)tile.start + q) * p.width_any + i];
+  const int q0 = blockIdx.y * kAnyTokens, count = min(tile.count - q0, kAnyTokens);
+  if (count <= 0 || (p.in_place && tile.rank == 0)) return;
+  if (threadIdx.x < kAnyTokens)
+    s_tok[threadIdx.x] = threadIdx.x < count ? token_at(p.plan, tile.start + q0 + threadIdx.x, p.err) : -1;
   __syncthreads();
-  const int o = blockIdx.z * blockDim.x + threadIdx.x;
-  if (tok < 0 || o >= (swiglu ? p.N / 2 : p.N)) return;
-  auto column = [&](int n) {
-    const float* sj = s_row + slice_of(p, n) * tile.rank;
-    const T* bn = b + (int64_t)tile.offset * p.N + n;
-    float v = 0.f;
-    for (int r = 0; r < tile.rank; ++r) v = fmaf(sj[r], to_f(bn[(int64_t)r * p.N]), v);
-    return p.base[tok * p.base_stride + n] + v;
-  };
-  float y;
-  if (swiglu) {
-    const int n = (o >> 3) * 16 + (o & 7);
-    const float gate = column(n);
-    y = gate / (1.f + expf(-gate)) * column(n + 8);
-  } else {
-    y = column(o);
+  const int o = blockIdx.z * kAnyThreads + threadIdx.x;
+  const bool in = o < (swiglu ? p.N / 2 : p.N);
+  const int n = swiglu ? (o >> 3) * 16 + (o & 7) : o;
+  float base[kAnyTokens], up[kAnyTokens];
+#pragma unroll
+  for (int k = 0; k < kAnyTokens; ++k) {
+    const float* row = p.base + max(s_tok[k], 0) * p.base_stride + n;
+    const bool has = in && s_tok[k] >= 0;
+    base[k] = has ? row[0] : 0.f;
+    up[k] = has && swiglu ? row[8] : 0.f;
   }
-  out[tok * p.out_stride + o] = from_f<TO>(y);
+  const int rows = p.ns * tile.rank;
+  if constexpr (FUSED) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (rows > 0) {
+      for (int k = warp; k < kAnyTokens; k += kAnyThreads / 32)
+        for (int i = lane; i < K; i += 32)
+          s_x[k * K + i] = s_tok[k] >= 0 ? to_f(x[s_tok[k] * x_stride + i]) : 0.f;
+      __syncthreads();
+    }
+    for (int row = 4 * warp; row < rows; row += kAnyThreads / 8) {
+      const float v = dots_4x8(a + (int64_t)p.ns * tile.offset * K, K, row, rows,
+                               [&](int t, int i) { return s_x[t * K + i]; }, 0, 32);
+      const int m = row + lane / kAnyTokens;
+      if (m < rows) s_any_mem[m * kAnyTokens + lane % kAnyTokens] = v * p.ad.scales[tile.adapter];
+    }
+  } else {
+    for (int i = threadIdx.x; i < kAnyTokens * rows; i += kAnyThreads) {
+      const int k = i / rows, m = i - k * rows;
+      s_any_mem[m * kAnyTokens + k] =
+          k < count ? p.s_any[((int64_t)tile.start + q0 + k) * p.width_any + m] : 0.f;
+    }
+  }
+  __syncthreads();
+  if (!in) return;
+  auto column = [&](int c, float (&y)[kAnyTokens]) {
+    const float4* sj = s_row + 2 * slice_of(p, c) * tile.rank;
+    const T* bn = b + (int64_t)tile.offset * p.N + c;
+    float v[kAnyTokens] = {};
+    for (int r0 = 0; r0 < tile.rank; r0 += 16) {  // 16 loads in flight
+      float w[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        w[r] = r0 + r < tile.rank ? to_f(bn[(int64_t)(r0 + r) * p.N]) : 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (r0 + r >= tile.rank) break;
+        const float4 lo = sj[2 * (r0 + r)], hi = sj[2 * (r0 + r) + 1];
+        v[0] = fmaf(lo.x, w[r], v[0]), v[1] = fmaf(lo.y, w[r], v[1]);
+        v[2] = fmaf(lo.z, w[r], v[2]), v[3] = fmaf(lo.w, w[r], v[3]);
+        v[4] = fmaf(hi.x, w[r], v[4]), v[5] = fmaf(hi.y, w[r], v[5]);
+        v[6] = fmaf(hi.z, w[r], v[6]), v[7] = fmaf(hi.w, w[r], v[7]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAnyTokens; ++k) y[k] += v[k];
+  };
+  column(n, base);
+  if (swiglu) column(n + 8, up);
+#pragma unroll
+  for (int k = 0; k < kAnyTokens; ++k) {
+    const int tok = s_tok[k];
+    if (tok < 0) continue;
+    const float y = swiglu ? base[k] / (1.f + expf(-base[k])) * up[k] : base[k];
+    out[tok * p.out_stride + o] = from_f<TO>(y);
+  }
 }
 
 constexpr int kMostSmem = 226 * 1024;
@@ -623,18 +843,53 @@ int dispatch_shrink(const ShrinkArgs& p, int rows, cudaStream_t s) {
   return rows <= 16 ? launch_shrink<1, NT>(p, rows, s) : launch_shrink<2, NT>(p, rows, s);
 }
 
+// Little work (the comment at lora_one_kernel): one launch, and no workspace.
+bool one_launch(const LoraCall& c, const ms_lora_plan& plan, int max_rank) {
+  return c.n_slices == 1 && max_rank <= kOneRank && c.N <= kOneN && plan.n_tokens <= 32 &&
+         plan.n_tokens <= kOneTokens * plan.n_tiles;
+}
+
+template <typename TO>
+int launch_one(ShrinkArgs p, const ExpandArgs& e, cudaStream_t s) {
+  p.k_per = ceil_div(ceil_div(p.K, kOneSplit), 32) * 32;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.plan.n_tiles, 1, kOneSplit);
+  cfg.blockDim = kShrinkWarps * 32;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {1, 1, kOneSplit};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  (void)cudaLaunchKernelEx(&cfg, lora_one_kernel<TO>, p, e);
+  return check_launch("lora_one_kernel");
+}
+
+// K and rank rows small enough for the second product's CTAs to make s: no workspace.
+bool any_fused(const LoraCall& c, int max_rank) {
+  return c.K <= kFusedK && c.n_slices * max_rank <= kFusedRows;
+}
+
 template <typename T, typename TO>
 int launch_any(const LoraCall& c, const ExpandArgs& e, cudaStream_t s) {
-  if (e.ad.max_rank > 0) {
-    launch_pdl(lora_shrink_any_kernel<T>, dim3(e.plan.n_tiles, kTile), 256, 0, s,
-               static_cast<const T*>(c.x), c.x_stride, static_cast<const T*>(c.a), c.K, c.n_slices,
-               e.width_any, e.ad, e.plan, const_cast<float*>(e.s_any), e.err);
+  const int outs = c.swiglu ? c.N / 2 : c.N, rows = c.n_slices * e.ad.max_rank;
+  const dim3 grid(e.plan.n_tiles, kTile / kAnyTokens, ceil_div(outs, kAnyThreads));
+  const T *x = static_cast<const T*>(c.x), *a = static_cast<const T*>(c.a), *b = static_cast<const T*>(c.b);
+  if (any_fused(c, e.ad.max_rank)) {
+    launch_pdl(lora_expand_any_kernel<T, TO, true>, grid, kAnyThreads, (rows + c.K) * kAnyTokens * 4, s,
+               x, c.x_stride, a, c.K, b, static_cast<TO*>(c.out), c.swiglu ? 1 : 0, e);
+    return check_launch("lora_expand_any_kernel");
+  }
+  if (rows > 0) {
+    launch_pdl(lora_shrink_any_kernel<T>,
+               dim3(e.plan.n_tiles, kTile / kAnyTokens, ceil_div(rows, 4)), kAnyThreads, 0, s, x, c.x_stride, a, c.K,
+               c.n_slices, e.width_any, e.ad, e.plan, const_cast<float*>(e.s_any), e.err);
     MS_TRY(check_launch("lora_shrink_any_kernel"));
   }
-  const int outs = c.swiglu ? c.N / 2 : c.N;
-  launch_pdl(lora_expand_any_kernel<T, TO>, dim3(e.plan.n_tiles, kTile, ceil_div(outs, 128)), 128,
-             c.n_slices * e.ad.max_rank * 4, s, static_cast<const T*>(c.b), static_cast<TO*>(c.out),
-             c.swiglu ? 1 : 0, e);
+  launch_pdl(lora_expand_any_kernel<T, TO, false>, grid, kAnyThreads, rows * kAnyTokens * 4, s, x,
+             c.x_stride, a, c.K, b, static_cast<TO*>(c.out), c.swiglu ? 1 : 0, e);
   return check_launch("lora_expand_any_kernel");
 }
 
@@ -662,11 +917,7 @@ int validate_lora(const ms_lora_adapters* ad, const ms_lora_plan* plan) {
 int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& plan,
              void* workspace, size_t workspace_bytes, cudaStream_t s) {
   if (plan.n_tiles == 0 || plan.n_tokens == 0) return MS_OK;
-  const size_t need = lora_workspace_size(plan.n_tokens, c.n_slices, ad.max_rank);
-  if (workspace_bytes < need || (need > 0 && workspace == nullptr))
-    return fail(MS_ERR_INVALID, "lora: workspace too small (%zu < %zu)", workspace_bytes, need);
   auto aligned = [](const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
-  MS_REQUIRE(aligned(workspace, 16), "lora: workspace not 16-byte aligned");
   const bool out_f32 = c.out_dtype == MS_DTYPE_F32;
   ExpandArgs e{};
   e.base = c.base;
@@ -697,6 +948,26 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
                       // 32-bit element offsets in the second product
                       plan.n_tokens * (c.base_stride > c.out_stride ? c.base_stride : c.out_stride) <=
                           (int64_t)UINT32_MAX;
+  ShrinkArgs p{};
+  p.x = static_cast<const __nv_bfloat16*>(c.x);
+  p.x_stride = c.x_stride;
+  p.a = static_cast<const __nv_bfloat16*>(c.a);
+  p.K = c.K;
+  p.ns = c.n_slices;
+  p.terms = e.terms;
+  p.s_stride = e.s_stride;
+  p.ad = ad;
+  p.plan = plan;
+  p.s = static_cast<__nv_bfloat16*>(workspace);
+  p.err = e.err;
+  if (tensor && one_launch(c, plan, ad.max_rank))
+    return out_f32 ? launch_one<float>(p, e, s) : launch_one<__nv_bfloat16>(p, e, s);
+  const size_t need = !tensor && any_fused(c, ad.max_rank)
+                          ? 0
+                          : lora_workspace_size(plan.n_tokens, c.n_slices, ad.max_rank);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr))
+    return fail(MS_ERR_WORKSPACE, "lora: workspace too small (%zu < %zu)", workspace_bytes, need);
+  MS_REQUIRE(need == 0 || aligned(workspace, 16), "lora: workspace not 16-byte aligned");
   if (!tensor) {
     if (c.dtype == MS_DTYPE_F32 && out_f32) return launch_any<float, float>(c, e, s);
     if (c.dtype == MS_DTYPE_F32) return launch_any<float, __nv_bfloat16>(c, e, s);
@@ -704,18 +975,6 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
     return launch_any<__nv_bfloat16, __nv_bfloat16>(c, e, s);
   }
   if (ad.max_rank > 0) {
-    ShrinkArgs p{};
-    p.x = static_cast<const __nv_bfloat16*>(c.x);
-    p.x_stride = c.x_stride;
-    p.a = static_cast<const __nv_bfloat16*>(c.a);
-    p.K = c.K;
-    p.ns = c.n_slices;
-    p.terms = e.terms;
-    p.s_stride = e.s_stride;
-    p.ad = ad;
-    p.plan = plan;
-    p.s = static_cast<__nv_bfloat16*>(workspace);
-    p.err = e.err;
     e.after_shrink = 1;
     // tokens at a time by the tiles' mean size
     const int rows = c.n_slices * e.rank_pm, mean = plan.n_tokens / plan.n_tiles;

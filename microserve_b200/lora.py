@@ -159,13 +159,21 @@ def lora_add(
         raise ValueError(f"out must be float32 or bfloat16, got {out.dtype}")
     if T == 0:
         return out
+    args = (x.data_ptr(), max(x_ld, K), base.data_ptr(), max(base_ld, N), out.data_ptr(),
+            max(out.stride(0), width), pa, pb, K, N, ns, _PACK_COLUMNS[ns](*slices),
+            int(proj.interleaved), int(swiglu), ad, pl, _CODES[dtype], _CODES[out.dtype])
+    # little work usually takes one launch without scratch (one_launch, any_fused)
+    if (T <= 32 and T <= 8 * n_tiles and N <= 4096 and proj.max_rank <= 16 and ns == 1) \
+            if dtype is torch.bfloat16 else (K <= 256 and ns * proj.max_rank <= 256):
+        rc = _lib.launch_status(dev, "ms_lora_add", *args, None, 0)
+        if rc != _lib.MS_ERR_WORKSPACE:
+            if rc:
+                _lib.check("ms_lora_add", rc)
+            return out
     # ms_lora_workspace_size: s as up to three bf16 terms of the padded rank
     need = T * ns * ((proj.max_rank + 15) // 16 * 16) * 6
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
-    cols = _PACK_COLUMNS[ns](*slices)
-    _lib.launch_on(dev, "ms_lora_add", x.data_ptr(), max(x_ld, K), base.data_ptr(),
-                   max(base_ld, N), out.data_ptr(), max(out.stride(0), width), pa, pb, K, N, ns,
-                   cols, int(proj.interleaved), int(swiglu), ad, pl, _CODES[dtype], _CODES[out.dtype], ws.data_ptr(), ws.numel())
+    _lib.launch_on(dev, "ms_lora_add", *args, ws.data_ptr(), ws.numel())
     return out
 
 

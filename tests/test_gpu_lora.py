@@ -94,6 +94,13 @@ CASES = {
     "one_token": dict(of=[0], ranks=[16], K=2048, slices=[2048], dtype="bfloat16"),
     "one_token_of_none": dict(of=[-1], ranks=[16], K=64, slices=[128], dtype="bfloat16"),
     "no_adapters": dict(of=[-1, -1, -1], ranks=[], K=64, slices=[128], dtype="bfloat16"),
+    "few": dict(of=[0, 1, -1, 1, 2, 0, 3], ranks=[16, 5, 0, 1], K=200, slices=[4096], dtype="bfloat16"),
+    "few_in_a_long_tile": dict(of=[0] * 20 + [1, 2, -1], ranks=[16, 8, 3], K=4104, slices=[1000], dtype="bfloat16"),
+    "few_and_small": dict(of=[0, -1], ranks=[7], K=8, slices=[8], dtype="bfloat16"),
+    "few_and_wider": dict(of=[0, 1, 0], ranks=[16, 5], K=64, slices=[4104], dtype="bfloat16"),
+    "few_of_rank_17": dict(of=[0, 1, 0], ranks=[17, 5], K=64, slices=[64], dtype="bfloat16"),
+    "few_at_the_most": dict(of=list(range(16)) + list(range(16)), ranks=[16] * 16, K=520, slices=[72], dtype="bfloat16"),
+    "one_more_than_few": dict(of=list(range(33)), ranks=[16] * 33, K=64, slices=[72], dtype="bfloat16"),
     "qkv_mixed": dict(of=mixed(77, 9), ranks=[8, 16, 32, 64, 1, 5, 24, 0, 128], K=2048,
                       slices=[2048, 256, 256], dtype="bfloat16"),
     "qkv_narrow_slices": dict(of=mixed(40, 3), ranks=[16, 8, 40], K=200, slices=[72, 8, 24], dtype="bfloat16"),
@@ -118,6 +125,11 @@ CASES = {
     "prompts_none": dict(of=[-1] * 200 + [0] * 64, ranks=[16], K=64, slices=[136], dtype="bfloat16"),
     "prompts_rank_256": dict(of=[0] * 140, ranks=[256], K=72, slices=[264], dtype="bfloat16"),
     "f32": dict(of=mixed(61, 3), ranks=[4, 5, 12], K=128, slices=[128, 128, 128], dtype="float32"),
+    "f32_long_k": dict(of=mixed(30, 3) + [-1], ranks=[4, 5, 12], K=259, slices=[70, 130], dtype="float32"),
+    "f32_many_rows": dict(of=mixed(13, 2), ranks=[129, 3], K=40, slices=[300, 21], dtype="float32"),
+    "f32_one_token": dict(of=[0], ranks=[3], K=256, slices=[257], dtype="float32"),
+    "f32_full_tiles": dict(of=[0] * 150 + [-1] * 9, ranks=[6], K=96, slices=[96], dtype="float32"),
+    "f32_most": dict(of=mixed(17, 2), ranks=[64, 64], K=256, slices=[33, 20, 1, 9], dtype="float32"),
     "f32_odd": dict(of=mixed(13, 2), ranks=[7, 1], K=33, slices=[29], dtype="float32"),
 }
 
@@ -195,10 +207,11 @@ def test_strides_and_rows_behind_the_batch() -> None:
     c.check(lora_add(xo[:, 1 : K + 1], c.base, c.proj, c.plan))
 
 
-def test_nan_of_one_token_stays_with_it() -> None:
+@pytest.mark.parametrize("ranks", [[16, 24], [16, 8]])
+def test_nan_of_one_token_stays_with_it(ranks: list[int]) -> None:
     from microserve_b200.lora import lora_add
 
-    c = Case([0, 1, 0, -1, 1, 0], [16, 24], 256, [128], "bfloat16")
+    c = Case([0, 1, 0, -1, 1, 0], ranks, 256, [128], "bfloat16")
     clean = lora_add(c.x, c.base, c.proj, c.plan)
     c.x[2] = float("nan")
     c.x[3] = float("inf")  # no adapter: not read
