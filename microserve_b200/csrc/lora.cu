@@ -421,7 +421,7 @@ __device__ __forceinline__ void expand_mma(float (&acc)[4][4], uint32_t sa, uint
 }
 
 template <int EPI, int WM, int WN>
-__global__ void __launch_bounds__(32 * WM * WN, WM * WN == 16 ? 2 : 1) lora_expand_kernel(ExpandArgs p) {
+__global__ void __launch_bounds__(32 * WM * WN, 1) lora_expand_kernel(ExpandArgs p) {
   constexpr int TERMS = EPI == kLoraF32 ? 3 : 2;
   constexpr int kTm = 16 * WM, kCols = 32 * WN, kThreads = 32 * WM * WN;
   constexpr int kBaseLd = kCols + kPad, kBLd = kCols + kPad;
@@ -445,7 +445,8 @@ __global__ void __launch_bounds__(32 * WM * WN, WM * WN == 16 ? 2 : 1) lora_expa
   const int stage_bytes = kBaseBytes + p.rank_pm * kBLd * 2;
   __nv_bfloat16* s_s = reinterpret_cast<__nv_bfloat16*>(smem);
   unsigned char* ring = smem + s_bytes;
-  const bool work = ok && tile.count > 0 && !(p.in_place && tile.rank == 0);
+  const int at = kTm * blockIdx.z;  // a long tile's tokens among the CTAs of z
+  const bool work = ok && tile.count > at && !(p.in_place && tile.rank == 0);
   const int step = kCols * gridDim.x, c_first = kCols * blockIdx.x;
 
   if (work)
@@ -502,9 +503,9 @@ __global__ void __launch_bounds__(32 * WM * WN, WM * WN == 16 ? 2 : 1) lora_expa
   if (p.after_shrink) pdl_enter();
   if (!work) return;
 
-  for (int first = 0; first < tile.count; first += kTm) {
+  for (int first = at; first < tile.count; first += kTm * gridDim.z) {
     const int here = min(tile.count - first, kTm);
-    if (first > 0) __syncthreads();  // the last pass is done with s and the ring
+    if (first > at) __syncthreads();  // the last pass is done with s and the ring
     find_rows(first, here);
     for (int i = threadIdx.x; i < here * (s_row / 8); i += kThreads) {
       const int row = i / (s_row / 8), q = 8 * (i - row * (s_row / 8));
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(32 * WM * WN, WM * WN == 16 ? 2 : 1) lora_expa
     }
     for (int k = 0; k + 1 < p.stages; ++k) {
       if (c_first + k * step < p.N) {
-        if (first > 0 || k > 0 || !p.after_shrink) load_b(c_first + k * step, k);
+        if (first > at || k > 0 || !p.after_shrink) load_b(c_first + k * step, k);
         load_base(c_first + k * step, k);
       }
       cp_commit();
@@ -783,6 +784,9 @@ int launch_expand(ExpandArgs p, cudaStream_t s) {
     if (smem() > kMostSmem) return launch_expand<EPI, 1, 2>(p, s);  // ranks of 128 and more
   static std::atomic<uint64_t> granted{0};
   MS_TRY(grant_dynamic_smem(lora_expand_kernel<EPI, WM, WN>, kMostSmem, granted));
+  // Where tiles are short on average, a long one (the tokens of no adapter) would
+  // take the longest: two CTAs share its tokens (256 tokens, 64 adapters, N = 2560:
+  // 20.8 -> 15.4 us; four 16.8).
   // CTAs per tile: the number whose rounds over the GPU take the fewest steps,
   // a CTA's start counted as three
   const int resident = max(1, min(64 / (WM * WN), 227 * 1024 / (smem() + 1536)));
@@ -796,22 +800,31 @@ int launch_expand(ExpandArgs p, cudaStream_t s) {
       gx = n;
     }
   }
-  launch_pdl(lora_expand_kernel<EPI, WM, WN>, dim3(gx, p.plan.n_tiles), 32 * WM * WN, smem(), s, p);
+  launch_pdl(lora_expand_kernel<EPI, WM, WN>, dim3(gx, p.plan.n_tiles, WM == 1 ? 2 : 1), 32 * WM * WN, smem(), s, p);
   return check_launch("lora_expand_kernel");
 }
 
-// Tokens per CTA by the tiles' mean size; tcgen05 above kTcTokens.
-constexpr int kTcTokens = 48;
+// By the tiles' mean size, the padded rank and N.  1024 tokens at N = 28672 with
+// the SwiGLU, first product of K = 512 included, in us, for 1 x 4 warps, 2 x 2 and
+// tcgen05:      rank 16           rank 32           rank 64           rank 128
+//   6 tokens    98  153  301      96  121  317      176  189  360     280  366  525
+//  12           62   89  167      64   76  182      109  108  200     170  203  289
+//  22           55   60   92      63   54   98      107   80  111     162  140  157
+//  40           47   63   59      57   57   64       94   80   74     140  140  102
+//  52           55   61   52      59   53   55       99   74   66     150  130   93
+// N = 2560 to 11264 agree, but that tcgen05 at 40 tokens pays from rank x N on
+// (rank 64: 24.3 to 23.0 us at 2560, 42.0 to 42.5 at 11264).
+constexpr int kTcTokens = 48;  // also where the first product goes to tcgen05
 template <int EPI>
 int dispatch_expand(const ExpandArgs& p, cudaStream_t s) {
   const int mean = p.plan.n_tokens / p.plan.n_tiles;
-  if (mean > kTcTokens) {
+  const bool wide = (int64_t)p.rank_pm * p.N >= 64 * 8192;
+  if (mean > (wide ? 32 : kTcTokens)) {
     const int rc = lora_expand_tc(p, EPI, s);
     if (rc != MS_ERR_UNSUPPORTED) return rc;
   }
-  if (mean <= 16) return launch_expand<EPI, 1, 4>(p, s);
-  if (mean <= 32) return launch_expand<EPI, 2, 4>(p, s);
-  return launch_expand<EPI, 4, 4>(p, s);
+  if (mean > 16 && p.rank_pm > 16) return launch_expand<EPI, 2, 2>(p, s);
+  return launch_expand<EPI, 1, 4>(p, s);
 }
 
 template <int MT, int NT>
