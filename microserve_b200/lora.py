@@ -112,7 +112,8 @@ def lora_add(
     contiguous rows.  ``swiglu`` returns ``silu(gate) * up`` (T, N/2) of an
     interleaved projection instead.  ``out`` (float32 or bfloat16) defaults to a
     new tensor of ``out_dtype``; it may be ``base`` itself (no SwiGLU): tokens
-    without an adapter are then not touched."""
+    without an adapter are then not touched.  Rows of tokens that no tile of
+    ``plan`` lists (``LoraPlan.build`` lists all) are not written."""
     dev = _lib.cuda_index(x)
     T, K = x.shape
     if base.dim() != 2 or base.shape[0] != T or base.dtype is not torch.float32 \
@@ -201,6 +202,8 @@ class LoraAdapters:
     def __init__(self, model: Transformer, rank_capacity: int = 64) -> None:
         if rank_capacity < 1:
             raise ValueError("rank_capacity must be at least 1")
+        if model.adapters is not None and any(model.adapters._users.values()):
+            raise ValueError("the model's adapters are held by requests")
         self.cfg, self.device, self.dtype = model.cfg, model.device, model.dtype
         c = model.cfg
         d, ff = c.d_model, c.ffn_hidden
@@ -247,6 +250,7 @@ class LoraAdapters:
             at = o + r
         if at + rank > self._capacity:
             capacity = max(2 * self._capacity, at + rank)
+            self._c = None  # it holds the old pools' addresses
             for name in self._shape:
                 ns = len(self._shape[name][1])
                 for pool, new, per in zip((self._a[name], self._b[name]),

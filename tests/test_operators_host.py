@@ -202,3 +202,35 @@ def test_adapter_pools_on_the_host() -> None:
     assert ads.id_of("z") == 0 and ads._offset[0] == 0
     assert (ads.projection("gate_up", 0).b[:2] == 0).all()  # nothing of x is left in z's rows
     assert ads.ids_of_tokens(["z", None, "y"], [2, 1, 3]).tolist() == [0, 0, -1, 1, 1, 1]
+
+
+def test_a_load_that_fails_leaves_the_adapters_usable(monkeypatch: pytest.MonkeyPatch) -> None:
+    """Growing the rank axis replaces the pools; their addresses are not kept past it."""
+    from types import SimpleNamespace
+
+    from microserve_b200.config import ModelConfig
+    from microserve_b200.lora import LoraAdapters
+
+    cfg = ModelConfig(vocab_size=65, n_layers=1, d_model=64, n_heads=4, d_ff=96)
+    model = SimpleNamespace(cfg=cfg, device=torch.device("cpu"), dtype=torch.float32, adapters=None)
+    ads = LoraAdapters(model, rank_capacity=2)
+    key = "blocks.0.attn.o_proj.lora_"
+    state = lambda r: {key + "A.weight": torch.ones(r, 64), key + "B.weight": torch.ones(64, r)}  # noqa: E731
+    ads.load("x", state(2))
+    assert ads.c_struct().a_o[0] == ads._a["o"][0].data_ptr()
+    grown = ads._reserve
+
+    def reserve(rank: int) -> int:
+        grown(rank)
+        raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(ads, "_reserve", reserve)
+    with pytest.raises(RuntimeError):
+        ads.load("y", state(5))
+    assert ads.names == ["x"]
+    assert ads.c_struct().a_o[0] == ads._a["o"][0].data_ptr()
+    assert (ads.projection("o", 0).a[:2] == 1).all()
+    ads.acquire("x")
+    with pytest.raises(ValueError, match="held"):
+        LoraAdapters(model)
+    assert model.adapters is ads
