@@ -225,7 +225,10 @@ __device__ __forceinline__ void edit_row(const ControlArgs& a, const Slice& sl, 
 // ---- out of place, through shared memory ------------------------------------
 // A CTA takes kSlice tokens of one request's rows.  Each row's slice comes in
 // by one bulk copy, is edited in shared memory and goes out by one bulk copy,
-// in a ring of rows.  The kernel moves 8 bytes per logit and is bound by HBM.
+// in a ring of rows.  The kernel moves 8 bytes per logit and is bound by HBM:
+// 256 requests x 6 rows x 128256 take 300 us (5.3 TB/s), x 5 x 32000 62 us.  A
+// deeper ring (347 us with 3 rows), half a slice (355) and 128 or 384 threads
+// (314, 327) take more: what hides the latency is the CTAs beside this one.
 // A row that does not start on 16 bytes keeps its misalignment in shared
 // memory; its up to 3 first and last logits are copied one by one.
 constexpr int kRing = 2;
@@ -357,7 +360,10 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
         issue(it + ahead);
       }
     }
-    if (loose) __syncthreads();  // its loose logits are out before the buffer is filled again
+    // Its loose logits are out before the buffer is filled again, and thread 0 has
+    // seen the store from the next row's buffer end before loose logits go there
+    // (rows of one alignment are all loose or none is).
+    if (loose || (a.in_stride & 3)) __syncthreads();
   }
   if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
@@ -366,7 +372,9 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
 // In place only what a control touches is read and written; else the slice is
 // copied first and then edited where it is.  128 threads a CTA: its work is
 // a chain of short dependent reads, so more CTAs per SM beat more threads
-// (grammar masks over 256 x 128256: 28.6 us, 33.9 with 256).
+// (grammar masks over 256 x 128256: 28.6 us, 33.9 with 256).  That case writes
+// 104 MB and is at the rate at which this GPU writes (a fill: 3.9 TB/s); reading
+// what a partly masked group of 4 holds, to write it whole, takes 36.7 us.
 constexpr int kDirectThreads = 128;
 __global__ void __launch_bounds__(kDirectThreads) logit_controls_direct_kernel(ControlArgs a) {
   pdl_enter();
@@ -465,9 +473,9 @@ int validate_controls(const ms_logit_controls* c, int n_requests, int rows_per_r
                "ms_logit_controls: %d proposals (1..%d)", c->n_proposals, kMaxProposals);
   }
   MS_REQUIRE(c->first_proposal >= 0, "ms_logit_controls: first_proposal %d", c->first_proposal);
-  MS_REQUIRE(!c->proposals || c->first_proposal + rows_per_request - 1 <= c->n_proposals,
-             "ms_logit_controls: the last row sees %d proposals of %d",
-             c->first_proposal + rows_per_request - 1, c->n_proposals);
+  MS_REQUIRE(!c->proposals || (int64_t)c->first_proposal + rows_per_request - 1 <= c->n_proposals,
+             "ms_logit_controls: rows after the first %d proposals, %d of them, see more than %d",
+             c->first_proposal, rows_per_request, c->n_proposals);
   if (c->bias_start)
     MS_REQUIRE(c->n_bias == 0 || (c->n_bias > 0 && c->bias_ids && c->bias_values),
                "ms_logit_controls: bias_start needs bias_ids and bias_values");

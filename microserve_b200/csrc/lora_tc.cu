@@ -72,6 +72,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop, int* err) {
   return __all_sync(0xffffffffu, bar_wait(bar, parity, stop, err));
 }
+// After a wait that ran out: the MMAs committed to `bar` end before the block goes.
+__device__ __forceinline__ void drain(uint32_t bar, int* err) {
+  int go_on = 0;
+  bar_wait(bar, 0, &go_on, err);
+}
 // Descriptors with the 128-byte swizzle.  K-major: rows of 64 k values, groups of
 // 8 rows 1024 bytes apart (lead 16: not used).  Adapter rows, MN-major: 64 columns per
 // 128-byte row, groups of 8 k rows 1024 bytes apart (stride offset), blocks of
@@ -157,7 +162,7 @@ __device__ int tiles_before(const ms_lora_plan& p, int i, int start, int adapter
     bool same = false;
     if (i - k >= 0) {
       const int4 q = tiles[i - k];
-      same = q.z == adapter && q.y == kTile && q.x == start - kTile * k;
+      same = q.z == adapter && q.y == kTile && q.x == start - kTile * k && q.x >= 0;
     }
     const uint32_t m = __ballot_sync(0xffffffffu, same);
     if (m != 0xffffffffu) return n + __ffs(~m) - 1;
@@ -302,7 +307,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
     // ---- MMA
     const uint32_t id = instr(here) & ~(1u << 16);  // B K-major as well
     bool fine = true;
-    for (int step = 0; step < steps && fine; ++step) {
+    int step = 0;
+    for (; step < steps; ++step) {
       const int slot = step % kSteps;
       if (!(fine = bar_wait(full + 8 * slot, (step / kSteps) & 1, stop, p.err))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -311,7 +317,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
       for (int k = 0; k < kStepK / 16; ++k) umma_ss(tmem, x + 2 * k, a + 2 * k, id, step > 0 || k > 0);
       umma_commit(empty + 8 * slot);
     }
-    if (fine && steps > 0) umma_commit(done);
+    if (step > 0) umma_commit(done);
+    if (!fine && step > 0) drain(done, p.err);
   }
   __syncwarp();
   if (splits > 1) cluster.sync(); else __syncthreads();
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   const uint32_t ring = base, stage_bytes = p.rank_pm * kChunk * 2;
   const uint32_t s_x = ring + kStages * stage_bytes, bars = s_x + kEpiWarps * kEpiBytes;
   const uint32_t full = bars, empty = full + 8 * kStages, s_ready = empty + 8 * kStages;
-  const uint32_t tfull = s_ready + 8, tempty = tfull + 16, slot_addr = tempty + 16;
+  const uint32_t tfull = s_ready + 8, tempty = tfull + 16, drained = tempty + 16, slot_addr = drained + 8;
   unsigned char* gbars = smem_raw + (bars - raw);
   volatile uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbars + (slot_addr - bars));
   volatile int* stop = reinterpret_cast<int*>(gbars + (slot_addr - bars) + 4);
@@ -376,6 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
       bar_init(empty + 8 * k, 1);
     }
     bar_init(s_ready, kEpiWarps);
+    bar_init(drained, 1);
     for (int k = 0; k < 2; ++k) {
       bar_init(tfull + 8 * k, 1);
       bar_init(tempty + 8 * k, kEpiWarps);
@@ -456,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
       bool fine = true;
       for (int ch = 0; ch < chunks && fine; ++ch) {
         const int buf = ch & 1, use = ch >> 1;
-        if (use >= 1 && !bar_wait(tempty + 8 * buf, (use - 1) & 1, stop, p.err)) break;
+        if (use >= 1 && !(fine = bar_wait(tempty + 8 * buf, (use - 1) & 1, stop, p.err))) break;
         const int c = column(ch), n = passes(c);
         const uint32_t d = tmem + buf * kChunk;
         uint32_t acc = 0;
@@ -492,6 +500,10 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
         }
         if (!fine) break;
         umma_commit(tfull + 8 * buf);
+      }
+      if (!fine) {
+        umma_commit(drained);
+        drain(drained, p.err);
       }
     }
     __syncwarp();
@@ -631,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
         }
       }
     }
+    cp_wait<0>();
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

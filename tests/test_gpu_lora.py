@@ -255,6 +255,19 @@ def test_bad_plans_and_adapters_are_skipped() -> None:
             assert torch.equal(out[keep], good[keep])
 
 
+@pytest.mark.parametrize("bad", [(-64, 64, 0, 0), (-1, 64, 0, 0), (0, 65, 0, 0), (0, 64, 3, 0)])
+def test_a_bad_tile_before_a_prompt_costs_only_itself(bad: tuple[int, ...]) -> None:
+    from microserve_b200 import _lib
+    from microserve_b200.lora import LoraPlan, lora_add
+
+    c = Case([0] * 256, [24], 128, [256], "bfloat16")
+    good = lora_add(c.x, c.base, c.proj, c.plan)
+    tiles = torch.cat([torch.tensor([bad], dtype=torch.int32, device=DEV), c.plan.tiles])
+    got = lora_add(c.x, c.base, c.proj, LoraPlan(c.plan.order, tiles))
+    assert _lib.device_error() != 0
+    assert torch.equal(got, good)
+
+
 def test_two_streams_and_replayed_graphs() -> None:
     """Each call has its own scratch: calls on two streams, and two captured graphs, do not mix."""
     from microserve_b200.lora import lora_add
