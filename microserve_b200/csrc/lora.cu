@@ -814,7 +814,7 @@ int launch_expand(ExpandArgs p, cudaStream_t s) {
 //  52           55   61   52      59   53   55       99   74   66     150  130   93
 // N = 2560 to 11264 agree, but that tcgen05 at 40 tokens pays from rank x N on
 // (rank 64: 24.3 to 23.0 us at 2560, 42.0 to 42.5 at 11264).
-constexpr int kTcTokens = 48;  // also where the first product goes to tcgen05
+constexpr int kTcTokens = 48;
 template <int EPI>
 int dispatch_expand(const ExpandArgs& p, cudaStream_t s) {
   const int mean = p.plan.n_tokens / p.plan.n_tiles;
@@ -989,13 +989,25 @@ int lora_add(const LoraCall& c, const ms_lora_adapters& ad, const ms_lora_plan& 
   }
   if (ad.max_rank > 0) {
     e.after_shrink = 1;
-    // tokens at a time by the tiles' mean size
+    // Tokens at a time by the tiles' mean size.  1024 tokens, K = 4096, two slices, in us
+    // (N = 128), for 8 and 16 tokens at a time and through shared memory:
+    //              rank 16           rank 64
+    //   6 tokens   23   26   32      50   58   60
+    //  12          26   20   22      50   40   38
+    //  22          30   25   18      47   41   28
+    //  40          27   21   14      55   43   22
+    // Shared memory with 64 rank rows a CTA or 128: 26 or 32 (4096 tokens, rank 16),
+    // 70 or 62 (8192, rank 64).  tcgen05 pays where tiles of one adapter follow one
+    // another in pairs, as only prompts' do, and there are enough of them: runs of 512
+    // tokens, rank 128, 50 us to 48 at 2048 tokens, 44 to 67 at 4096, 66 to 107 at
+    // 8192; 8192 tokens of 128 adapters, rank 64, 74 to 63.
     const int rows = c.n_slices * e.rank_pm, mean = plan.n_tokens / plan.n_tiles;
+    const bool long_runs = plan.n_tiles >= 64 && plan.n_tiles >= 2 * (ad.n_adapters + 1);
     if (mean <= 8)
       MS_TRY(dispatch_shrink<1>(p, rows, s));
     else if (mean <= 16)
       MS_TRY(dispatch_shrink<2>(p, rows, s));
-    else if (mean > kTcTokens)
+    else if (mean > kTcTokens && long_runs)
       MS_TRY(lora_shrink_tc(p, rows, s));
     else if (rows <= 64)
       MS_TRY(launch_shrink_tile<64>(p, rows, s));

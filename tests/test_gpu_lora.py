@@ -124,6 +124,9 @@ CASES = {
     "prompts_narrow_slices": dict(of=[0] * 130, ranks=[24], K=128, slices=[30, 40, 58], dtype="bfloat16"),
     "prompts_none": dict(of=[-1] * 200 + [0] * 64, ranks=[16], K=64, slices=[136], dtype="bfloat16"),
     "prompts_rank_256": dict(of=[0] * 140, ranks=[256], K=72, slices=[264], dtype="bfloat16"),
+    "long_prompts": dict(of=[0] * 2070 + [-1] * 70 + [1] * 2150, ranks=[24, 64], K=200, slices=[136], dtype="bfloat16"),
+    "long_prompts_shared_k": dict(of=[0] * 4300, ranks=[16], K=1096, slices=[72, 24], dtype="bfloat16"),
+    "long_prompts_rank_256": dict(of=[0] * 4225, ranks=[256], K=72, slices=[64, 32, 40], dtype="bfloat16"),
     "f32": dict(of=mixed(61, 3), ranks=[4, 5, 12], K=128, slices=[128, 128, 128], dtype="float32"),
     "f32_long_k": dict(of=mixed(30, 3) + [-1], ranks=[4, 5, 12], K=259, slices=[70, 130], dtype="float32"),
     "f32_many_rows": dict(of=mixed(13, 2), ranks=[129, 3], K=40, slices=[300, 21], dtype="float32"),
