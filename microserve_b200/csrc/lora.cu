@@ -757,12 +757,14 @@ __global__ void __launch_bounds__(kAnyThreads)
 
 constexpr int kMostSmem = 226 * 1024;
 
-// CTAs of a cluster that share out k: enough CTAs for the GPU, at least 256 k
-// values for each.
+// CTAs of a cluster that share out k: as many as one round over the GPU takes (two
+// a SM), at least 256 k values for each.  Sharing on into a second round costs:
+// 256 tiles of 6 tokens, K = 14336, rank 16, 33.7 us by two CTAs and 28.9 by one;
+// 64 tiles of 4, 22.5 us by eight and 15.9 by four.
 int shrink_split(int n_tiles, int K, int rows, int mt) {
   const int64_t ctas = (int64_t)n_tiles * ceil_div(rows, 16 * mt);
   int split = 1;
-  while (split < 8 && ctas * split < 2 * 148 && K / (2 * split) >= 256) split *= 2;
+  while (split < 8 && ctas * split <= 148 && K / (2 * split) >= 256) split *= 2;
   return split;
 }
 
@@ -844,7 +846,7 @@ int launch_shrink_tile(ShrinkArgs p, int rows, cudaStream_t s) {
   MS_TRY(grant_dynamic_smem(lora_shrink_tile_kernel<RB>, smem, granted));
   const int blocks = ceil_div(rows, RB);
   int split = 1;
-  while (split < 8 && (int64_t)p.plan.n_tiles * blocks * split < 2 * 148 && p.K / (2 * split) >= 256)
+  while (split < 8 && (int64_t)p.plan.n_tiles * blocks * split <= 148 && p.K / (2 * split) >= 256)
     split *= 2;
   p.k_per = ceil_div(ceil_div(p.K, split), kBigK) * kBigK;
   return launch_cluster(lora_shrink_tile_kernel<RB>, dim3(p.plan.n_tiles, blocks, split), 256, smem,
