@@ -9,7 +9,9 @@
 // The plan lists tiles of up to 64 tokens that share an adapter (adapter -1:
 // none).  Two launches: lora_shrink computes s (k shared out over the CTAs of
 // a cluster when there are few tiles, the parts summed in a fixed order, so
-// results do not depend on timing), lora_expand adds B s to the base.
+// results do not depend on timing), lora_expand adds B s to the base.  Calls of
+// little work take one (lora_one_kernel; the any-shape kernels for small K);
+// tiles of many tokens go to the tcgen05 kernels of lora_tc.cu.
 //
 // s is a float32 sum.  The second product takes it in bf16 terms (s rounded,
 // then what is left rounded, ...) whose sum is s: one term would put 2^-9 of
@@ -52,7 +54,8 @@ namespace {
 // A CTA takes 16 * MT rank rows, 8 * NT tokens at a time; its 8 warps and the CTAs of its
 // cluster share out k, and the parts meet in (distributed) shared memory.
 // Each slice's rank rows are padded to a multiple of 16 (`rank_p`), with
-// zeros in s.
+// zeros in s.  Bound by HBM where every few tokens bring an adapter of their own:
+// 1536 tokens of 256 adapters of rank 16, K = 14336 (161 MB), 28.7 us (5.6 TB/s).
 constexpr int kShrinkWarps = 8;
 
 template <int MT, int NT>
@@ -144,7 +147,8 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
 // The same for larger tiles: 64 tokens x RB rank rows per CTA, both operands
 // through shared memory (each is read RB / 16 and 4 times), k in steps of 64
 // behind a ring of cp.async.  Warp (m, n) of the 4 x 2 has 16 tokens and RB / 2
-// rank rows.
+// rank rows.  1280 tokens of 32 adapters, K = 2048, two slices, rank 16-32 (11 MB):
+// 9.5 us, the latency of the ring's first steps and of the cluster's sum.
 constexpr int kBigK = 64;
 constexpr int kBigLd = kBigK + 8;  // padded row (elements): conflict-free ldmatrix
 constexpr int kBigStages = 4;
@@ -362,10 +366,17 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_one_kernel(ShrinkArgs 
 // ---- second product, bf16 -----------------------------------------------------
 // A CTA keeps the s rows of up to 16 WM tokens of a tile in shared memory and
 // goes through its share of the columns, 32 WN at a step: their base values
-// and adapter rows come in by cp.async, up to two steps ahead.  mma m16n8k16
+// and adapter rows come in by cp.async, up to three steps ahead.  mma m16n8k16
 // with tokens as M, columns as N, the rank as K; warp (m, n) of the WM x WN
 // has 16 tokens and 32 columns.  The sums start from the base and leave
 // through its buffer, in whole 32-byte sectors.
+// 1536 tokens of 256 adapters, rank 16, N = 4096 (84 MB): 21.8 us (3.9 TB/s, near the
+// rate at which half of it can be written).  1280 tokens of 32 adapters, rank 16-32,
+// N = 11264 with the SwiGLU (89 MB): 26 us after the first product (3.4 TB/s); 14
+// warps a SM keep the issue slots half busy, and what they wait for most is the
+// result of the last instruction.  Small CTAs do best: 512 threads took 42 us for the
+// call's two products, 256 38 and 128 36; more of them per SM by fewer registers (96
+// of 122) take 8B's two products from 57 to 76 us.
 constexpr int kPad = 8;  // elements after each shared-memory row: conflict-free fragment reads
 
 // Which slice a warp's 32 columns take their s from.

@@ -1,5 +1,5 @@
 """Per-request logit controls and low-rank adapters restated in 64-bit numpy --
-test infrastructure (checker only).  Each function also returns the sum of the
+test infrastructure.  Each function also returns the sum of the
 magnitudes that enter a result, from which rounding bounds are derived."""
 
 from __future__ import annotations

@@ -271,11 +271,18 @@ def test_a_bad_tile_before_a_prompt_costs_only_itself(bad: tuple[int, ...]) -> N
     assert torch.equal(got, good)
 
 
-def test_two_streams_and_replayed_graphs() -> None:
+@pytest.mark.parametrize("tokens,ranks,K,dtype", [
+    (90, [16, 8, 32, 16], 1024, "bfloat16"),
+    (9, [16, 8, 3, 16], 1024, "bfloat16"),  # one launch
+    (40, [16, 8, 3, 16], 200, "float32"),
+    (40, [16, 8, 3, 16], 1024, "float32"),
+    (4500, [16, 8], 520, "bfloat16"),
+])
+def test_two_streams_and_replayed_graphs(tokens: int, ranks: list[int], K: int, dtype: str) -> None:
     """Each call has its own scratch: calls on two streams, and two captured graphs, do not mix."""
     from microserve_b200.lora import lora_add
 
-    cs = [Case(mixed(90, 4, s), [16, 8, 32, 16], 1024, [512], "bfloat16", seed=s) for s in range(2)]
+    cs = [Case(mixed(tokens, len(ranks), s), ranks, K, [512], dtype, seed=s) for s in range(2)]
     want = [lora_add(c.x, c.base, c.proj, c.plan) for c in cs]
     streams = [torch.cuda.Stream() for _ in cs]
     torch.cuda.synchronize()
