@@ -156,32 +156,42 @@ __device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int te
 // This CTA's share of a cluster's outputs: the parts ([token][ld] floats in each
 // CTA's shared memory) of tokens [0, count) and rank rows [m0, m0 + here), `here`
 // a multiple of 16, summed in cluster order, scaled, and stored as terms.
-template <typename Cluster>
-__device__ __forceinline__ void finish_s(const ShrinkArgs& p, const Cluster& cluster, const float* part,
-                                         int ld, int start, int count, int m0, int here, int rank_p,
-                                         float scale) {
-  const int splits = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
-  const int quads = here / 4;
-#pragma unroll 2
-  for (int o = split * blockDim.x + threadIdx.x; o < count * quads; o += splits * blockDim.x) {
+template <int SPLITS, typename Cluster>
+__device__ __forceinline__ void finish_part(const ShrinkArgs& p, const Cluster& cluster, const float* part,
+                                            int ld, int start, int count, int m0, int here, int rank_p,
+                                            float scale) {
+  const int split = SPLITS > 1 ? (int)cluster.block_rank() : 0, quads = here / 4;
+#pragma unroll (SPLITS > 2 ? 2 : 4)
+  for (int o = split * blockDim.x + threadIdx.x; o < count * quads; o += SPLITS * blockDim.x) {
     const int col = o / quads, row = 4 * (o - col * quads);
     const float* at = part + col * ld + row;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (splits > 1) {
-#pragma unroll 4
-      for (int k = 0; k < splits; ++k) {
-        const float4 q = *reinterpret_cast<const float4*>(cluster.map_shared_rank(at, k));
-        v.x += q.x;
-        v.y += q.y;
-        v.z += q.z;
-        v.w += q.w;
-      }
-    } else {
-      v = *reinterpret_cast<const float4*>(at);
+    float4 q[SPLITS];
+#pragma unroll
+    for (int k = 0; k < SPLITS; ++k)
+      q[k] = *reinterpret_cast<const float4*>(SPLITS > 1 ? cluster.map_shared_rank(at, k) : at);
+    float4 v = q[0];
+#pragma unroll
+    for (int k = 1; k < SPLITS; ++k) {
+      v.x += q[k].x;
+      v.y += q[k].y;
+      v.z += q[k].z;
+      v.w += q[k].w;
     }
     const int j = (m0 + row) / rank_p, r = m0 + row - j * rank_p;
     store_terms(p.s + (start + col) * p.s_stride + j * p.terms * rank_p + r, rank_p, p.terms,
                 make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
+  }
+}
+
+template <typename Cluster>
+__device__ __forceinline__ void finish_s(const ShrinkArgs& p, const Cluster& cluster, const float* part,
+                                         int ld, int start, int count, int m0, int here, int rank_p,
+                                         float scale) {
+  switch ((int)cluster.num_blocks()) {  // 1, 2, 4 or 8
+    case 1: return finish_part<1>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
+    case 2: return finish_part<2>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
+    case 4: return finish_part<4>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
+    default: return finish_part<8>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
   }
 }
 

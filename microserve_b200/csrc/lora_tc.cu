@@ -200,7 +200,7 @@ __device__ bool load_pair(const ms_lora_plan& p, const ms_lora_adapters& ad, int
 // of 64 through a ring of four slots, two loading warps each; k is shared out
 // over a cluster, whose parts meet in distributed shared memory, summed in
 // cluster order.  x is read once, A by every pair of tiles out of L2.  8192 tokens,
-// K = 4096, two slices of rank 64-128 (73 MB): 49 us, by mma.sync 95; about 18 us of
+// K = 4096, two slices of rank 64-128 (73 MB): 46 us, by mma.sync 95; about 15 us of
 // it start, the hand-over of 128 KB of sums per CTA through shared memory, and the
 // stores of s.
 constexpr int kSteps = 4;                       // ring slots
