@@ -887,6 +887,7 @@ class SpeculativeDecoder:
     # -- lifecycle ----------------------------------------------------------------
     def free(self, seq_id: int) -> None:
         self.draft_cache.free(seq_id)
+        self.controls.free(seq_id)
 
     def reset(self) -> None:
         self._pending = None
