@@ -407,7 +407,8 @@ typedef struct {
  * n_slices entries) gives the column counts, or interleaved != 0: two slices
  * alternating every 8 columns, as w_gate_up.  swiglu: out (N/2 columns) =
  * silu(gate) * up of those.  out may be base (float32, no SwiGLU): then tokens
- * without an adapter are not touched; otherwise the two must not overlap.
+ * without an adapter are not touched; otherwise the two must not overlap, and
+ * out never overlaps x.
  * The workspace is 16-byte aligned scratch of this call alone.  Calls of little
  * work take one launch that needs none (NULL, 0 bytes); MS_ERR_WORKSPACE, before
  * anything is launched, says that a call does need it.  Tokens of no tile are

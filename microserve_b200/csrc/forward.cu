@@ -127,6 +127,13 @@ extern "C" int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache,
     MS_TRY(validate_lora(&lora->adapters, plan));
     MS_REQUIRE(plan->n_tokens == T, "ms_forward_lora: the plan has %d tokens, the batch %d",
                plan->n_tokens, T);
+    const void* const* const pairs[][2] = {{lora->a_qkv, lora->b_qkv}, {lora->a_o, lora->b_o},
+                                           {lora->a_gate_up, lora->b_gate_up},
+                                           {lora->a_down, lora->b_down}};
+    for (const auto& ab : pairs)
+      for (int l = 0; ab[0] && l < m.n_layers; ++l)
+        MS_REQUIRE(!ab[0][l] || (ab[1] && ab[1][l]),
+                   "ms_forward_lora: an A without its B in layer %d", l);
   }
   const Workspace w = carve(m, T, R, static_cast<unsigned char*>(workspace),
                             adapted ? lora->adapters.max_rank : 0);

@@ -1083,6 +1083,15 @@ extern "C" int ms_lora_add(const void* x, int64_t x_stride, const float* base, i
                               ((int64_t)(plan->n_tokens - 1) * out_stride + outs);
     MS_REQUIRE(o1 <= b0 || b1 <= o0, "ms_lora_add: base and out overlap");
   }
+  {
+    const char* x0 = static_cast<const char*>(x);
+    const char* x1 = x0 + (dtype == MS_DTYPE_F32 ? 4 : 2) *
+                              ((int64_t)(plan->n_tokens - 1) * x_stride + K);
+    const char* o0 = static_cast<const char*>(out);
+    const char* o1 = o0 + (out_dtype == MS_DTYPE_F32 ? 4 : 2) *
+                              ((int64_t)(plan->n_tokens - 1) * out_stride + outs);
+    MS_REQUIRE(o1 <= x0 || x1 <= o0, "ms_lora_add: x and out overlap");
+  }
   c.x = x;
   c.x_stride = x_stride;
   c.base = base;

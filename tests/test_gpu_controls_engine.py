@@ -173,6 +173,29 @@ def test_a_caller_that_changes_the_tokens_gets_them_counted_afresh(golden) -> No
                           np.bincount(req.output_ids, minlength=V))
 
 
+def test_an_id_used_again_starts_without_counts(golden) -> None:
+    """The decoder used directly: a freed id's next request has the length that was counted."""
+    from microserve_b200.cache import PagedKVCache
+    from microserve_b200.config import CacheConfig, SamplingConfig
+    from microserve_b200.scheduler import Request
+    from microserve_b200.speculative import SpeculativeDecoder
+
+    target, draft = device_model(golden, "target"), device_model(golden, "draft")
+    dec = SpeculativeDecoder(target, draft, CacheConfig(8, 64), gamma=2)
+    cache = PagedKVCache(target.cfg, CacheConfig(8, 64, target.cfg.dtype), DEV)
+    cfg = SamplingConfig(temperature=0.0, max_new_tokens=500, repetition_penalty=1.4)
+    first = Request(7, _prompts(golden, 1)[0], cfg)
+    new = dec.step([first], cache, {7: torch.Generator().manual_seed(0)})[0]
+    cache.free(7)
+    dec.free(7)
+    second = Request(7, [3] * (first.num_tokens + len(new)), cfg)
+    dec.controls.prepare([second])
+    slot = dec.controls._slot[7]
+    assert not dec.controls.counts.counts[slot].any()
+    seen = dec.controls.counts.seen[slot].cpu().tolist()
+    assert seen[0] == 1 << 3 and not any(seen[1:])
+
+
 def test_sampled_speculation_follows_the_controlled_distribution(golden) -> None:
     """Chi-square of the first token of 4096 requests against the controlled softmax: the accept
     rule has to use controlled draft and target rows alike."""
@@ -332,8 +355,8 @@ def _again(model, tokens):
 
 
 def test_adapters_on_the_tensor_core_path() -> None:
-    """bf16: tokens without an adapter keep their logits, bit for bit; the others agree with a
-    merged model to the bf16 models' 2e-2 of the row's scale."""
+    """bf16: tokens without an adapter agree with the shared weights, the others with a merged
+    model, to the bf16 models' 2e-2 of the row's scale."""
     from microserve_b200.batching import build_paged_batch
     from microserve_b200.cache import PagedKVCache
     from microserve_b200.config import CacheConfig, ModelConfig
@@ -367,6 +390,27 @@ def test_adapters_on_the_tensor_core_path() -> None:
         assert_bf16_close(got[rows].cpu().numpy(), want[rows].cpu().numpy())
         if n is not None:  # and the adapter does something
             assert (got[rows] - plain[rows]).abs().max() > 0.05
+
+
+def test_an_array_of_a_without_b_is_refused(golden) -> None:
+    import ctypes
+
+    from microserve_b200 import _lib
+    from microserve_b200.batching import build_paged_batch
+    from microserve_b200.cache import PagedKVCache
+    from microserve_b200.config import CacheConfig
+    from microserve_b200.lora import LoraAdapters
+
+    model = device_model(golden, "target")
+    ads = LoraAdapters(model)
+    ads.load("a", adapter_state(model.cfg, 4, 1, ALL))
+    cache = PagedKVCache(model.cfg, CacheConfig(8, 64, model.cfg.dtype), DEV)
+    batch = build_paged_batch(cache, [0], [_prompts(golden, 1)[0]], [0])
+    n = batch.n_tokens
+    ads.c_struct().b_o = ctypes.POINTER(ctypes.c_void_p)()
+    with pytest.raises(_lib.MicroserveError, match="without its B"):
+        model.forward_paged(batch, cache, lora=ads.plan(["a"], [n]))
+    assert _lib.device_error() == 0
 
 
 def test_loading_refusals_change_nothing(golden) -> None:

@@ -103,6 +103,7 @@ def test_c_entry_points_refuse_before_launching() -> None:
     assert lora(x=0) == bad and lora(x_ld=63) == bad and lora(base_ld=63) == bad
     assert lora(out_ld=63) == bad and lora(out=(1 << 16) + 32) == bad  # overlaps the base
     assert lora(out=1 << 16, od=1) == bad  # bf16 over the float32 base
+    assert lora(x=(1 << 20) + 512) == bad and lora(x=(1 << 20) - 256) == bad  # x overlaps out
     assert lora(ws=1 << 24, n_ws=8, K=263, x_ld=263) == _lib.MS_ERR_WORKSPACE  # too small
     assert lora(a=0) == bad
     assert lora(ad=_lib.MsLoraAdapters(1, 16, 257, 0, 1, 1, 1)) == bad
