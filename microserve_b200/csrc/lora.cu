@@ -368,14 +368,14 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_one_kernel(ShrinkArgs 
 // goes through its share of the columns, 32 WN at a step: their base values
 // and adapter rows come in by cp.async, up to three steps ahead.  mma m16n8k16
 // with tokens as M, columns as N, the rank as K; warp (m, n) of the WM x WN
-// has 16 tokens and 32 columns.  The sums start from the base and leave
-// through its buffer, in whole 32-byte sectors.
+// has 16 tokens and 32 columns.  The result leaves through the base's buffer, in
+// whole 32-byte sectors.
 // 1536 tokens of 256 adapters, rank 16, N = 4096 (84 MB): 21.8 us (3.9 TB/s, near the
 // rate at which half of it can be written).  1280 tokens of 32 adapters, rank 16-32,
 // N = 11264 with the SwiGLU (89 MB): 26 us after the first product (3.4 TB/s); 14
 // warps a SM keep the issue slots half busy, and what they wait for most is the
 // result of the last instruction.  Small CTAs do best: 512 threads took 42 us for the
-// call's two products, 256 38 and 128 36; more of them per SM by fewer registers (96
+// call's two products, 256 38 and 128 36 (37 with the base added last); more of them per SM by fewer registers (96
 // of 122) take 8B's two products from 57 to 76 us.
 constexpr int kPad = 8;  // elements after each shared-memory row: conflict-free fragment reads
 
@@ -548,16 +548,6 @@ __global__ void __launch_bounds__(32 * WM * WN, 1) lora_expand_kernel(ExpandArgs
       if (m >= here || c >= p.N) continue;
       const bool upper = here - m > 8;  // tokens in the upper 8 rows
       float acc[4][4] = {};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == 1 && !upper) break;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float2 v = *reinterpret_cast<const float2*>(s_base + (g + 8 * h) * kBaseLd + 8 * n + 2 * t);
-          acc[n][2 * h] = v.x;
-          acc[n][2 * h + 1] = v.y;
-        }
-      }
       const uint32_t sa = s_addr(s_s + (m + (lane & 15)) * s_ld + 8 * (lane >> 4));
       const uint32_t sb = s_addr(s_b + (lane & 15) * kBLd + 8 * (lane >> 4));
       if (p.interleaved) {
@@ -568,6 +558,17 @@ __global__ void __launch_bounds__(32 * WM * WN, 1) lora_expand_kernel(ExpandArgs
           expand_mma<TERMS, kOneSlice>(acc, sa, sb, rank_p, 32 * kBLd, p, c, j0, j0);
         else
           expand_mma<TERMS, kMixed>(acc, sa, sb, rank_p, 32 * kBLd, p, c, j0, j1);
+      }
+      // the base is added last: an MMA truncates its sum to the accumulator's 24 bits
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !upper) break;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float2 v = *reinterpret_cast<const float2*>(s_base + (g + 8 * h) * kBaseLd + 8 * n + 2 * t);
+          acc[n][2 * h] += v.x;
+          acc[n][2 * h + 1] += v.y;
+        }
       }
       // out through this warp's part of the base rows, which all its lanes have read
       __syncwarp();

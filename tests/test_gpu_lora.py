@@ -188,6 +188,26 @@ def test_swiglu_epilogue(dtype: str, of: list[int], ranks: list[int], K: int, N:
         assert (err <= bound).all()
 
 
+@pytest.mark.parametrize("of,ranks,K,dtype", [
+    ([0, 1, 0], [16, 8], 64, "bfloat16"),
+    (mixed(40, 6), [256, 16, 40, 64, 3, 128], 64, "bfloat16"),
+    ([0] * 24 + [1] * 30, [256, 40], 64, "bfloat16"),
+    ([0] * 300, [128], 64, "bfloat16"),
+    (mixed(30, 3), [256, 7, 20], 64, "float32"),
+])
+def test_the_base_is_rounded_once(of: list[int], ranks: list[int], K: int, dtype: str) -> None:
+    """A base far above the adapters' part, a float32 result: beside the part's own error
+    (Case.tolerance), one rounding of the sum."""
+    from microserve_b200.lora import lora_add
+
+    c = Case(of, ranks, K, [136], dtype)
+    c.base *= 4096.0
+    y, _, terms = c.want()
+    got = lora_add(c.x, c.base, c.proj, c.plan).double().cpu().numpy()
+    part = c.tolerance(np.zeros_like(y), terms, torch.float32)
+    assert (np.abs(got - y) <= part * (1 + 2.0 ** -20) + np.abs(y) * 2.0 ** -24 * (1 + 2.0 ** -20)).all()
+
+
 def test_strides_and_rows_behind_the_batch() -> None:
     from microserve_b200.lora import lora_add
 
