@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_one_kernel(ShrinkArgs 
 // N = 11264 with the SwiGLU (89 MB): 26 us after the first product (3.4 TB/s); 14
 // warps a SM keep the issue slots half busy, and what they wait for most is the
 // result of the last instruction.  Small CTAs do best: 512 threads took 42 us for the
-// call's two products, 256 38 and 128 36 (37 with the base added last); more of them per SM by fewer registers (96
-// of 122) take 8B's two products from 57 to 76 us.
+// call's two products, 256 38 and 128 36 (37 with the base added last); more of them
+// per SM by fewer registers (96 of 122) take 8B's two products from 57 to 76 us.
 constexpr int kPad = 8;  // elements after each shared-memory row: conflict-free fragment reads
 
 // Which slice a warp's 32 columns take their s from.
