@@ -53,6 +53,10 @@ namespace {
 // MMAs at once, instead of the four separate pairs of the nominal layout.
 // A CTA takes 16 * MT rank rows, 8 * NT tokens at a time; its 8 warps and the CTAs of its
 // cluster share out k, and the parts meet in (distributed) shared memory.
+// An MMA truncates its sum to the accumulator's 24 bits, always towards zero: four or
+// eight of them make a partial sum, which is added in float32 with rounding (a running
+// sum of n MMAs comes out about n 2^-26 too small: 1.6e-6 for K = 14336 over 8 warps).
+// The steps of a partial sum have their loads in flight together.
 // Each slice's rank rows are padded to a multiple of 16 (`rank_p`), with
 // zeros in s.  Bound by HBM where every few tokens bring an adapter of their own:
 // 1536 tokens of 256 adapters of rank 16, K = 14336 (161 MB), 28.7 us (5.6 TB/s).
@@ -96,27 +100,38 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
       xr[n] = p.x + (int64_t)max(tok, 0) * p.x_stride + 8 * t;
     }
     float acc[MT][NT][4] = {};
-#pragma unroll (MT + NT <= 3 ? 4 : 2)
-    for (int k0 = split * p.k_per + 32 * warp; k0 < k_end; k0 += 32 * kShrinkWarps) {
-      const bool in = k0 + 8 * t < k_end;
-      uint4 xv[NT], av[MT][2];
+    constexpr int kParts = MT + NT <= 3 ? 4 : 2;  // steps of a partial sum
+    for (int k1 = split * p.k_per + 32 * warp; k1 < k_end; k1 += 32 * kShrinkWarps * kParts) {
+      float sum[MT][NT][4] = {};
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const int k0 = k1 + 32 * kShrinkWarps * i;
+        const bool in = k0 + 8 * t < k_end;
+        uint4 xv[NT], av[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            av[m][h] = in && row_in[m][h] ? __ldg(reinterpret_cast<const uint4*>(ar[m][h] + k0)) : zero;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          xv[n] = in && 8 * n < count ? __ldg(reinterpret_cast<const uint4*>(xr[n] + k0)) : zero;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (8 * n >= count) break;
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma_bf16(sum[m][n], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv[n].x, xv[n].y);
+            mma_bf16(sum[m][n], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv[n].z, xv[n].w);
+          }
+        }
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          av[m][h] = in && row_in[m][h] ? __ldg(reinterpret_cast<const uint4*>(ar[m][h] + k0)) : zero;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        xv[n] = in && 8 * n < count ? __ldg(reinterpret_cast<const uint4*>(xr[n] + k0)) : zero;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (8 * n >= count) break;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          mma_bf16(acc[m][n], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv[n].x, xv[n].y);
-          mma_bf16(acc[m][n], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv[n].z, xv[n].w);
-        }
-      }
+          for (int e = 0; e < 4; ++e) acc[m][n][e] += sum[m][n][e];
     }
     // the warps' parts, summed in warp order
 #pragma unroll
@@ -147,7 +162,7 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
 // The same for larger tiles: 64 tokens x RB rank rows per CTA, both operands
 // through shared memory (each is read RB / 16 and 4 times), k in steps of 64
 // behind a ring of cp.async.  Warp (m, n) of the 4 x 2 has 16 tokens and RB / 2
-// rank rows.  1280 tokens of 32 adapters, K = 2048, two slices, rank 16-32 (11 MB):
+// rank rows; each step's four MMAs make a partial sum, added with rounding.  1280 tokens of 32 adapters, K = 2048, two slices, rank 16-32 (11 MB):
 // 9.5 us, the latency of the ring's first steps and of the cluster's sum.
 constexpr int kBigK = 64;
 constexpr int kBigLd = kBigK + 8;  // padded row (elements): conflict-free ldmatrix
@@ -216,6 +231,7 @@ __global__ void __launch_bounds__(256, 2) lora_shrink_tile_kernel(ShrinkArgs p) 
     const uint32_t xa = s_addr(xs + (16 * wm + (lane & 15)) * kBigLd + 8 * (lane >> 4));
     const uint32_t aa = s_addr(xs + (kTile + wn * (RB / 2) + (lane & 7) + 8 * (lane >> 4)) * kBigLd +
                                8 * ((lane >> 3) & 1));
+    float sum[NT][4];
 #pragma unroll
     for (int k = 0; k < kBigK; k += 16) {
       uint32_t xf[4];
@@ -224,10 +240,19 @@ __global__ void __launch_bounds__(256, 2) lora_shrink_tile_kernel(ShrinkArgs p) 
       for (int n = 0; n < NT; n += 2) {
         uint32_t af[4];  // rank rows 8n .. 8n+15: b0, b1 of n, then of n + 1
         ldsm4(af, aa + n * 8 * kBigLd * 2 + 2 * k);
-        mma_bf16(acc[n], xf[0], xf[1], xf[2], xf[3], af[0], af[1]);
-        mma_bf16(acc[n + 1], xf[0], xf[1], xf[2], xf[3], af[2], af[3]);
+        if (k == 0) {
+          mma_bf16_first(sum[n], xf[0], xf[1], xf[2], xf[3], af[0], af[1]);
+          mma_bf16_first(sum[n + 1], xf[0], xf[1], xf[2], xf[3], af[2], af[3]);
+        } else {
+          mma_bf16(sum[n], xf[0], xf[1], xf[2], xf[3], af[0], af[1]);
+          mma_bf16(sum[n + 1], xf[0], xf[1], xf[2], xf[3], af[2], af[3]);
+        }
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] += sum[n][e];
   }
   cp_wait<0>();
   __syncthreads();
@@ -314,8 +339,11 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_one_kernel(ShrinkArgs 
         const uint4 xv = kin ? __ldg(reinterpret_cast<const uint4*>(xr + k0)) : zero;
         const uint4 a0 = kin && g < tile.rank ? __ldg(reinterpret_cast<const uint4*>(ar[0] + k0)) : zero;
         const uint4 a1 = kin && 8 + g < tile.rank ? __ldg(reinterpret_cast<const uint4*>(ar[1] + k0)) : zero;
-        mma_bf16(acc, a0.x, a1.x, a0.y, a1.y, xv.x, xv.y);
-        mma_bf16(acc, a0.z, a1.z, a0.w, a1.w, xv.z, xv.w);
+        float sum[4];
+        mma_bf16_first(sum, a0.x, a1.x, a0.y, a1.y, xv.x, xv.y);
+        mma_bf16(sum, a0.z, a1.z, a0.w, a1.w, xv.z, xv.w);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q] += sum[q];
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) s_red[warp][2 * t + (q & 1)][g + 8 * (q >> 1)] = acc[q];

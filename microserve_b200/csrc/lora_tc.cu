@@ -139,6 +139,16 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint4& a, const ui
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+// The load and its wait in one, so that nothing that uses the values comes between.
+__device__ __forceinline__ void tmem_ld8_wait(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ void st4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
@@ -199,17 +209,24 @@ __device__ bool load_pair(const ms_lora_plan& p, const ms_lora_adapters& ad, int
 // s of up to 128 tokens x 256 rank rows per CTA: both operands K-major, k in steps
 // of 64 through a ring of four slots, two loading warps each; k is shared out
 // over a cluster, whose parts meet in distributed shared memory, summed in
-// cluster order.  x is read once, A by every pair of tiles out of L2.  8192 tokens,
-// K = 4096, two slices of rank 64-128 (73 MB): 46 us, by mma.sync 95; about 15 us of
+// cluster order.  The MMAs of eight steps make a partial sum in one of two
+// accumulators; the loading warps add it up in float32 registers while their next
+// copies are in flight.  (An MMA truncates its sum to 24 bits, always towards zero: a
+// running sum over K = 14336 comes out 1.4e-5 too small, over 512 k values 5e-7.  The
+// call below takes 302 us with one running sum, 304 with eight steps each, 308 with four.)
+// x is read once, A by every pair of tiles out of L2.  8192 tokens,
+// K = 4096, two slices of rank 64-128 (73 MB): 48 us, by mma.sync 95; about 15 us of
 // it start, the hand-over of 128 KB of sums per CTA through shared memory, and the
 // stores of s.
 constexpr int kSteps = 4;                       // ring slots
+constexpr int kSumSteps = 8;                    // steps of a partial sum, a multiple of kSteps
 constexpr int kStepK = 64;
 constexpr int kRankRows = 256;                  // most rank rows per CTA
 constexpr int kStepBytes = (kRows + kRankRows) * 128;
 constexpr int kPartLd = kRankRows + 4;          // floats per token of the parts
 constexpr int kShrinkBytes = 1024 + kBarBytes + kSteps * kStepBytes;
 constexpr int kShrinkThreads = 288;             // 8 loading warps, 1 for the MMAs
+constexpr int kShrinkTmem = 2 * kRankRows;      // two accumulators
 static_assert(kRows * kPartLd * 4 <= kSteps * kStepBytes, "the parts fit the ring");
 
 __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(ShrinkArgs p) {
@@ -222,7 +239,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
   const int splits = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
   const uint32_t raw = s_addr(smem_raw);
   const uint32_t ring = raw + ((1024u - (raw & 1023u)) & 1023u), bars = ring + kSteps * kStepBytes;
-  const uint32_t full = bars, empty = full + 8 * kSteps, done = empty + 8 * kSteps, slot_addr = done + 8;
+  const uint32_t full = bars, empty = full + 8 * kSteps, summed = empty + 8 * kSteps, taken = summed + 16,
+                 ended = taken + 16, slot_addr = ended + 8;
   unsigned char* gbars = smem_raw + (bars - raw);
   volatile uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbars + (slot_addr - bars));
   volatile int* stop = reinterpret_cast<int*>(gbars + (slot_addr - bars) + 4);
@@ -245,14 +263,18 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
       bar_init(full + 8 * k, 64);
       bar_init(empty + 8 * k, 1);
     }
-    bar_init(done, 1);
+    for (int k = 0; k < 2; ++k) {
+      bar_init(summed + 8 * k, 1);
+      bar_init(taken + 8 * k, 8);
+    }
+    bar_init(ended, 1);
     *stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_addr),
-                 "r"(kRankRows));
+                 "r"(kShrinkTmem));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -262,13 +284,35 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
   const int k_begin = split * p.k_per, k_end = min(p.K, k_begin + p.k_per);
   const int steps = k_end > k_begin ? (k_end - k_begin + kStepK - 1) / kStepK : 0;
 
+  const int sums = (steps + kSumSteps - 1) / kSumSteps;
   if (warp < 8) {
     // ---- loads: 16 bytes at k offset 8 i of rows r0, r0 + 8, ...
     const int group = warp >> 1, t = tid & 63, i = t & 7, r0 = t >> 3;
+    // ---- the partial sums: lane quarter warp & 3, half the columns
+    const int row0 = 32 * (warp & 3), c0 = (warp >> 2) * 128;
+    float acc[128] = {};
     bool alive = true;
+    auto take = [&](int sum) {
+      alive = alive && warp_wait(summed + 8 * (sum & 1), (sum >> 1) & 1, stop, p.err);
+      if (!alive) return;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t from = tmem + (sum & 1) * kRankRows + c0 + ((uint32_t)row0 << 16);
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+        if (c0 + c >= here) break;
+        uint32_t r[8];
+        tmem_ld8_wait(from + c, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[c + e] += __uint_as_float(r[e]);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(taken + 8 * (sum & 1));
+    };
+    int taken_sums = 0;
     for (int step = group; step < steps; step += kSteps) {
       if (step >= kSteps) {
-        alive = warp_wait(empty + 8 * group, (step / kSteps - 1) & 1, stop, p.err);
+        alive = alive && warp_wait(empty + 8 * group, (step / kSteps - 1) & 1, stop, p.err);
         if (!alive) break;
       }
       const int k = k_begin + step * kStepK + 8 * i;
@@ -288,45 +332,41 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
         cp_async16(to + kRows * 128 + r * 128, a + (int64_t)max(row, 0) * p.K, in && row >= 0);
       }
       cp_commit();
+      if (taken_sums < step / kSumSteps) take(taken_sums++);  // while the copies are in flight
       cp_wait<0>();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(full + 8 * group);
     }
-    // ---- the accumulators: lane quarter warp & 3, half the columns
-    if (steps > 0) alive = alive && warp_wait(done, 0, stop, p.err);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    while (taken_sums < sums) take(taken_sums++);  // (all MMAs have ended: the ring is free)
     float* part = reinterpret_cast<float*>(smem_raw + (ring - raw));  // [token][kPartLd]
-    const int row0 = 32 * (warp & 3), c0 = (warp >> 2) * 128;
-    for (int c = c0; c < min(here, c0 + 128); c += 16) {
-      uint32_t r[16];
-      if (steps > 0) {
-        tmem_ld16(tmem + c + ((uint32_t)row0 << 16), r);
-        tmem_wait_ld();
-      } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) r[e] = 0u;
-      }
-      uint4* dst = reinterpret_cast<uint4*>(part + (row0 + lane) * kPartLd + c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dst[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+    for (int c = 0; c < 128; c += 4) {
+      if (c0 + c >= here) break;
+      *reinterpret_cast<float4*>(part + (row0 + lane) * kPartLd + c0 + c) =
+          make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   } else if (lane == 0) {
     // ---- MMA
     const uint32_t id = instr(here) & ~(1u << 16);  // B K-major as well
     bool fine = true;
     int step = 0;
     for (; step < steps; ++step) {
-      const int slot = step % kSteps;
+      const int slot = step % kSteps, sum = step / kSumSteps;
+      const bool first = step % kSumSteps == 0;
+      if (first && sum > 1 && !(fine = bar_wait(taken + 8 * (sum & 1), ((sum >> 1) - 1) & 1, stop, p.err))) break;
       if (!(fine = bar_wait(full + 8 * slot, (step / kSteps) & 1, stop, p.err))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint64_t x = desc(ring + slot * kStepBytes, 16), a = desc(ring + slot * kStepBytes + kRows * 128, 16);
+      const uint32_t d = tmem + (sum & 1) * kRankRows;
 #pragma unroll
-      for (int k = 0; k < kStepK / 16; ++k) umma_ss(tmem, x + 2 * k, a + 2 * k, id, step > 0 || k > 0);
+      for (int k = 0; k < kStepK / 16; ++k) umma_ss(d, x + 2 * k, a + 2 * k, id, !first || k > 0);
       umma_commit(empty + 8 * slot);
+      if (step % kSumSteps == kSumSteps - 1 || step == steps - 1) umma_commit(summed + 8 * (sum & 1));
     }
-    if (step > 0) umma_commit(done);
-    if (!fine && step > 0) drain(done, p.err);
+    if (!fine && step > 0) {
+      umma_commit(ended);
+      drain(ended, p.err);
+    }
   }
   __syncwarp();
   if (splits > 1) cluster.sync(); else __syncthreads();
@@ -334,7 +374,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
            count, m0, here, rank_p, p.ad.scales[tile.adapter]);
   if (splits > 1) cluster.sync(); else __syncthreads();  // no CTA leaves while another reads its part
   if (warp == 8)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kRankRows));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kShrinkTmem));
 }
 
 // Shared memory for a rank; 0 when it or TMEM do not do.
