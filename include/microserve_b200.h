@@ -164,8 +164,8 @@ typedef struct {
  * b * rows_per_request + i is row i of request b): repetition penalty on
  * tokens in the prompt or generated, minus frequency * count and presence on
  * generated tokens, plus bias, and -inf where the row's mask forbids the
- * token (a row whose mask allows nothing is all -inf).  In place when out ==
- * logits: only the changed logits are then read and written.  Otherwise the
+ * token (a row whose mask and biases leave nothing is all -inf: there is
+ * nothing to draw from it).  In place when out == logits: only the changed logits are then read and written.  Otherwise the
  * two must not overlap.  A bad slot, token, mask row or bias order sets the
  * device error word and is skipped. */
 MS_API int ms_apply_logit_controls(const float* logits, int64_t row_stride, float* out,

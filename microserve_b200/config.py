@@ -147,9 +147,10 @@ class SamplingConfig:
     # logits.py).  Tokens of the prompt or generated so far have positive
     # logits divided and negative ones multiplied by ``repetition_penalty``;
     # generated tokens lose ``frequency_penalty`` per occurrence and
-    # ``presence_penalty`` once; ``logit_bias`` adds to single tokens;
+    # ``presence_penalty`` once; ``logit_bias`` adds to single tokens (-inf bans one);
     # ``allowed_tokens`` maps the tokens generated so far to the tokens allowed
-    # next: a bool array over the vocabulary, or None for all of them.
+    # next: a bool array over the vocabulary, or None for all of them.  Settings
+    # that leave no token are refused with ``ValueError``.
     repetition_penalty: float = 1.0
     presence_penalty: float = 0.0
     frequency_penalty: float = 0.0

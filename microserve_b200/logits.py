@@ -22,7 +22,7 @@ speculative decoder use.
 from __future__ import annotations
 
 import struct
-from collections.abc import Sequence
+from collections.abc import Iterable, Sequence
 from dataclasses import dataclass
 from typing import TYPE_CHECKING
 
@@ -168,8 +168,8 @@ def apply_logit_controls(
     ``i`` of a request treats its first ``first_proposal + i`` as generated.
     ``out`` may be ``logits`` itself (only the changed logits are then touched)
     or a tensor that does not overlap it; by default a new one is returned.
-    Masked tokens become ``-inf``; a row whose mask allows nothing is all
-    ``-inf``.  Rows may be strided; a row's logits must be contiguous."""
+    Masked tokens become ``-inf``; a row whose mask and biases leave nothing is all
+    ``-inf`` (there is nothing to draw from it: do not).  Rows may be strided; a row's logits must be contiguous."""
     dev = _lib.cuda_index(logits)
     if logits.dim() != 2 or logits.dtype is not torch.float32 or logits.stride(1) != 1:
         raise ValueError("logits must be a float32 (rows, vocab) tensor with contiguous rows")
@@ -256,16 +256,28 @@ class RequestControls:
         self._recount_upload = HostStaging(device)
 
     def check(self, sampling: SamplingConfig) -> None:
-        """Raise ``ValueError`` for biases of no token, or that are no number or +inf."""
+        """Raise ``ValueError`` for biases of no token, that are no number or +inf, or that ban
+        every token."""
         if sampling.logit_bias:
             self._check_bias(np.array(list(sampling.logit_bias)),
-                             np.array(list(sampling.logit_bias.values()), np.float32))
+                             self._bias_values(sampling.logit_bias.values()), [len(sampling.logit_bias)])
 
-    def _check_bias(self, ids: np.ndarray, values: np.ndarray) -> None:
+    @staticmethod
+    def _bias_values(values: Iterable[float]) -> np.ndarray:
+        with np.errstate(over="ignore"):  # below float32's range: -inf, a ban
+            return np.array(list(values), np.float32)
+
+    def _check_bias(self, ids: np.ndarray, values: np.ndarray, counts: Sequence[int]) -> None:
+        """Biases of requests that have ``counts`` of them each."""
         if ids.dtype.kind not in "iu" or ids.min() < 0 or ids.max() >= self.vocab_size:
             raise ValueError("logit_bias names a token outside the vocabulary")
         if not np.all(values < np.inf):
             raise ValueError("logit_bias values must be numbers below +inf")  # -inf bans a token
+        end = 0
+        for n in counts:
+            end += n
+            if n >= self.vocab_size and np.all(values[end - n : end] == -np.inf):
+                raise ValueError("logit_bias bans every token")
 
     @staticmethod
     def wanted(requests: Sequence[Request]) -> bool:
@@ -273,7 +285,7 @@ class RequestControls:
 
     def masks_of(self, requests: Sequence[Request]) -> dict[int, np.ndarray]:
         """The allowed tokens of the requests that restrict them, by index.  Raises ``ValueError``
-        for an array of the wrong shape or one that allows nothing."""
+        for an array of the wrong shape or one that allows nothing the request's biases leave."""
         out: dict[int, np.ndarray] = {}
         for i, r in enumerate(requests):
             if r.sampling.allowed_tokens is None:
@@ -285,8 +297,16 @@ class RequestControls:
             if allowed.shape != (self.vocab_size,) or allowed.dtype != np.bool_:
                 raise ValueError(f"request {r.request_id}: allowed_tokens must give a bool array of "
                                  f"{self.vocab_size} entries")
-            if not allowed.any():
-                raise ValueError(f"request {r.request_id}: allowed_tokens allows no token")
+            left = allowed
+            if r.sampling.logit_bias:
+                ids = np.array(list(r.sampling.logit_bias))
+                values = self._bias_values(r.sampling.logit_bias.values())
+                self._check_bias(ids, values, [len(ids)])
+                left = allowed.copy()
+                left[ids[values == -np.inf]] = False
+            if not left.any():
+                raise ValueError(f"request {r.request_id}: allowed_tokens allows no token"
+                                 + (" that logit_bias does not ban" if allowed.any() else ""))
             out[i] = allowed
         return out
 
@@ -333,8 +353,8 @@ class RequestControls:
         if any(r.sampling.logit_bias for r in requests):
             lists = [sorted((r.sampling.logit_bias or {}).items()) for r in requests]
             ids = np.array([v for x in lists for v, _ in x])
-            values = np.array([b for x in lists for _, b in x], np.float32)
-            self._check_bias(ids, values)
+            values = self._bias_values(b for x in lists for _, b in x)
+            self._check_bias(ids, values, [len(x) for x in lists])
             parts["bias_start"] = np.cumsum([0] + [len(x) for x in lists]).astype(np.int32)
             parts["bias_ids"] = ids.astype(np.int32)
             parts["bias_values"] = values.view(np.int32)
