@@ -250,14 +250,16 @@ class LoraAdapters:
             at = o + r
         if at + rank > self._capacity:
             capacity = max(2 * self._capacity, at + rank)
-            self._c = None  # it holds the old pools' addresses
-            for name in self._shape:
+            # all of them before any is replaced: memory may run out in between
+            grown = {name: self._pools(name, capacity) for name in self._shape}
+            for name, (a, b) in grown.items():
                 ns = len(self._shape[name][1])
-                for pool, new, per in zip((self._a[name], self._b[name]),
-                                          self._pools(name, capacity), (ns, 1)):
-                    for i, (old, fresh) in enumerate(zip(pool, new)):
+                for pool, new, per in ((self._a[name], a, ns), (self._b[name], b, 1)):
+                    for old, fresh in zip(pool, new):
                         fresh[: per * self._capacity].copy_(old)
-                        pool[i] = fresh
+            self._c = None  # it holds the old pools' addresses
+            for name, (a, b) in grown.items():
+                self._a[name], self._b[name] = a, b
             self._capacity = capacity
         return at
 
