@@ -16,8 +16,6 @@ uniforms, plus a chi-square test against the reference itself.
 
 from __future__ import annotations
 
-import math
-
 import numpy as np
 import torch
 
@@ -25,6 +23,7 @@ from . import _lib
 from .config import SamplingConfig
 
 NEG_INF = float("-inf")
+_F32_OVERFLOW = 2.0 ** 128 - 2.0 ** 103  # rounds to inf in float32
 
 
 def make_params(
@@ -47,10 +46,12 @@ def validate(cfg: SamplingConfig) -> None:
         raise ValueError("top_k must be positive")
     if cfg.top_p is not None and not 0.0 < cfg.top_p <= 1.0:
         raise ValueError("top_p must be in (0, 1]")
-    if not (0.0 < cfg.repetition_penalty < math.inf):
+    # the kernel has them in float32, where they have to be finite (and the first one not 0)
+    if not (2.0 ** -150 < cfg.repetition_penalty < _F32_OVERFLOW):
         raise ValueError("repetition_penalty must be positive and finite")
-    if not (math.isfinite(cfg.presence_penalty) and math.isfinite(cfg.frequency_penalty)):
-        raise ValueError("presence_penalty and frequency_penalty must be finite")
+    if not (abs(cfg.presence_penalty) < _F32_OVERFLOW
+            and abs(cfg.frequency_penalty) * max(cfg.max_new_tokens, 1) < _F32_OVERFLOW):
+        raise ValueError("presence_penalty and frequency_penalty times max_new_tokens must be finite")
 
 
 def params_to_device(params: np.ndarray, device: torch.device) -> torch.Tensor:

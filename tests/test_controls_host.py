@@ -50,3 +50,34 @@ def test_biases_that_ban_the_whole_vocabulary_are_refused() -> None:
     assert not rc._slot
     every[3] = -1e30
     rc.check(request(logit_bias=every).sampling)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(repetition_penalty=1e-46),  # 0 in float32: x / 0
+    dict(repetition_penalty=2.0 ** -150),
+    dict(repetition_penalty=1e39),
+    dict(presence_penalty=1e39), dict(presence_penalty=-1e39),
+    dict(frequency_penalty=1e39),  # inf * 0 occurrences
+    dict(frequency_penalty=-1e39),
+    dict(frequency_penalty=1e37, max_new_tokens=100),  # beyond the range once a token repeats enough
+])
+def test_penalties_beyond_float32_are_refused(kw: dict) -> None:
+    from microserve_b200.config import SamplingConfig
+    from microserve_b200.sampling import validate
+
+    with pytest.raises(ValueError, match="penalty"):
+        validate(SamplingConfig(**kw))
+
+
+def test_penalties_within_float32_are_accepted() -> None:
+    from microserve_b200.config import SamplingConfig
+    from microserve_b200.sampling import validate
+
+    for kw in (dict(repetition_penalty=1e-45), dict(repetition_penalty=3e38), dict(presence_penalty=-3e38),
+               dict(frequency_penalty=1e36, max_new_tokens=100), dict(frequency_penalty=3e38, max_new_tokens=1),
+               dict(frequency_penalty=0.5, max_new_tokens=0)):
+        cfg = SamplingConfig(**kw)
+        validate(cfg)
+        for v in (cfg.repetition_penalty, cfg.presence_penalty, cfg.frequency_penalty):
+            assert np.isfinite(np.float32(v))
+        assert np.float32(cfg.repetition_penalty) > 0
