@@ -26,7 +26,8 @@ A request may bring logit controls (``SamplingConfig`` penalties, biases and
 allowed tokens) and the name of a low-rank adapter loaded beside the model
 (``add_request(adapter=...)``); both work inside the shared batch.  While a
 scheduled request restricts its tokens (``allowed_tokens`` asks the host between
-tokens), the iteration is an ordinary pass.
+tokens), or has penalties where a round has more than 64 proposals, the iteration
+is an ordinary pass.
 """
 
 from __future__ import annotations
@@ -246,9 +247,8 @@ class LLMEngine:
     def _round_fits(self, plan: SchedulerOutput) -> bool:
         """A speculative round needs every request decoding (one uncomputed
         token), room for gamma + 1 tokens per request, and no request whose
-        allowed tokens the host has to name one token at a time."""
-        if self.spec is None or any(r.sampling.allowed_tokens is not None
-                                    for r in plan.scheduled):
+        controls a round cannot apply (``SpeculativeDecoder.can_control``)."""
+        if self.spec is None or not all(self.spec.can_control(r.sampling) for r in plan.scheduled):
             return False
         width = self.config.speculative.gamma + 1
         return all(not r.is_prefill and self.cache.can_append(r.request_id, width)

@@ -37,7 +37,7 @@ from . import _lib
 from .batching import HostStaging, batch_from_host, pack_int32
 from .cache import OutOfCacheMemory, PagedKVCache
 from .config import CacheConfig, SamplingConfig
-from .logits import LogitControls, RequestControls, apply_logit_controls
+from .logits import MAX_PROPOSALS, LogitControls, RequestControls, apply_logit_controls
 from .lora import LoraPlan
 from .model import PagedBatch, Transformer
 from .sampling import generator_seed_and_step, make_params, validate
@@ -256,8 +256,9 @@ class SpeculativeDecoder:
     draft's and the target's logits alike: row i of a verify pass sees the
     proposals before it as generated, and the tokens a round emits are counted
     on the device right after the accept kernel, before a chained round's draft
-    passes.  ``allowed_tokens`` needs the host between tokens and is refused here
-    (the engine serves such requests with ordinary passes).  A request's
+    passes.  ``allowed_tokens`` needs the host between tokens and is refused here, and so
+    are penalties when gamma is above 64, the proposals that they count (the
+    engine serves such requests with ordinary passes).  A request's
     adapter applies to the target; the draft proposes with its shared weights."""
 
     def __init__(
@@ -315,6 +316,12 @@ class SpeculativeDecoder:
         self.lookahead_hits = 0
         self.lookahead_misses = 0
 
+    def can_control(self, sampling: SamplingConfig) -> bool:
+        """Whether a round can apply a request's controls: no allowed tokens, which the host
+        names one token at a time, and no penalties beside more proposals than they count."""
+        return sampling.allowed_tokens is None and not (self.gamma > MAX_PROPOSALS
+                                                        and sampling.penalised)
+
     # -- one round ------------------------------------------------------------
     def step(
         self,
@@ -332,6 +339,9 @@ class SpeculativeDecoder:
             validate(cfg)
             if cfg.allowed_tokens is not None:
                 raise ValueError("allowed_tokens cannot be combined with a speculative round")
+            if not self.can_control(cfg):
+                raise ValueError(f"penalties count at most {MAX_PROPOSALS} proposals of a "
+                                 f"speculative round, gamma is {G}")
         for r in requests:
             if r.adapter is not None and (self.target.adapters is None
                                           or r.adapter not in self.target.adapters):
