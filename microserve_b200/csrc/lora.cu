@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
       s_red[i] = v;  // only this thread reads or writes column i of the parts
     }
     if (splits > 1) cluster.sync(); else __syncthreads();
-    finish_s(p, cluster, s_red, 16 * MT, tile.start + first, count, m0, min(16 * MT, rows - m0), rank_p,
+    finish_s(p, cluster, s_red, 16 * MT, tile.start + first, count, m0, min(16 * MT, rows - m0), tile.rank,
              p.ad.scales[tile.adapter]);
     // no CTA leaves, or starts on s_red again, while another reads its part
     if (splits > 1) cluster.sync(); else __syncthreads();
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(256, 2) lora_shrink_tile_kernel(ShrinkArgs p) 
     for (int e = 0; e < 4; ++e)
       part[(16 * wm + g + 8 * (e >> 1)) * kOutLd + wn * (RB / 2) + 8 * n + 2 * t + (e & 1)] = acc[n][e];
   if (splits > 1) cluster.sync(); else __syncthreads();
-  finish_s(p, cluster, part, kOutLd, tile.start, tile.count, m0, min(RB, rows - m0), rank_p,
+  finish_s(p, cluster, part, kOutLd, tile.start, tile.count, m0, min(RB, rows - m0), tile.rank,
            tile.rank > 0 ? p.ad.scales[tile.adapter] : 0.f);
   if (splits > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
@@ -407,7 +407,9 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_one_kernel(ShrinkArgs 
 // per SM by fewer registers (96 of 122) take 8B's two products from 57 to 76 us.
 constexpr int kPad = 8;  // elements after each shared-memory row: conflict-free fragment reads
 
-// Which slice a warp's 32 columns take their s from.
+// Which slice a warp's 32 columns take their s from.  kMixed: several slices', one after
+// another with the other columns' B as zeros (an infinite s of one slice then makes NaN
+// of the other's columns among the 32).
 enum SliceMode { kOneSlice, kInterleaved, kMixed };
 
 // acc += s B for one warp: sa, sb the shared addresses of this lane's ldmatrix

@@ -1,6 +1,8 @@
 // What the adapter kernels share (lora.cu, lora_tc.cu): the plan's tiles, the
 // second product's arguments and epilogues, and small PTX helpers.
 #pragma once
+#include <cmath>
+
 #include "lora.cuh"
 
 namespace ms {
@@ -146,6 +148,11 @@ __device__ __forceinline__ float silu(float x) {
   return x * r;
 }
 
+// What a bf16 term leaves of a value: nothing of an infinite one (inf - inf is NaN).
+__device__ __forceinline__ float rest(float v, float term) {
+  return fabsf(term) == INFINITY ? 0.f : v - term;
+}
+
 // Four neighbouring values as `terms` bf16 terms each, at dst, dst + step, ...
 __device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int terms, float4 v) {
   for (int k = 0; k < terms; ++k) {
@@ -155,20 +162,22 @@ __device__ __forceinline__ void store_terms(__nv_bfloat16* dst, int step, int te
     w.y = *reinterpret_cast<const uint32_t*>(&b);
     *reinterpret_cast<uint2*>(dst + k * step) = w;
     const float2 fa = __bfloat1622float2(a), fb = __bfloat1622float2(b);
-    v.x -= fa.x;
-    v.y -= fa.y;
-    v.z -= fb.x;
-    v.w -= fb.y;
+    v.x = rest(v.x, fa.x);
+    v.y = rest(v.y, fa.y);
+    v.z = rest(v.z, fb.x);
+    v.w = rest(v.w, fb.y);
   }
 }
 
 // This CTA's share of a cluster's outputs: the parts ([token][ld] floats in each
 // CTA's shared memory) of tokens [0, count) and rank rows [m0, m0 + here), `here`
-// a multiple of 16, summed in cluster order, scaled, and stored as terms.
+// a multiple of 16, summed in cluster order, scaled, and stored as terms.  The rows
+// that pad a slice's rank are stored as zeros: 0 times an infinite x is NaN.
 template <int SPLITS, typename Cluster>
 __device__ __forceinline__ void finish_part(const ShrinkArgs& p, const Cluster& cluster, const float* part,
-                                            int ld, int start, int count, int m0, int here, int rank_p,
+                                            int ld, int start, int count, int m0, int here, int rank,
                                             float scale) {
+  const int rank_p = pad16(rank);
   const int split = SPLITS > 1 ? (int)cluster.block_rank() : 0, quads = here / 4;
 #pragma unroll (SPLITS > 2 ? 2 : 4)
   for (int o = split * blockDim.x + threadIdx.x; o < count * quads; o += SPLITS * blockDim.x) {
@@ -188,19 +197,20 @@ __device__ __forceinline__ void finish_part(const ShrinkArgs& p, const Cluster& 
     }
     const int j = (m0 + row) / rank_p, r = m0 + row - j * rank_p;
     store_terms(p.s + (start + col) * p.s_stride + j * p.terms * rank_p + r, rank_p, p.terms,
-                make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
+                make_float4(r < rank ? v.x * scale : 0.f, r + 1 < rank ? v.y * scale : 0.f,
+                            r + 2 < rank ? v.z * scale : 0.f, r + 3 < rank ? v.w * scale : 0.f));
   }
 }
 
 template <typename Cluster>
 __device__ __forceinline__ void finish_s(const ShrinkArgs& p, const Cluster& cluster, const float* part,
-                                         int ld, int start, int count, int m0, int here, int rank_p,
+                                         int ld, int start, int count, int m0, int here, int rank,
                                          float scale) {
   switch ((int)cluster.num_blocks()) {  // 1, 2, 4 or 8
-    case 1: return finish_part<1>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
-    case 2: return finish_part<2>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
-    case 4: return finish_part<4>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
-    default: return finish_part<8>(p, cluster, part, ld, start, count, m0, here, rank_p, scale);
+    case 1: return finish_part<1>(p, cluster, part, ld, start, count, m0, here, rank, scale);
+    case 2: return finish_part<2>(p, cluster, part, ld, start, count, m0, here, rank, scale);
+    case 4: return finish_part<4>(p, cluster, part, ld, start, count, m0, here, rank, scale);
+    default: return finish_part<8>(p, cluster, part, ld, start, count, m0, here, rank, scale);
   }
 }
 

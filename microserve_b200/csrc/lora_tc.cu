@@ -13,7 +13,8 @@
 //               column) in memory, so B is MN-major.  Gate | up columns
 //               (alternating every 8) are parted by the load into two blocks of
 //               64, one accumulator each; columns where one slice ends and
-//               another begins take two passes, the other slice's columns zero;
+//               another begins take two passes, the other slice's columns zero
+//               (an infinite s of one slice makes NaN of the other's columns there);
 //   warps 4-19  epilogue: TMEM lane quarter warp % 4, 32 of the columns each; a
 //               thread has one row.  Each warp brings its own base in by cp.async,
 //               two steps ahead (16 warps keep more copies in flight than a few
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 1) lora_shrink_tc_kernel(Shrin
   __syncwarp();
   if (splits > 1) cluster.sync(); else __syncthreads();
   finish_s(p, cluster, reinterpret_cast<const float*>(smem_raw + (ring - raw)), kPartLd, tile.start,
-           count, m0, here, rank_p, p.ad.scales[tile.adapter]);
+           count, m0, here, tile.rank, p.ad.scales[tile.adapter]);
   if (splits > 1) cluster.sync(); else __syncthreads();  // no CTA leaves while another reads its part
   if (warp == 8)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kShrinkTmem));
