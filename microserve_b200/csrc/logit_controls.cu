@@ -26,7 +26,7 @@ struct ControlArgs {
   int64_t in_stride;
   float* out;
   int64_t out_stride;
-  int n_requests, rows, rows_per_cta, vocab, words;
+  int n_requests, rows, vocab, words;
   ms_logit_controls c;
   int* err;
 };
@@ -223,7 +223,7 @@ __device__ __forceinline__ void edit_row(const ControlArgs& a, const Slice& sl, 
 }
 
 // ---- out of place, through shared memory ------------------------------------
-// A CTA takes kSlice tokens of one request's rows.  Each row's slice comes in
+// A CTA takes kSlice tokens of all rows of one request.  Each row's slice comes in
 // by one bulk copy, is edited in shared memory and goes out by one bulk copy,
 // in a ring of rows.  The kernel moves 8 bytes per logit and is bound by HBM:
 // 256 requests x 6 rows x 128256 take 300 us (5.3 TB/s), x 5 x 32000 62 us.  A
@@ -278,10 +278,8 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
   const int tid = threadIdx.x;
   const int t0 = blockIdx.x * kSlice;
   const int b = blockIdx.y;
-  const int r0 = blockIdx.z * a.rows_per_cta;
-  const int n_rows = min(a.rows - r0, a.rows_per_cta);
   const int n_here = min(kSlice, a.vocab - t0);
-  const int64_t row0 = (int64_t)b * a.rows + r0;
+  const int64_t row0 = (int64_t)b * a.rows;
 
   // Row it: misalignment (in floats), loose first logits, bulk-copied logits.
   struct Cut {
@@ -314,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
   }
   pdl_enter();
   if (tid == 0)
-    for (int it = 0; it < min(ahead, n_rows); ++it) issue(it);
+    for (int it = 0; it < min(ahead, a.rows); ++it) issue(it);
   const int slot = valid_slot(a, b);
   Penalty p{1.f, 0.f, 0.f};
   if (slot >= 0) p = Penalty{c.penalties[3 * b], c.penalties[3 * b + 1], c.penalties[3 * b + 2]};
@@ -322,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
   load_slice(a, b, slot, row0, t0, n_here, sl, masked);
   const Entry own = list_entry(a, sl, slot, t0, tid);
 
-  for (int it = 0; it < n_rows; ++it) {
+  for (int it = 0; it < a.rows; ++it) {
     float* buf = smem + (it % ring) * kRowFloats;
     const Cut q = cut(it);
     const float* xin = a.in + (row0 + it) * a.in_stride + t0;
@@ -333,11 +331,11 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
     if (tid >= 32 && tail0 + tid - 32 < n_here) buf[q.mis + tail0 + tid - 32] = xin[tail0 + tid - 32];
     bool next_masked = false;
     uint32_t next_mask = 0;
-    if (it + 1 < n_rows) next_mask = mask_word(a, row0 + it + 1, t0, next_masked);
+    if (it + 1 < a.rows) next_mask = mask_word(a, row0 + it + 1, t0, next_masked);
     const bool ok = wait_full(s_addr(&bars[it % ring]), (it / ring) & 1, a.err);
     if (loose) __syncthreads();
     float* x = buf + q.mis;
-    edit_row<true>(a, sl, b, slot, p, own, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
+    edit_row<true>(a, sl, b, slot, p, own, c.first_proposal + it, t0, n_here, sl.mask[it & 1],
                    masked, x, q.mis);
     if (tid < kSlice / 32) sl.mask[(it + 1) & 1][tid] = next_mask;
     masked = next_masked;
@@ -345,7 +343,7 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
     // all threads agree to stop when a copy did not arrive in time
     if (__syncthreads_or(!ok)) {
       if (tid == 0)  // no copy may arrive after the block has gone
-        for (int k = it; k < min(it + ahead, n_rows); ++k)
+        for (int k = it; k < min(it + ahead, a.rows); ++k)
           wait_full(s_addr(&bars[k % ring]), (k / ring) & 1, a.err);
       break;
     }
@@ -354,7 +352,7 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
     if (tid == 0) {
       if (q.body) bulk_store(yout + q.head, s_addr(x + q.head), 4u * q.body);
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      if (it + ahead < n_rows) {
+      if (it + ahead < a.rows) {
         // the row `ahead` from here takes the buffer of the row before this one
         asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         issue(it + ahead);
@@ -383,17 +381,15 @@ __global__ void __launch_bounds__(kDirectThreads) logit_controls_direct_kernel(C
   const int tid = threadIdx.x;
   const int t0 = blockIdx.x * kSlice;
   const int b = blockIdx.y;
-  const int r0 = blockIdx.z * a.rows_per_cta;
-  const int n_rows = min(a.rows - r0, a.rows_per_cta);
   const int n_here = min(kSlice, a.vocab - t0);
-  const int64_t row0 = (int64_t)b * a.rows + r0;
+  const int64_t row0 = (int64_t)b * a.rows;
   const int slot = valid_slot(a, b);
   Penalty p{1.f, 0.f, 0.f};
   if (slot >= 0) p = Penalty{c.penalties[3 * b], c.penalties[3 * b + 1], c.penalties[3 * b + 2]};
   bool masked;
   load_slice(a, b, slot, row0, t0, n_here, sl, masked);
   const Entry own = list_entry(a, sl, slot, t0, tid);
-  for (int it = 0; it < n_rows; ++it) {
+  for (int it = 0; it < a.rows; ++it) {
     float* x = a.out + (row0 + it) * a.out_stride + t0;
     if (a.in != a.out) {
       const float* xin = a.in + (row0 + it) * a.in_stride + t0;
@@ -403,10 +399,10 @@ __global__ void __launch_bounds__(kDirectThreads) logit_controls_direct_kernel(C
     }
     bool next_masked = false;
     uint32_t next_mask = 0;
-    if (it + 1 < n_rows) next_mask = mask_word(a, row0 + it + 1, t0, next_masked);
-    edit_row<false>(a, sl, b, slot, p, own, c.first_proposal + r0 + it, t0, n_here, sl.mask[it & 1],
+    if (it + 1 < a.rows) next_mask = mask_word(a, row0 + it + 1, t0, next_masked);
+    edit_row<false>(a, sl, b, slot, p, own, c.first_proposal + it, t0, n_here, sl.mask[it & 1],
                     masked, x, (int)(reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-    if (it + 1 < n_rows) {
+    if (it + 1 < a.rows) {
       if (tid < kSlice / 32) sl.mask[(it + 1) & 1][tid] = next_mask;
       masked = next_masked;
       __syncthreads();
@@ -502,8 +498,7 @@ extern "C" int ms_apply_logit_controls(const float* logits, int64_t row_stride, 
   MS_REQUIRE(logits && out, "ms_apply_logit_controls: null pointer");
   MS_REQUIRE(row_stride >= vocab && out_stride >= vocab,
              "ms_apply_logit_controls: row stride below the vocabulary");
-  MS_REQUIRE(n_requests <= 65535 && rows_per_request <= 65535,
-             "ms_apply_logit_controls: more than 65535 requests or rows per request");
+  MS_REQUIRE(n_requests <= 65535, "ms_apply_logit_controls: more than 65535 requests");
   const bool in_place = logits == out;
   MS_REQUIRE(!in_place || row_stride == out_stride,
              "ms_apply_logit_controls: in place with two row strides");
@@ -526,16 +521,14 @@ extern "C" int ms_apply_logit_controls(const float* logits, int64_t row_stride, 
   a.c = *controls;
   a.err = device_error_word();
   const int slices = ceil_div(vocab, kSlice);
-  a.rows_per_cta = rows_per_request;
-  const dim3 grid(slices, n_requests, ceil_div(rows_per_request, a.rows_per_cta));
+  const dim3 grid(slices, n_requests);
   const uintptr_t pi = reinterpret_cast<uintptr_t>(logits), po = reinterpret_cast<uintptr_t>(out);
   cudaStream_t s = as_stream(stream);
   ProfScope prof(kClsSample, s);
   // every row of the input and of the output equally far from 16 bytes
   if (!in_place && ((pi ^ po) & 15) == 0 && (row_stride - out_stride) % 4 == 0) {
-    const int ring = a.rows_per_cta < kRing ? a.rows_per_cta : kRing;
-    static std::atomic<uint64_t> granted{0};  // with the static part past the default 48 KB
-    MS_TRY(grant_dynamic_smem(logit_controls_kernel, kRing * kRowFloats * 4, granted));
+    const int ring = rows_per_request < kRing ? rows_per_request : kRing;
+    static_assert(sizeof(Slice) + kRing * (kRowFloats * 4 + 8) <= 48 * 1024, "the default shared memory");
     launch_pdl(logit_controls_kernel, grid, kThreads, ring * kRowFloats * 4, s, a, ring);
     return check_launch("logit_controls_kernel");
   }
