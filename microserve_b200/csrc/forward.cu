@@ -121,10 +121,12 @@ extern "C" int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache,
   const int T = bt.n_tokens;
   const int R = logit_rows ? n_logit_rows : T;
   MS_REQUIRE(R >= 0 && (R == 0 || logits), "ms_forward: logits output missing");
-  const bool adapted = lora != nullptr && plan != nullptr && plan->n_tiles > 0 &&
-                       lora->adapters.max_rank > 0;
-  if (adapted) {
+  if (lora != nullptr) {
+    MS_REQUIRE(plan != nullptr, "ms_forward_lora: adapters without a plan");
     MS_TRY(validate_lora(&lora->adapters, plan));
+  }
+  const bool adapted = lora != nullptr && plan->n_tiles > 0 && lora->adapters.max_rank > 0;
+  if (adapted) {
     MS_REQUIRE(plan->n_tokens == T, "ms_forward_lora: the plan has %d tokens, the batch %d",
                plan->n_tokens, T);
     const void* const* const pairs[][2] = {{lora->a_qkv, lora->b_qkv}, {lora->a_o, lora->b_o},

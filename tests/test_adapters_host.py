@@ -53,3 +53,32 @@ def test_a_growth_that_runs_out_of_memory_changes_nothing(fails_at: int, monkeyp
         assert (p.a[o : o + rank] == value).all() and (p.b[o : o + rank] == -value).all()
     assert all(ads._b[n][0].shape[0] == ads._capacity for n in ads._b)
     assert ads.c_struct().adapters.total_rank == ads._capacity
+
+
+def test_a_forward_with_adapters_needs_their_plan() -> None:
+    """Adapters without a plan, or with a bad one, are refused before anything is launched (the
+    workspace is missing as well, so that nothing could be)."""
+    import ctypes
+
+    from microserve_b200 import _lib
+
+    one = (ctypes.c_void_p * 1)(1 << 12)
+    ptrs = ctypes.cast(one, ctypes.POINTER(ctypes.c_void_p))
+    model = _lib.MsModel(65, 64, 1, 4, 4, 16, 96, 128, _lib.DTYPE_F32, 1e-5, 1 << 12, 1 << 12, 1 << 12,
+                         1 << 12, *[ptrs] * 6)
+    cache = _lib.MsKVCache(1, 8, 8, 4, 16, _lib.DTYPE_F32, ptrs, ptrs)
+    batch = _lib.MsBatch(4, 1, 8, 4, 4, 0, *[1 << 12] * 6)
+    lora = _lib.MsLoraModel(_lib.MsLoraAdapters(1, 16, 16, 0, 1 << 12, 1 << 12, 1 << 12))
+    null = ctypes.POINTER(_lib.MsLoraPlan)()
+
+    def refused(plan, match: str, adapters=lora) -> None:
+        with pytest.raises(_lib.MicroserveError, match=match):
+            _lib.call("ms_forward_lora", ctypes.byref(model), ctypes.byref(cache), ctypes.byref(batch),
+                      ctypes.byref(adapters), plan, None, 0, 1 << 12, 0, None, 0, None)
+
+    refused(null, "without a plan")
+    refused(ctypes.byref(_lib.MsLoraPlan(4, -1, 1 << 12, 1 << 12)), "plan sizes")
+    refused(ctypes.byref(_lib.MsLoraPlan(4, 1, 1 << 12, 1 << 12)), "adapter sizes",
+            _lib.MsLoraModel(_lib.MsLoraAdapters(1, 16, -1, 0, 1 << 12, 1 << 12, 1 << 12)))
+    refused(ctypes.byref(_lib.MsLoraPlan(4, 1, 1 << 12, 1 << 12)), "workspace")  # nothing else is wrong
+    refused(ctypes.byref(_lib.MsLoraPlan(4, 0, None, None)), "workspace")  # ms_forward
