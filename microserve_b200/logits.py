@@ -227,8 +227,11 @@ def apply_logit_controls(
     s = _PACK_CONTROLS(slots, penalties, p_counts, p_seen, n_slots, n_props, props,
                        first_proposal if props else 0, n_bias, starts, ids, values, mask_rows, masks,
                        n_masks, 0)
-    _lib.launch_on(dev, "ms_apply_logit_controls", logits.data_ptr(), logits.stride(0),
-                   out.data_ptr(), out.stride(0), B, rows_per_request, vocab, s)
+    in_ld, out_ld = logits.stride(0), out.stride(0)
+    if rows == 1:  # the stride of a single row says nothing
+        in_ld = out_ld = vocab
+    _lib.launch_on(dev, "ms_apply_logit_controls", logits.data_ptr(), in_ld, out.data_ptr(), out_ld,
+                   B, rows_per_request, vocab, s)
     return out
 
 

@@ -36,3 +36,14 @@ def test_rows_of_two_alignments(V: int, src: tuple[int, int], dst: tuple[int, in
         view.fill_(7.0)
         assert (buf == 7.0).all()
     assert _lib.device_error() == 0
+
+
+def test_a_single_row_of_any_stride() -> None:
+    """A column of logits, transposed, is one row whose stride is 1."""
+    c = Case(1, 1, 4100, seed=3)
+    want, mag = c.want()
+    x = torch.from_numpy(c.x).to(DEV).reshape(4100, 1).t()
+    assert x.shape == (1, 4100) and x.stride(0) == 1
+    assert_controlled(c.run(x).cpu().numpy(), want, mag)
+    assert c.run(x, out=x) is x
+    assert_controlled(x.cpu().numpy(), want, mag)
