@@ -226,7 +226,7 @@ __device__ __forceinline__ void edit_row(const ControlArgs& a, const Slice& sl, 
 // A CTA takes kSlice tokens of all rows of one request.  Each row's slice comes in
 // by one bulk copy, is edited in shared memory and goes out by one bulk copy,
 // in a ring of rows.  The kernel moves 8 bytes per logit and is bound by HBM:
-// 256 requests x 6 rows x 128256 take 300 us (5.3 TB/s), x 5 x 32000 62 us.  A
+// 256 requests x 6 rows x 128256 take 290 us (5.5 TB/s), x 5 x 32000 61 us.  A
 // deeper ring (347 us with 3 rows), half a slice (355) and 128 or 384 threads
 // (314, 327) take more: what hides the latency is the CTAs beside this one.
 // A row that does not start on 16 bytes keeps its misalignment in shared
@@ -371,8 +371,10 @@ __global__ void __launch_bounds__(kThreads) logit_controls_kernel(ControlArgs a,
 // copied first and then edited where it is.  128 threads a CTA: its work is
 // a chain of short dependent reads, so more CTAs per SM beat more threads
 // (grammar masks over 256 x 128256: 28.6 us, 33.9 with 256).  That case writes
-// 104 MB and is at the rate at which this GPU writes (a fill: 3.9 TB/s); reading
-// what a partly masked group of 4 holds, to write it whole, takes 36.7 us.
+// 104 MB (a plain fill: 3.9 TB/s) as 190 MB of sectors at L2; reading what a partly
+// masked group of 4 holds, to write it whole, takes 36.7 us.  Penalties in place, 256 x 5
+// rows x 32000 with 1114 tokens touched in each: 44 us, for 110 MB of sectors read and 35
+// written around 11 MB of logits.
 constexpr int kDirectThreads = 128;
 __global__ void __launch_bounds__(kDirectThreads) logit_controls_direct_kernel(ControlArgs a) {
   pdl_enter();

@@ -5,8 +5,8 @@
 // with the epilogues of lora.cu.  A CTA takes up to 128 tokens of one adapter
 // (two neighbouring tiles of the plan) and goes through its share of the
 // columns, 128 at a step:
-//   warps 0-2   load each step's adapter rows by cp.async, a ring slot per warp, into
-//               the 128-byte swizzle that the MMA reads;
+//   warps 0, 1  load each step's adapter rows by cp.async, a ring slot per warp, into
+//               the 128-byte swizzle that the MMA reads (warp 2 only fills the group);
 //   warp 3      allocates TMEM; lane 0 issues tcgen05.mma with s (bf16 terms side
 //               by side along k) as A in TMEM, copied there once, so that the
 //               MMAs read only B from shared memory.  The adapter rows are (rank,
@@ -23,7 +23,7 @@
 // TMEM: two accumulators of 128 columns, then s (up to 256).  One CTA per SM.
 // The kernel moves 4 bytes in per column and token and 1 to 4 out: HBM is its
 // floor, and shared memory sees the base twice and little else.  8192 tokens, rank
-// 64-128, N = 28672 with the SwiGLU (1.2 GB): 302 us (4.0 TB/s) on 130 of the 148
+// 64-128, N = 28672 with the SwiGLU (1.2 GB): 304 us (3.9 TB/s) on 130 of the 148
 // SMs, one wave of a CTA per pair of tiles and half of the columns, about 3700
 // cycles for each step of 128 x 128; issue slots 44%, tensor pipe 23%, L2 54% busy.
 // The same with s as A in shared memory and both slices against all columns 447 us,
@@ -38,7 +38,7 @@ namespace {
 constexpr int kRows = 128;          // tokens per CTA
 constexpr int kChunk = 128;         // columns per step
 constexpr int kSAt = 2 * kChunk;    // TMEM column of s
-constexpr int kLoadThreads = 96;  // (three warps: the fourth of their group issues the MMAs)
+constexpr int kLoadThreads = 96;  // two loading warps and an idle one: the fourth of their group issues the MMAs
 constexpr int kEpiWarps = 16;
 constexpr int kThreads = kLoadThreads + 32 + 32 * kEpiWarps;
 constexpr int kSegment = 32 * 128;                    // base of 32 rows x 32 columns
