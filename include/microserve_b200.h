@@ -414,8 +414,7 @@ typedef struct {
  * anything is launched, says that a call does need it.  Tokens of no tile are
  * left as they were.  A bad tile, token or adapter sets the device error word
  * and is skipped.  A token whose A x is infinite gets the formula's +-inf and
- * NaN, but NaN may stand for +-inf in columns within 128 of a boundary between
- * slices; other tokens never see it. */
+ * NaN; other tokens never see it. */
 MS_API size_t ms_lora_workspace_size(const ms_lora_adapters* adapters, const ms_lora_plan* plan,
                                      int n_slices);
 MS_API int ms_lora_add(const void* x, int64_t x_stride, const float* base, int64_t base_stride,

@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) lora_one_kernel(ShrinkArgs 
 constexpr int kPad = 8;  // elements after each shared-memory row: conflict-free fragment reads
 
 // Which slice a warp's 32 columns take their s from.  kMixed: several slices', one after
-// another with the other columns' B as zeros (an infinite s of one slice then makes NaN
-// of the other's columns among the 32).
+// another for all columns, of which the other slices' keep what they had (B as zeros
+// there would do, but for an infinite s).
 enum SliceMode { kOneSlice, kInterleaved, kMixed };
 
 // acc += s B for one warp: sa, sb the shared addresses of this lane's ldmatrix
@@ -419,8 +419,8 @@ __device__ __forceinline__ void expand_mma(float (&acc)[4][4], uint32_t sa, uint
                                            uint32_t b_step, const ExpandArgs& p, int c, int j0,
                                            int j1) {
   const uint32_t term = 2u * rank_p, slice = TERMS * term;
-  const int g = (threadIdx.x & 31) >> 2;
-#pragma unroll 2
+  const int t = threadIdx.x & 3;
+#pragma unroll (MODE == kMixed ? 1 : 2)
   for (int k = 0; k < rank_p; k += 16, sa += 32, sb += b_step) {
     uint32_t b[8];  // n-tile n: b[2n], b[2n + 1]
     {
@@ -437,11 +437,15 @@ __device__ __forceinline__ void expand_mma(float (&acc)[4][4], uint32_t sa, uint
         for (int e = 0; e < TERMS; ++e) ldsm4(a[e], sa + j * slice + e * term);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const bool mine = slice_of(p, c + 8 * n + g) == j;  // this lane's column
-          const uint32_t w0 = mine ? b[2 * n] : 0u, w1 = mine ? b[2 * n + 1] : 0u;
+          float had[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) had[e] = acc[n][e];
 #pragma unroll
           for (int e = TERMS - 1; e >= 0; --e)
-            mma_bf16(acc[n], a[e][0], a[e][1], a[e][2], a[e][3], w0, w1);
+            mma_bf16(acc[n], a[e][0], a[e][1], a[e][2], a[e][3], b[2 * n], b[2 * n + 1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)  // this lane's columns 2t and 2t + 1 of the 8
+            if (slice_of(p, c + 8 * n + 2 * t + (e & 1)) != j) acc[n][e] = had[e];
         }
       }
     } else {

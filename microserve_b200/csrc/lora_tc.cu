@@ -13,8 +13,7 @@
 //               column) in memory, so B is MN-major.  Gate | up columns
 //               (alternating every 8) are parted by the load into two blocks of
 //               64, one accumulator each; columns where one slice ends and
-//               another begins take two passes, the other slice's columns zero
-//               (an infinite s of one slice makes NaN of the other's columns there);
+//               another begins take a step for each, which stores its own slice's;
 //   warps 4-19  epilogue: TMEM lane quarter warp % 4, 32 of the columns each; a
 //               thread has one row.  Each warp brings its own base in by cp.async,
 //               two steps ahead (16 warps keep more copies in flight than a few
@@ -23,7 +22,7 @@
 // TMEM: two accumulators of 128 columns, then s (up to 256).  One CTA per SM.
 // The kernel moves 4 bytes in per column and token and 1 to 4 out: HBM is its
 // floor, and shared memory sees the base twice and little else.  8192 tokens, rank
-// 64-128, N = 28672 with the SwiGLU (1.2 GB): 304 us (3.9 TB/s) on 130 of the 148
+// 64-128, N = 28672 with the SwiGLU (1.2 GB): 301 us (4.0 TB/s) on 130 of the 148
 // SMs, one wave of a CTA per pair of tiles and half of the columns, about 3700
 // cycles for each step of 128 x 128; issue slots 44%, tensor pipe 23%, L2 54% busy.
 // The same with s as A in shared memory and both slices against all columns 447 us,
@@ -43,7 +42,7 @@ constexpr int kEpiWarps = 16;
 constexpr int kThreads = kLoadThreads + 32 + 32 * kEpiWarps;
 constexpr int kSegment = 32 * 128;                    // base of 32 rows x 32 columns
 constexpr int kEpiBytes = 2 * kSegment + 32 * 64;     // two of them, and the exchange, per warp
-constexpr int kStages = 2;          // passes in the ring, a loading warp each
+constexpr int kStages = 2;          // steps in the ring, a loading warp each
 constexpr int kBarBytes = 256;
 constexpr int kMostBytes = 226 * 1024;
 constexpr long long kWaitCycles = 1ll << 32;  // ~2.2 s
@@ -214,7 +213,7 @@ __device__ bool load_pair(const ms_lora_plan& p, const ms_lora_adapters& ad, int
 // accumulators; the loading warps add it up in float32 registers while their next
 // copies are in flight.  (An MMA truncates its sum to 24 bits, always towards zero: a
 // running sum over K = 14336 comes out 1.4e-5 too small, over 512 k values 5e-7.  The
-// call below takes 302 us with one running sum, 304 with eight steps each, 308 with four.)
+// whole call below took 302 us with one running sum, 304 with eight steps, 308 with four.)
 // x is read once, A by every pair of tiles out of L2.  8192 tokens,
 // K = 4096, two slices of rank 64-128 (73 MB): 48 us, by mma.sync 95; about 15 us of
 // it start, the hand-over of 128 KB of sums per CTA through shared memory, and the
@@ -392,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   __shared__ int s_tok[kRows];
   const uint32_t raw = s_addr(smem_raw);
   const uint32_t base = raw + ((1024u - (raw & 1023u)) & 1023u);
-  // adapter rows of a pass in two blocks of 64 columns; each epilogue warp's base
+  // adapter rows of a step in two blocks of 64 columns; each epilogue warp's base
   // rows and exchange
   const uint32_t ring = base, stage_bytes = p.rank_pm * kChunk * 2;
   const uint32_t s_x = ring + kStages * stage_bytes, bars = s_x + kEpiWarps * kEpiBytes;
@@ -417,11 +416,20 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
   const int n_chunks = (p.N + kChunk - 1) / kChunk;
   const int chunks = (n_chunks - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   auto column = [&](int chunk) { return ((int)blockIdx.x + chunk * (int)gridDim.x) * kChunk; };
-  // The passes of a chunk: one, or one per slice where a slice ends inside.
-  auto first_slice = [&](int c) { return parted ? 0 : slice_of(p, c); };
-  auto passes = [&](int c) {
-    return parted ? 1 : slice_of(p, min(c + kChunk, p.N) - 1) - slice_of(p, c) + 1;
+  // The steps of this CTA, the same for every warp: a chunk of columns each, or one for
+  // each slice (pass) where a slice ends inside the chunk.
+  struct Walk {
+    int chunk, pass, c, passes;
   };
+  auto enter = [&](int chunk) {
+    const int c = column(chunk);
+    return Walk{chunk, 0, c, parted ? 1 : slice_of(p, min(c + kChunk, p.N) - 1) - slice_of(p, c) + 1};
+  };
+  auto next = [&](Walk w) {
+    if (++w.pass < w.passes) return w;
+    return w.chunk + 1 < chunks ? enter(w.chunk + 1) : Walk{chunks, 0, 0, 1};
+  };
+  auto slice_at = [&](const Walk& w) { return parted ? 0 : slice_of(p, w.c) + w.pass; };
 
   if (threadIdx.x < kRows)
     s_tok[threadIdx.x] =
@@ -455,53 +463,29 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
     // ---- loads of the adapter rows.  Each warp fills its own slot of the ring, so
     // that a slot waiting to be free does not hold up the others.
     const int q = lane & 15, r0 = lane >> 4;
-    auto load_b = [&](uint32_t dst, int c0, int pass) {
+    auto load_b = [&](uint32_t dst, int c0) {
       const int c = c0 + 8 * q;
       // block and place of these 8 columns: gate | up parted, else in order
       const int block = parted ? q & 1 : q >> 3, at = parted ? q >> 1 : q & 7;
       const uint32_t to = dst + block * (rank_p * 128);
       const bool in = c < p.N;
-      const bool split = passes(c0) > 1;
-      const int j = first_slice(c0) + pass;
-      const bool mine = in && (!split || (slice_of(p, c) == j && slice_of(p, c + 7) == j));
-      const bool some = in && split && !mine && (slice_of(p, c) <= j && slice_of(p, c + 7) >= j);
       const __nv_bfloat16* src = p.b + ((int64_t)tile.offset + r0) * p.N + (in ? c : 0);
       constexpr int kStep = 2;
-      if (!some) {
-        const int64_t jump = (int64_t)kStep * p.N;
-        const int last = mine ? tile.rank : 0;  // rows past it: zeros
+      const int64_t jump = (int64_t)kStep * p.N;
+      const int last = in ? tile.rank : 0;  // rows past it: zeros
 #pragma unroll 8
-        for (int r = r0; r < rank_p; r += kStep, src += jump)
-          cp_async16(to + r * 128 + ((at ^ (r & 7)) << 4), r < last ? src : p.b, r < last);
-      } else {  // the slice ends within the 8 columns
-        for (int r = r0; r < rank_p; r += kStep, src += (int64_t)kStep * p.N) {
-          uint32_t w[4] = {0u, 0u, 0u, 0u};
-          if (r < tile.rank) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-            for (int e = 0; e < 8; ++e)
-              if (slice_of(p, c + e) != j) w[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
-          }
-          st4(to + r * 128 + ((at ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
-        }
-      }
+      for (int r = r0; r < rank_p; r += kStep, src += jump)
+        cp_async16(to + r * 128 + ((at ^ (r & 7)) << 4), r < last ? src : p.b, r < last);
     };
     int step = 0;
-    bool alive = warp < kStages;
-    for (int chunk = 0; chunk < chunks && alive; ++chunk) {
-      const int c = column(chunk), n = passes(c);
-      for (int pass = 0; pass < n; ++pass, ++step) {
-        if (step % kStages != warp) continue;
-        if (step >= kStages) {
-          alive = warp_wait(empty + 8 * warp, (step / kStages - 1) & 1, stop, p.err);
-          if (!alive) break;
-        }
-        load_b(ring + warp * stage_bytes, c, pass);
-        cp_commit();
-        cp_wait<0>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        bar_arrive(full + 8 * warp);
-      }
+    for (Walk w = enter(0); warp < kStages && w.chunk < chunks; w = next(w), ++step) {
+      if (step % kStages != warp) continue;
+      if (step >= kStages && !warp_wait(empty + 8 * warp, (step / kStages - 1) & 1, stop, p.err)) break;
+      load_b(ring + warp * stage_bytes, w.c);
+      cp_commit();
+      cp_wait<0>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(full + 8 * warp);
     }
     if (p.after_shrink) pdl_enter();  // lora_shrink does not write the adapter rows
   } else if (warp == 3) {
@@ -511,43 +495,30 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       int step = 0;
       bool fine = true;
-      for (int ch = 0; ch < chunks && fine; ++ch) {
-        const int buf = ch & 1, use = ch >> 1;
+      for (Walk w = enter(0); w.chunk < chunks; w = next(w), ++step) {
+        const int buf = step & 1, use = step >> 1, slot = step % kStages;
         if (use >= 1 && !(fine = bar_wait(tempty + 8 * buf, (use - 1) & 1, stop, p.err))) break;
-        const int c = column(ch), n = passes(c);
-        const uint32_t d = tmem + buf * kChunk;
-        uint32_t acc = 0;
-        for (int pass = 0; pass < n; ++pass, ++step) {
-          const int slot = step % kStages;
-          if (!(fine = bar_wait(full + 8 * slot, (step / kStages) & 1, stop, p.err))) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t lead = rank_p * 128;
-          const uint64_t b0 = desc(ring + slot * stage_bytes, lead);
-          const uint32_t term = rank_p / 2, slice = TERMS * term;  // TMEM columns
-          // all terms and rank steps of one slice into d
-          auto products = [&](uint32_t to, uint32_t a, uint64_t bj, uint32_t id) {
-            for (int e = TERMS - 1; e >= 0; --e) {  // the small terms first
-              const uint32_t ae = a + e * term;
-              if (acc)
-                umma(to, ae, bj, id, 1u);
-              else
-                umma(to, ae, bj, id, 0u);
-              acc = 1;
+        if (!(fine = bar_wait(full + 8 * slot, (step / kStages) & 1, stop, p.err))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + buf * kChunk, lead = rank_p * 128;
+        const uint64_t b0 = desc(ring + slot * stage_bytes, lead);
+        const uint32_t term = rank_p / 2, slice = TERMS * term;  // TMEM columns
+        // all terms and rank steps of one slice into `to`
+        auto products = [&](uint32_t to, uint32_t a, uint64_t bj, uint32_t id) {
+          for (int e = TERMS - 1; e >= 0; --e) {  // the small terms first
+            const uint32_t ae = a + e * term;
+            umma(to, ae, bj, id, e < TERMS - 1);
 #pragma unroll 4
-              for (int k = 16; k < rank_p; k += 16) umma(to, ae + k / 2, bj + k * 8, id, 1u);
-            }
-          };
-          if (rank_p > 0 && parted) {
-            for (int j = 0; j < 2; ++j) {
-              acc = 0;
-              products(d + 64 * j, tmem + kSAt + j * slice, b0 + j * (lead >> 4), instr(64));
-            }
-          } else if (rank_p > 0) {
-            products(d, tmem + kSAt + (first_slice(c) + pass) * slice, b0, instr(kChunk));
+            for (int k = 16; k < rank_p; k += 16) umma(to, ae + k / 2, bj + k * 8, id, 1u);
           }
-          umma_commit(empty + 8 * slot);
+        };
+        if (rank_p > 0 && parted) {
+          for (int j = 0; j < 2; ++j)
+            products(d + 64 * j, tmem + kSAt + j * slice, b0 + j * (lead >> 4), instr(64));
+        } else if (rank_p > 0) {
+          products(d, tmem + kSAt + slice_at(w) * slice, b0, instr(kChunk));
         }
-        if (!fine) break;
+        umma_commit(empty + 8 * slot);
         umma_commit(tfull + 8 * buf);
       }
       if (!fine) {
@@ -595,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
       has |= (uint32_t)(tok >= 0) << i;
       out_at[i] = (uint32_t)(max(tok, 0) * p.out_stride + at % kChunks * kPer);
     }
-    // The base comes by cp.async, two chunks ahead, into this warp's own rows
+    // The base comes by cp.async, two steps ahead, into this warp's own rows
     // (16-byte chunk k of row r at k ^ (r & 7)); lane l loads chunk l & 7 of rows
     // (l >> 3) + 4 i.
     uint32_t base_at[8];
@@ -604,11 +575,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
       const int r = 4 * i + (lane >> 3);
       base_at[i] = (uint32_t)(max(r < rows ? s_tok[row0 + r] : 0, 0) * p.base_stride + 4 * (lane & 7));
     }
-    auto load_base = [&](int ch) {
-      if (ch < chunks && rows > 0) {
-        const int c = column(ch) + 32 * part;
+    auto load_base = [&](const Walk& w, int buf) {
+      if (w.chunk < chunks && rows > 0) {
+        const int c = w.c + 32 * part;
         const bool in = c + 4 * (lane & 7) < p.N;
-        const uint32_t to = base_buf + (ch & 1) * kSegment + (lane >> 3) * 128;
+        const uint32_t to = base_buf + buf * kSegment + (lane >> 3) * 128;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           cp_async16(to + 512 * i + (((lane & 7) ^ ((4 * i + (lane >> 3)) & 7)) << 4),
@@ -616,10 +587,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
       }
       cp_commit();
     };
-    load_base(0);
-    load_base(1);
-    for (int ch = 0; ch < chunks; ++ch) {
-      const int buf = ch & 1, c = column(ch) + 32 * part;
+    Walk w = enter(0), ahead = next(w);
+    load_base(w, 0);
+    load_base(ahead, 1);
+    for (int step = 0; w.chunk < chunks; w = next(w), ++step) {
+      const int buf = step & 1, c = w.c + 32 * part;
       float y[32];
       // the base of this thread's row
       cp_wait<1>();
@@ -636,8 +608,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
         }
       }
       __syncwarp();
-      load_base(ch + 2);
-      if (!warp_wait(tfull + 8 * buf, (ch >> 1) & 1, stop, p.err)) break;
+      ahead = next(ahead);
+      load_base(ahead, buf);
+      if (!warp_wait(tfull + 8 * buf, (step >> 1) & 1, stop, p.err)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (rows > 0 && rank_p > 0) {
         uint32_t acc[32];
@@ -680,13 +653,27 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_tc_kernel(ExpandArgs 
           for (int i = 0; i < kChunks; ++i) {
             const int at = 32 * i + lane, r = at / kChunks, k = at % kChunks;
             const int col = c_out + 16 * h;
-            if ((has >> i & 1u) && col + k * kPer < n_out) {
-              const uint4 q = ld4(place(r, k));
-              if constexpr (EPI == kLoraF32)
-                *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + (out_at[i] + col)) = q;
-              else
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + (out_at[i] + col)) = q;
+            if (!(has >> i & 1u) || col + k * kPer >= n_out) continue;
+            const uint4 q = ld4(place(r, k));
+            if (EPI != kLoraSwiGLU && w.passes > 1) {  // this slice's columns alone
+              const int n = col + k * kPer, j = slice_at(w);
+              if (slice_of(p, n) != j || slice_of(p, n + kPer - 1) != j) {
+                const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                  if (slice_of(p, n + e) != j) continue;
+                  if constexpr (EPI == kLoraF32)
+                    static_cast<uint32_t*>(p.out)[out_at[i] + col + e] = word[e];
+                  else
+                    static_cast<uint16_t*>(p.out)[out_at[i] + col + e] = (uint16_t)(word[e >> 1] >> 16 * (e & 1));
+                }
+                continue;
+              }
             }
+            if constexpr (EPI == kLoraF32)
+              *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + (out_at[i] + col)) = q;
+            else
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + (out_at[i] + col)) = q;
           }
           __syncwarp();
         }

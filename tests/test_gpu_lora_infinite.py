@@ -17,6 +17,10 @@ CASES = {
     "tiles": dict(of=np.arange(200) % 6, ranks=[40, 5, 24, 16, 1, 72], K=264, slices=[128, 32, 32]),
     "prompt": dict(of=np.arange(200) // 100, ranks=[24, 5], K=256, slices=[256, 128]),
     "long_prompt": dict(of=np.arange(4300) // 4000, ranks=[24, 5], K=256, slices=[256, 128]),
+    # slices that end inside the columns of one step
+    "some_slice_edges": dict(of=np.arange(60) % 5, ranks=[40, 5, 24, 16, 1], K=264, slices=[72, 8, 27, 21]),
+    "prompt_slice_edges": dict(of=np.arange(200) // 100, ranks=[24, 5], K=256, slices=[203, 150, 47]),
+    "prompt_narrow_slices": dict(of=np.arange(200) // 100, ranks=[24, 5], K=256, slices=[30, 40, 58]),
     "rows_off_16_bytes": dict(of=np.arange(60) % 3, ranks=[40, 5, 24], K=67, slices=[50]),
     "f32": dict(of=np.arange(60) % 3, ranks=[40, 5, 24], K=67, slices=[50], dtype="float32"),
     "f32_long_k": dict(of=np.arange(60) % 3, ranks=[40, 5, 24], K=300, slices=[50], dtype="float32"),
