@@ -162,8 +162,9 @@ __global__ void __launch_bounds__(kShrinkWarps * 32, 2) lora_shrink_kernel(Shrin
 // The same for larger tiles: 64 tokens x RB rank rows per CTA, both operands
 // through shared memory (each is read RB / 16 and 4 times), k in steps of 64
 // behind a ring of cp.async.  Warp (m, n) of the 4 x 2 has 16 tokens and RB / 2
-// rank rows; each step's four MMAs make a partial sum, added with rounding.  1280 tokens of 32 adapters, K = 2048, two slices, rank 16-32 (11 MB):
-// 9.7 us, the latency of the ring's first steps and of the cluster's sum.
+// rank rows; each step's four MMAs make a partial sum, added with rounding.  1280
+// tokens of 32 adapters, K = 2048, two slices, rank 16-32 (11 MB): 9.7 us, the
+// latency of the ring's first steps and of the cluster's sum.
 constexpr int kBigK = 64;
 constexpr int kBigLd = kBigK + 8;  // padded row (elements): conflict-free ldmatrix
 constexpr int kBigStages = 4;
