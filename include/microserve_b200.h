@@ -287,6 +287,24 @@ MS_API int ms_kv_gather(const ms_kv_cache* cache, int layer,
                  const int32_t* block_tables, int n_seqs, int max_blocks,
                  int max_context, float* keys, float* values, void* stream);
 
+/* Copy pages: block dst_blocks[i] of every layer's K and V pools gets the content of
+ * src_blocks[i] (device arrays, n_blocks entries).  A source may repeat (a
+ * fork's own pages, PagedKVCache.unshare_last_block over a batch, reference
+ * cache.py:189-204; a pool made compact); a destination must not, nor be a
+ * source.  A block outside the pool sets the device error word and its pair is skipped. */
+MS_API int ms_kv_copy_blocks(const ms_kv_cache* cache, const int32_t* src_blocks,
+                             const int32_t* dst_blocks, int n_blocks, void* stream);
+
+/* Move tokens: slot dst_slots[i] of every layer's pools gets the content of src_slots[i].  The arrays
+ * are (n_groups, per_group); within a group every source is read before any
+ * destination is written, so the two may overlap (the accepted path of a tree
+ * made contiguous); groups must not touch one another's slots, nor a group one
+ * destination twice.  A pair with a negative slot is skipped; one outside the
+ * pool too, and sets the device error word.  At most MS_KV_MOVE_MAX a group. */
+#define MS_KV_MOVE_MAX 256
+MS_API int ms_kv_move_tokens(const ms_kv_cache* cache, const int32_t* src_slots,
+                             const int32_t* dst_slots, int n_groups, int per_group, void* stream);
+
 /* ---- model forward ------------------------------------------------------- */
 /* Pre-norm RMSNorm / RoPE / SwiGLU decoder with tied embeddings (reference
  * model.py:265-354) and grouped-query attention (n_kv_heads <= n_heads).
@@ -450,6 +468,85 @@ MS_API int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache, cons
                            const int32_t* logit_rows, int n_logit_rows, float* logits,
                            int64_t logits_row_stride, void* workspace, size_t workspace_bytes,
                            void* stream);
+
+/* ---- score forms and trees ---------------------------------------------------- */
+/* What a query's scores are and which keys it sees, instead of plain causal
+ * attention.  No reference counterpart, like everything in this section.
+ *   x = c - slopes[h] * |p_q - p_k|,  c = softcap * tanh(s / softcap) (softcap
+ *   0: c = s),  s = scale * q . k (scale 0: 1 / sqrt(d_head));
+ * the query at position p_q sees key j when j < prefix_lens[b], or when it is seen and
+ * p_q - p_k < window (window 0: any): without a tree mask p_k = j <= p_q; with one
+ * every key before the pass's own tokens is seen, and of those, which stand at
+ * context_lens[b] - q_len onwards, token i if bit i % 32 of word i / 32 of the query's mask
+ * row is set (p_k is then that token's position).  A query that sees nothing gives 0; what
+ * stands in keys and values that a query does not see never reaches its result.
+ * Device arrays, each nullable. */
+typedef struct {
+  float scale;
+  float softcap;
+  int32_t window;
+  int32_t mask_words;          /* words of a mask row, >= ceil(q_len / 32) */
+  const float* slopes;         /* (n_heads) */
+  const int32_t* prefix_lens;  /* (n_seqs) */
+  const uint32_t* tree_mask;   /* (n_tokens, mask_words) */
+} ms_attention_form;
+
+/* ms_paged_attention with a form (NULL: plain causal).  Token t's head h is at
+ * q + t * q_stride + h * d_head, its result at out + t * out_stride + h * d_head.  out
+ * must not overlap q or the pools.  The workspace is 16-byte aligned scratch of this call
+ * alone; fewer bytes than the size call says (NULL, 0 too) cost parallelism over long
+ * contexts, not results.  Lengths that do not fit the batch's arrays, max_q_len or the block
+ * tables set the device error word and are cut. */
+MS_API size_t ms_attention_form_workspace_size(const ms_kv_cache* cache, int n_heads,
+                                               const ms_batch* batch,
+                                               const ms_attention_form* form);
+MS_API int ms_paged_attention_form(const void* q, int64_t q_stride, const ms_kv_cache* cache,
+                                   int layer, const ms_batch* batch, int n_heads,
+                                   const ms_attention_form* form, void* out, int64_t out_stride,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* ms_forward_lora with a form for every layer's attention (NULL: plain causal;
+ * lora NULL: the shared weights alone).  The batch's positions are the tokens' own (a
+ * tree's siblings share one); its slots say where their K/V go. */
+MS_API size_t ms_forward_form_workspace_size(const ms_model* model, const ms_kv_cache* cache,
+                                             const ms_batch* batch, const ms_attention_form* form,
+                                             const ms_lora_model* lora, int max_logit_rows);
+MS_API int ms_forward_form(const ms_model* model, const ms_kv_cache* cache, const ms_batch* batch,
+                           const ms_attention_form* form, const ms_lora_model* lora,
+                           const ms_lora_plan* plan, const int32_t* logit_rows, int n_logit_rows,
+                           float* logits, int64_t logits_row_stride, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Trees of tokens, one per sequence: sequence b's nodes are tokens [q_start[b],
+ * q_start[b+1]), and parents[] gives each node's parent by its number in its tree, an earlier node
+ * (-1: none, a root).  Sizes up to max_nodes, at most MS_TREE_MAX.
+ *
+ * masks: (n_tokens, mask_words) rows for ms_attention_form (a node sees its ancestors and
+ * itself), depths (n_tokens; nullable): ancestors of each node.  A parent that is no earlier node
+ * sets the device error word and counts as none. */
+#define MS_TREE_MAX 1024
+MS_API int ms_tree_masks(const int32_t* parents, const int32_t* q_start, int n_seqs, int n_tokens,
+                         int max_nodes, uint32_t* masks, int mask_words, int32_t* depths,
+                         void* stream);
+
+/* Walk down each tree along the target's tokens: from node 0, the token that the target gives after
+ * a node is emitted, and the lowest child with that token is the next node, up to max_accept of
+ * them.  With target tokens drawn from the target's distribution this leaves the emitted
+ * tokens distributed as the target alone would, whatever the tree.  Exactly one of
+ *   logits: float32 rows of the nodes, logits_stride apart; the token is the largest
+ *     logit's (lowest index of equals; NaN is never the largest).  Only rows on the path are read;
+ *   target_tokens: (n_tokens), the tokens themselves.
+ * batch: input_ids (the nodes' tokens), q_start, context_lens, block_tables, sizes; a sequence's
+ * nodes stand at the last places of its context.
+ * Outputs, -1 past the accepted ones: out_tokens (n_seqs, max_accept + 1), out_num_accepted (n_seqs),
+ * out_nodes (n_seqs, max_accept) the accepted nodes after node 0, and src_slots and
+ * dst_slots (n_seqs, max_accept), both or neither: the moves for ms_kv_move_tokens that put them behind
+ * node 0.  A sequence without nodes accepts and emits nothing (all -1, 0 accepted). */
+MS_API int ms_tree_accept(const float* logits, int64_t logits_stride, int vocab,
+                          const int32_t* target_tokens, const ms_batch* batch,
+                          const int32_t* parents, int max_accept, int block_size, int num_blocks,
+                          int32_t* out_tokens, int32_t* out_num_accepted, int32_t* out_nodes,
+                          int32_t* src_slots, int32_t* dst_slots, void* stream);
 
 /* ---- building blocks, exported for tests and for callers that compose
  *      their own forward ---------------------------------------------- */

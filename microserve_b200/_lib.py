@@ -166,6 +166,18 @@ class MsLoraModel(ctypes.Structure):
     ]
 
 
+class MsAttentionForm(ctypes.Structure):
+    _fields_ = [
+        ("scale", c_float),
+        ("softcap", c_float),
+        ("window", c_int32),
+        ("mask_words", c_int32),
+        ("slopes", c_void_p),
+        ("prefix_lens", c_void_p),
+        ("tree_mask", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ms_version": (c_int, []),
@@ -249,6 +261,33 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_void_p],
     ),
     "ms_attention_scratch_size": (c_size_t, [POINTER(MsKVCache), c_int, POINTER(MsBatch)]),
+    # (the structures of these may also come as packed bytes)
+    "ms_attention_form_workspace_size": (c_size_t, [c_void_p, c_int, c_void_p, c_void_p]),
+    "ms_paged_attention_form": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "ms_kv_copy_blocks": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "ms_kv_move_tokens": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "ms_tree_masks": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                              c_void_p]),
+    "ms_tree_accept": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "ms_forward_form_workspace_size": (
+        c_size_t,
+        [POINTER(MsModel), POINTER(MsKVCache), POINTER(MsBatch), POINTER(MsAttentionForm),
+         POINTER(MsLoraModel), c_int],
+    ),
+    "ms_forward_form": (
+        c_int,
+        [POINTER(MsModel), POINTER(MsKVCache), POINTER(MsBatch), POINTER(MsAttentionForm),
+         POINTER(MsLoraModel), POINTER(MsLoraPlan), c_void_p, c_int, c_void_p, c_int64, c_void_p,
+         c_size_t, c_void_p],
+    ),
     "ms_paged_attention": (c_int, [c_void_p, POINTER(MsKVCache), c_int, POINTER(MsBatch), c_int,
                                    c_void_p, c_void_p]),
 }

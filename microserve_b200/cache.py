@@ -21,6 +21,7 @@ tensor methods raise (there is no CPU compute path).
 from __future__ import annotations
 
 import ctypes
+import struct
 from collections.abc import Iterator, Sequence
 
 import numpy as np
@@ -28,6 +29,62 @@ import torch
 
 from . import _lib
 from .config import CacheConfig, ModelConfig
+
+
+# ms_kv_cache as bytes (a third of the time a ctypes structure takes to fill)
+_PACK_CACHE = struct.Struct("=iiiiiiQQ").pack
+_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+MAX_MOVES = 256  # MS_KV_MOVE_MAX
+
+
+def _pack_pool(pool: torch.Tensor, index: int) -> tuple[bytes, np.ndarray]:
+    """``ms_kv_cache`` of a pool tensor, and the array of its layers' addresses (to be kept until
+    the call)."""
+    if pool.dim() != 6 or pool.shape[0] != 2 or pool.dtype not in _CODES:
+        raise ValueError("a pool is a float32 or bfloat16 tensor (2, layers, blocks, n_kv_heads, "
+                         "block_size, d_head)")
+    shape = pool.shape
+    base = _lib.check_tensor(pool, "pool", pool.dtype, index, shape)
+    layers = shape[1]
+    at = np.arange(base, base + 2 * layers * pool.stride(1) * pool.element_size(),
+                   pool.stride(1) * pool.element_size(), dtype=np.uint64) if pool.numel() else \
+        np.zeros(2 * layers, np.uint64)
+    where = _addr(at)
+    return _PACK_CACHE(layers, shape[2], shape[4], shape[3], shape[5], _CODES[pool.dtype], where,
+                       where + 8 * layers), at
+
+
+def copy_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Block ``dst[i]`` of every layer of ``pool`` (:attr:`PagedKVCache.pool`) becomes a copy of block
+    ``src[i]``, in one launch.  ``src`` and ``dst`` (n,) int32 on the pool's device; a source
+    may repeat, a destination must not, nor be a source."""
+    index = _lib.cuda_index(pool)
+    n = src.numel()
+    s = _lib.check_tensor(src, "src", torch.int32, index, (n,))
+    d = _lib.check_tensor(dst, "dst", torch.int32, index, (n,))
+    cache, _keep = _pack_pool(pool, index)
+    if n and pool.numel():
+        _lib.launch_on(index, "ms_kv_copy_blocks", cache, s, d, n)
+
+
+def move_tokens(pool: torch.Tensor, src_slots: torch.Tensor, dst_slots: torch.Tensor) -> None:
+    """Slot ``dst_slots[b, i]`` of every layer of ``pool`` gets the keys and values of ``src_slots[b,
+    i]``, as if a row's sources were all read before any of its destinations is written.
+
+    ``src_slots`` and ``dst_slots`` (B, n) int32 on the pool's device, n at most 256; a pair
+    with a negative slot is skipped.  Rows must not touch one another's slots, nor a row one
+    destination twice."""
+    index = _lib.cuda_index(pool)
+    if src_slots.dim() != 2:
+        raise ValueError("src_slots and dst_slots must be (B, n)")
+    B, n = src_slots.shape
+    s = _lib.check_tensor(src_slots, "src_slots", torch.int32, index, (B, n))
+    d = _lib.check_tensor(dst_slots, "dst_slots", torch.int32, index, (B, n))
+    if n > MAX_MOVES:  # (each row would be staged as a whole)
+        raise ValueError(f"{n} moves in a row (at most {MAX_MOVES})")
+    cache, _keep = _pack_pool(pool, index)
+    if B and n and pool.numel():
+        _lib.launch_on(index, "ms_kv_move_tokens", cache, s, d, B, n)
 
 
 def _addr(a: np.ndarray) -> int:
@@ -113,6 +170,18 @@ class BlockAllocator:
             raise ValueError(f"double free of block {bad}")
         self._refcount[arr] -= 1
         self._free.extend(arr[self._refcount[arr] == 0].tolist())
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Rename the used blocks from the upper end to the free ids below them: the old and the
+        new ids.  The lowest free id is handed out first from then on."""
+        used = self.num_used
+        held = np.flatnonzero(self._refcount > 0)
+        src = held[held >= used]
+        below = np.flatnonzero(self._refcount[:used] == 0)
+        self._refcount[below] = self._refcount[src]
+        self._refcount[src] = 0
+        self._free = list(range(self.num_blocks - 1, used - 1, -1))
+        return src.tolist(), below.tolist()
 
     def check_invariants(self) -> None:
         """Assert internal consistency; used by tests."""
@@ -218,6 +287,8 @@ class PagedKVCache:
         # Bumped whenever a sequence gains or loses its table row, so callers
         # may keep ``rows_of`` results while it is unchanged.
         self.generation = 0
+        # Bumped whenever blocks change places (:meth:`compact`).
+        self.moves = 0
         self._table = np.zeros((8, self._max_blocks), dtype=np.int32)
         self._freed = np.empty(cache.num_blocks, dtype=np.int32)  # truncate_many's output
         self._nblk = np.zeros(8, dtype=np.int32)
@@ -465,6 +536,82 @@ class PagedKVCache:
             self.pool[:, :, new].copy_(self.pool[:, :, old])
         self._table[row, n - 1] = new
         self.allocator.free(old)
+
+    def fork_many(self, parent_id: int, child_ids: Sequence[int]) -> None:
+        """:meth:`fork` for several children, each with its own copy of a last block that is not
+        full: all of them may append at once.  All-or-nothing."""
+        if len(set(child_ids)) != len(child_ids):
+            raise ValueError("fork_many: a child appears twice")
+        for c in child_ids:
+            if c in self._rows:
+                raise ValueError(f"sequence {c} already exists")
+        parent = self._rows[parent_id]
+        n = int(self._nblk[parent])
+        held = int(self._ntok[parent])
+        # blocks behind the tokens (reserved capacity) are not shared, nor a last one in part
+        full = held // self.block_size
+        part = held % self.block_size != 0
+        if part * len(child_ids) > self.allocator.num_free:
+            raise OutOfCacheMemory(f"need {len(child_ids)} blocks, {self.allocator.num_free} free")
+        assert full + part <= n
+        shared = self._table[parent, :full].copy()
+        last = int(self._table[parent, full]) if part else -1
+        new = self.allocator.allocate_many(len(child_ids)) if part else []
+        for i, c in enumerate(child_ids):
+            for block in shared.tolist():
+                self.allocator.incref(block)
+            row = self._row_of(c)
+            self._table[row, :full] = shared
+            if part:
+                self._table[row, full] = new[i]
+            self._nblk[row] = full + part
+            self._ntok[row] = held
+        self._copy([last] * len(new), new)
+
+    def unshare_many(self, seq_ids: Sequence[int]) -> None:
+        """:meth:`unshare_last_block` for several sequences, in one copy.  All-or-nothing."""
+        rows = [self._rows[s] for s in dict.fromkeys(seq_ids)]
+        refs: dict[int, int] = {}
+        todo = []
+        for row in rows:
+            n = int(self._nblk[row])
+            if n == 0:
+                continue
+            old = int(self._table[row, n - 1])
+            left = refs.setdefault(old, self.allocator.refcount(old))
+            if left > 1:  # the last holder keeps it
+                refs[old] = left - 1
+                todo.append((row, n - 1, old))
+        new = self.allocator.allocate_many(len(todo))
+        for (row, col, old), block in zip(todo, new, strict=True):
+            self._table[row, col] = block
+            self.allocator.free(old)
+        self._copy([old for _, _, old in todo], new)
+
+    def compact(self) -> int:
+        """Move blocks from the upper end of the pool to free places below, so that the blocks in use are
+        the first :attr:`BlockAllocator.num_used`; returns how many moved.  Block ids handed
+        out before (tables on the device, slots of a batch not run yet) are stale afterwards."""
+        used = self.allocator.num_used
+        src, dst = self.allocator.compact()
+        if not src:
+            return 0
+        new = np.arange(self.allocator.num_blocks, dtype=np.int32)
+        new[src] = dst
+        for row in self._rows.values():
+            n = int(self._nblk[row])
+            self._table[row, :n] = new[self._table[row, :n]]
+        assert max(dst) < used
+        self.moves += 1
+        self._copy(src, dst)
+        return len(src)
+
+    def _copy(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Copy blocks of every layer (a cache without a device has nothing to copy)."""
+        if self.pool is None or not len(src):
+            return
+        both = torch.from_numpy(np.array([src, dst], np.int32)).to(self.device)
+        copy_blocks(self.pool, both[0], both[1])
 
     def truncate(self, seq_id: int, num_tokens: int) -> None:
         """Shrink a sequence to ``num_tokens``, releasing blocks past the end."""

@@ -1,0 +1,359 @@
+// Paged attention with score forms: entry points, the plan, the kernel on the
+// CUDA cores (float32 caches, and bf16 ones whose head or block size the
+// matrix kernels do not take) and the joining of KV ranges.
+#include <cfloat>
+
+#include "attention_form.cuh"
+#include "model_kernels.cuh"
+
+namespace ms {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kChunk = 32;
+template <int DH> constexpr int rows_per_warp() { return DH <= 64 ? 4 : 2; }
+
+// One CTA per (row tile, KV range, kv head, sequence); row r of a tile is
+// (token r / group, head-in-group r % group).  32 keys at a time in shared
+// memory, a lane a key for the scores and a dimension for the sums; online
+// softmax in base e, everything in float32.
+template <typename T, int DH>
+__global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
+  pdl_enter();
+  constexpr int PER_LANE = DH >= 32 ? DH / 32 : 1;
+  constexpr int RPW = rows_per_warp<DH>();
+  constexpr int ROWS = kWarps * RPW;
+  __shared__ float Qs[ROWS][DH];
+  __shared__ float Ks[kChunk][DH + 1];
+  __shared__ float Vs[kChunk][DH];
+  __shared__ int s_min, s_max;
+
+  const int b = blockIdx.z, g = blockIdx.y;
+  const int split = blockIdx.x % a.n_splits, tile = blockIdx.x / a.n_splits;
+  const FormSeq s = form_seq(a, b);
+  const int nrows = s.qlen * a.group, r0 = tile * ROWS;
+  if (r0 >= nrows) return;
+  const int nr = min(ROWS, nrows - r0);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    s_min = INT_MAX;
+    s_max = INT_MIN;
+  }
+  __syncthreads();
+  const T* q = static_cast<const T*>(a.q);
+  for (int idx = threadIdx.x; idx < ROWS * DH; idx += blockDim.x) {
+    const int r = idx / DH, d = idx - r * DH, rr = r0 + r;
+    Qs[r][d] = r < nr ? to_f(q[(int64_t)(s.t0 + rr / a.group) * a.q_stride +
+                               (int64_t)(g * a.group + rr % a.group) * DH + d])
+                      : 0.f;
+  }
+  for (int r = threadIdx.x; r < nr; r += blockDim.x) {
+    const int p = a.positions[s.t0 + (r0 + r) / a.group];
+    atomicMin(&s_min, p);
+    atomicMax(&s_max, p);
+  }
+  __syncthreads();
+  const FormKeys keys = form_keys(a, s, s_min, s_max);
+  const int xbeg = min(split * a.split_len, keys.total);
+  const int xend = split == a.n_splits - 1 ? keys.total : min(keys.total, xbeg + a.split_len);
+
+  float m[RPW], l[RPW], acc[RPW][PER_LANE];
+  int tok[RPW], pos[RPW];
+  float slope[RPW];
+#pragma unroll
+  for (int i = 0; i < RPW; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER_LANE; ++e) acc[i][e] = 0.f;
+    const int r = warp + i * kWarps, rr = r0 + r;
+    tok[i] = s.t0 + (r < nr ? rr / a.group : 0);
+    pos[i] = a.positions[tok[i]];
+    slope[i] = a.slopes && r < nr ? a.slopes[g * a.group + rr % a.group] : 0.f;
+  }
+  const T *kp = static_cast<const T*>(a.k), *vp = static_cast<const T*>(a.v);
+  const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
+  const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  for (int x0 = xbeg; x0 < xend; x0 += kChunk) {
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < kChunk * DH; idx += blockDim.x) {
+      const int kk = idx / DH, d = idx - kk * DH;
+      float kv = 0.f, vv = 0.f;
+      if (x0 + kk < xend) {
+        const int j = keys.key(x0 + kk);
+        const int64_t o =
+            (((int64_t)form_block(a, table, j / a.bs) * a.hkv + g) * a.bs + (j % a.bs)) * DH + d;
+        kv = to_f(kp[o]);
+        vv = to_f(vp[o]);
+      }
+      Ks[kk][d] = kv;
+      Vs[kk][d] = vv;
+    }
+    __syncthreads();
+    const int j = keys.key(x0 + lane);
+    const bool in = x0 + lane < xend;
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+      const int r = warp + i * kWarps;
+      if (r >= nr) continue;
+      float x = 0.f;
+#pragma unroll 8
+      for (int d = 0; d < DH; ++d) x = fmaf(Qs[r][d], Ks[lane][d], x);
+      int distance = 0;
+      const bool seen = in && form_sees(a, s, tok[i], pos[i], j, distance);
+      x = a.softcap > 0.f ? a.softcap * tanhf(x * inv_cap) : x * a.scale;
+      if (a.slopes) x -= slope[i] * fabsf((float)distance);
+      x = seen ? x : -INFINITY;
+      const uint32_t seen_mask = __ballot_sync(0xffffffffu, seen);
+      if (seen_mask == 0) continue;
+      const float mn = fmaxf(m[i], warp_max(x));
+      const float sub = mn == -INFINITY ? 0.f : mn;
+      const float alpha = m[i] == -INFINITY ? 0.f : expf(m[i] - sub);
+      const float p = seen ? expf(x - sub) : 0.f;
+      l[i] = l[i] * alpha + warp_sum(p);
+#pragma unroll
+      for (int e = 0; e < PER_LANE; ++e) acc[i][e] *= alpha;
+#pragma unroll 4
+      for (int kk = 0; kk < kChunk; ++kk) {
+        const float pk = __shfl_sync(0xffffffffu, p, kk);
+        if (!((seen_mask >> kk) & 1)) continue;  // an unseen value may be anything
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e)
+          if (DH >= 32 || lane < DH) acc[i][e] = fmaf(pk, Vs[kk][lane + 32 * e], acc[i][e]);
+      }
+      m[i] = mn;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RPW; ++i) {
+    const int r = warp + i * kWarps;
+    if (r >= nr) continue;
+    const int rr = r0 + r;
+    if (a.n_splits == 1) {
+      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+      T* o = static_cast<T*>(a.out) + (int64_t)(s.t0 + rr / a.group) * a.out_stride +
+             (int64_t)(g * a.group + rr % a.group) * DH;
+#pragma unroll
+      for (int e = 0; e < PER_LANE; ++e)
+        if (DH >= 32 || lane < DH) o[lane + 32 * e] = from_f<T>(acc[i][e] * inv);
+    } else {
+      const int64_t unit = (((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split;
+#pragma unroll
+      for (int e = 0; e < PER_LANE; ++e)
+        if (DH >= 32 || lane < DH) a.part_o[(unit * ROWS + r) * DH + lane + 32 * e] = acc[i][e];
+      if (lane == 0) {
+        a.part_ml[(unit * ROWS + r) * 2] = m[i];
+        a.part_ml[(unit * ROWS + r) * 2 + 1] = l[i];
+      }
+    }
+  }
+}
+
+// A warp a row: the ranges' maxima first, then their sums with the weights
+// exp(m - max).  Ranges in order, so that the result does not depend on timing.
+template <typename T, bool kBase2>
+__global__ void __launch_bounds__(128) form_combine_kernel(FormArgs a, int rows, int dh) {
+  pdl_enter();
+  const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 31;
+  const FormSeq s = form_seq(a, b);
+  const int rr = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (rr >= s.qlen * a.group) return;
+  const int tile = rr / rows, r = rr - tile * rows;
+  const int64_t unit0 = (((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + unit0 * rows + r;
+  float mx = -INFINITY;
+  for (int i = lane; i < a.n_splits; i += 32) mx = fmaxf(mx, ml[(int64_t)i * rows].x);
+  mx = warp_max(mx);
+  const float sub = mx == -INFINITY ? 0.f : mx;
+  float l = 0.f, acc[4] = {};
+  const float* po = a.part_o + (unit0 * rows + r) * dh;
+#pragma unroll 4
+  for (int i = 0; i < a.n_splits; ++i) {
+    const float2 v = ml[(int64_t)i * rows];
+    if (v.y == 0.f) continue;  // a range without a key for this row: its sums may be unset
+    const float w = kBase2 ? exp2f(v.x - sub) : expf(v.x - sub);
+    l = fmaf(w, v.y, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane + 32 * e < dh) acc[e] = fmaf(w, po[(int64_t)i * rows * dh + lane + 32 * e], acc[e]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* o = static_cast<T*>(a.out) + (int64_t)(s.t0 + rr / a.group) * a.out_stride +
+         (int64_t)(g * a.group + rr % a.group) * dh;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (lane + 32 * e < dh) o[lane + 32 * e] = from_f<T>(acc[e] * inv);
+}
+
+// Tiles of `rows` rows; KV ranges where the tiles alone leave SMs without work,
+// of at least `least` keys and in whole chunks of `chunk`, up to `wave` CTAs in all.
+void plan(FormArgs& a, int max_context, int rows, int chunk, int least, int wave) {
+  int64_t span = max_context;
+  if (a.window > 0 && !a.prefix) span = min(span, (int64_t)a.window + a.max_q + 2 * a.bs);
+  a.row_tiles = ceil_div(a.max_q * a.group, rows);
+  const int64_t units = (int64_t)a.n_seqs * a.hkv * a.row_tiles;
+  int64_t splits = units < wave ? wave / units : 1;
+  splits = max((int64_t)1, min(splits, (span + least - 1) / least));
+  int64_t len = (span + splits - 1) / splits;
+  len = max((int64_t)chunk, (len + chunk - 1) / chunk * chunk);
+  a.split_len = (int)len;
+  a.n_splits = (int)max((int64_t)1, (span + len - 1) / len);
+}
+
+size_t part_bytes(const FormArgs& a, int rows, int dh) {
+  if (a.n_splits == 1) return 0;
+  const size_t units = (size_t)a.n_seqs * a.hkv * a.row_tiles * a.n_splits;
+  return units * rows * (dh + 2) * sizeof(float);
+}
+
+int simt_rows(int dh) { return kWarps * (dh <= 64 ? 4 : 2); }
+
+template <typename T, int DH>
+int launch_simt(FormArgs& a, cudaStream_t s) {
+  dim3 grid(a.row_tiles * a.n_splits, a.hkv, a.n_seqs);
+  launch_pdl(form_simt_kernel<T, DH>, grid, kWarps * 32, 0, s, a);
+  MS_TRY(check_launch("form_simt_kernel"));
+  return a.n_splits > 1 ? form_combine<T, false>(a, simt_rows(DH), DH, s) : MS_OK;
+}
+
+template <typename T>
+int simt_by_dh(FormArgs& a, int dh, cudaStream_t s) {
+  switch (dh) {
+    case 8: return launch_simt<T, 8>(a, s);
+    case 16: return launch_simt<T, 16>(a, s);
+    case 32: return launch_simt<T, 32>(a, s);
+    case 64: return launch_simt<T, 64>(a, s);
+    default: return launch_simt<T, 128>(a, s);
+  }
+}
+
+// Everything of a call that does not depend on the device's data, checked.
+int form_args(FormArgs& a, const ms_kv_cache& c, int layer, const ms_batch& bt, int hq,
+              const ms_attention_form* form, int* max_context) {
+  MS_REQUIRE(bt.n_seqs >= 0 && bt.n_tokens >= 0, "ms_paged_attention_form: bad batch sizes");
+  MS_REQUIRE(hq > 0 && hq % c.n_kv_heads == 0,
+             "ms_paged_attention_form: n_heads %d not a multiple of n_kv_heads %d", hq, c.n_kv_heads);
+  if (c.dtype != MS_DTYPE_F32 && c.dtype != MS_DTYPE_BF16)
+    return fail(MS_ERR_UNSUPPORTED, "ms_paged_attention_form: dtype %d", c.dtype);
+  if (c.d_head != 8 && c.d_head != 16 && c.d_head != 32 && c.d_head != 64 && c.d_head != 128)
+    return fail(MS_ERR_UNSUPPORTED, "ms_paged_attention_form: d_head %d (8/16/32/64/128)", c.d_head);
+  const bool empty = bt.n_seqs == 0 || bt.n_tokens == 0;
+  MS_REQUIRE(empty || (bt.max_q_len > 0 && bt.max_blocks > 0),
+             "ms_paged_attention_form: max_q_len and max_blocks must be > 0");
+  MS_REQUIRE((int64_t)bt.max_blocks * c.block_size <= INT_MAX && (int64_t)bt.max_q_len * hq <= INT_MAX / 2,
+             "ms_paged_attention_form: contexts or queries beyond 2^31");
+  if (bt.n_seqs > 65535 || c.n_kv_heads > 65535)
+    return fail(MS_ERR_TOO_LARGE, "ms_paged_attention_form: more than 65535 sequences or kv heads");
+  a.q_start = bt.q_start;
+  a.context_lens = bt.context_lens;
+  a.positions = bt.positions;
+  a.tables = bt.block_tables;
+  a.n_tokens = bt.n_tokens;
+  a.n_seqs = bt.n_seqs;
+  a.max_blocks = bt.max_blocks;
+  a.max_q = bt.max_q_len;
+  a.bs = c.block_size;
+  a.num_blocks = c.num_blocks;
+  a.hq = hq;
+  a.hkv = c.n_kv_heads;
+  a.group = hq / c.n_kv_heads;
+  a.k = c.k_pool[layer];
+  a.v = c.v_pool[layer];
+  a.scale = 1.f / sqrtf((float)c.d_head);
+  if (form) {
+    MS_REQUIRE(form->scale >= 0.f && form->scale <= FLT_MAX && form->softcap >= 0.f &&
+                   form->softcap <= FLT_MAX && form->window >= 0 && form->mask_words >= 0,
+               "ms_paged_attention_form: scale, softcap, window and mask_words must be >= 0 and finite");
+    MS_REQUIRE(!form->tree_mask || form->mask_words > 0, "ms_paged_attention_form: a mask of no words");
+    if (form->scale > 0.f) a.scale = form->scale;
+    a.softcap = form->softcap;
+    a.window = form->window;
+    a.slopes = form->slopes;
+    a.prefix = form->prefix_lens;
+    a.mask = form->tree_mask;
+    a.mask_words = form->mask_words;
+  }
+  const int bound = bt.max_blocks * c.block_size;
+  *max_context = bt.max_context > 0 ? min(bt.max_context, bound) : bound;
+  return MS_OK;
+}
+
+}  // namespace
+
+template <typename T, bool kBase2>
+int form_combine(const FormArgs& a, int rows, int dh, cudaStream_t s) {
+  dim3 grid(ceil_div(a.max_q * a.group, 4), a.hkv, a.n_seqs);
+  launch_pdl(form_combine_kernel<T, kBase2>, grid, 128, 0, s, a, rows, dh);
+  return check_launch("form_combine_kernel");
+}
+
+int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& c, int layer,
+                   const ms_batch& bt, int hq, const ms_attention_form* form, void* out,
+                   int64_t out_stride, void* workspace, size_t workspace_bytes, cudaStream_t s) {
+  FormArgs a{};
+  int max_context = 0;
+  MS_TRY(form_args(a, c, layer, bt, hq, form, &max_context));
+  if (bt.n_seqs == 0 || bt.n_tokens == 0) return MS_OK;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.err = device_error_word();
+  ProfScope prof(kClsAttention, s);
+  const int rows = simt_rows(c.d_head);
+  plan(a, max_context, rows, kChunk, 128, 148 * 4);
+  if (part_bytes(a, rows, c.d_head) > workspace_bytes) {  // one range a tile
+    a.n_splits = 1;
+    a.split_len = INT_MAX;
+  }
+  if (a.n_splits > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)a.n_seqs * a.hkv * a.row_tiles * a.n_splits * rows * c.d_head;
+  }
+  return c.dtype == MS_DTYPE_F32 ? simt_by_dh<float>(a, c.d_head, s)
+                                 : simt_by_dh<__nv_bfloat16>(a, c.d_head, s);
+}
+
+size_t attention_form_workspace(const ms_kv_cache& c, const ms_batch& bt, int hq,
+                                const ms_attention_form* form) {
+  FormArgs a{};
+  int max_context = 0;
+  if (form_args(a, c, 0, bt, hq, form, &max_context) != MS_OK || bt.n_seqs == 0 || bt.n_tokens == 0)
+    return 0;
+  const int rows = simt_rows(c.d_head);
+  plan(a, max_context, rows, kChunk, 128, 148 * 4);
+  return part_bytes(a, rows, c.d_head);
+}
+
+}  // namespace ms
+
+using namespace ms;
+
+extern "C" size_t ms_attention_form_workspace_size(const ms_kv_cache* cache, int n_heads,
+                                                   const ms_batch* batch,
+                                                   const ms_attention_form* form) {
+  if (validate_cache(cache, 0) != MS_OK || batch == nullptr) return 0;
+  return attention_form_workspace(*cache, *batch, n_heads, form);
+}
+
+extern "C" int ms_paged_attention_form(const void* q, int64_t q_stride, const ms_kv_cache* cache,
+                                       int layer, const ms_batch* batch, int n_heads,
+                                       const ms_attention_form* form, void* out, int64_t out_stride,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  MS_TRY(validate_cache(cache, layer));
+  MS_REQUIRE(batch != nullptr, "ms_paged_attention_form: null batch");
+  if (batch->n_seqs > 0 && batch->n_tokens > 0) {
+    MS_REQUIRE(q && out, "ms_paged_attention_form: null pointer");
+    MS_REQUIRE(batch->q_start && batch->context_lens && batch->positions && batch->block_tables,
+               "ms_paged_attention_form: batch has null arrays");
+    const int64_t width = (int64_t)n_heads * cache->d_head;
+    MS_REQUIRE(q_stride >= width && out_stride >= width,
+               "ms_paged_attention_form: strides below n_heads * d_head");
+    MS_REQUIRE(workspace != nullptr || workspace_bytes == 0,
+               "ms_paged_attention_form: workspace missing");
+    MS_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+               "ms_paged_attention_form: workspace must be 16-byte aligned");
+  }
+  return attention_form(q, q_stride, *cache, layer, *batch, n_heads, form, out, out_stride,
+                        workspace, workspace_bytes, as_stream(stream));
+}

@@ -118,6 +118,8 @@ enum DeviceError : int {
   kErrMask = 6,      // mask row outside the masks
   kErrOrder = 7,     // a list that has to be ascending (bias ids, offsets) is not
   kErrAdapter = 8,   // adapter id, rank or segment outside the adapters' arrays
+  kErrLength = 9,    // a sequence's length beyond the call's arrays or its declared maximum
+  kErrTree = 10,     // a node's parent that is not an earlier node of its tree
 };
 __device__ __forceinline__ void raise_device_error(int* err, int code) {
   atomicCAS(err, 0, code);

@@ -99,11 +99,14 @@ extern "C" int ms_forward(const ms_model* model, const ms_kv_cache* cache, const
                          logits_row_stride, workspace, workspace_bytes, stream);
 }
 
-extern "C" int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache,
-                               const ms_batch* batch, const ms_lora_model* lora,
-                               const ms_lora_plan* plan, const int32_t* logit_rows,
-                               int n_logit_rows, float* logits, int64_t logits_row_stride,
-                               void* workspace, size_t workspace_bytes, void* stream) {
+namespace ms {
+namespace {
+
+// `forms`: attention with a score form (which may be null), else plain causal attention.
+int forward(const ms_model* model, const ms_kv_cache* cache, const ms_batch* batch, bool forms,
+            const ms_attention_form* form, const ms_lora_model* lora, const ms_lora_plan* plan,
+            const int32_t* logit_rows, int n_logit_rows, float* logits, int64_t logits_row_stride,
+            void* workspace, size_t workspace_bytes, void* stream) {
   MS_TRY(validate_model(model));
   MS_TRY(validate_cache(cache, 0));
   MS_REQUIRE(batch != nullptr, "ms_forward: null batch");
@@ -211,8 +214,12 @@ extern "C" int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache,
       MS_TRY(rc);
     }
     // q occupies the first hq*dh columns of each qkv row.
-    MS_TRY(paged_attention(w.qkv, qkv_w, c, l, bt, hq, w.attn, attn_scratch, attn_scratch_bytes,
-                           s, order));
+    if (forms)
+      MS_TRY(attention_form(w.qkv, qkv_w, c, l, bt, hq, form, w.attn, hq * dh, attn_scratch,
+                            attn_scratch_bytes, s));
+    else
+      MS_TRY(paged_attention(w.qkv, qkv_w, c, l, bt, hq, w.attn, attn_scratch, attn_scratch_bytes,
+                             s, order));
     MS_TRY(gemm_dispatch(w.attn, m.w_o[l], w.x, w.x, T, d, hq * dh, 0, dt, MS_DTYPE_F32,
                          kEpiResidual, s, true));
     if (o_a)
@@ -239,4 +246,34 @@ extern "C" int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache,
              "ms_forward: logits_row_stride < vocab");
   return gemm_dispatch(w.xl, m.embed, logits, nullptr, R, m.vocab_size, d, logits_row_stride, dt,
                        MS_DTYPE_F32, kEpiStore, s, true);
+}
+
+}  // namespace
+}  // namespace ms
+
+extern "C" int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache,
+                               const ms_batch* batch, const ms_lora_model* lora,
+                               const ms_lora_plan* plan, const int32_t* logit_rows,
+                               int n_logit_rows, float* logits, int64_t logits_row_stride,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  return forward(model, cache, batch, false, nullptr, lora, plan, logit_rows, n_logit_rows, logits,
+                 logits_row_stride, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t ms_forward_form_workspace_size(const ms_model* model, const ms_kv_cache* cache,
+                                                 const ms_batch* batch,
+                                                 const ms_attention_form* form,
+                                                 const ms_lora_model* lora, int max_logit_rows) {
+  if (model == nullptr || batch == nullptr || batch->n_tokens < 0) return 0;
+  return carve(*model, batch->n_tokens, max_logit_rows, nullptr, lora ? lora->adapters.max_rank : 0).bytes +
+         ms_attention_form_workspace_size(cache, model->n_heads, batch, form);
+}
+
+extern "C" int ms_forward_form(const ms_model* model, const ms_kv_cache* cache, const ms_batch* batch,
+                               const ms_attention_form* form, const ms_lora_model* lora,
+                               const ms_lora_plan* plan, const int32_t* logit_rows, int n_logit_rows,
+                               float* logits, int64_t logits_row_stride, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return forward(model, cache, batch, true, form, lora, plan, logit_rows, n_logit_rows, logits,
+                 logits_row_stride, workspace, workspace_bytes, stream);
 }

@@ -23,6 +23,15 @@ int paged_attention(const void* q, int q_stride, const ms_kv_cache& cache, int l
                     const ms_batch& batch, int hq, void* out, void* scratch, size_t scratch_bytes,
                     cudaStream_t s, const int32_t* seq_order = nullptr);
 
+// The same with a score form (attention_form.cu); form may be null.  q_stride and
+// out_stride: elements between tokens.  Fewer workspace bytes than
+// attention_form_workspace: one KV range per tile.
+int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& cache, int layer,
+                   const ms_batch& batch, int hq, const ms_attention_form* form, void* out,
+                   int64_t out_stride, void* workspace, size_t workspace_bytes, cudaStream_t s);
+size_t attention_form_workspace(const ms_kv_cache& cache, const ms_batch& batch, int hq,
+                                const ms_attention_form* form);
+
 // order[r] = the sequence with the r-th longest context (ties by index), so
 // the attention grid starts the longest sequences first and the short ones
 // fill the last wave.  Scheduling order only: every output is unchanged.

@@ -32,6 +32,7 @@ from .cache import PagedKVCache
 from .config import ModelConfig
 
 if TYPE_CHECKING:
+    from .attention import AttentionForm
     from .lora import LoraAdapters, LoraPlan
 
 
@@ -325,8 +326,12 @@ class Transformer:
         out: torch.Tensor | None = None,
         out_row_stride: int = 0,
         lora: LoraPlan | None = None,
+        form: AttentionForm | None = None,
     ) -> torch.Tensor:
         """Paged forward; returns float32 logits ``(rows, vocab)``.
+
+        ``form``: every layer's attention takes this form (a tree of drafted tokens, say)
+        instead of plain causal attention; the batch's positions are the tokens' own.
 
         ``lora`` says which of :attr:`adapters` each token of the batch uses
         (``adapters.plan``); None: the shared weights alone.
@@ -348,6 +353,9 @@ class Transformer:
             rows_ptr, out_ptr = self._placeholder().data_ptr(), self._placeholder().data_ptr()
         cb = batch.c_struct()
         cc = cache.c_struct()
+        if form is not None:
+            return self._forward_form(form, batch, cb, cc, lora, rows_ptr, n_rows, out, out_ptr,
+                                      out_row_stride)
         scratch = int(_lib.load().ms_attention_scratch_size(ctypes.byref(cc), self.cfg.n_heads,
                                                             ctypes.byref(cb)))
         if lora is not None:
@@ -367,4 +375,24 @@ class Transformer:
             ctypes.byref(cb), rows_ptr, n_rows, out_ptr, out_row_stride,
             ws.data_ptr(), ws.numel(), _lib.stream_ptr(self.device),
         )
+        return out
+
+    def _forward_form(self, form: AttentionForm, batch: PagedBatch, cb: _lib.MsBatch,
+                      cc: _lib.MsKVCache, lora: LoraPlan | None, rows_ptr: int | None, n_rows: int,
+                      out: torch.Tensor, out_ptr: int, out_row_stride: int) -> torch.Tensor:
+        ref = ctypes.byref
+        index = torch.cuda.current_device() if self.device.index is None else self.device.index
+        cf = ref(form.c_struct(index, self.cfg.n_heads, batch))
+        cl = cp = None
+        if lora is not None:
+            if self.adapters is None:
+                raise ValueError("the model has no adapters loaded")
+            cl, cp = ref(self.adapters.c_struct()), ref(lora.c_struct(batch.n_tokens, self.device))
+        need = int(_lib.load().ms_forward_form_workspace_size(ref(self._c_model), ref(cc), ref(cb), cf,
+                                                              cl, n_rows))
+        if self._ws is None or self._ws.numel() < need:
+            self._ws = torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
+        _lib.call("ms_forward_form", ref(self._c_model), ref(cc), ref(cb), cf, cl, cp, rows_ptr, n_rows,
+                  out_ptr, out_row_stride, self._ws.data_ptr(), self._ws.numel(),
+                  _lib.stream_ptr(self.device))
         return out

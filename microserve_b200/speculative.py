@@ -226,6 +226,7 @@ class _Lookahead:
     events: tuple[torch.cuda.Event, torch.cuda.Event] | None
     controls: LogitControls | None = None
     controls_version: int = 0  # the upload that `controls` views
+    draft_moves: int = 0  # draft_cache.moves: its tables are on the device
     # filled once the round's results are read
     n_tok: np.ndarray = field(default_factory=_empty)  # token counts with the round's tokens
     last: list[int] = field(default_factory=list)  # last tokens then
@@ -449,7 +450,7 @@ class SpeculativeDecoder:
             samplings=[r.sampling for r in plan.requests],
             seeds=[g.initial_seed() for g in plan.gens], target_cache=plan.target_cache,
             max_ctx=max_ctx, params=params, idsv=idsv, events=ev, controls=plan.controls,
-            controls_version=self.controls.version)
+            controls_version=self.controls.version, draft_moves=self.draft_cache.moves)
 
     def _chain_buffers(self, B: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Device buffers of the chained round: its metadata, its sampling
@@ -520,6 +521,8 @@ class SpeculativeDecoder:
         if target_cache is not ahead.target_cache or len(requests) != len(ahead.ids):
             return False
         if ahead.controls is not None and self.controls.version != ahead.controls_version:
+            return False
+        if self.draft_cache.moves != ahead.draft_moves:
             return False
         for i, r in enumerate(requests):
             if r.request_id != ahead.ids[i] or r.sampling is not ahead.samplings[i]:
