@@ -208,6 +208,22 @@ size_t part_bytes(const FormArgs& a, int rows, int dh) {
 
 int simt_rows(int dh) { return kWarps * (dh <= 64 ? 4 : 2); }
 
+// How a call is cut up: which kernel, its rows per tile, the KV ranges.
+struct Way {
+  bool tma;
+  int rows;
+};
+Way choose(FormArgs& a, const ms_kv_cache& c, int max_context) {
+  Way w{form_tma_takes(c), 64};
+  if (w.tma) {
+    plan(a, max_context, w.rows, 64, 256, 148 * 4);
+  } else {
+    w.rows = simt_rows(c.d_head);
+    plan(a, max_context, w.rows, kChunk, 128, 148 * 4);
+  }
+  return w;
+}
+
 template <typename T, int DH>
 int launch_simt(FormArgs& a, cudaStream_t s) {
   dim3 grid(a.row_tiles * a.n_splits, a.hkv, a.n_seqs);
@@ -286,6 +302,7 @@ int form_combine(const FormArgs& a, int rows, int dh, cudaStream_t s) {
   launch_pdl(form_combine_kernel<T, kBase2>, grid, 128, 0, s, a, rows, dh);
   return check_launch("form_combine_kernel");
 }
+template int form_combine<__nv_bfloat16, true>(const FormArgs& a, int rows, int dh, cudaStream_t s);
 
 int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& c, int layer,
                    const ms_batch& bt, int hq, const ms_attention_form* form, void* out,
@@ -300,8 +317,8 @@ int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& c, int la
   a.out_stride = out_stride;
   a.err = device_error_word();
   ProfScope prof(kClsAttention, s);
-  const int rows = simt_rows(c.d_head);
-  plan(a, max_context, rows, kChunk, 128, 148 * 4);
+  const Way way = choose(a, c, max_context);
+  const int rows = way.rows;
   if (part_bytes(a, rows, c.d_head) > workspace_bytes) {  // one range a tile
     a.n_splits = 1;
     a.split_len = INT_MAX;
@@ -310,6 +327,7 @@ int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& c, int la
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + (size_t)a.n_seqs * a.hkv * a.row_tiles * a.n_splits * rows * c.d_head;
   }
+  if (way.tma) return form_tma(a, c.d_head, s);
   return c.dtype == MS_DTYPE_F32 ? simt_by_dh<float>(a, c.d_head, s)
                                  : simt_by_dh<__nv_bfloat16>(a, c.d_head, s);
 }
@@ -320,9 +338,8 @@ size_t attention_form_workspace(const ms_kv_cache& c, const ms_batch& bt, int hq
   int max_context = 0;
   if (form_args(a, c, 0, bt, hq, form, &max_context) != MS_OK || bt.n_seqs == 0 || bt.n_tokens == 0)
     return 0;
-  const int rows = simt_rows(c.d_head);
-  plan(a, max_context, rows, kChunk, 128, 148 * 4);
-  return part_bytes(a, rows, c.d_head);
+  const Way way = choose(a, c, max_context);
+  return part_bytes(a, way.rows, c.d_head);
 }
 
 }  // namespace ms

@@ -114,4 +114,8 @@ __device__ __forceinline__ bool form_sees(const FormArgs& a, const FormSeq& s, i
 template <typename T, bool kBase2>
 int form_combine(const FormArgs& a, int rows, int dh, cudaStream_t s);
 
+// attention_form_tma.cu: tiles of 64 rows.
+bool form_tma_takes(const ms_kv_cache& c);
+int form_tma(const FormArgs& a, int dh, cudaStream_t s);
+
 }  // namespace ms

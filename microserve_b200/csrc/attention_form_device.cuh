@@ -1,0 +1,164 @@
+// Device helpers of the matrix kernels of attention with score forms
+// (attention_form_tma.cu, attention_form_tc.cu), and their tensor maps.
+#pragma once
+
+#include <cuda.h>
+
+#include "attention_form.cuh"
+
+namespace ms {
+
+constexpr int kErrTimeout = 5;
+constexpr long long kFormWaitCycles = 1ll << 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ uint32_t s_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Waits for a phase, up to a limit; after that (or when another thread of the block gave
+// up) false.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* stop, int* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*stop) return false;
+    if (clock64() - t0 > kFormWaitCycles) {
+      *stop = 1;
+      atomicCAS(err, 0, kErrTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+// 2^x by the SFU (ftz; 2^-inf = 0): 2 ulp of a result that is rounded to bf16 next.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float low_half(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high_half(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// Smallest and largest position of the tokens of rows [r0, r0 + nr) (the whole warp calls it).
+__device__ __forceinline__ void position_range(const FormArgs& a, const FormSeq& s, int r0, int nr,
+                                               int& lo, int& hi) {
+  lo = INT_MAX;
+  hi = INT_MIN;
+  const int last = (r0 + nr - 1) / a.group;
+  for (int t = r0 / a.group + (threadIdx.x & 31); t <= last; t += 32) {
+    const int p = a.positions[s.t0 + t];
+    lo = min(lo, p);
+    hi = max(hi, p);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+}
+
+// Whether every row of the tile sees all N keys from place x0 on.
+template <int N>
+__device__ __forceinline__ bool all_see(const FormArgs& a, const FormSeq& s, const FormKeys& k, int x0,
+                                        int xend, int minpos, int maxpos) {
+  if (x0 + N > xend || (x0 < k.a && x0 + N > k.a)) return false;
+  const int j0 = k.key(x0);
+  if (j0 + N <= s.pfx) return true;
+  return (a.mask ? j0 + N <= s.base : j0 + N - 1 <= minpos) &&
+         (a.window <= 0 || maxpos - j0 < a.window);
+}
+
+__device__ __forceinline__ uint64_t low_bits(int n) {
+  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+
+// How many keys from j0 on (up to 64) lie before the window of a token at `pos`.
+__device__ __forceinline__ int before_window(const FormArgs& a, int pos, int j0) {
+  return (int)min(max((int64_t)pos - a.window - j0 + 1, (int64_t)0), (int64_t)64);
+}
+
+// Bit i: whether the token at row t of the batch (position pos) sees key j0 + i.
+__device__ __forceinline__ uint64_t seen_from(const FormArgs& a, const FormSeq& s, int t, int pos, int j0) {
+  uint64_t seen;
+  if (a.mask) {
+    const int node0 = j0 - s.base, w0 = node0 >> 5, sh = node0 & 31;
+    const uint32_t* row = a.mask + (int64_t)t * a.mask_words;
+    auto word = [&](int w) { return w >= 0 && w < a.mask_words ? (uint64_t)row[w] : 0ull; };
+    seen = (word(w0) | word(w0 + 1) << 32) >> sh;
+    if (sh) seen |= word(w0 + 2) << (64 - sh);
+    seen = (seen & low_bits(s.qlen - node0)) | low_bits(-node0);
+    if (a.window > 0) {
+      // keys before the pass's own tokens by their place, those by their positions
+      seen &= ~(low_bits(before_window(a, pos, j0)) & low_bits(-node0));
+      for (int i = max(0, -node0); i < 64 && node0 + i < s.qlen; ++i)
+        if (pos - a.positions[s.t0 + node0 + i] >= a.window) seen &= ~(1ull << i);
+    }
+  } else {
+    seen = pos < j0 ? 0ull : low_bits(min(pos - j0, 63) + 1);
+    if (a.window > 0) seen &= ~low_bits(before_window(a, pos, j0));
+  }
+  return seen | low_bits(s.pfx - j0);
+}
+
+// The same for the 64 places from x0 on, cut to those below xend.
+__device__ __forceinline__ uint64_t seen_places(const FormArgs& a, const FormSeq& s, const FormKeys& k,
+                                                int t, int pos, int x0, int xend) {
+  uint64_t seen;
+  if (x0 >= k.a) {
+    seen = seen_from(a, s, t, pos, x0 + k.shift);
+  } else {
+    seen = seen_from(a, s, t, pos, x0);
+    if (x0 + 64 > k.a) {
+      const uint64_t first = low_bits(k.a - x0);
+      seen = (seen & first) | (seen_from(a, s, t, pos, x0 + k.shift) & ~first);
+    }
+  }
+  return seen & low_bits(xend - x0);
+}
+
+// The position of the key at place x.
+__device__ __forceinline__ int key_position(const FormArgs& a, const FormSeq& s, const FormKeys& k, int x) {
+  const int j = k.key(x), node = j - s.base;
+  return a.mask && node >= 0 ? a.positions[s.t0 + min(node, s.qlen - 1)] : j;
+}
+
+// attention_form_tma.cu: the pool as [rows][dh] bf16, boxes of 64 columns x `box` rows, 128-byte swizzle.
+int form_pool_map(const void* pool, int64_t rows, int dh, int box, CUtensorMap* out);
+
+}  // namespace ms
