@@ -209,19 +209,25 @@ size_t part_bytes(const FormArgs& a, int rows, int dh) {
 int simt_rows(int dh) { return kWarps * (dh <= 64 ? 4 : 2); }
 
 // How a call is cut up: which kernel, its rows per tile, the KV ranges.
+enum Kernel { kSimt, kTma, kTc };
 struct Way {
-  bool tma;
+  Kernel kernel;
   int rows;
 };
 Way choose(FormArgs& a, const ms_kv_cache& c, int max_context) {
-  Way w{form_tma_takes(c), 64};
-  if (w.tma) {
-    plan(a, max_context, w.rows, 64, 256, 148 * 4);
-  } else {
-    w.rows = simt_rows(c.d_head);
+  const int64_t rows = (int64_t)a.max_q * a.group;
+  if (!form_tma_takes(c)) {
+    const Way w{kSimt, simt_rows(c.d_head)};
     plan(a, max_context, w.rows, kChunk, 128, 148 * 4);
+    return w;
   }
-  return w;
+  if (rows <= 32) {
+    plan(a, max_context, 64, 64, 256, 148 * 4);
+    return {kTma, 64};
+  }
+  const int tile = rows > 128 ? 256 : 128;
+  plan(a, max_context, tile, 128, 512, tile == 256 ? 148 : 2 * 148);
+  return {kTc, tile};
 }
 
 template <typename T, int DH>
@@ -327,7 +333,8 @@ int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& c, int la
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + (size_t)a.n_seqs * a.hkv * a.row_tiles * a.n_splits * rows * c.d_head;
   }
-  if (way.tma) return form_tma(a, c.d_head, s);
+  if (way.kernel == kTma) return form_tma(a, c.d_head, s);
+  if (way.kernel == kTc) return form_tc(a, c.d_head, rows, s);
   return c.dtype == MS_DTYPE_F32 ? simt_by_dh<float>(a, c.d_head, s)
                                  : simt_by_dh<__nv_bfloat16>(a, c.d_head, s);
 }
