@@ -225,7 +225,7 @@ Way choose(FormArgs& a, const ms_kv_cache& c, int max_context) {
     plan(a, max_context, 64, 64, 256, 148 * 4);
     return {kTma, 64};
   }
-  const int tile = rows > 128 ? 256 : 128;
+  const int tile = rows > 128 ? 256 : rows > 64 ? 128 : 64;
   plan(a, max_context, tile, 128, 512, tile == 256 ? 148 : 2 * 148);
   return {kTc, tile};
 }
@@ -264,6 +264,8 @@ int form_args(FormArgs& a, const ms_kv_cache& c, int layer, const ms_batch& bt, 
              "ms_paged_attention_form: max_q_len and max_blocks must be > 0");
   MS_REQUIRE((int64_t)bt.max_blocks * c.block_size <= INT_MAX && (int64_t)bt.max_q_len * hq <= INT_MAX / 2,
              "ms_paged_attention_form: contexts or queries beyond 2^31");
+  if ((int64_t)bt.max_q_len * (hq / c.n_kv_heads) > 65535 * 128)
+    return fail(MS_ERR_TOO_LARGE, "ms_paged_attention_form: %d tokens of a sequence", bt.max_q_len);
   if (bt.n_seqs > 65535 || c.n_kv_heads > 65535)
     return fail(MS_ERR_TOO_LARGE, "ms_paged_attention_form: more than 65535 sequences or kv heads");
   a.q_start = bt.q_start;
