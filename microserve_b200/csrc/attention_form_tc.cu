@@ -38,23 +38,27 @@ template <int DH, int SH>
 struct TcCfg {
   static constexpr int ST = SH == kTwo ? 2 : 1;                  // streams of 128 rows
   static constexpr bool kTwin = SH == kHalf;
-  static constexpr int KC = kTwin && DH == 64 ? 128 : 64;        // keys per step
-  static constexpr int SB = kTwin ? 1 : 2;                       // score buffers
-  static constexpr int kWidth = kTwin ? KC / 2 : KC;             // scores of a step per thread
+  static constexpr bool kSep = kTwin || DH == 64;                // p behind the scores, or over them
+  static constexpr int KC = DH == 64 || SH == kTwo ? 128 : 64;   // keys per step
+  static constexpr int SB = kSep || SH == kTwo ? 1 : 2;          // score buffers
+  static constexpr int kParts = kTwin && DH == 128 ? 1 : 2;      // threads that share a row's scores
+  static constexpr int kWidth = KC / (kTwin ? 2 : 1) / kParts;   // scores of a step per thread
   static constexpr int kTile = KC * DH * 2;                      // K or V of a step
-  static constexpr int kSlots = SH == kTwo ? 144 : kTwin && DH == 64 ? 96 : DH == 64 ? 96 : 80;  // KB of K and V
+  static constexpr int kSlots = SH == kTwo ? 160 : DH == 64 || kTwin ? 80 : 64;  // KB of K and V
   static constexpr int NK = (kSlots * 1024 / kTile + 1) / 2, NV = kSlots * 1024 / kTile / 2;
   static constexpr int kQ = kTileRows * DH * 2;
-  static constexpr int kPCol = kTwin ? KC : 0;                   // p stands behind the scores, or over them
-  static constexpr int kOCol = kTwin ? KC + KC / 2 : SB * KC;
+  static constexpr int kPCol = kSep ? KC : 0;
+  static constexpr int kOCol = kSep ? KC + KC / 2 : SB * KC;
   static constexpr int kStreamCols = kOCol + DH;
   static constexpr int kCols = ST == 2 ? 512 : 256;
-  static constexpr int kWarps = 4 * ST + (ST == 2 ? 4 : 2);
+  static constexpr int kSoft = 4 * kParts;                       // softmax warps of a stream
+  static constexpr int kWarps = kSoft * ST + (ST == 2 ? 4 : 2);
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kBars = 2 * NK + 2 * NV + 3 + ST * (2 * SB + 2);
-  static constexpr int kSmem = ST * kQ + (NK + NV) * kTile + kBars * 8 + 16;
+  static constexpr int kBars = 2 * NK + 2 * NV + 2 + ST * (2 * SB + 3);
+  static constexpr int kShare = ST * kParts * kTileRows * 4;     // what the threads of a row tell one another
+  static constexpr int kSmem = ST * kQ + (NK + NV) * kTile + kShare + kBars * 8 + 16;
   static_assert(ST * kStreamCols <= kCols, "TMEM columns");
-  static_assert((3 - ST) * (kSmem + 1024) <= 228 * 1024, "shared memory of the CTAs of an SM");
+  static_assert((3 - ST) * (kSmem + 1024) <= 228 * 1024 && kSmem <= 227 * 1024, "shared memory of an SM's CTAs");
   static_assert(!kTwin || 64 * DH * 4 + 64 * 8 <= NK * kTile, "the copies meet in the K ring");
 };
 
@@ -114,47 +118,41 @@ __device__ __forceinline__ uint32_t elect_one() {
       : "=r"(one));
   return one;
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+// 32 lanes x N columns, N a multiple of 16 (loads) or 8 (stores).  Nothing that uses the values of a
+// load comes between it and its wait: the outputs of the empty asm are the values.
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-      "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-      "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// Nothing that uses r comes before this (the loads' outputs are there only after the wait).
-__device__ __forceinline__ void pin32(uint32_t* r) {
+__device__ __forceinline__ void pin16(uint32_t* r) {
   asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]));
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]));
   asm volatile(""
-               : "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                 "+r"(r[29]));
-  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+               : "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[N]) {
+  static_assert(N % 16 == 0, "whole loads");
+#pragma unroll
+  for (int c = 0; c < N; c += 16) tmem_ld16(addr + c, r + c);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < N; c += 16) pin16(r + c);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[N]) {
+  static_assert(N % 8 == 0, "whole stores");
+#pragma unroll
+  for (int c = 0; c < N; c += 8) tmem_st8(addr + c, r + c);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() {
@@ -221,6 +219,20 @@ __device__ __forceinline__ float min3(float a, uint32_t b, uint32_t c) {
   return d;
 }
 
+// The largest (or smallest) of 32 values.
+template <bool kMax>
+__device__ __forceinline__ float reduce(const uint32_t (&x)[32]) {
+  float v[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = __uint_as_float(x[c]);
+#pragma unroll
+  for (int c = 4; c < 32; c += 2) {
+    float& to = v[(c >> 1) & 3];
+    to = kMax ? max3(to, x[c], x[c + 1]) : min3(to, x[c], x[c + 1]);
+  }
+  return kMax ? fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) : fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
+}
+
 // Adds the two bf16 of a word to two float32 sums.
 __device__ __forceinline__ void add_bf16(uint32_t v, float& lo, float& hi) {
   asm("{\n\t.reg .b16 l, h;\n\t"
@@ -252,39 +264,54 @@ struct Cap {
   __device__ __forceinline__ float exact(float s) const {
     return fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(s * in)), cap2);
   }
-  __device__ __forceinline__ float series(float s) const {
-    const float w = s * s;
-    return s * fmaf(w, fmaf(w, fmaf(w, fmaf(w, d4, d3), d2), d1), d0);
-  }
 };
 
-// p = 2^(x - sub) of 2 kWords values, rounded to bf16; `sum` gets the rounded values.
-// kWay 0: x * mul; 1: the cap's series of x; 2: x as it is.
-template <int kWay, int kWords>
-__device__ __forceinline__ void exps(const uint32_t* x, uint32_t* p, float mul, float sub, const Cap& cap,
-                                     float (&sum)[4]) {
+// p = 2^(x - sub) of 32 values, rounded to bf16, into TMEM; returns the sum of the rounded values.
+// kWay 0: x * mul; 1: the cap's series of x; 2: x as it is.  16 values at a time, each operation
+// over all of them before the next: a packed operation with three fresh operands takes 3
+// cycles, with one repeated from the operation before 2.
+template <int kWay>
+__device__ __forceinline__ float exps(const uint32_t (&x)[32], uint32_t p_at, float mul, float sub, const Cap& cap) {
   const uint64_t minus = twice(-sub);
+  float sum[4] = {};
 #pragma unroll
-  for (int e = 0; e < kWords; ++e) {
-    const uint64_t v = pair(x[2 * e], x[2 * e + 1]);
-    uint64_t arg;
+  for (int g = 0; g < 32; g += 16) {
+    uint64_t v[8], c[8];
+    uint32_t p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = pair(x[g + 2 * j], x[g + 2 * j + 1]);
     if constexpr (kWay == 0) {
-      arg = fma2(v, twice(mul), minus);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = fma2(v[j], twice(mul), minus);
     } else if constexpr (kWay == 1) {
-      const uint64_t w = mul2(v, v);
-      uint64_t c = fma2(w, twice(cap.d4), twice(cap.d3));
-      c = fma2(w, c, twice(cap.d2));
-      c = fma2(w, c, twice(cap.d1));
-      c = fma2(w, c, twice(cap.d0));
-      arg = fma2(v, c, minus);
+      uint64_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = mul2(v[j], v[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = fma2(w[j], twice(cap.d4), twice(cap.d3));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = fma2(w[j], c[j], twice(cap.d2));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = fma2(w[j], c[j], twice(cap.d1));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = fma2(w[j], c[j], twice(cap.d0));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = fma2(v[j], c[j], minus);
     } else {
-      arg = add2(v, minus);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = add2(v[j], minus);
     }
-    float lo, hi;
-    unpair(arg, lo, hi);
-    p[e] = pack2(fast_exp2(lo), fast_exp2(hi));
-    add_bf16(p[e], sum[2 * (e & 1)], sum[2 * (e & 1) + 1]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float lo, hi;
+      unpair(c[j], lo, hi);
+      p[j] = pack2(fast_exp2(lo), fast_exp2(hi));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) add_bf16(p[j], sum[2 * (j & 1)], sum[2 * (j & 1) + 1]);
+    tmem_st8(p_at + g / 2, p);
   }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // The rows of a CTA once more, a warp a row: every seen key by itself, a lane a key for the
@@ -352,9 +379,10 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
   constexpr int ST = C::ST, KC = C::KC, SB = C::SB, NK = C::NK, NV = C::NV, W = C::kWidth;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = s_addr(smem_raw), q_s = raw;  // (1024-byte aligned, as declared)
-  const uint32_t k_s = q_s + ST * C::kQ, v_s = k_s + NK * C::kTile, bars = v_s + NV * C::kTile;
+  const uint32_t k_s = q_s + ST * C::kQ, v_s = k_s + NK * C::kTile, share = v_s + NV * C::kTile;
+  const uint32_t bars = share + C::kShare;
   const uint32_t k_full = bars, k_empty = k_full + 8 * NK, v_full = k_empty + 8 * NK, v_empty = v_full + 8 * NV;
-  const uint32_t q_ready = v_empty + 8 * NV, ended = q_ready + 8, s_read = ended + 8, s_full = s_read + 8;
+  const uint32_t q_ready = v_empty + 8 * NV, ended = q_ready + 8, s_read = ended + 8, s_full = s_read + 8 * ST;
   const uint32_t p_ready = s_full + 8 * ST * SB, pv_done = p_ready + 8 * ST * SB, slot_at = pv_done + 16 * ST;
   unsigned char* words = smem_raw + (slot_at - raw);
   volatile uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(words);
@@ -381,7 +409,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
   const int xend = split == a.n_splits - 1 ? keys.total : min(keys.total, xbeg + a.split_len);
   const int steps = (xend - xbeg + KC - 1) / KC;
   const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-  constexpr int kProducer = 4 * ST, kMma = kProducer + 1;
+  constexpr int kProducer = C::kSoft * ST, kMma = kProducer + 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NK; ++i) {
@@ -392,12 +420,12 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       mbar_init(v_full + 8 * i, 1);
       mbar_init(v_empty + 8 * i, 1);
     }
-    mbar_init(q_ready, 4 * ST);
+    mbar_init(q_ready, C::kSoft * ST);
     mbar_init(ended, 1);
-    mbar_init(s_read, 4);
+    for (int i = 0; i < ST; ++i) mbar_init(s_read + 8 * i, C::kSoft);
     for (int i = 0; i < ST * SB; ++i) {
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_ready + 8 * i, 4);
+      mbar_init(p_ready + 8 * i, C::kSoft);
     }
     for (int i = 0; i < 2 * ST; ++i) mbar_init(pv_done + 8 * i, 1);
     *stop = 0;
@@ -416,7 +444,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= kProducer) {
-    if constexpr (ST == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if constexpr (ST == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == kProducer) {
       // ---- loads
       constexpr int kHalves = DH / 64;
@@ -480,7 +508,11 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
         const uint32_t p = cols + st * C::kStreamCols + C::kPCol + (it % SB) * KC;
         const uint64_t vd = smem_desc(v_s + (it % NV) * C::kTile, KC * 128);
 #pragma unroll
-        for (int k = 0; k < KC / 16; ++k) mma_ts(o, p + 8 * k, vd + k * (2048 / 16), id_o, it > 0 || k > 0, one);
+        for (int k = 0; k < KC / 16; ++k) {
+          // over the scores, each part's p starts where its scores did
+          const int at = C::kSep ? 8 * k : 8 * (k % (W / 16)) + k / (W / 16) * W;
+          mma_ts(o, p + at, vd + k * (2048 / 16), id_o, it > 0 || k > 0, one);
+        }
         mma_commit(pv_done + 8 * (2 * st + (it & 1)), one);
       };
       bool ok = wait(q_ready, 0);
@@ -493,7 +525,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       }
       for (int it = 0; it < n && ok; ++it) {
         const int ahead = it + SB;
-        if constexpr (C::kTwin) {  // the next scores as soon as these are read
+        if constexpr (C::kSep && ST == 1) {  // the next scores as soon as these are read
           if (ahead < n) {
             ok = wait(k_full + 8 * (ahead % NK), (ahead / NK) & 1) && wait(s_read, it & 1);
             if (!ok) break;
@@ -511,10 +543,15 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           fence_after();
           add_values(it, st);
           if (st == ST - 1) mma_commit(v_empty + 8 * (it % NV), one);
-          if constexpr (!C::kTwin) {
+          if constexpr (!C::kSep || ST == 2) {
             if (ahead < n) {
               if (st == 0) {
                 ok = wait(k_full + 8 * (ahead % NK), (ahead / NK) & 1);
+                if (!ok) break;
+                fence_after();
+              }
+              if constexpr (C::kSep) {  // (read before p was ready)
+                ok = wait(s_read + 8 * st, it & 1);
                 if (!ok) break;
                 fence_after();
               }
@@ -531,53 +568,82 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       }
     }
   } else {
-    if constexpr (ST == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    // ---- softmax: stream st, row t of its tile
-    const int st = warp >> 2, t = threadIdx.x & 127;
-    // which half of a step's keys a copy of a row has (one copy: all of them)
-    const int mine = C::kTwin ? (t >> 6) * W : 0;
-    const int r = C::kTwin ? t & 63 : st * kTileRows + t;  // row of the CTA
+    if constexpr (ST == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ---- softmax: lane t of stream st.  A row has kParts threads, in warps of one scheduler, that
+    // share its maximum; in a twin two copies (lanes t and t + 64) with a maximum each
+    const int st = warp / C::kSoft, part = (warp >> 2) % C::kParts, t = threadIdx.x & 127;
+    const int mine = (C::kTwin ? (t >> 6) * (KC / 2) : 0) + part * W;  // the first of its keys in a step
+    const int r = C::kTwin ? t & 63 : st * kTileRows + t;              // row of the CTA
     const bool live = r < nr;
     const bool warp_live = __any_sync(0xffffffffu, live);
     const int rr = r0 + (live ? r : 0), tok = s.t0 + rr / a.group, head = g * a.group + rr % a.group;
     const int pos = a.positions[tok];
+    constexpr int kMyDims = DH / C::kParts;  // of the row's O and result
+    const int dim0 = part * kMyDims;
     {
-      const __nv_bfloat16* q =
-          static_cast<const __nv_bfloat16*>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * DH;
-      uint4 v[DH / 8];
-      if (vec) {
+      // ---- Q into the swizzled tile: DH / 8 lanes a row, so that whole rows are read
+      constexpr int kLanes = DH / 8, kRowsAtOnce = 32 / kLanes, kMine = kTileRows / C::kSoft;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q);
+      const int c = lane % kLanes, first = (warp % C::kSoft) * kMine + lane / kLanes;
+      uint4 v[kMine / kRowsAtOnce];
 #pragma unroll
-        for (int c = 0; c < DH / 8; ++c)
-          v[c] = live ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int c = 0; c < DH / 8; ++c) {
-          uint32_t w[4];
-          for (int e = 0; e < 4; ++e)
-            w[e] = !live ? 0u
-                         : (uint32_t)__bfloat16_as_ushort(q[c * 8 + 2 * e]) |
-                               (uint32_t)__bfloat16_as_ushort(q[c * 8 + 2 * e + 1]) << 16;
-          v[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int i = 0; i < kMine / kRowsAtOnce; ++i) {
+        const int at = first + i * kRowsAtOnce, row = C::kTwin ? at & 63 : st * kTileRows + at;
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (row < nr) {
+          const int k = r0 + row, tk = k / a.group;
+          const __nv_bfloat16* src =
+              q + (int64_t)(s.t0 + tk) * a.q_stride + (int64_t)(g * a.group + k - tk * a.group) * DH + c * 8;
+          if (vec) {
+            v[i] = *reinterpret_cast<const uint4*>(src);
+          } else {
+            uint32_t w[4];
+            for (int e = 0; e < 4; ++e)
+              w[e] = (uint32_t)__bfloat16_as_ushort(src[2 * e]) | (uint32_t)__bfloat16_as_ushort(src[2 * e + 1]) << 16;
+            v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
       }
-      const uint32_t to = q_s + st * C::kQ + t * 128;
 #pragma unroll
-      for (int c = 0; c < DH / 8; ++c)
-        sts128(to + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (t & 7)) << 4), v[c]);
+      for (int i = 0; i < kMine / kRowsAtOnce; ++i) {
+        const int at = first + i * kRowsAtOnce;
+        sts128(q_s + st * C::kQ + at * 128 + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (at & 7)) << 4), v[i]);
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
+    // whether any thread of the warps that share these rows says so
+    auto any_part = [&](bool pred) {
+      if constexpr (C::kParts == 1) return __any_sync(0xffffffffu, pred) != 0;
+      uint32_t any;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %1, 0;\n\t"
+          "bar.red.or.pred q, %2, 64, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(any)
+          : "r"((uint32_t)pred), "r"(2 + 4 * st + (warp & 3))
+          : "memory");
+      return any != 0;
+    };
+    // a wait that gives up sets `stop`: the later ones return at once, and nothing is written
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      mbar_wait(bar, parity, stop, a.err);
+      __syncwarp();
+      fence_after();
+    };
+    const uint32_t mine_at = share + ((st * C::kParts + part) * kTileRows + t) * 4;
+    const uint32_t other_at = share + ((st * C::kParts + (part ^ (C::kParts - 1))) * kTileRows + t) * 4;
     const bool capped = a.softcap > 0.f, sloped = a.slopes != nullptr;
     Cap cap{};
     if (capped) cap.set(a);
     const float lin = a.scale * kLog2e, slope = sloped ? a.slopes[head] * kLog2e : 0.f;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_col = tmem + st * C::kStreamCols + lanes, o_col = s_col + C::kOCol;
+    const uint32_t s_col = tmem + st * C::kStreamCols + lanes, o_col = s_col + C::kOCol + dim0;
     if constexpr (C::kTwin) {  // p of the other copy's keys: 0 for good
-      uint32_t zero[32] = {};
-      const uint32_t to = s_col + C::kPCol + (W - mine) / 2;
-      if constexpr (W == 64) tmem_st32(to, zero); else tmem_st16(to, zero);
+      uint32_t zero[W / 2] = {};
+      tmem_st(s_col + C::kPCol + (KC / 4) * (1 - (t >> 6)) + part * (W / 2), zero);
     }
     // the steps that every row sees in full: those inside the prefix, and [free0, free1)
     const int lead = max(0, min(keys.a > 0 ? min(keys.a, s.pfx) : s.pfx, xend) - xbeg) / KC;
@@ -585,17 +651,18 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     const int free0 = (max(0, max(keys.a, oldest - keys.shift) - xbeg) + KC - 1) / KC;
     const int free1 = max(0, min((a.mask ? s.base : min(minpos, INT_MAX - 1) + 1) - keys.shift, xend) - xbeg) / KC;
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    // scores (as they come out of the product) above and below which a step is not plain
+    float plain_top = -INFINITY;
+    const float plain_bottom = capped ? -cap.limit : -INFINITY;
     for (int it = 0; it < steps; ++it) {
       const int x0 = xbeg + it * KC;
       const bool free = it < lead || (it >= free0 && it < free1);
       if (!free) {
         // ---- the step's values: nothing that is not finite may enter the product
-        ok = mbar_wait(v_full + 8 * (it % NV), (it / NV) & 1, stop, a.err);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        wait(v_full + 8 * (it % NV), (it / NV) & 1);
         const uint32_t vt = v_s + (it % NV) * C::kTile;
 #pragma unroll 4
-        for (int i = t; i < KC * DH / 8; i += kTileRows) {
+        for (int i = part * kTileRows + t; i < KC * DH / 8; i += C::kParts * kTileRows) {
           uint4 v = lds128(vt + i * 16);
           const uint4 n = make_uint4(not_finite(v.x), not_finite(v.y), not_finite(v.z), not_finite(v.w));
           if (n.x | n.y | n.z | n.w) {
@@ -605,146 +672,150 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      ok = mbar_wait(s_full + 8 * (st * SB + it % SB), (it / SB) & 1, stop, a.err);
-      // (these scores came after the values of step it - SB or earlier were added: of pv_done's
-      // two barriers, each has at most one phase open)
-      if (!__all_sync(0xffffffffu, ok)) break;
-      fence_after();
-      const uint32_t s_at = s_col + (it % SB) * KC, p_at = s_at + C::kPCol + mine / 2;
+      // (the scores of this step came after the values of step it - SB or earlier were added: of
+      // pv_done's two barriers, each has at most one phase open)
+      wait(s_full + 8 * (st * SB + it % SB), (it / SB) & 1);
+      const uint32_t s_at = s_col + (it % SB) * KC + mine;
+      const uint32_t p_at = C::kSep ? s_col + C::kPCol + mine / 2 : s_at;
+      const uint32_t added = pv_done + 8 * (2 * st + ((it - 1) & 1)), added_parity = ((it - 1) >> 1) & 1;
       if (warp_live) {
-        uint32_t x[W];
-#pragma unroll
-        for (int c = 0; c < W; c += 32) tmem_ld32(s_at + mine + c, x + c);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < W; c += 32) pin32(x + c);
-        if constexpr (C::kTwin) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_read);
+        // 32 scores at a time: with more of them they are read again for the exponentials
+        constexpr int kBlocks = W / 32;
+        uint32_t x[32];
+        float top = -INFINITY, bottom = INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < kBlocks; ++h) {
+          tmem_ld(s_at + 32 * h, x);
+          top = fmaxf(top, reduce<true>(x));
+          if (capped) bottom = fminf(bottom, reduce<false>(x));
         }
-        // `way` says what the exponent still has to do (see exps)
-        int way = capped ? 2 : 0;
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (capped) {
-          float mn[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
+        // `way` says what the exponent still has to do (see exps).  Almost every step of a long context
+        // is plain: all keys seen, no maximum grown, the cap's series good for all
+        int way = capped ? 1 : 0;
+        // the scores of block h as the exponent takes them: capped, with the distance, -inf where unseen
+        auto finish = [&](int h) {
+          const int x1 = x0 + mine + 32 * h;
+          if (capped) {
 #pragma unroll
-          for (int c = 0; c < W; c += 2) {
-            mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], x[c], x[c + 1]);
-            mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], x[c], x[c + 1]);
+            for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
           }
-          const float far = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                  -fminf(fminf(mn[0], mn[1]), fminf(mn[2], mn[3])));
-          if (free && !sloped && __all_sync(0xffffffffu, far <= cap.limit)) {
-            way = 1;
-          } else {
+          if (sloped) {
+            const float in = capped ? 1.f : lin;
+            if (free) {
+              const float away = (float)(pos - keys.key(x1));
 #pragma unroll
-            for (int c = 0; c < W; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
-          }
-        }
-        if (sloped) {
-          way = 2;
-          const float in = capped ? 1.f : lin;
-          if (free) {
-            const float away = (float)(pos - keys.key(x0 + mine));
+              for (int c = 0; c < 32; ++c)
+                x[c] = __float_as_uint(fmaf(-slope, fabsf(away - (float)c), __uint_as_float(x[c]) * in));
+            } else {
 #pragma unroll
-            for (int c = 0; c < W; ++c)
-              x[c] = __float_as_uint(fmaf(-slope, fabsf(away - (float)c), __uint_as_float(x[c]) * in));
-          } else {
-#pragma unroll
-            for (int c = 0; c < W; ++c)
-              x[c] = __float_as_uint(fmaf(-slope, fabsf((float)(pos - key_position(a, s, keys, x0 + mine + c))),
-                                          __uint_as_float(x[c]) * in));
-          }
-        }
-        if (!free) {
-          const uint64_t see = live ? seen_places(a, s, keys, tok, pos, x0 + mine, xend) : 0ull;
-#pragma unroll
-          for (int c = 0; c < W; ++c)
-            if (!(((uint32_t)(see >> (c & 32)) >> (c & 31)) & 1)) x[c] = 0xff800000u;  // -inf
-        }
-        if (way != 1) {
-          mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < W; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], x[c], x[c + 1]);
-        }
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        top = way == 0 ? top * lin : way == 1 ? cap.series(top) : top;
-        const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float mn = grow ? top : m;
-          const float al = grow ? fast_exp2(m - mn) : 1.f;
-          m = mn;
-          l *= al;
-          if (it > 0) {
-            ok = mbar_wait(pv_done + 8 * (2 * st + ((it - 1) & 1)), ((it - 1) >> 1) & 1, stop, a.err);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            fence_after();
-#pragma unroll
-            for (int c = 0; c < DH; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_col + c, o);
-              tmem_wait_ld();
-              pin32(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
-              tmem_st32(o_col + c, o);
+              for (int c = 0; c < 32; ++c)
+                x[c] = __float_as_uint(fmaf(-slope, fabsf((float)(pos - key_position(a, s, keys, x1 + c))),
+                                            __uint_as_float(x[c]) * in));
             }
           }
+          if (!free) {
+            const uint32_t see = live ? (uint32_t)seen_places(a, s, keys, tok, pos, x1, xend) : 0u;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!((see >> c) & 1)) x[c] = 0xff800000u;  // -inf
+          }
+        };
+        const bool special = any_part(!free || sloped || top > plain_top || bottom < plain_bottom);
+        if (special) {
+          way = capped || sloped ? 2 : 0;
+          top = -INFINITY;
+#pragma unroll 1
+          for (int h = 0; h < kBlocks; ++h) {
+            if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
+            finish(h);
+            top = fmaxf(top, reduce<true>(x));
+          }
+          if (way == 0) top *= lin;
+          if constexpr (C::kParts == 2) {
+            st32(mine_at, top);
+            any_part(false);
+            top = fmaxf(top, ld32(other_at));
+          }
+          const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+          // (the same for all threads of a row, and the barrier keeps `share` until all have read it)
+          if (any_part(grow)) {
+            const float mn = grow ? top : m;
+            const float al = grow ? fast_exp2(m - mn) : 1.f;
+            m = mn;
+            l *= al;
+            if (it > 0) {
+              wait(added, added_parity);
+#pragma unroll 1
+              for (int c = 0; c < kMyDims; c += 16) {
+                uint32_t o[16];
+                tmem_ld(o_col + c, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+                tmem_st(o_col + c, o);
+              }
+            }
+          }
+          // (tanh(u) <= u for u >= 0: a capped score grows past the limit only if s * lin does)
+          plain_top = !capped ? (m + 8.f) / lin : m + 8.f >= 0.f ? fminf((m + 8.f) / lin, cap.limit) : -INFINITY;
+        }
+        if constexpr (C::kSep) {  // the values of the step before have been added: p may be replaced
+          if (it > 0) wait(added, added_parity);
         }
         const float sub = m == -INFINITY ? 0.f : m;
-        float sum[4] = {};
-        uint32_t p[W / 2];
-        if (way == 0)
-          exps<0, W / 2>(x, p, lin, sub, cap, sum);
-        else if (way == 1)
-          exps<1, W / 2>(x, p, lin, sub, cap, sum);
-        else
-          exps<2, W / 2>(x, p, lin, sub, cap, sum);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if constexpr (C::kTwin) {  // the values of the step before have been added: p may be replaced
-          if (it > 0) ok = mbar_wait(pv_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, stop, a.err);
-          if (!__all_sync(0xffffffffu, ok)) break;
-          fence_after();
+#pragma unroll 1
+        for (int h = 0; h < kBlocks; ++h) {
+          if constexpr (kBlocks > 1) {
+            tmem_ld(s_at + 32 * h, x);
+            if (special) finish(h);
+          }
+          if constexpr (C::kSep) {
+            if (h == kBlocks - 1) {
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(s_read + 8 * st);
+            }
+          }
+          if (way == 0)
+            l += exps<0>(x, p_at + 16 * h, lin, sub, cap);
+          else if (way == 1)
+            l += exps<1>(x, p_at + 16 * h, lin, sub, cap);
+          else
+            l += exps<2>(x, p_at + 16 * h, lin, sub, cap);
         }
-        if constexpr (W == 64) tmem_st32(p_at, p); else tmem_st16(p_at, p);
         tmem_wait_st();
-      } else if (C::kTwin) {
-        if (lane == 0) mbar_arrive(s_read);
+      } else if (C::kSep) {
+        if (lane == 0) mbar_arrive(s_read + 8 * st);
         // (p_ready has one phase open at a time: not ahead of the other warps' step before)
-        if (it > 0) ok = mbar_wait(pv_done + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, stop, a.err);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        if (it > 0) wait(added, added_parity);
       }
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_ready + 8 * (st * SB + it % SB));
     }
-    if (ok && steps > 0)
-      ok = mbar_wait(pv_done + 8 * (2 * st + ((steps - 1) & 1)), ((steps - 1) >> 1) & 1, stop, a.err);
-    ok = __all_sync(0xffffffffu, ok);
-    fence_after();
-    asm volatile("bar.sync 1, %0;" ::"r"(ST * 128) : "memory");
+    if (steps > 0) wait(pv_done + 8 * (2 * st + ((steps - 1) & 1)), ((steps - 1) >> 1) & 1);
+    if constexpr (C::kParts == 2) {
+      st32(mine_at, l);
+      asm volatile("bar.sync 1, %0;" ::"r"(ST * C::kSoft * 32) : "memory");
+      l += ld32(other_at);
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(ST * C::kSoft * 32) : "memory");
     const int64_t part_row0 = ((((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split) * kCtaRows;
-    // the copies' parts: the second one's (m, l, O) through shared memory (all copies and MMAs have ended)
+    // the second copies' (m, l, O) through shared memory (all copies and MMAs have ended)
     float w0 = 1.f, w1 = 0.f;
-    const uint32_t meet = k_s + (t & 63) * 4;
+    const uint32_t meet = k_s + (t & 63) * 4, meet_o = meet + 512 + dim0 * 256;  // floats [value][row]
     if constexpr (C::kTwin) {
       if (t >= 64 && warp_live) {
         st32(meet, m);
         st32(meet + 256, l);
 #pragma unroll
-        for (int c = 0; c < DH; c += 32) {
+        for (int c = 0; c < kMyDims; c += 32) {
           uint32_t o[32] = {};
-          if (steps > 0) {
-            tmem_ld32(o_col + c, o);
-            tmem_wait_ld();
-            pin32(o);
-          }
+          if (steps > 0) tmem_ld(o_col + c, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) st32(meet + 512 + (c + e) * 256, __uint_as_float(o[e]));
+          for (int e = 0; e < 32; ++e) st32(meet_o + (c + e) * 256, __uint_as_float(o[e]));
         }
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"r"(ST * C::kSoft * 32) : "memory");
       if (t < 64 && warp_live) {
         const float m1 = ld32(meet), l1 = ld32(meet + 256), top = fmaxf(m, m1), sub = top == -INFINITY ? 0.f : top;
         w0 = fast_exp2(m - sub);
@@ -755,52 +826,82 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     }
     if (*stop) {
     } else if (*odd) {
-      rows_by_key<DH>(a, s, keys, table, g, r0, nr, xbeg, xend, part_row0, warp, 4 * ST);
+      rows_by_key<DH>(a, s, keys, table, g, r0, nr, xbeg, xend, part_row0, warp, C::kSoft * ST);
     } else if (warp_live && (!C::kTwin || t < 64)) {
-      // ---- a thread writes its row
+      // ---- the warp's rows through its share of the Q tile, so that whole lines are written
       const float inv = l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst =
-          static_cast<__nv_bfloat16*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * DH;
-      float* po = a.part_o + (part_row0 + r) * DH;
-      if (a.n_splits > 1 && live)
+          static_cast<__nv_bfloat16*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * DH + dim0;
+      if (a.n_splits > 1 && live && part == 0)
         *reinterpret_cast<float2*>(a.part_ml + (part_row0 + r) * 2) = make_float2(m, l);
-#pragma unroll
-      for (int c = 0; c < DH; c += 32) {
-        uint32_t o[32] = {};
-        if (steps > 0) {
-          tmem_ld32(o_col + c, o);
-          tmem_wait_ld();
-          pin32(o);
-        }
+      constexpr int kPitch = kMyDims * 2, kPieces = kPitch / 16;  // bytes and 16-byte pieces of a row
+      const uint32_t stage = q_s + warp * 32 * kPitch;
+      auto piece = [&](int row, int c) {
+        return stage + row * kPitch + ((kPieces >= 8 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4);
+      };
+      // the sums of 16 dimensions
+      auto sums = [&](int c, uint32_t (&o)[16]) {
+        if (steps > 0)
+          tmem_ld(o_col + c, o);
+        else
+          for (int e = 0; e < 16; ++e) o[e] = 0u;
         if constexpr (C::kTwin) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            // (a copy without a key has sums of 0, its m - sub may be -inf)
-            const float v = __uint_as_float(o[e]) * w0, u = ld32(meet + 512 + (c + e) * 256) * w1;
-            o[e] = __float_as_uint(v + u);
+          for (int e = 0; e < 16; ++e)
+            o[e] = __float_as_uint(__uint_as_float(o[e]) * w0 + ld32(meet_o + (c + e) * 256) * w1);
+        }
+      };
+      // rows that are read back: 32 / kPieces at once
+      const int back = lane / kPieces, c_back = lane % kPieces;
+      if (a.n_splits == 1) {
+#pragma unroll
+        for (int c = 0; c < kMyDims; c += 16) {
+          uint32_t o[16], w[8];
+          sums(c, o);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[e] = l == 0.f ? 0u : pack2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          sts128(piece(lane, c / 8), make_uint4(w[0], w[1], w[2], w[3]));
+          sts128(piece(lane, c / 8 + 1), make_uint4(w[4], w[5], w[6], w[7]));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int row = i * (32 / kPieces) + back;
+          __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+          if (!__shfl_sync(0xffffffffu, (int)live, row)) continue;
+          const uint4 v = lds128(piece(row, c_back));
+          if (vec) {
+            *reinterpret_cast<uint4*>(to + c_back * 8) = v;
+          } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            for (int e = 0; e < 4; ++e) {
+              to[c_back * 8 + 2 * e] = __ushort_as_bfloat16((unsigned short)(w[e] & 0xffffu));
+              to[c_back * 8 + 2 * e + 1] = __ushort_as_bfloat16((unsigned short)(w[e] >> 16));
+            }
           }
         }
-        if (!live) continue;
-        if (a.n_splits > 1) {
+      } else {
+        float* po = a.part_o + (part_row0 + r - lane) * DH + dim0;  // of the warp's first row
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(po + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          continue;
-        }
-        uint32_t w[16];
+        for (int half = 0; half < kMyDims; half += kMyDims / 2) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          w[e] = l == 0.f ? 0u : pack2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-        if (vec) {
+          for (int c = 0; c < kMyDims / 2; c += 16) {
+            uint32_t o[16];
+            sums(half + c, o);
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<uint4*>(dst + c + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            dst[c + 2 * e] = __ushort_as_bfloat16((unsigned short)(w[e] & 0xffffu));
-            dst[c + 2 * e + 1] = __ushort_as_bfloat16((unsigned short)(w[e] >> 16));
+            for (int e = 0; e < 16; e += 4)
+              sts128(piece(lane, (c + e) / 4), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
           }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            const int row = i * (32 / kPieces) + back;
+            if (__shfl_sync(0xffffffffu, (int)live, row))
+              *reinterpret_cast<uint4*>(po + (int64_t)row * DH + half + c_back * 4) = lds128(piece(row, c_back));
+          }
+          __syncwarp();
         }
       }
     }
