@@ -261,6 +261,13 @@ struct Cap {
     d4 = d0 * (0.0127505842f * kk * kk * kk * kk);
     limit = k <= 1024.f ? 0.75f / k : -1.f;  // (k^8 stays within float32)
   }
+  __device__ __forceinline__ uint64_t series(uint64_t v) const {
+    const uint64_t w = mul2(v, v);
+    uint64_t c = fma2(w, twice(d4), twice(d3));
+    c = fma2(w, c, twice(d2));
+    c = fma2(w, c, twice(d1));
+    return mul2(v, fma2(w, c, twice(d0)));
+  }
   __device__ __forceinline__ float exact(float s) const {
     return fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(s * in)), cap2);
   }
@@ -692,12 +699,23 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
         // `way` says what the exponent still has to do (see exps).  Almost every step of a long context
         // is plain: all keys seen, no maximum grown, the cap's series good for all
         int way = capped ? 1 : 0;
+        bool far = false;  // some score is beyond the cap's series
         // the scores of block h as the exponent takes them: capped, with the distance, -inf where unseen
         auto finish = [&](int h) {
           const int x1 = x0 + mine + 32 * h;
           if (capped) {
+            if (far) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
+              for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
+            } else {
+#pragma unroll
+              for (int c = 0; c < 32; c += 2) {
+                float lo, hi;
+                unpair(cap.series(pair(x[c], x[c + 1])), lo, hi);
+                x[c] = __float_as_uint(lo);
+                x[c + 1] = __float_as_uint(hi);
+              }
+            }
           }
           if (sloped) {
             const float in = capped ? 1.f : lin;
@@ -720,15 +738,21 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
               if (!((see >> c) & 1)) x[c] = 0xff800000u;  // -inf
           }
         };
-        const bool special = any_part(!free || sloped || top > plain_top || bottom < plain_bottom);
-        if (special) {
-          way = capped || sloped ? 2 : 0;
-          top = -INFINITY;
+        bool finished = false;
+        if (any_part(!free || sloped || top > plain_top || bottom < plain_bottom)) {
+          if (capped) far = any_part(!(top <= cap.limit && bottom >= -cap.limit));
+          if (!free || sloped || far) {
+            finished = true;
+            way = capped || sloped ? 2 : 0;
+            top = -INFINITY;
 #pragma unroll 1
-          for (int h = 0; h < kBlocks; ++h) {
-            if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
-            finish(h);
-            top = fmaxf(top, reduce<true>(x));
+            for (int h = 0; h < kBlocks; ++h) {
+              if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
+              finish(h);
+              top = fmaxf(top, reduce<true>(x));
+            }
+          } else if (capped) {
+            top = cap.exact(top);
           }
           if (way == 0) top *= lin;
           if constexpr (C::kParts == 2) {
@@ -766,7 +790,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
         for (int h = 0; h < kBlocks; ++h) {
           if constexpr (kBlocks > 1) {
             tmem_ld(s_at + 32 * h, x);
-            if (special) finish(h);
+            if (finished) finish(h);
           }
           if constexpr (C::kSep) {
             if (h == kBlocks - 1) {
