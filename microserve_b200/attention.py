@@ -75,22 +75,22 @@ class AttentionForm:
         return _lib.MsAttentionForm(*self.fields(index, n_heads, batch))
 
 
-def pack_batch(batch: PagedBatch, index: int) -> bytes:
-    """``ms_batch`` of a batch, its arrays checked (the token arrays may be absent here)."""
+def pack_batch(batch: PagedBatch, index: int, tokens: bool = False) -> bytes:
+    """``ms_batch`` of a batch, its arrays checked; ``tokens``: with its token ids (attention
+    reads none, nor the slots)."""
     T, B = batch.n_tokens, batch.q_lens.numel()
     i32 = torch.int32
     tables = batch.block_tables
-    if tables.dim() != 2:
+    shape = tables.shape
+    if len(shape) != 2:
         raise ValueError("block_tables must be (B, max_blocks)")
-    width = tables.shape[1]
     return _PACK_BATCH(
-        T, B, width, batch.max_q, batch.max_context, 0,
-        _check(batch.input_ids, "input_ids", i32, index, (T,)),
-        _check(batch.positions, "positions", i32, index, (T,)),
-        _check(batch.slot_mapping, "slot_mapping", i32, index, (T,)),
+        T, B, shape[1], batch.max_q, batch.max_context, 0,
+        _check(batch.input_ids, "input_ids", i32, index, (T,)) if tokens else 0,
+        _check(batch.positions, "positions", i32, index, (T,)), 0,
         _check(batch.q_start, "q_start", i32, index, (B + 1,)),
         _check(batch.context_lens, "context_lens", i32, index, (B,)),
-        _check(tables, "block_tables", i32, index, (B, width)))
+        _check(tables, "block_tables", i32, index, (B, shape[1])))
 
 
 def _heads(t: torch.Tensor, name: str, index: int, dtype: torch.dtype, n_tokens: int, heads: int,
@@ -120,16 +120,16 @@ def paged_attention(
     projection); ``out`` too, and it must not overlap ``q`` or the pools.  A query that sees no
     key gives 0.  float32 or bfloat16, d_head 8, 16, 32, 64 or 128."""
     index = _lib.cuda_index(q)
-    if q.dim() != 3 or k_pool.dim() != 4:
+    q_shape, shape = q.shape, k_pool.shape
+    if len(q_shape) != 3 or len(shape) != 4:
         raise ValueError("q must be (T, n_heads, d_head) and a pool (blocks, n_kv_heads, block_size, d_head)")
-    T, heads, dh = q.shape
+    T, heads, dh = q_shape
     dt = q.dtype
     code = _CODES.get(dt)
     if code is None:
         raise ValueError(f"q must be float32 or bfloat16, got {dt}")
     if batch.n_tokens != T:
         raise ValueError(f"q has {T} tokens, the batch {batch.n_tokens}")
-    shape = k_pool.shape
     blocks, hkv, block, pool_dh = shape
     pointers = (c_void_p * 2)(_check(k_pool, "k_pool", dt, index, shape),
                               _check(v_pool, "v_pool", dt, index, shape))
@@ -137,7 +137,7 @@ def paged_attention(
         raise ValueError(f"q has {heads} heads of {dh}, the pools {hkv} of {pool_dh}")
     q_stride = _heads(q, "q", index, dt, T, heads, dh)
     if out is None:
-        out = torch.empty((T, heads, dh), dtype=dt, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         out_stride = heads * dh
     else:
         out_stride = _heads(out, "out", index, dt, T, heads, dh)
@@ -149,7 +149,7 @@ def paged_attention(
     cb = pack_batch(batch, index)
     cf = None if form is None else _PACK_FORM(*form.fields(index, heads, batch))
     need = (_lib._lib or _lib.load()).ms_attention_form_workspace_size(cache, heads, cb, cf)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _lib.launch_on(index, "ms_paged_attention_form", q.data_ptr(), q_stride, cache, 0, cb, heads, cf,
                    out.data_ptr(), out_stride, None if ws is None else ws.data_ptr(), need)
     return out

@@ -3,30 +3,44 @@
 // matrix kernels do not take) and the joining of KV ranges.
 #include <cfloat>
 
-#include "attention_form.cuh"
+#include "attention_form_device.cuh"
 #include "model_kernels.cuh"
 
 namespace ms {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kChunk = 32;
 template <int DH> constexpr int rows_per_warp() { return DH <= 64 ? 4 : 2; }
+// Keys per step: as many as 48 KB hold beside the queries (a step costs a round trip to memory).
+template <int DH> constexpr int step_keys() { return DH <= 32 ? 128 : DH == 64 ? 64 : 32; }
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u),
+                       __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+  }
+}
 
 // One CTA per (row tile, KV range, kv head, sequence); row r of a tile is
-// (token r / group, head-in-group r % group).  32 keys at a time in shared
-// memory, a lane a key for the scores and a dimension for the sums; online
-// softmax in base e, everything in float32.
+// (token r / group, head-in-group r % group).  A step's keys in shared memory (rows
+// padded by 4 floats: the lanes of a quarter warp read 16 bytes each from different
+// banks), a lane a key for the scores and a dimension for the sums; online softmax in base
+// e, everything in float32.  The small models that take this kernel are bound by latency:
+// 8 trees of 7 tokens, 4 heads of 32, contexts up to 97: 14.2 us with 32 keys a step.
 template <typename T, int DH>
 __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
   pdl_enter();
   constexpr int PER_LANE = DH >= 32 ? DH / 32 : 1;
   constexpr int RPW = rows_per_warp<DH>();
   constexpr int ROWS = kWarps * RPW;
-  __shared__ float Qs[ROWS][DH];
-  __shared__ float Ks[kChunk][DH + 1];
-  __shared__ float Vs[kChunk][DH];
-  __shared__ int s_min, s_max;
+  constexpr int CK = step_keys<DH>(), SUB = CK / 32, LD = DH + 4;
+  __shared__ __align__(16) float Qs[ROWS * DH];
+  __shared__ __align__(16) float Ks[CK * LD];
+  __shared__ __align__(16) float Vs[CK * DH];
 
   const int b = blockIdx.z, g = blockIdx.y;
   const int split = blockIdx.x % a.n_splits, tile = blockIdx.x / a.n_splits;
@@ -35,25 +49,15 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
   if (r0 >= nrows) return;
   const int nr = min(ROWS, nrows - r0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
-    s_min = INT_MAX;
-    s_max = INT_MIN;
-  }
-  __syncthreads();
+  int minpos, maxpos;
+  position_range(a, s, r0, nr, minpos, maxpos);
   const T* q = static_cast<const T*>(a.q);
-  for (int idx = threadIdx.x; idx < ROWS * DH; idx += blockDim.x) {
+  for (int idx = threadIdx.x; idx < nr * DH; idx += blockDim.x) {
     const int r = idx / DH, d = idx - r * DH, rr = r0 + r;
-    Qs[r][d] = r < nr ? to_f(q[(int64_t)(s.t0 + rr / a.group) * a.q_stride +
-                               (int64_t)(g * a.group + rr % a.group) * DH + d])
-                      : 0.f;
+    Qs[idx] = to_f(q[(int64_t)(s.t0 + rr / a.group) * a.q_stride +
+                     (int64_t)(g * a.group + rr % a.group) * DH + d]);
   }
-  for (int r = threadIdx.x; r < nr; r += blockDim.x) {
-    const int p = a.positions[s.t0 + (r0 + r) / a.group];
-    atomicMin(&s_min, p);
-    atomicMax(&s_max, p);
-  }
-  __syncthreads();
-  const FormKeys keys = form_keys(a, s, s_min, s_max);
+  const FormKeys keys = form_keys(a, s, minpos, maxpos);
   const int xbeg = min(split * a.split_len, keys.total);
   const int xend = split == a.n_splits - 1 ? keys.total : min(keys.total, xbeg + a.split_len);
 
@@ -74,54 +78,81 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
   const T *kp = static_cast<const T*>(a.k), *vp = static_cast<const T*>(a.v);
   const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
   const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
-  for (int x0 = xbeg; x0 < xend; x0 += kChunk) {
+  // (rows of 4 values are aligned to them where the pools are)
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) == 0;
+  for (int x0 = xbeg; x0 < xend; x0 += CK) {
+    const int n = min(CK, xend - x0);
     __syncthreads();
-    for (int idx = threadIdx.x; idx < kChunk * DH; idx += blockDim.x) {
-      const int kk = idx / DH, d = idx - kk * DH;
-      float kv = 0.f, vv = 0.f;
-      if (x0 + kk < xend) {
-        const int j = keys.key(x0 + kk);
-        const int64_t o =
-            (((int64_t)form_block(a, table, j / a.bs) * a.hkv + g) * a.bs + (j % a.bs)) * DH + d;
-        kv = to_f(kp[o]);
-        vv = to_f(vp[o]);
+#pragma unroll 4
+    for (int idx = threadIdx.x; idx < n * (DH / 4); idx += kWarps * 32) {
+      const int kk = idx / (DH / 4), d = (idx - kk * (DH / 4)) * 4, j = keys.key(x0 + kk);
+      const int64_t o = (((int64_t)form_block(a, table, j / a.bs) * a.hkv + g) * a.bs + (j % a.bs)) * DH + d;
+      float4 kv, vv;
+      if (vec) {
+        kv = load4(kp + o);
+        vv = load4(vp + o);
+      } else {
+        kv = make_float4(to_f(kp[o]), to_f(kp[o + 1]), to_f(kp[o + 2]), to_f(kp[o + 3]));
+        vv = make_float4(to_f(vp[o]), to_f(vp[o + 1]), to_f(vp[o + 2]), to_f(vp[o + 3]));
       }
-      Ks[kk][d] = kv;
-      Vs[kk][d] = vv;
+      *reinterpret_cast<float4*>(Ks + kk * LD + d) = kv;
+      *reinterpret_cast<float4*>(Vs + kk * DH + d) = vv;
     }
     __syncthreads();
-    const int j = keys.key(x0 + lane);
-    const bool in = x0 + lane < xend;
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
       const int r = warp + i * kWarps;
       if (r >= nr) continue;
-      float x = 0.f;
+      float x[SUB];
+      uint32_t seen[SUB];
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        seen[u] = 0;
+        if (u * 32 >= n) continue;
+        const int kk = u * 32 + lane;
+        // (keys behind the last one are rows of an earlier step, or never written: not seen)
+        float v = 0.f;
+        const float4* kr = reinterpret_cast<const float4*>(Ks + kk * LD);
+        const float4* qr = reinterpret_cast<const float4*>(Qs + r * DH);
 #pragma unroll 8
-      for (int d = 0; d < DH; ++d) x = fmaf(Qs[r][d], Ks[lane][d], x);
-      int distance = 0;
-      const bool seen = in && form_sees(a, s, tok[i], pos[i], j, distance);
-      x = a.softcap > 0.f ? a.softcap * tanhf(x * inv_cap) : x * a.scale;
-      if (a.slopes) x -= slope[i] * fabsf((float)distance);
-      x = seen ? x : -INFINITY;
-      const uint32_t seen_mask = __ballot_sync(0xffffffffu, seen);
-      if (seen_mask == 0) continue;
-      const float mn = fmaxf(m[i], warp_max(x));
+        for (int d = 0; d < DH / 4; ++d) {
+          const float4 k4 = kr[d], q4 = qr[d];
+          v = fmaf(q4.x, k4.x, v);
+          v = fmaf(q4.y, k4.y, v);
+          v = fmaf(q4.z, k4.z, v);
+          v = fmaf(q4.w, k4.w, v);
+        }
+        int distance = 0;
+        const bool sees = kk < n && form_sees(a, s, tok[i], pos[i], keys.key(x0 + min(kk, n - 1)), distance);
+        v = a.softcap > 0.f ? a.softcap * tanhf(v * inv_cap) : v * a.scale;
+        if (a.slopes) v -= slope[i] * fabsf((float)distance);
+        x[u] = sees ? v : -INFINITY;
+        seen[u] = __ballot_sync(0xffffffffu, sees);
+        top = fmaxf(top, x[u]);
+      }
+      const float mn = fmaxf(m[i], warp_max(top));
       const float sub = mn == -INFINITY ? 0.f : mn;
       const float alpha = m[i] == -INFINITY ? 0.f : expf(m[i] - sub);
-      const float p = seen ? expf(x - sub) : 0.f;
-      l[i] = l[i] * alpha + warp_sum(p);
+      m[i] = mn;
+      float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < PER_LANE; ++e) acc[i][e] *= alpha;
-#pragma unroll 4
-      for (int kk = 0; kk < kChunk; ++kk) {
-        const float pk = __shfl_sync(0xffffffffu, p, kk);
-        if (!((seen_mask >> kk) & 1)) continue;  // an unseen value may be anything
 #pragma unroll
-        for (int e = 0; e < PER_LANE; ++e)
-          if (DH >= 32 || lane < DH) acc[i][e] = fmaf(pk, Vs[kk][lane + 32 * e], acc[i][e]);
+      for (int u = 0; u < SUB; ++u) {
+        if (seen[u] == 0) continue;
+        const float p = (seen[u] >> lane) & 1 ? expf(x[u] - sub) : 0.f;
+        sum += p;
+        const float* vr = Vs + u * 32 * DH + (DH >= 32 ? lane : lane % DH);
+#pragma unroll 8
+        for (int kk = 0; kk < 32; ++kk) {
+          const float pk = __shfl_sync(0xffffffffu, p, kk);
+          if (!((seen[u] >> kk) & 1)) continue;  // an unseen value may be anything
+#pragma unroll
+          for (int e = 0; e < PER_LANE; ++e) acc[i][e] = fmaf(pk, vr[kk * DH + 32 * e], acc[i][e]);
+        }
       }
-      m[i] = mn;
+      l[i] = l[i] * alpha + warp_sum(sum);
     }
   }
 #pragma unroll
@@ -218,11 +249,11 @@ Way choose(FormArgs& a, const ms_kv_cache& c, int max_context) {
   const int64_t rows = (int64_t)a.max_q * a.group;
   if (!form_tma_takes(c)) {
     const Way w{kSimt, simt_rows(c.d_head)};
-    plan(a, max_context, w.rows, kChunk, 128, 148 * 4);
+    plan(a, max_context, w.rows, 128, 256, 148 * 4);
     return w;
   }
   if (rows <= 32) {
-    plan(a, max_context, 64, 64, 256, 148 * 4);
+    plan(a, max_context, 64, 64, 512, 148 * 4);
     return {kTma, 64};
   }
   const int tile = rows > 128 ? 256 : rows > 64 ? 128 : 64;

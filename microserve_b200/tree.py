@@ -96,13 +96,15 @@ def accept_trees(target: torch.Tensor, batch: PagedBatch, parents: torch.Tensor,
         logits = target.data_ptr()
     else:
         tokens = _check(target, "target tokens", torch.int32, index, (T,))
-    cb = pack_batch(batch, index)
+    cb = pack_batch(batch, index, True)
     p = _check(parents, "parents", torch.int32, index, (T,))
     # one allocation: tokens, nodes, sources, destinations, counts
     A = max_accept
-    flat = torch.empty(B * (4 * A + 2), dtype=torch.int32, device=target.device)
-    said, nodes, src, dst, num = flat.split((B * (A + 1), B * A, B * A, B * A, B))
-    out = TreeAccept(said.view(B, A + 1), num, nodes.view(B, A), src.view(B, A), dst.view(B, A))
+    flat = parents.new_empty(B * (4 * A + 2))
+    view, o, rows = flat.as_strided, flat.storage_offset(), (A, 1)
+    out = TreeAccept(view((B, A + 1), (A + 1, 1), o), view((B,), (1,), o + B * (4 * A + 1)),
+                     view((B, A), rows, o + B * (A + 1)), view((B, A), rows, o + B * (2 * A + 1)),
+                     view((B, A), rows, o + B * (3 * A + 1)))
     if B:
         at = flat.data_ptr()
         _lib.launch_on(index, "ms_tree_accept", logits or None, stride, vocab, tokens or None, cb,
