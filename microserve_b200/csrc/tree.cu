@@ -92,7 +92,7 @@ __device__ __forceinline__ Best better(Best a, Best b) {
 
 // The best of x[lo, hi): 16 bytes at a time from the first aligned element on.
 __device__ __forceinline__ Best best_of(const float* x, int lo, int hi) {
-  constexpr int kUnroll = 8;
+  constexpr int kUnroll = 16;
   Best m{-INFINITY, INT_MAX};
   const int tid = threadIdx.x;
   const int head = min(hi, lo + (int)((4 - ((reinterpret_cast<uintptr_t>(x + lo) >> 2) & 3)) & 3));
