@@ -90,14 +90,19 @@ __device__ __forceinline__ Best better(Best a, Best b) {
   return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a;
 }
 
-// The best of x[lo, hi): 16 bytes at a time from the first aligned element on.
+// The best of x[lo, hi): 16 bytes at a time from the first aligned element on.  A thread's
+// indices ascend, so only a larger value replaces its best; of four values their maximum
+// is compared first (a row of -inf or NaN leaves the index at INT_MAX).
 __device__ __forceinline__ Best best_of(const float* x, int lo, int hi) {
-  constexpr int kUnroll = 16;
+  constexpr int kUnroll = 4;
   Best m{-INFINITY, INT_MAX};
   const int tid = threadIdx.x;
   const int head = min(hi, lo + (int)((4 - ((reinterpret_cast<uintptr_t>(x + lo) >> 2) & 3)) & 3));
   const int quads = (hi - head) >> 2;
-  if (tid < head - lo) m = better(m, Best{x[lo + tid], lo + tid});
+  auto take = [&](float v, int i) {
+    if (v > m.v) m = Best{v, i};
+  };
+  if (tid < head - lo) take(x[lo + tid], lo + tid);
   const float4* x4 = reinterpret_cast<const float4*>(x + head);
   for (int q0 = tid; q0 < quads; q0 += kUnroll * kTreeThreads) {
     float4 v[kUnroll];
@@ -107,17 +112,17 @@ __device__ __forceinline__ Best best_of(const float* x, int lo, int hi) {
                                            : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (q0 + u * kTreeThreads >= quads) break;
-      const int i = head + 4 * (q0 + u * kTreeThreads);
-      // a thread's indices ascend, so only a larger value (or the first -inf) replaces
-      m = better(m, Best{v[u].x, i});
-      m = better(m, Best{v[u].y, i + 1});
-      m = better(m, Best{v[u].z, i + 2});
-      m = better(m, Best{v[u].w, i + 3});
+      if (fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w)) > m.v) {
+        const int i = head + 4 * (q0 + u * kTreeThreads);
+        take(v[u].x, i);
+        take(v[u].y, i + 1);
+        take(v[u].z, i + 2);
+        take(v[u].w, i + 3);
+      }
     }
   }
   const int tail = head + 4 * quads + tid;
-  if (tail < hi) m = better(m, Best{x[tail], tail});
+  if (tail < hi) take(x[tail], tail);
   return m;
 }
 
