@@ -50,11 +50,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
   return true;
 }
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+// `row`: the first of the box's rows (a multiple of 8) of a pool's map (form_pool_map).
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %3, %3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(row >> 3)
       : "memory");
 }
 // 2^x by the SFU (ftz; 2^-inf = 0): 2 ulp of a result that is rounded to bf16 next.
@@ -158,7 +159,11 @@ __device__ __forceinline__ int key_position(const FormArgs& a, const FormSeq& s,
   return a.mask && node >= 0 ? a.positions[s.t0 + min(node, s.qlen - 1)] : j;
 }
 
-// attention_form_tma.cu: the pool as [rows][dh] bf16, boxes of 64 columns x `box` rows, 128-byte swizzle.
+// attention_form_tma.cu: the pool's rows of dh bf16 as (64 columns, 8 rows, dh / 64 column blocks, groups of
+// 8 rows), boxes of `box` rows with the 128-byte swizzle: a whole page in one copy, of which a
+// group of 8 rows fills dh / 64 swizzle atoms of 1024 bytes, one behind the other.  (A copy of 2
+// KB costs 73 cycles of an SM's copy unit, one of 4 KB 96: with a copy for each column block
+// the unit's 28 bytes a cycle were the bound.)
 int form_pool_map(const void* pool, int64_t rows, int dh, int box, CUtensorMap* out);
 
 }  // namespace ms

@@ -9,7 +9,7 @@
 //        2^(x - m) rounded to bf16 back into TMEM over the scores, and the sum of the
 //        rounded values.  m is raised only when a row's maximum has grown by
 //        more than 2^8, so O is rescaled a few times a row at most;
-//   producer warp  TMA loads of whole pages (or parts of one), a box a lane, into
+//   producer warp  TMA loads of whole pages (or parts of one), a lane a page, into
 //        rings of their own for K and V;
 //   MMA warp  one thread issues S = Q K^T (both from shared memory) and O += P V (P in
 //        TMEM, V MN-major as it lies in the page).  With SB score buffers the
@@ -62,13 +62,13 @@ struct TcCfg {
   static_assert(!kTwin || 64 * DH * 4 + 64 * 8 <= NK * kTile, "the copies meet in the K ring");
 };
 
-// Descriptors with the 128-byte swizzle.  K-major (Q, K): rows of 64 values, 8-row
-// groups 1024 bytes apart.  MN-major (V): 64 dimensions a row, groups of 8 keys
-// 1024 bytes apart, blocks of 64 dimensions `lead` bytes apart.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+// Descriptors with the 128-byte swizzle: atoms of 8 rows x 128 bytes, groups of 8 rows `stride` bytes
+// apart.  K-major (Q, K): rows of 64 values (`lead` not used).  MN-major (V): 64 dimensions a row,
+// blocks of 64 dimensions `lead` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
   uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);
   d |= (uint64_t)(lead >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)(stride >> 4) << 32;
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
@@ -454,10 +454,8 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     if constexpr (ST == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == kProducer) {
       // ---- loads
-      constexpr int kHalves = DH / 64;
-      static_assert(KC / 8 * kHalves <= 32, "a lane for each box");
-      const int box = min(a.bs, KC), boxes = KC / box;
-      const int i = lane / kHalves, half = lane % kHalves;
+      static_assert(KC / 8 <= 32, "a lane for each box");
+      const int box = min(a.bs, KC), boxes = KC / box, i = lane;
       auto row_of = [&](int step) {  // the pool row of this lane's box (-1: none)
         const int x = xbeg + step * KC + i * box;
         if (i >= boxes || x >= xend) return -1;
@@ -469,19 +467,19 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
         const int row = next;
         if (it + 1 < steps) next = row_of(it + 1);
         const int n = (min(KC, xend - (xbeg + it * KC)) + box - 1) / box;
-        const uint32_t bytes = (uint32_t)(n * box * DH * 2), off = half * (KC * 128) + i * box * 128;
+        const uint32_t bytes = (uint32_t)(n * box * DH * 2), off = i * box * DH * 2;
         const int ks = it % NK, vs = it % NV;
         bool ok = it < NK || mbar_wait(k_empty + 8 * ks, (it / NK - 1) & 1, stop, a.err);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) mbar_expect_tx(k_full + 8 * ks, bytes);
         __syncwarp();
-        if (row >= 0) tma_load_2d(k_s + ks * C::kTile + off, &kmap, k_full + 8 * ks, half * 64, row);
+        if (row >= 0) tma_load_rows(k_s + ks * C::kTile + off, &kmap, k_full + 8 * ks, row);
         ++k_issued;
         ok = it < NV || mbar_wait(v_empty + 8 * vs, (it / NV - 1) & 1, stop, a.err);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) mbar_expect_tx(v_full + 8 * vs, bytes);
         __syncwarp();
-        if (row >= 0) tma_load_2d(v_s + vs * C::kTile + off, &vmap, v_full + 8 * vs, half * 64, row);
+        if (row >= 0) tma_load_rows(v_s + vs * C::kTile + off, &vmap, v_full + 8 * vs, row);
         ++v_issued;
       }
       if (*stop) {  // a block that gave up still waits for its loads in flight
@@ -503,22 +501,23 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       };
       auto scores = [&](int it, int st) {
         const uint32_t d = cols + st * C::kStreamCols + (it % SB) * KC;
-        const uint64_t qd = smem_desc(q_s + st * C::kQ, 16), kd = smem_desc(k_s + (it % NK) * C::kTile, 16);
+        const uint64_t qd = smem_desc(q_s + st * C::kQ, 16, 1024);
+        const uint64_t kd = smem_desc(k_s + (it % NK) * C::kTile, 16, DH * 16);
 #pragma unroll
         for (int k = 0; k < DH / 16; ++k)
           mma_ss(d, qd + (k >> 2) * (kTileRows * 128 / 16) + (k & 3) * 2,
-                 kd + (k >> 2) * (KC * 128 / 16) + (k & 3) * 2, id_s, k > 0, one);
+                 kd + (k >> 2) * (1024 / 16) + (k & 3) * 2, id_s, k > 0, one);
         mma_commit(s_full + 8 * (st * SB + it % SB), one);
       };
       auto add_values = [&](int it, int st) {
         const uint32_t o = cols + st * C::kStreamCols + C::kOCol;
         const uint32_t p = cols + st * C::kStreamCols + C::kPCol + (it % SB) * KC;
-        const uint64_t vd = smem_desc(v_s + (it % NV) * C::kTile, KC * 128);
+        const uint64_t vd = smem_desc(v_s + (it % NV) * C::kTile, 1024, DH * 16);
 #pragma unroll
         for (int k = 0; k < KC / 16; ++k) {
           // over the scores, each part's p starts where its scores did
           const int at = C::kSep ? 8 * k : 8 * (k % (W / 16)) + k / (W / 16) * W;
-          mma_ts(o, p + at, vd + k * (2048 / 16), id_o, it > 0 || k > 0, one);
+          mma_ts(o, p + at, vd + k * (2 * DH * 16 / 16), id_o, it > 0 || k > 0, one);
         }
         mma_commit(pv_done + 8 * (2 * st + (it & 1)), one);
       };
@@ -673,7 +672,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           uint4 v = lds128(vt + i * 16);
           const uint4 n = make_uint4(not_finite(v.x), not_finite(v.y), not_finite(v.z), not_finite(v.w));
           if (n.x | n.y | n.z | n.w) {
-            if (x0 + (i >> 3) % KC < xend) *odd = 1;
+            if (x0 + (i >> 6) / (DH / 64) * 8 + ((i >> 3) & 7) < xend) *odd = 1;
             sts128(vt + i * 16, make_uint4(v.x & ~n.x, v.y & ~n.y, v.z & ~n.z, v.w & ~n.w));
           }
         }

@@ -5,7 +5,7 @@
 // (token r / group, head-in-group r % group), so that keys and values are
 // read once per kv head.
 //   producer warp   TMA loads of each chunk of 64 places (whole pages or parts
-//                   of one) into a ring, one box a lane;
+//                   of one) into a ring, a lane a page;
 //   consumer warps  one for each 16 rows: S = Q K^T and O += P V by mma.sync
 //                   m16n8k16, online softmax in base 2 in float32.  P enters the
 //                   second product rounded to bf16 (its operand type); the sum
@@ -52,9 +52,10 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 16-byte chunk c of key row k in a tile of 64-column halves, 128-byte swizzle.
+// 16-byte chunk c of key row k in a tile (see form_pool_map).
+template <int DH>
 __device__ __forceinline__ uint32_t tile_addr(uint32_t tile, int k, int c) {
-  return tile + (uint32_t)((c >> 3) * (kCh * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4));
+  return tile + (uint32_t)((k >> 3) * (DH * 16) + (c >> 3) * 1024 + (k & 7) * 128 + (((c & 7) ^ (k & 7)) << 4));
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
@@ -104,11 +105,10 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
   __syncthreads();
 
   if (warp == MT) {
-    // ---- producer: lane l loads box l / (2 * DH / 64) of the chunk, K or V, a half of its columns
-    constexpr int kPer = 2 * DH / 64;
-    static_assert(kCh / 8 * kPer <= 32, "a lane for each box");
+    // ---- producer: lane l loads box l / 2 of the chunk, K or V
+    static_assert(kCh / 8 * 2 <= 32, "a lane for each box");
     const int box = min(a.bs, kCh), boxes = kCh / box;
-    const int i = lane / kPer, half = lane % (DH / 64), is_v = (lane / (DH / 64)) & 1;
+    const int i = lane / 2, is_v = lane & 1;
     const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
     auto row_of = [&](int chunk) {  // the pool row of this lane's box (-1: none)
       const int x = xbeg + chunk * kCh + i * box;
@@ -127,8 +127,8 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
       if (lane == 0) mbar_expect_tx(full + 8 * slot, (uint32_t)(n * box * DH * 2 * 2));
       __syncwarp();
       if (row >= 0) {
-        const uint32_t dst = ring + slot * 2 * C::kTile + is_v * C::kTile + half * (kCh * 128) + i * box * 128;
-        tma_load_2d(dst, is_v ? &vmap : &kmap, full + 8 * slot, half * 64, row);
+        const uint32_t dst = ring + slot * 2 * C::kTile + is_v * C::kTile + i * box * DH * 2;
+        tma_load_rows(dst, is_v ? &vmap : &kmap, full + 8 * slot, row);
       }
       ++issued;
     }
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
         ldm_x4(q_lane + k * 32, qf);
 #pragma unroll
         for (int p = 0; p < kCh / 16; ++p)
-          ldm_x4(tile_addr(Kt, p * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), kb[p]);
+          ldm_x4(tile_addr<DH>(Kt, p * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), kb[p]);
 #pragma unroll
         for (int p = 0; p < kCh / 16; ++p) {
           mma_bf16(sc[2 * p], qf, kb[p][0], kb[p][1]);
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
         uint32_t vb[NT / 2][4];
 #pragma unroll
         for (int p = 0; p < NT / 2; ++p)
-          ldm_x4_t(tile_addr(Vt, kt * 16 + (lane & 15), 2 * p + (lane >> 4)), vb[p]);
+          ldm_x4_t(tile_addr<DH>(Vt, kt * 16 + (lane & 15), 2 * p + (lane >> 4)), vb[p]);
         if (!free) {
 #pragma unroll
           for (int p = 0; p < NT / 2; ++p)
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
         for (int k = 0; k < kCh && x0 + k < xend; ++k)
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            const uint32_t v = lds32(tile_addr(Vt, k, i) + 4 * (lane & 3));
+            const uint32_t v = lds32(tile_addr<DH>(Vt, k, i) + 4 * (lane & 3));
             const uint32_t bad = __vcmpeq2(v & 0x7f807f80u, 0x7f807f80u);
             if ((bad & 0xffffu) && ((see_a >> k) & 1)) o[i][0] += low_half(v);
             if ((bad >> 16) && ((see_a >> k) & 1)) o[i][1] += high_half(v);
@@ -406,10 +406,10 @@ int launch(const FormArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int 
 int form_pool_map(const void* pool, int64_t rows, int dh, int box, CUtensorMap* out) {
   EncodeFn enc = encode_fn();
   if (!enc) return fail(MS_ERR_CUDA, "form_pool_map: cuTensorMapEncodeTiled unavailable");
-  const cuuint64_t dims[2] = {(cuuint64_t)dh, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)dh * 2};
-  const cuuint32_t sizes[2] = {64, (cuuint32_t)box}, estr[2] = {1, 1};
-  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides,
+  const cuuint64_t dims[4] = {64, 8, (cuuint64_t)dh / 64, (cuuint64_t)rows / 8};
+  const cuuint64_t strides[3] = {(cuuint64_t)dh * 2, 128, (cuuint64_t)dh * 16};
+  const cuuint32_t sizes[4] = {64, 8, (cuuint32_t)dh / 64, (cuuint32_t)box / 8}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides,
                          sizes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MS_ERR_CUDA, "form_pool_map: tensor map encode failed (%d)", (int)r);
