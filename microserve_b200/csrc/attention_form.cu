@@ -262,26 +262,32 @@ size_t part_bytes(const FormArgs& a, int rows, int dh) {
 
 int simt_rows(int dh) { return kWarps * (dh <= 64 ? 4 : 2); }
 
-// How a call is cut up: which kernel, its rows per tile, the KV ranges.
+// How a call is cut up: which kernel, its rows per tile, the KV ranges, and whether the sequences are
+// put in order first.
 enum Kernel { kSimt, kTma, kTc };
 struct Way {
   Kernel kernel;
   int rows;
+  bool order;
 };
 Way choose(FormArgs& a, const ms_kv_cache& c, int max_context) {
   const int64_t rows = (int64_t)a.max_q * a.group;
   if (!form_tma_takes(c)) {
-    const Way w{kSimt, simt_rows(c.d_head)};
+    const Way w{kSimt, simt_rows(c.d_head), false};
     plan(a, max_context, w.rows, 128, 256, 148 * 4);
     return w;
   }
-  if (rows <= 32) {
-    plan(a, max_context, 64, 64, 512, 148 * 4);
-    return {kTma, 64};
-  }
-  const int tile = rows > 128 ? 256 : rows > 64 ? 128 : 64;
-  plan(a, max_context, tile, 128, 512, tile == 256 ? 148 : 2 * 148);
-  return {kTc, tile};
+  Way w{rows <= 32 ? kTma : kTc, rows <= 64 ? 64 : rows <= 128 ? 128 : 256, false};
+  const int resident = 148 * (w.kernel == kTma ? 3 : w.rows == 256 ? 1 : 2);
+  if (w.kernel == kTma)
+    plan(a, max_context, w.rows, 64, 512, 148 * 4);
+  else
+    plan(a, max_context, w.rows, 128, 512, resident);
+  // Longest first where the CTAs take more than one wave: the last wave is then of short ones.
+  // (ordering: a launch of about 2 us, n_seqs^2 comparisons)
+  w.order = a.n_seqs > 1 && a.n_seqs <= 4096 &&
+            (int64_t)a.n_seqs * a.hkv * a.row_tiles * a.n_splits > resident;
+  return w;
 }
 
 template <typename T, int DH>
@@ -370,7 +376,8 @@ template int form_combine<__nv_bfloat16, true>(const FormArgs& a, int rows, int 
 
 int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& c, int layer,
                    const ms_batch& bt, int hq, const ms_attention_form* form, void* out,
-                   int64_t out_stride, void* workspace, size_t workspace_bytes, cudaStream_t s) {
+                   int64_t out_stride, void* workspace, size_t workspace_bytes, cudaStream_t s,
+                   const int32_t* seq_order) {
   FormArgs a{};
   int max_context = 0;
   MS_TRY(form_args(a, c, layer, bt, hq, form, &max_context));
@@ -383,13 +390,23 @@ int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& c, int la
   ProfScope prof(kClsAttention, s);
   const Way way = choose(a, c, max_context);
   const int rows = way.rows;
-  if (part_bytes(a, rows, c.d_head) > workspace_bytes) {  // one range a tile
+  size_t parts = part_bytes(a, rows, c.d_head);
+  if (parts > workspace_bytes) {  // one range a tile
     a.n_splits = 1;
     a.split_len = INT_MAX;
+    parts = 0;
   }
   if (a.n_splits > 1) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + (size_t)a.n_seqs * a.hkv * a.row_tiles * a.n_splits * rows * c.d_head;
+  }
+  if (way.order) {
+    a.order = seq_order;
+    if (!seq_order && workspace_bytes - parts >= (size_t)a.n_seqs * sizeof(int32_t)) {
+      int32_t* order = reinterpret_cast<int32_t*>(static_cast<unsigned char*>(workspace) + parts);
+      MS_TRY(attn_seq_order(bt.context_lens, a.n_seqs, order, s));
+      a.order = order;
+    }
   }
   if (way.kernel == kTma) return form_tma(a, c.d_head, s);
   if (way.kernel == kTc) return form_tc(a, c.d_head, rows, s);
@@ -404,7 +421,7 @@ size_t attention_form_workspace(const ms_kv_cache& c, const ms_batch& bt, int hq
   if (form_args(a, c, 0, bt, hq, form, &max_context) != MS_OK || bt.n_seqs == 0 || bt.n_tokens == 0)
     return 0;
   const Way way = choose(a, c, max_context);
-  return part_bytes(a, way.rows, c.d_head);
+  return part_bytes(a, way.rows, c.d_head) + (way.order ? a.n_seqs * sizeof(int32_t) : 0);
 }
 
 }  // namespace ms

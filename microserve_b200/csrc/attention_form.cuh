@@ -24,6 +24,7 @@ struct FormArgs {
   const int32_t *q_start, *context_lens, *positions, *tables;
   const int32_t* prefix;  // null: none
   const float* slopes;    // null: none
+  const int32_t* order;   // the sequences, longest first (null: as they come)
   const uint32_t* mask;   // null: causal
   int mask_words, window;
   float scale, softcap;   // softcap 0: none

@@ -273,18 +273,18 @@ struct Cap {
   }
 };
 
-// p = 2^(x - sub) of 32 values, rounded to bf16, into TMEM; returns the sum of the rounded values.
+// p = 2^(x - sub) of 32 values, rounded to bf16; returns the sum of the rounded values.
 // kWay 0: x * mul; 1: the cap's series of x; 2: x as it is.  16 values at a time, each operation
 // over all of them before the next: a packed operation with three fresh operands takes 3
 // cycles, with one repeated from the operation before 2.
 template <int kWay>
-__device__ __forceinline__ float exps(const uint32_t (&x)[32], uint32_t p_at, float mul, float sub, const Cap& cap) {
+__device__ __forceinline__ float exps(const uint32_t (&x)[32], uint32_t* p16, float mul, float sub, const Cap& cap) {
   const uint64_t minus = twice(-sub);
   float sum[4] = {};
 #pragma unroll
   for (int g = 0; g < 32; g += 16) {
     uint64_t v[8], c[8];
-    uint32_t p[8];
+    uint32_t* p = p16 + g / 2;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = pair(x[g + 2 * j], x[g + 2 * j + 1]);
     if constexpr (kWay == 0) {
@@ -316,7 +316,6 @@ __device__ __forceinline__ float exps(const uint32_t (&x)[32], uint32_t p_at, fl
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) add_bf16(p[j], sum[2 * (j & 1)], sum[2 * (j & 1) + 1]);
-    tmem_st8(p_at + g / 2, p);
   }
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     return;
   }
   // the last tiles of the sequences, which see the most keys, come first
-  const int g = blockIdx.x / a.n_splits, b = blockIdx.y, split = blockIdx.x % a.n_splits;
+  const int g = blockIdx.x / a.n_splits, b = a.order ? a.order[blockIdx.y] : blockIdx.y, split = blockIdx.x % a.n_splits;
   const int tile = (int)gridDim.z - 1 - (int)blockIdx.z;
   const FormSeq s = form_seq(a, b);
   constexpr int kCtaRows = C::kTwin ? 64 : ST * kTileRows;
@@ -685,64 +684,88 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       const uint32_t p_at = C::kSep ? s_col + C::kPCol + mine / 2 : s_at;
       const uint32_t added = pv_done + 8 * (2 * st + ((it - 1) & 1)), added_parity = ((it - 1) >> 1) & 1;
       if (warp_live) {
-        // 32 scores at a time: with more of them they are read again for the exponentials
+        // Almost every step of a long context is plain: all keys seen, no maximum grown by more than
+        // 2^8, the cap's series good for all scores.  So p is computed with the maximum as it is, and the
+        // scores' range beside it: a maximum first would put a pass over the scores and a barrier
+        // before the exponentials.  A step that turns out otherwise starts over (its scores are still there).
         constexpr int kBlocks = W / 32;
-        uint32_t x[32];
-        float top = -INFINITY, bottom = INFINITY;
-#pragma unroll 1
-        for (int h = 0; h < kBlocks; ++h) {
-          tmem_ld(s_at + 32 * h, x);
-          top = fmaxf(top, reduce<true>(x));
-          if (capped) bottom = fminf(bottom, reduce<false>(x));
+        uint32_t x[32], p[W / 2];
+        bool special = !free || sloped;
+        float sum = 0.f;
+        if constexpr (kBlocks == 1) {  // (kept in registers: the next scores may be computed now)
+          tmem_ld(s_at, x);
+          if constexpr (C::kSep) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_read + 8 * st);
+          }
         }
-        // `way` says what the exponent still has to do (see exps).  Almost every step of a long context
-        // is plain: all keys seen, no maximum grown, the cap's series good for all
-        int way = capped ? 1 : 0;
-        bool far = false;  // some score is beyond the cap's series
-        // the scores of block h as the exponent takes them: capped, with the distance, -inf where unseen
-        auto finish = [&](int h) {
-          const int x1 = x0 + mine + 32 * h;
-          if (capped) {
-            if (far) {
+        if (!special) {
+          float top = -INFINITY, bottom = INFINITY;
+          const float sub = m == -INFINITY ? 0.f : m;
 #pragma unroll
-              for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
+          for (int h = 0; h < kBlocks; ++h) {
+            if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
+            if (capped) {
+              sum += exps<1>(x, p + 16 * h, lin, sub, cap);
+              bottom = fminf(bottom, reduce<false>(x));
             } else {
+              sum += exps<0>(x, p + 16 * h, lin, sub, cap);
+            }
+            top = fmaxf(top, reduce<true>(x));
+          }
+          special = any_part(top > plain_top || bottom < plain_bottom);
+        }
+        if (special) {
+          float top = -INFINITY, bottom = INFINITY;
+#pragma unroll 1
+          for (int h = 0; h < kBlocks; ++h) {
+            if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
+            top = fmaxf(top, reduce<true>(x));
+            if (capped) bottom = fminf(bottom, reduce<false>(x));
+          }
+          // some score is beyond the cap's series
+          const bool far = capped && any_part(!(top <= cap.limit && bottom >= -cap.limit));
+          // the scores of block h as the exponent takes them: capped, with the distance, -inf where unseen
+          auto finish = [&](int h) {
+            const int x1 = x0 + mine + 32 * h;
+            if (capped) {
+              if (far) {
 #pragma unroll
-              for (int c = 0; c < 32; c += 2) {
-                float lo, hi;
-                unpair(cap.series(pair(x[c], x[c + 1])), lo, hi);
-                x[c] = __float_as_uint(lo);
-                x[c + 1] = __float_as_uint(hi);
+                for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
+              } else {
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                  float lo, hi;
+                  unpair(cap.series(pair(x[c], x[c + 1])), lo, hi);
+                  x[c] = __float_as_uint(lo);
+                  x[c + 1] = __float_as_uint(hi);
+                }
               }
             }
-          }
-          if (sloped) {
-            const float in = capped ? 1.f : lin;
-            if (free) {
-              const float away = (float)(pos - keys.key(x1));
+            if (sloped) {
+              const float in = capped ? 1.f : lin;
+              if (free) {
+                const float away = (float)(pos - keys.key(x1));
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                x[c] = __float_as_uint(fmaf(-slope, fabsf(away - (float)c), __uint_as_float(x[c]) * in));
-            } else {
+                for (int c = 0; c < 32; ++c)
+                  x[c] = __float_as_uint(fmaf(-slope, fabsf(away - (float)c), __uint_as_float(x[c]) * in));
+              } else {
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                x[c] = __float_as_uint(fmaf(-slope, fabsf((float)(pos - key_position(a, s, keys, x1 + c))),
-                                            __uint_as_float(x[c]) * in));
+                for (int c = 0; c < 32; ++c)
+                  x[c] = __float_as_uint(fmaf(-slope, fabsf((float)(pos - key_position(a, s, keys, x1 + c))),
+                                              __uint_as_float(x[c]) * in));
+              }
             }
-          }
-          if (!free) {
-            const uint32_t see = live ? (uint32_t)seen_places(a, s, keys, tok, pos, x1, xend) : 0u;
+            if (!free) {
+              const uint32_t see = live ? (uint32_t)seen_places(a, s, keys, tok, pos, x1, xend) : 0u;
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (!((see >> c) & 1)) x[c] = 0xff800000u;  // -inf
-          }
-        };
-        bool finished = false;
-        if (any_part(!free || sloped || top > plain_top || bottom < plain_bottom)) {
-          if (capped) far = any_part(!(top <= cap.limit && bottom >= -cap.limit));
-          if (!free || sloped || far) {
-            finished = true;
-            way = capped || sloped ? 2 : 0;
+              for (int c = 0; c < 32; ++c)
+                if (!((see >> c) & 1)) x[c] = 0xff800000u;  // -inf
+            }
+          };
+          const bool finished = !free || sloped || far;
+          if (finished) {
             top = -INFINITY;
 #pragma unroll 1
             for (int h = 0; h < kBlocks; ++h) {
@@ -750,10 +773,10 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
               finish(h);
               top = fmaxf(top, reduce<true>(x));
             }
-          } else if (capped) {
-            top = cap.exact(top);
+            if (!capped && !sloped) top *= lin;
+          } else {
+            top = capped ? cap.exact(top) : top * lin;
           }
-          if (way == 0) top *= lin;
           if constexpr (C::kParts == 2) {
             st32(mine_at, top);
             any_part(false);
@@ -780,31 +803,33 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           }
           // (tanh(u) <= u for u >= 0: a capped score grows past the limit only if s * lin does)
           plain_top = !capped ? (m + 8.f) / lin : m + 8.f >= 0.f ? fminf((m + 8.f) / lin, cap.limit) : -INFINITY;
+          const float sub = m == -INFINITY ? 0.f : m;
+          sum = 0.f;
+#pragma unroll
+          for (int h = 0; h < kBlocks; ++h) {
+            if constexpr (kBlocks > 1) {
+              tmem_ld(s_at + 32 * h, x);
+              if (finished) finish(h);
+            }
+            if (!finished && capped)
+              sum += exps<1>(x, p + 16 * h, lin, sub, cap);
+            else if (capped || sloped)
+              sum += exps<2>(x, p + 16 * h, lin, sub, cap);
+            else
+              sum += exps<0>(x, p + 16 * h, lin, sub, cap);
+          }
         }
-        if constexpr (C::kSep) {  // the values of the step before have been added: p may be replaced
+        l += sum;
+        if constexpr (C::kSep) {
+          if constexpr (kBlocks > 1) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_read + 8 * st);
+          }
+          // the values of the step before have been added: p may be replaced
           if (it > 0) wait(added, added_parity);
         }
-        const float sub = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-        for (int h = 0; h < kBlocks; ++h) {
-          if constexpr (kBlocks > 1) {
-            tmem_ld(s_at + 32 * h, x);
-            if (finished) finish(h);
-          }
-          if constexpr (C::kSep) {
-            if (h == kBlocks - 1) {
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(s_read + 8 * st);
-            }
-          }
-          if (way == 0)
-            l += exps<0>(x, p_at + 16 * h, lin, sub, cap);
-          else if (way == 1)
-            l += exps<1>(x, p_at + 16 * h, lin, sub, cap);
-          else
-            l += exps<2>(x, p_at + 16 * h, lin, sub, cap);
-        }
+        tmem_st(p_at, p);
         tmem_wait_st();
       } else if (C::kSep) {
         if (lane == 0) mbar_arrive(s_read + 8 * st);

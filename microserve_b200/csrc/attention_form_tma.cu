@@ -79,7 +79,7 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
   const uint32_t full = s_addr(bars), empty = full + 8 * NS;
   volatile int* stop = reinterpret_cast<volatile int*>(bars + 2 * NS);
 
-  const int g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.y, b = a.order ? a.order[blockIdx.z] : blockIdx.z;
   const int split = blockIdx.x % a.n_splits, tile = blockIdx.x / a.n_splits;
   const FormSeq s = form_seq(a, b);
   const int r0 = tile * kRows;

@@ -216,7 +216,7 @@ int forward(const ms_model* model, const ms_kv_cache* cache, const ms_batch* bat
     // q occupies the first hq*dh columns of each qkv row.
     if (forms)
       MS_TRY(attention_form(w.qkv, qkv_w, c, l, bt, hq, form, w.attn, hq * dh, attn_scratch,
-                            attn_scratch_bytes, s));
+                            attn_scratch_bytes, s, order));
     else
       MS_TRY(paged_attention(w.qkv, qkv_w, c, l, bt, hq, w.attn, attn_scratch, attn_scratch_bytes,
                              s, order));

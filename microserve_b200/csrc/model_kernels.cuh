@@ -28,7 +28,8 @@ int paged_attention(const void* q, int q_stride, const ms_kv_cache& cache, int l
 // attention_form_workspace: one KV range per tile.
 int attention_form(const void* q, int64_t q_stride, const ms_kv_cache& cache, int layer,
                    const ms_batch& batch, int hq, const ms_attention_form* form, void* out,
-                   int64_t out_stride, void* workspace, size_t workspace_bytes, cudaStream_t s);
+                   int64_t out_stride, void* workspace, size_t workspace_bytes, cudaStream_t s,
+                   const int32_t* seq_order = nullptr);
 size_t attention_form_workspace(const ms_kv_cache& cache, const ms_batch& batch, int hq,
                                 const ms_attention_form* form);
 
