@@ -38,25 +38,24 @@ template <int DH, int SH>
 struct TcCfg {
   static constexpr int ST = SH == kTwo ? 2 : 1;                  // streams of 128 rows
   static constexpr bool kTwin = SH == kHalf;
-  static constexpr bool kSep = kTwin || DH == 64;                // p behind the scores, or over them
-  static constexpr int KC = DH == 64 || SH == kTwo ? 128 : 64;   // keys per step
-  static constexpr int SB = kSep || SH == kTwo ? 1 : 2;          // score buffers
+  static constexpr int KC = kTwin && DH == 64 ? 128 : 64;        // keys per step
+  static constexpr int SB = kTwin ? 1 : 2;                       // score buffers
   static constexpr int kParts = kTwin && DH == 128 ? 1 : 2;      // threads that share a row's scores
-  static constexpr int kWidth = KC / (kTwin ? 2 : 1) / kParts;   // scores of a step per thread
   static constexpr int kTile = KC * DH * 2;                      // K or V of a step
-  static constexpr int kSlots = SH == kTwo ? 160 : DH == 64 || kTwin ? 80 : 64;  // KB of K and V
+  static constexpr int kSlots = SH == kTwo ? 144 : DH == 64 || kTwin ? 80 : 64;  // KB of K and V
   static constexpr int NK = (kSlots * 1024 / kTile + 1) / 2, NV = kSlots * 1024 / kTile / 2;
   static constexpr int kQ = kTileRows * DH * 2;
-  static constexpr int kPCol = kSep ? KC : 0;
-  static constexpr int kOCol = kSep ? KC + KC / 2 : SB * KC;
+  static constexpr int kPCol = kTwin ? KC : 0;                   // p behind the scores, or over them
+  static constexpr int kOCol = kTwin ? KC + KC / 2 : SB * KC;
   static constexpr int kStreamCols = kOCol + DH;
   static constexpr int kCols = ST == 2 ? 512 : 256;
   static constexpr int kSoft = 4 * kParts;                       // softmax warps of a stream
   static constexpr int kWarps = kSoft * ST + (ST == 2 ? 4 : 2);
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kBars = 2 * NK + 2 * NV + 2 + ST * (2 * SB + 3);
+  static constexpr int kBars = 2 * NK + 2 * NV + 3 + ST * (2 * SB + 2);
   static constexpr int kShare = ST * kParts * kTileRows * 4;     // what the threads of a row tell one another
   static constexpr int kSmem = ST * kQ + (NK + NV) * kTile + kShare + kBars * 8 + 16;
+  static_assert(KC / (kTwin ? 2 : 1) / kParts == 32, "32 scores of a step per thread");
   static_assert(ST * kStreamCols <= kCols, "TMEM columns");
   static_assert((3 - ST) * (kSmem + 1024) <= 228 * 1024 && kSmem <= 227 * 1024, "shared memory of an SM's CTAs");
   static_assert(!kTwin || 64 * DH * 4 + 64 * 8 <= NK * kTile, "the copies meet in the K ring");
@@ -273,11 +272,33 @@ struct Cap {
   }
 };
 
+// 2^x of two values on the FMA units: x = n + f, |f| <= 1/2 (n by adding and taking off 1.5 2^23), 2^f
+// by a cubic (fitted to the least maximum of the relative error, 1.0e-4, a fortieth of bf16's
+// rounding), n into the exponent.  From -128 down that leaves a negative word, and 0 (an unseen key's p
+// has to be 0: its value may be anything finite).
+__device__ __forceinline__ void exp2_fma(uint64_t v, float& lo, float& hi) {
+  float a, b;
+  unpair(v, a, b);
+  v = pair(__float_as_uint(fmaxf(a, -128.f)), __float_as_uint(fmaxf(b, -128.f)));
+  const uint64_t t = add2(v, twice(12582912.f)), n = add2(t, twice(-12582912.f));
+  const uint64_t f = fma2(n, twice(-1.f), v);
+  uint64_t c = fma2(f, twice(0.0551716684f), twice(0.242611122f));
+  c = fma2(f, c, twice(0.693260986f));
+  c = fma2(f, c, twice(0.999928074f));
+  float tl, th, cl, ch;
+  unpair(t, tl, th);
+  unpair(c, cl, ch);
+  lo = __int_as_float(max((int)(__float_as_uint(cl) + (__float_as_uint(tl) << 23)), 0));
+  hi = __int_as_float(max((int)(__float_as_uint(ch) + (__float_as_uint(th) << 23)), 0));
+}
+
 // p = 2^(x - sub) of 32 values, rounded to bf16; returns the sum of the rounded values.
 // kWay 0: x * mul; 1: the cap's series of x; 2: x as it is.  16 values at a time, each operation
 // over all of them before the next: a packed operation with three fresh operands takes 3
 // cycles, with one repeated from the operation before 2.
-template <int kWay>
+// kFma: a quarter of the exponentials on the FMA units, where the SFU (8 cycles a warp and value) is the
+// bound (8B trees of 61 nodes 223 -> 207 us; half of them 213).
+template <int kWay, bool kFma>
 __device__ __forceinline__ float exps(const uint32_t (&x)[32], uint32_t* p16, float mul, float sub, const Cap& cap) {
   const uint64_t minus = twice(-sub);
   float sum[4] = {};
@@ -311,8 +332,14 @@ __device__ __forceinline__ float exps(const uint32_t (&x)[32], uint32_t* p16, fl
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float lo, hi;
-      unpair(c[j], lo, hi);
-      p[j] = pack2(fast_exp2(lo), fast_exp2(hi));
+      if (kFma && (j == 1 || j == 4)) {
+        exp2_fma(c[j], lo, hi);
+      } else {
+        unpair(c[j], lo, hi);
+        lo = fast_exp2(lo);
+        hi = fast_exp2(hi);
+      }
+      p[j] = pack2(lo, hi);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) add_bf16(p[j], sum[2 * (j & 1)], sum[2 * (j & 1) + 1]);
@@ -382,13 +409,13 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
                    const __grid_constant__ FormArgs a, int log2_bs, int vec) {
   pdl_enter();
   using C = TcCfg<DH, SH>;
-  constexpr int ST = C::ST, KC = C::KC, SB = C::SB, NK = C::NK, NV = C::NV, W = C::kWidth;
+  constexpr int ST = C::ST, KC = C::KC, SB = C::SB, NK = C::NK, NV = C::NV, W = 32;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = s_addr(smem_raw), q_s = raw;  // (1024-byte aligned, as declared)
   const uint32_t k_s = q_s + ST * C::kQ, v_s = k_s + NK * C::kTile, share = v_s + NV * C::kTile;
   const uint32_t bars = share + C::kShare;
   const uint32_t k_full = bars, k_empty = k_full + 8 * NK, v_full = k_empty + 8 * NK, v_empty = v_full + 8 * NV;
-  const uint32_t q_ready = v_empty + 8 * NV, ended = q_ready + 8, s_read = ended + 8, s_full = s_read + 8 * ST;
+  const uint32_t q_ready = v_empty + 8 * NV, ended = q_ready + 8, s_read = ended + 8, s_full = s_read + 8;
   const uint32_t p_ready = s_full + 8 * ST * SB, pv_done = p_ready + 8 * ST * SB, slot_at = pv_done + 16 * ST;
   unsigned char* words = smem_raw + (slot_at - raw);
   volatile uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(words);
@@ -428,7 +455,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     }
     mbar_init(q_ready, C::kSoft * ST);
     mbar_init(ended, 1);
-    for (int i = 0; i < ST; ++i) mbar_init(s_read + 8 * i, C::kSoft);
+    mbar_init(s_read, C::kSoft);
     for (int i = 0; i < ST * SB; ++i) {
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_ready + 8 * i, C::kSoft);
@@ -515,7 +542,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
 #pragma unroll
         for (int k = 0; k < KC / 16; ++k) {
           // over the scores, each part's p starts where its scores did
-          const int at = C::kSep ? 8 * k : 8 * (k % (W / 16)) + k / (W / 16) * W;
+          const int at = C::kTwin ? 8 * k : 8 * (k % (W / 16)) + k / (W / 16) * W;
           mma_ts(o, p + at, vd + k * (2 * DH * 16 / 16), id_o, it > 0 || k > 0, one);
         }
         mma_commit(pv_done + 8 * (2 * st + (it & 1)), one);
@@ -530,7 +557,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       }
       for (int it = 0; it < n && ok; ++it) {
         const int ahead = it + SB;
-        if constexpr (C::kSep && ST == 1) {  // the next scores as soon as these are read
+        if constexpr (C::kTwin) {  // the next scores as soon as these are read
           if (ahead < n) {
             ok = wait(k_full + 8 * (ahead % NK), (ahead / NK) & 1) && wait(s_read, it & 1);
             if (!ok) break;
@@ -548,15 +575,10 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           fence_after();
           add_values(it, st);
           if (st == ST - 1) mma_commit(v_empty + 8 * (it % NV), one);
-          if constexpr (!C::kSep || ST == 2) {
+          if constexpr (!C::kTwin) {
             if (ahead < n) {
               if (st == 0) {
                 ok = wait(k_full + 8 * (ahead % NK), (ahead / NK) & 1);
-                if (!ok) break;
-                fence_after();
-              }
-              if constexpr (C::kSep) {  // (read before p was ready)
-                ok = wait(s_read + 8 * st, it & 1);
                 if (!ok) break;
                 fence_after();
               }
@@ -681,99 +703,61 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       // pv_done's two barriers, each has at most one phase open)
       wait(s_full + 8 * (st * SB + it % SB), (it / SB) & 1);
       const uint32_t s_at = s_col + (it % SB) * KC + mine;
-      const uint32_t p_at = C::kSep ? s_col + C::kPCol + mine / 2 : s_at;
+      const uint32_t p_at = C::kTwin ? s_col + C::kPCol + mine / 2 : s_at;
       const uint32_t added = pv_done + 8 * (2 * st + ((it - 1) & 1)), added_parity = ((it - 1) >> 1) & 1;
       if (warp_live) {
-        // Almost every step of a long context is plain: all keys seen, no maximum grown by more than
-        // 2^8, the cap's series good for all scores.  So p is computed with the maximum as it is, and the
-        // scores' range beside it: a maximum first would put a pass over the scores and a barrier
-        // before the exponentials.  A step that turns out otherwise starts over (its scores are still there).
-        constexpr int kBlocks = W / 32;
-        uint32_t x[32], p[W / 2];
-        bool special = !free || sloped;
-        float sum = 0.f;
-        if constexpr (kBlocks == 1) {  // (kept in registers: the next scores may be computed now)
-          tmem_ld(s_at, x);
-          if constexpr (C::kSep) {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_read + 8 * st);
-          }
+        uint32_t x[W], p[W / 2];
+        tmem_ld(s_at, x);
+        if constexpr (C::kTwin) {  // the next scores may be computed
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_read);
         }
-        if (!special) {
-          float top = -INFINITY, bottom = INFINITY;
-          const float sub = m == -INFINITY ? 0.f : m;
-#pragma unroll
-          for (int h = 0; h < kBlocks; ++h) {
-            if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
-            if (capped) {
-              sum += exps<1>(x, p + 16 * h, lin, sub, cap);
-              bottom = fminf(bottom, reduce<false>(x));
-            } else {
-              sum += exps<0>(x, p + 16 * h, lin, sub, cap);
-            }
-            top = fmaxf(top, reduce<true>(x));
-          }
-          special = any_part(top > plain_top || bottom < plain_bottom);
-        }
-        if (special) {
-          float top = -INFINITY, bottom = INFINITY;
-#pragma unroll 1
-          for (int h = 0; h < kBlocks; ++h) {
-            if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
-            top = fmaxf(top, reduce<true>(x));
-            if (capped) bottom = fminf(bottom, reduce<false>(x));
-          }
+        float top = reduce<true>(x), bottom = INFINITY;
+        if (capped) bottom = reduce<false>(x);
+        // `way` says what the exponent still has to do (see exps).  Almost every step of a long context
+        // is plain: all keys seen, no maximum grown, the cap's series good for all
+        int way = capped ? 1 : 0;
+        if (any_part(!free || sloped || top > plain_top || bottom < plain_bottom)) {
           // some score is beyond the cap's series
           const bool far = capped && any_part(!(top <= cap.limit && bottom >= -cap.limit));
-          // the scores of block h as the exponent takes them: capped, with the distance, -inf where unseen
-          auto finish = [&](int h) {
-            const int x1 = x0 + mine + 32 * h;
-            if (capped) {
-              if (far) {
+          if (!free || sloped || far) {
+            // ---- the scores as the exponent takes them: capped, with the distance, -inf where unseen
+            way = capped || sloped ? 2 : 0;
+            if (capped && far) {
 #pragma unroll
-                for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
-              } else {
+              for (int c = 0; c < W; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
+            } else if (capped) {
 #pragma unroll
-                for (int c = 0; c < 32; c += 2) {
-                  float lo, hi;
-                  unpair(cap.series(pair(x[c], x[c + 1])), lo, hi);
-                  x[c] = __float_as_uint(lo);
-                  x[c + 1] = __float_as_uint(hi);
-                }
+              for (int c = 0; c < W; c += 2) {
+                float lo, hi;
+                unpair(cap.series(pair(x[c], x[c + 1])), lo, hi);
+                x[c] = __float_as_uint(lo);
+                x[c + 1] = __float_as_uint(hi);
               }
             }
             if (sloped) {
               const float in = capped ? 1.f : lin;
               if (free) {
-                const float away = (float)(pos - keys.key(x1));
+                const float away = (float)(pos - keys.key(x0 + mine));
 #pragma unroll
-                for (int c = 0; c < 32; ++c)
+                for (int c = 0; c < W; ++c)
                   x[c] = __float_as_uint(fmaf(-slope, fabsf(away - (float)c), __uint_as_float(x[c]) * in));
               } else {
 #pragma unroll
-                for (int c = 0; c < 32; ++c)
-                  x[c] = __float_as_uint(fmaf(-slope, fabsf((float)(pos - key_position(a, s, keys, x1 + c))),
+                for (int c = 0; c < W; ++c)
+                  x[c] = __float_as_uint(fmaf(-slope, fabsf((float)(pos - key_position(a, s, keys, x0 + mine + c))),
                                               __uint_as_float(x[c]) * in));
               }
             }
             if (!free) {
-              const uint32_t see = live ? (uint32_t)seen_places(a, s, keys, tok, pos, x1, xend) : 0u;
+              const uint32_t see = live ? (uint32_t)seen_places(a, s, keys, tok, pos, x0 + mine, xend) : 0u;
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
+              for (int c = 0; c < W; ++c)
                 if (!((see >> c) & 1)) x[c] = 0xff800000u;  // -inf
             }
-          };
-          const bool finished = !free || sloped || far;
-          if (finished) {
-            top = -INFINITY;
-#pragma unroll 1
-            for (int h = 0; h < kBlocks; ++h) {
-              if constexpr (kBlocks > 1) tmem_ld(s_at + 32 * h, x);
-              finish(h);
-              top = fmaxf(top, reduce<true>(x));
-            }
-            if (!capped && !sloped) top *= lin;
+            top = reduce<true>(x);
+            if (way == 0) top *= lin;
           } else {
             top = capped ? cap.exact(top) : top * lin;
           }
@@ -803,36 +787,21 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           }
           // (tanh(u) <= u for u >= 0: a capped score grows past the limit only if s * lin does)
           plain_top = !capped ? (m + 8.f) / lin : m + 8.f >= 0.f ? fminf((m + 8.f) / lin, cap.limit) : -INFINITY;
-          const float sub = m == -INFINITY ? 0.f : m;
-          sum = 0.f;
-#pragma unroll
-          for (int h = 0; h < kBlocks; ++h) {
-            if constexpr (kBlocks > 1) {
-              tmem_ld(s_at + 32 * h, x);
-              if (finished) finish(h);
-            }
-            if (!finished && capped)
-              sum += exps<1>(x, p + 16 * h, lin, sub, cap);
-            else if (capped || sloped)
-              sum += exps<2>(x, p + 16 * h, lin, sub, cap);
-            else
-              sum += exps<0>(x, p + 16 * h, lin, sub, cap);
-          }
         }
-        l += sum;
-        if constexpr (C::kSep) {
-          if constexpr (kBlocks > 1) {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_read + 8 * st);
-          }
-          // the values of the step before have been added: p may be replaced
+        const float sub = m == -INFINITY ? 0.f : m;
+        if (way == 0)
+          l += exps<0, !C::kTwin>(x, p, lin, sub, cap);
+        else if (way == 1)
+          l += exps<1, false>(x, p, lin, sub, cap);
+        else
+          l += exps<2, !C::kTwin>(x, p, lin, sub, cap);
+        if constexpr (C::kTwin) {  // the values of the step before have been added: p may be replaced
           if (it > 0) wait(added, added_parity);
         }
         tmem_st(p_at, p);
         tmem_wait_st();
-      } else if (C::kSep) {
-        if (lane == 0) mbar_arrive(s_read + 8 * st);
+      } else if (C::kTwin) {
+        if (lane == 0) mbar_arrive(s_read);
         // (p_ready has one phase open at a time: not ahead of the other warps' step before)
         if (it > 0) wait(added, added_parity);
       }

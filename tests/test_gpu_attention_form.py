@@ -285,3 +285,21 @@ def test_refusals() -> None:
     q = torch.zeros((8, 4, 64), device=DEV, dtype=BF16)
     with pytest.raises(ValueError, match="overlap"):
         run(x, q=q[:4], out=q[2:6])
+
+
+@pytest.mark.parametrize("dh,hq,n", [(64, 4, 9), (128, 4, 9), (64, 16, 40), (128, 16, 40), (128, 16, 10), (64, 16, 10)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_the_largest_values_in_unseen_places(dh, hq, n, tree) -> None:
+    """Stale places hold the type's largest finite value: an unseen key's weight is exactly 0."""
+    big = float(torch.finfo(BF16).max)
+    x = make(21, BF16, hq, 2, dh, 16, [50, 130, 0], [n, n - 1, 1], tree=tree, stale=big, window=0 if tree else 30)
+    for _ in range(2):
+        check(run(x), x)
+    for b, c in enumerate((50, 130)):  # and so do other branches' values, and keys that come later
+        page = int(x.tables[b, (c + 2) // 16])
+        x.v[page, :, (c + 2) % 16] = big
+    seen = [r for b in range(2) for r in range(int(x.q_start[b]), int(x.q_start[b + 1]))
+            if x.context[b] - x.q_lens[b] + 2 not in visible(x, b, r - int(x.q_start[b]))[0]]
+    got = run(x).double().cpu()
+    ref, tol = reference(x)
+    assert seen and bool(((got - ref).abs() <= tol)[seen].all())
