@@ -303,3 +303,20 @@ def test_the_largest_values_in_unseen_places(dh, hq, n, tree) -> None:
     got = run(x).double().cpu()
     ref, tol = reference(x)
     assert seen and bool(((got - ref).abs() <= tol)[seen].all())
+
+
+@pytest.mark.parametrize("dtype,hq,dh", [(F32, 2, 64), (BF16, 2, 64), (BF16, 16, 128), (BF16, 2, 32)])
+def test_pools_beyond_four_gigabytes(dtype, hq, dh) -> None:
+    """Pages whose offsets pass 32 bits, in bytes and in elements."""
+    from microserve_b200.attention import paged_attention
+
+    x = make(22, dtype, hq, 1, dh, 16, [40, 100], [5, 9], tree=True)
+    blocks = x.k.shape[0]
+    total = (2 ** 32 + 2 ** 28) // (16 * dh)
+    big = torch.empty((2, total, 1, 16, dh), dtype=dtype, device=DEV)  # (not filled: only the pages in use are)
+    batch = x.batch()
+    high = total - blocks
+    batch.block_tables += high
+    big[0, high:].copy_(x.k)
+    big[1, high:].copy_(x.v)
+    check(paged_attention(x.q.to(DEV), big[0], big[1], batch, x.form()), x)

@@ -203,3 +203,20 @@ def test_compact_keeps_every_sequence() -> None:
         cache.free(s)
     cache.allocator.check_invariants()
     assert cache.num_free_blocks == 40
+
+
+def test_pools_beyond_four_gigabytes() -> None:
+    """Blocks and slots whose offsets pass 32 bits, in bytes and in elements."""
+    from microserve_b200.cache import copy_blocks, move_tokens
+
+    blocks = (2 ** 32 + 2 ** 26) // (16 * 64)
+    pool = torch.empty((2, 1, blocks, 1, 16, 64), dtype=torch.bfloat16, device=DEV)
+    at = torch.tensor([3, blocks - 2], device=DEV)
+    pool[:, :, at] = torch.randn((2, 1, 2, 1, 16, 64), device=DEV).to(torch.bfloat16)
+    was = pool[:, :, at].clone()
+    copy_blocks(pool, _i32([3, blocks - 2]), _i32([blocks - 1, 4]))
+    assert torch.equal(pool[:, :, blocks - 1], was[:, :, 0]) and torch.equal(pool[:, :, 4], was[:, :, 1])
+    last = (blocks - 2) * 16
+    move_tokens(pool, _i32([[last + 5, 3 * 16 + 1]]), _i32([[3 * 16 + 1, last + 9]]))
+    assert torch.equal(pool[:, :, 3, :, 1], was[:, :, 1, :, 5])
+    assert torch.equal(pool[:, :, blocks - 2, :, 9], was[:, :, 0, :, 1])
