@@ -272,12 +272,21 @@ struct Way {
 };
 Way choose(FormArgs& a, const ms_kv_cache& c, int max_context) {
   const int64_t rows = (int64_t)a.max_q * a.group;
-  if (!form_tma_takes(c)) {
+  if (!form_tma_takes(c) || ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15)) {
     const Way w{kSimt, simt_rows(c.d_head), false};
     plan(a, max_context, w.rows, 128, 256, 148 * 4);
     return w;
   }
-  Way w{rows <= 32 ? kTma : kTc, rows <= 64 ? 64 : rows <= 128 ? 128 : 256, false};
+  // mma.sync for few rows, tcgen05 for many, where 128 rows of a tile cost what 16 do (us, mma.sync and
+  // tcgen05; 128 sequences of 2 k keys, cap and window): heads of 128, 4, 16 and 32 rows 185 and
+  // 201, 210 and 204, 258 and 208 (without either 335 and 354, 345 and 358, 382 and 365); heads of
+  // 64, 4, 16 and 32 rows 104 and 126, 119 and 129, 149 and 128; trees of 256 sequences, heads of
+  // 64, 32, 40 and 64 rows 78 and 94, 90 and 94, 120 and 95.
+  Way w{rows <= (c.d_head == 128 ? 16 : 32) ? kTma : kTc, 0, false};
+  // The least tile that holds a sequence (us; trees of 64 sequences, heads of 128): 64 rows in a tile of
+  // 64 and of 128 127 and 137; 128 rows in 128 and 256 145 and 185; 192 rows in two of 128 and one of
+  // 256 257 and 221.
+  w.rows = w.kernel == kTma ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
   const int resident = 148 * (w.kernel == kTma ? 3 : w.rows == 256 ? 1 : 2);
   if (w.kernel == kTma)
     plan(a, max_context, w.rows, 64, 512, 148 * 4);

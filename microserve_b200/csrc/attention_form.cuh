@@ -115,10 +115,10 @@ __device__ __forceinline__ bool form_sees(const FormArgs& a, const FormSeq& s, i
 template <typename T, bool kBase2>
 int form_combine(const FormArgs& a, int rows, int dh, cudaStream_t s);
 
-// attention_form_tma.cu: tiles of 64 rows.
+// attention_form_tma.cu: one tile of up to 32 rows a sequence (16 at heads of 128).
 bool form_tma_takes(const ms_kv_cache& c);
 int form_tma(const FormArgs& a, int dh, cudaStream_t s);
-// attention_form_tc.cu: tiles of 128 or 256 rows, for the caches that form_tma_takes.
+// attention_form_tc.cu: tiles of 64, 128 or 256 rows, for the caches that form_tma_takes.
 int form_tc(const FormArgs& a, int dh, int rows, cudaStream_t s);
 
 }  // namespace ms

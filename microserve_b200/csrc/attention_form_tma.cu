@@ -1,9 +1,8 @@
-// Attention with score forms over bf16 caches, for few rows: up to 64 per
-// tile (single tokens and small trees of a kv head's query heads).
+// Attention with score forms over bf16 caches, for few rows: up to 32 (16 at heads
+// of 128) a sequence and kv head, as single tokens and small trees have.
 //
-// One CTA per (64-row tile, KV range, kv head, sequence).  Row r of a tile is
-// (token r / group, head-in-group r % group), so that keys and values are
-// read once per kv head.
+// One CTA per (KV range, kv head, sequence).  Row r is (token r / group, head-in-group
+// r % group), so that keys and values are read once per kv head.
 //   producer warp   TMA loads of each chunk of 64 places (whole pages or parts
 //                   of one) into a ring, a lane a page;
 //   consumer warps  one for each 16 rows: S = Q K^T and O += P V by mma.sync
@@ -23,7 +22,7 @@
 namespace ms {
 namespace {
 
-constexpr int kRows = 64;
+constexpr int kRows = 32;
 constexpr int kCh = 64;  // keys per chunk
 
 template <int DH, int MT, int NS>
@@ -430,21 +429,8 @@ int form_tma(const FormArgs& a, int dh, cudaStream_t s) {
   MS_TRY(form_pool_map(a.v, rows, dh, min(a.bs, kCh), &vm));
   const int vec = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 &&
                   a.q_stride % 8 == 0 && a.out_stride % 8 == 0;
-  const int mt = (min(a.max_q * a.group, kRows) + 15) / 16;
-  if (dh == 64) {
-    switch (mt) {
-      case 1: return launch<64, 1, 2, 6>(a, km, vm, vec, s);
-      case 2: return launch<64, 2, 3, 4>(a, km, vm, vec, s);
-      case 3: return launch<64, 3, 2, 4>(a, km, vm, vec, s);
-      default: return launch<64, 4, 2, 3>(a, km, vm, vec, s);
-    }
-  }
-  switch (mt) {
-    case 1: return launch<128, 1, 2, 3>(a, km, vm, vec, s);
-    case 2: return launch<128, 2, 2, 3>(a, km, vm, vec, s);
-    case 3: return launch<128, 3, 2, 2>(a, km, vm, vec, s);
-    default: return launch<128, 4, 2, 2>(a, km, vm, vec, s);
-  }
+  if (dh == 128) return launch<128, 1, 2, 3>(a, km, vm, vec, s);
+  return a.max_q * a.group <= 16 ? launch<64, 1, 2, 6>(a, km, vm, vec, s) : launch<64, 2, 3, 4>(a, km, vm, vec, s);
 }
 
 }  // namespace ms

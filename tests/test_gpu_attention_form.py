@@ -320,3 +320,17 @@ def test_pools_beyond_four_gigabytes(dtype, hq, dh) -> None:
     big[0, high:].copy_(x.k)
     big[1, high:].copy_(x.v)
     check(paged_attention(x.q.to(DEV), big[0], big[1], batch, x.form()), x)
+
+
+@pytest.mark.parametrize("dtype,shift", [(F32, 1), (F32, 2), (BF16, 1), (BF16, 4)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_pools_that_start_anywhere(dtype, shift, n) -> None:
+    """Pools that are not aligned to 16 bytes."""
+    from microserve_b200.attention import paged_attention
+
+    x = make(23, dtype, 4, 2, 64, 16, [70, 20], [n, n], tree=True)
+    pools = []
+    for t in (x.k, x.v):
+        flat = torch.empty(t.numel() + shift, dtype=dtype, device=DEV)
+        pools.append(flat[shift:].view(t.shape).copy_(t))
+    check(paged_attention(x.q.to(DEV), *pools, x.batch(), x.form()), x)
