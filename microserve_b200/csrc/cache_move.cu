@@ -17,10 +17,11 @@ struct Pools {
 
 // The (layer, K or V) pools are copied side by side: element e of a page is
 // copied by one thread of the CTA that has its tile of kUnroll * kThreads
-// elements; all loads of a thread are in flight before its stores.
+// elements; all loads of a thread are in flight before its stores.  Bound by HBM: 4001 pages of 22 layers, 4
+// heads of 64 (2.9 GB moved) take 430 us, 6.7 TB/s.
 template <typename V>
 __global__ void __launch_bounds__(kThreads)
-    kv_copy_blocks_kernel(const __grid_constant__ Pools pools, int n_pools, const int32_t* __restrict__ src,
+    kv_copy_blocks_kernel(const __grid_constant__ Pools pools, const int32_t* __restrict__ src,
                           const int32_t* __restrict__ dst, int n, int page, int num_blocks, int* err) {
   pdl_enter();
   constexpr int kUnroll = 4;
@@ -64,60 +65,66 @@ __device__ __forceinline__ bool move_pair(const int32_t* src, const int32_t* dst
   return true;
 }
 
-// A warp a (group, kv head) and kPools pools: the group's rows of `row` elements, at most
-// kRegs elements a lane and pool, are all in registers before the first is stored.  Rows of
-// 128 to 256 bytes lie anywhere, so what counts is how many are in flight: one pool a
-// warp took 34 us for 192 groups of up to 5 moves in 32 layers, 8 heads of 128; four take 16.
+// `team` threads (a power of two, 32 to kThreads) a (group, kv head): they hold the group's rows, up to
+// kRegs elements of `row` a thread, in registers before the first is stored, kPools pools
+// at a time, and go through the pools of their slice (blockIdx.y of gridDim.y).  The
+// places are worked out once a slice: their divisions take longer than the copies of a pool.
+// Rows of 128 to 256 bytes lie anywhere, so what counts is how many are in flight: 192 groups, 32
+// layers, 8 heads of 128 take 20, 27 and 42 us for up to 5, 8 and 24 moves (6 us of which are the
+// launch and its gaps, 25, 40 and 115 MB), and at most 5 of them with 1, 2, 4 and 8 pools at a time 37,
+// 24, 20 and 20 us.  4 elements a thread: 23, 26 and 58 us.
 template <typename V, int kRegs, int kPools>
 __global__ void __launch_bounds__(kThreads)
     kv_move_kernel(const __grid_constant__ Pools pools, int n_pools, const int32_t* __restrict__ src,
                    const int32_t* __restrict__ dst, int n_groups, int per_group, int row, int bs,
-                   int hkv, int num_slots, int* err) {
+                   int hkv, int num_slots, int team, int* err) {
   pdl_enter();
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (unit >= (int64_t)n_groups * hkv) return;
+  const int member = threadIdx.x & (team - 1), elements = per_group * row;
+  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / team;
   const int group = (int)(unit / hkv), h = (int)(unit - (int64_t)group * hkv);
   int64_t from[kRegs], to[kRegs];
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const int e = lane + 32 * i, m = e / row, at = e - m * row;
-    if (m < per_group &&
-        move_pair(src, dst, (int64_t)group * per_group + m, bs, hkv, num_slots, from[i], to[i], err)) {
+    to[i] = -1;
+    const int e = member + team * i;
+    if (e >= elements || group >= n_groups) continue;
+    const int m = e / row, at = e - m * row;
+    if (move_pair(src, dst, (int64_t)group * per_group + m, bs, hkv, num_slots, from[i], to[i], err)) {
       from[i] = (from[i] + (int64_t)h * bs) * row + at;
       to[i] = (to[i] + (int64_t)h * bs) * row + at;
-    } else {
-      to[i] = -1;
     }
   }
-  V v[kPools][kRegs];
+  const int p0 = (int)((int64_t)n_pools * blockIdx.y / gridDim.y);
+  const int p1 = (int)((int64_t)n_pools * (blockIdx.y + 1) / gridDim.y);
+  for (int p = p0; p < p1; p += kPools) {
+    V v[kPools][kRegs];
 #pragma unroll
-  for (int p = 0; p < kPools; ++p) {
-    const int pool = blockIdx.y * kPools + p;
-    if (pool >= n_pools) break;
-    const V* base = static_cast<const V*>(pools.p[pool]);
+    for (int u = 0; u < kPools; ++u) {
+      if (p + u >= p1) break;
+      const V* base = static_cast<const V*>(pools.p[p + u]);
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-      if (to[i] >= 0) v[p][i] = base[from[i]];
-  }
-  __syncwarp();
+      for (int i = 0; i < kRegs; ++i)
+        if (to[i] >= 0) v[u][i] = base[from[i]];
+    }
+    if (team > 32) __syncthreads(); else __syncwarp();
 #pragma unroll
-  for (int p = 0; p < kPools; ++p) {
-    const int pool = blockIdx.y * kPools + p;
-    if (pool >= n_pools) break;
-    V* base = static_cast<V*>(pools.p[pool]);
+    for (int u = 0; u < kPools; ++u) {
+      if (p + u >= p1) break;
+      V* base = static_cast<V*>(pools.p[p + u]);
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-      if (to[i] >= 0) base[to[i]] = v[p][i];
+      for (int i = 0; i < kRegs; ++i)
+        if (to[i] >= 0) base[to[i]] = v[u][i];
+    }
   }
 }
 
-// Larger groups: a CTA a (group, kv head, pool), the rows in shared memory.
+// Groups of more than kRegs * kThreads elements: a CTA a (group, kv head, pool), the rows in shared
+// memory (the three groups above would take 118, 128 and 206 us).
 template <typename V>
 __global__ void __launch_bounds__(kThreads)
-    kv_move_shared_kernel(const __grid_constant__ Pools pools, int n_pools, const int32_t* __restrict__ src,
-                          const int32_t* __restrict__ dst, int n_groups, int per_group, int row,
-                          int bs, int hkv, int num_slots, int* err) {
+    kv_move_shared_kernel(const __grid_constant__ Pools pools, const int32_t* __restrict__ src,
+                          const int32_t* __restrict__ dst, int per_group, int row, int bs, int hkv,
+                          int num_slots, int* err) {
   pdl_enter();
   extern __shared__ __align__(16) unsigned char smem[];
   V* rows = reinterpret_cast<V*>(smem);
@@ -175,7 +182,7 @@ int copy_blocks(const ms_kv_cache& c, const int32_t* src, const int32_t* dst, in
   const int64_t tiles = ((int64_t)n * page + 4 * kThreads - 1) / (4 * kThreads);
   MS_REQUIRE(tiles <= INT32_MAX, "ms_kv_copy_blocks: too many blocks");
   return over_layers(c, [&](const Pools& p, int count) {
-    launch_pdl(kv_copy_blocks_kernel<V>, dim3((unsigned)tiles, count), kThreads, 0, s, p, count, src,
+    launch_pdl(kv_copy_blocks_kernel<V>, dim3((unsigned)tiles, count), kThreads, 0, s, p, src,
                dst, n, page, c.num_blocks, device_error_word());
     return check_launch("kv_copy_blocks_kernel");
   });
@@ -185,28 +192,29 @@ template <typename V>
 int move_tokens(const ms_kv_cache& c, const int32_t* src, const int32_t* dst, int n_groups,
                 int per_group, int row_bytes, cudaStream_t s) {
   const int row = row_bytes / (int)sizeof(V), num_slots = c.num_blocks * c.block_size;
-  const int regs = ceil_div(per_group * row, 32);
   const int64_t units = (int64_t)n_groups * c.n_kv_heads;
   MS_REQUIRE(units <= INT32_MAX, "ms_kv_move_tokens: too many groups");
-  const unsigned warps = (unsigned)((units + kThreads / 32 - 1) / (kThreads / 32));
+  constexpr int kRegs = 3, kPools = 4;
+  int team = 32;
+  while (team < kThreads && team * kRegs < per_group * row) team *= 2;
+  const bool in_registers = team * kRegs >= per_group * row;
+  const int64_t ctas = (units * team + kThreads - 1) / kThreads;
   const int bytes = per_group * row_bytes;
   static std::atomic<uint64_t> granted{0};
-  if (regs > 8 && bytes > 48 * 1024) {
+  if (!in_registers && bytes > 48 * 1024) {
     if (bytes > 227 * 1024)
       return fail(MS_ERR_TOO_LARGE, "ms_kv_move_tokens: %d rows of %d bytes a group", per_group, row_bytes);
     MS_TRY(grant_dynamic_smem(kv_move_shared_kernel<V>, 227 * 1024, granted));
   }
   return over_layers(c, [&](const Pools& p, int count) {
     int* err = device_error_word();
-    if (regs <= 3)
-      launch_pdl(kv_move_kernel<V, 3, 4>, dim3(warps, ceil_div(count, 4)), kThreads, 0, s, p, count, src, dst, n_groups,
-                 per_group, row, c.block_size, c.n_kv_heads, num_slots, err);
-    else if (regs <= 8)
-      launch_pdl(kv_move_kernel<V, 8, 2>, dim3(warps, ceil_div(count, 2)), kThreads, 0, s, p, count, src, dst, n_groups,
-                 per_group, row, c.block_size, c.n_kv_heads, num_slots, err);
+    const int slices = (int)min((int64_t)ceil_div(count, kPools), (148 * 4 + ctas - 1) / ctas);
+    if (in_registers)
+      launch_pdl(kv_move_kernel<V, kRegs, kPools>, dim3((unsigned)ctas, slices), kThreads, 0, s, p, count, src, dst,
+                 n_groups, per_group, row, c.block_size, c.n_kv_heads, num_slots, team, err);
     else
-      launch_pdl(kv_move_shared_kernel<V>, dim3((unsigned)units, count), kThreads, bytes, s, p, count,
-                 src, dst, n_groups, per_group, row, c.block_size, c.n_kv_heads, num_slots, err);
+      launch_pdl(kv_move_shared_kernel<V>, dim3((unsigned)units, count), kThreads, bytes, s, p,
+                 src, dst, per_group, row, c.block_size, c.n_kv_heads, num_slots, err);
     return check_launch("kv_move_kernel");
   });
 }
