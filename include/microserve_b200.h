@@ -536,8 +536,8 @@ MS_API int ms_tree_masks(const int32_t* parents, const int32_t* q_start, int n_s
  *   logits: float32 rows of the nodes, logits_stride apart; the token is the largest
  *     logit's (lowest index of equals; NaN is never the largest).  Only rows on the path are read;
  *   target_tokens: (n_tokens), the tokens themselves.
- * batch: input_ids (the nodes' tokens), q_start, context_lens, block_tables, sizes; a sequence's
- * nodes stand at the last places of its context.
+ * batch: input_ids (the nodes' tokens), q_start, sizes, and for slots context_lens and
+ * block_tables; a sequence's nodes stand at the last places of its context.
  * Outputs, -1 past the accepted ones: out_tokens (n_seqs, max_accept + 1), out_num_accepted (n_seqs),
  * out_nodes (n_seqs, max_accept) the accepted nodes after node 0, and src_slots and
  * dst_slots (n_seqs, max_accept), both or neither: the moves for ms_kv_move_tokens that put them behind

@@ -138,7 +138,9 @@ __device__ __forceinline__ Best warp_best(Best m) {
 // node's row, a slice a CTA, the slices' bests exchanged through distributed
 // shared memory (two buffers in turn, so one cluster barrier a step), then the
 // lowest child with that token.  All CTAs of a cluster take the same steps.
-// Short rows, and tokens that are given, take one warp (8 trees of 7 nodes, 65 logits: 11.4 -> 8.8 us).
+// Short rows, and tokens that are given, take one warp: 256 trees take 8.7 us with it and 9.7 with 8
+// warps at 65 logits, 9.7 and 8.9 at 1024.  Long ones are bound by HBM, less the steps' barriers and
+// the rows' ends: 192 trees of 128256 logits, 672 rows of which are read (345 MB), 53 us, 6.5 TB/s.
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads) tree_accept_kernel(AcceptArgs a) {
   pdl_enter();
@@ -156,8 +158,8 @@ __global__ void __launch_bounds__(kThreads) tree_accept_kernel(AcceptArgs a) {
   load_parents(a.parents, t0, n, s_parent, a.err);
   for (int i = tid; i < n; i += kThreads) s_token[i] = a.ids[t0 + i];
   const int64_t held = (int64_t)a.max_blocks * a.bs;
-  int ctx = a.context_lens[b];
-  if (ctx < n || ctx > held) {
+  int ctx = a.src ? a.context_lens[b] : n;
+  if (a.src && (ctx < n || ctx > held)) {
     if (tid == 0) raise_device_error(a.err, kErrLength);
     ctx = ctx < n ? n : (int)held;
   }
@@ -172,7 +174,8 @@ __global__ void __launch_bounds__(kThreads) tree_accept_kernel(AcceptArgs a) {
     }
     return blk * a.bs + j % a.bs;
   };
-  __syncthreads();
+  // (shared memory of another CTA may be written once that CTA has started)
+  if (parts > 1) cluster.sync(); else __syncthreads();
 
   const int per = ((a.vocab + parts - 1) / parts + 3) & ~3;
   const int lo = min(rank * per, a.vocab), hi = min(lo + per, a.vocab);
@@ -275,7 +278,7 @@ extern "C" int ms_tree_accept(const float* logits, int64_t logits_stride, int vo
     return fail(MS_ERR_TOO_LARGE, "ms_tree_accept: trees of %d nodes (at most %d)", batch->max_q_len,
                 MS_TREE_MAX);
   if (batch->n_seqs == 0) return MS_OK;
-  MS_REQUIRE(batch->q_start && batch->context_lens && batch->block_tables && out_tokens &&
+  MS_REQUIRE(batch->q_start && (!src_slots || (batch->context_lens && batch->block_tables)) && out_tokens &&
                  out_num_accepted && (out_nodes || max_accept == 0) &&
                  (batch->n_tokens == 0 || (batch->input_ids && parents)),
              "ms_tree_accept: null pointer");
@@ -302,16 +305,17 @@ extern "C" int ms_tree_accept(const float* logits, int64_t logits_stride, int vo
   a.src = src_slots;
   a.dst = dst_slots;
   a.err = device_error_word();
-  // A cluster as wide as leaves all sequences resident (8 CTAs an SM), slices of at
-  // least 2048 logits.
+  // A cluster as wide as leaves all sequences resident (8 CTAs an SM), slices of at least 2560
+  // logits: 8 trees, 4096 logits, 1 CTA 8.7 us and 2 CTAs 10.7; 32000 logits, 1, 4 and 8 CTAs 19.3,
+  // 12.6 and 11.2 us; 192 trees, 128256 logits, 1 and 4 CTAs 103.6 and 52.9 us.
   int parts = 1;
-  while (logits && parts < 8 && (int64_t)batch->n_seqs * parts * 2 <= 148 * 8 && vocab / (parts * 2) >= 2048)
+  while (logits && parts < 8 && (int64_t)batch->n_seqs * parts * 2 <= 148 * 8 && vocab / (parts * 2) >= 2560)
     parts *= 2;
   if ((int64_t)batch->n_seqs * parts > INT_MAX)
     return fail(MS_ERR_TOO_LARGE, "ms_tree_accept: too many sequences");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(batch->n_seqs * parts));
-  const bool narrow = !logits || vocab <= 1024;
+  const bool narrow = !logits || vocab <= 512;
   cfg.blockDim = dim3(narrow ? 32 : kWide);
   cfg.stream = as_stream(stream);
   cudaLaunchAttribute attr[2] = {};

@@ -136,6 +136,26 @@ def test_the_walk(lens, most, vocab, by_logits) -> None:
     assert _lib.device_error() == 0
 
 
+def test_a_walk_without_moves_needs_no_cache() -> None:
+    """The C call with neither slots nor a cache's sizes: contexts are not looked at."""
+    from microserve_b200 import _lib
+    from microserve_b200.attention import pack_batch
+    from microserve_b200.tree import accept_trees
+
+    lens, most = [7, 33, 1], 5
+    batch, parents, ids, target, cached, tables, q_start, blocks = _case(5, lens, 65, 16, 0.9)
+    want = accept_trees(_i32(target), batch, _i32(parents), most, 16, blocks)
+    batch.context_lens = _i32([2 ** 30, -5, 0])
+    batch.block_tables = _i32(np.zeros((3, 0)))
+    target, parents = _i32(target), _i32(parents)
+    tokens, nodes, num = (torch.empty(n, dtype=torch.int32, device=DEV) for n in (18, 15, 3))
+    _lib.launch_on(_lib.cuda_index(tokens), "ms_tree_accept", None, 0, 0, target.data_ptr(),
+                   pack_batch(batch, _lib.cuda_index(tokens), True), parents.data_ptr(), most, 0, 0, tokens.data_ptr(),
+                   num.data_ptr(), nodes.data_ptr(), None, None)
+    assert torch.equal(tokens.view(3, 6), want.tokens) and torch.equal(num, want.num_accepted)
+    assert torch.equal(nodes.view(3, 5), want.nodes) and _lib.device_error() == 0
+
+
 def test_rows_of_infinities() -> None:
     """A row of -inf alone, or of NaN alone, gives token 0; +inf is the largest."""
     from microserve_b200.tree import accept_trees
