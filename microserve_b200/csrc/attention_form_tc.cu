@@ -1,22 +1,34 @@
 // Attention with score forms over bf16 caches on tcgen05, for many rows:
 // prompts and the rows of larger trees.
 //
+// With t = scale q k (capped, less slope x distance, -inf where unseen): p = 2^(t log2 e - m), O = sum p v,
+// l = sum p, out = O / l, and where m grows O and l are scaled by 2^(old - new).
+//
 // A CTA takes ST streams of 128 rows each of one kv head of one sequence (row r is
 // (token r / group, head-in-group r % group)) and a range of its keys, KC places
 // at a step; the streams share the keys and values.
-//   softmax warps (4 a stream)  a thread has a row: scores out of TMEM, cap,
-//        distance, mask (bits, only where some row does not see all keys), p =
-//        2^(x - m) rounded to bf16 back into TMEM over the scores, and the sum of the
-//        rounded values.  m is raised only when a row's maximum has grown by
-//        more than 2^8, so O is rescaled a few times a row at most;
+//   softmax warps  two threads (kParts) share a row, 32 scores of a step each: scores out of
+//        TMEM, cap, distance, mask (bits, only where some row does not see all keys), p
+//        rounded to bf16 back into TMEM over the scores, and the sum of the rounded values
+//        (the rounding of a dominant p cancels).  m is raised only when a row's maximum has
+//        grown by more than 2^8, so O is rescaled a few times a row at most;
 //   producer warp  TMA loads of whole pages (or parts of one), a lane a page, into
 //        rings of their own for K and V;
-//   MMA warp  one thread issues S = Q K^T (both from shared memory) and O += P V (P in
-//        TMEM, V MN-major as it lies in the page).  With SB score buffers the
-//        scores of the next SB steps are there when p of this one is.
-// Two shapes: ST 2, KC 128, SB 1, one CTA an SM (all 512 TMEM columns at d_head 128): the
-// streams' softmax and MMAs take turns; and ST 1, KC 64, SB 2, two CTAs an SM, for up to 128
-// rows, where HBM is the bound.
+//   MMA warp  S = Q K^T (both from shared memory) and O += P V (P in TMEM, V MN-major as it
+//        lies in the page).  With SB score buffers the scores of the next SB steps are
+//        there when p of this one is.
+// Three shapes.  kTwo: 256 rows in two streams, all of TMEM, one CTA an SM.  kOne: 128 rows, two CTAs an
+// SM.  kHalf: up to 64 rows, twice in the tile; each copy takes half of the step's keys, so that no
+// lane of the softmax idles, and the copies meet at the end; two CTAs an SM.
+//
+// What it measured: 64 trees of 33 to 61 nodes, 32 heads over 8 of 128, 1 to 4 k keys (127 GFLOP, 733 MB)
+// 221 us, 0.57 PFLOP/s and 3.3 TB/s; 4 prompts of up to 4096 with cap and prefix (309 GFLOP) 481 us,
+// 0.64 PFLOP/s; 256 trees of 8 nodes, 32 heads over 4 of 64, 1.3 k keys (351 MB) 95 us, 3.7
+// TB/s; one tree of 16 nodes over 32 k keys (134 MB) 42 us with the joining of its 37 ranges.
+// Every pipe is half idle (tensor 24 to 39%, issue 42 to 56%, SFU 24 to 32%): the bound is the chain of a
+// step, scores -> softmax (about 2400 cycles) -> values (1300 with the hand-offs), which two
+// streams or two CTAs overlap only in part, and what a CTA does before its first and after its
+// last step (8 to 10 thousand cycles of dependent loads, Q and the result).
 //
 // Values that no row should meet: where a mask is needed the softmax warps look
 // at the step's values first and put 0 for what is not finite.  If one of those belongs
@@ -31,7 +43,8 @@ namespace {
 
 constexpr int kTileRows = 128;
 
-// The shape of a CTA: up to 64 rows (twice, each copy half of the keys), 128, or 256 in two streams.
+// The shape of a CTA: up to 64 rows (twice, each copy half of the keys), 128, or 256 in two streams.  64 keys
+// a step with two score buffers took trees of heads of 64 from 215 to 197 us against 128 with one.
 enum Shape { kHalf, kOne, kTwo };
 
 template <int DH, int SH>

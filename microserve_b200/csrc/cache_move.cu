@@ -70,9 +70,9 @@ __device__ __forceinline__ bool move_pair(const int32_t* src, const int32_t* dst
 // at a time, and go through the pools of their slice (blockIdx.y of gridDim.y).  The
 // places are worked out once a slice: their divisions take longer than the copies of a pool.
 // Rows of 128 to 256 bytes lie anywhere, so what counts is how many are in flight: 192 groups, 32
-// layers, 8 heads of 128 take 20, 27 and 42 us for up to 5, 8 and 24 moves (6 us of which are the
-// launch and its gaps, 25, 40 and 115 MB), and at most 5 of them with 1, 2, 4 and 8 pools at a time 37,
-// 24, 20 and 20 us.  4 elements a thread: 23, 26 and 58 us.
+// layers, 8 heads of 128 take 20, 27 and 42 us for up to 5, 8 and 24 moves (82, 95 and 113 MB:
+// 4.2, 3.5 and 2.7 TB/s); with 4 elements a thread 23, 26 and 58 us, with 8 pools at a time
+// instead of 4 20, 27 and 43.
 template <typename V, int kRegs, int kPools>
 __global__ void __launch_bounds__(kThreads)
     kv_move_kernel(const __grid_constant__ Pools pools, int n_pools, const int32_t* __restrict__ src,

@@ -139,8 +139,9 @@ __device__ __forceinline__ Best warp_best(Best m) {
 // shared memory (two buffers in turn, so one cluster barrier a step), then the
 // lowest child with that token.  All CTAs of a cluster take the same steps.
 // Short rows, and tokens that are given, take one warp: 256 trees take 8.7 us with it and 9.7 with 8
-// warps at 65 logits, 9.7 and 8.9 at 1024.  Long ones are bound by HBM, less the steps' barriers and
-// the rows' ends: 192 trees of 128256 logits, 672 rows of which are read (345 MB), 53 us, 6.5 TB/s.
+// warps at 65 logits, 9.7 and 8.9 at 1024.  Long ones wait for HBM, at a rate that
+// falls as paths end: 192 trees of 128256 logits, 511 rows of which are read (262 MB), 53 us, 5.0 TB/s
+// (8 values of 16 bytes a thread in flight instead of 4 57 us, 2 of them 83; 512 threads 58).
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads) tree_accept_kernel(AcceptArgs a) {
   pdl_enter();
