@@ -473,7 +473,7 @@ MS_API int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache, cons
 /* What a query's scores are and which keys it sees, instead of plain causal
  * attention.  No reference counterpart, like everything in this section.
  *   x = c - slopes[h] * |p_q - p_k|,  c = softcap * tanh(s / softcap) (softcap
- *   0: c = s),  s = scale * q . k (scale 0: 1 / sqrt(d_head));
+ *   0: c = s; at least 1e-30 scale else),  s = scale * q . k (scale 0: 1 / sqrt(d_head));
  * the query at position p_q sees key j when j < prefix_lens[b], or when it is seen and
  * p_q - p_k < window (window 0: any): without a tree mask p_k = j <= p_q; with one
  * every key before the pass's own tokens is seen, and of those, which stand at

@@ -359,6 +359,9 @@ int form_args(FormArgs& a, const ms_kv_cache& c, int layer, const ms_batch& bt, 
                "ms_paged_attention_form: scale, softcap, window and mask_words must be >= 0 and finite");
     MS_REQUIRE(!form->tree_mask || form->mask_words > 0, "ms_paged_attention_form: a mask of no words");
     if (form->scale > 0.f) a.scale = form->scale;
+    // (scale / softcap is a factor of its own in the kernels)
+    MS_REQUIRE(form->softcap == 0.f || a.scale / form->softcap <= 1e30f,
+               "ms_paged_attention_form: a softcap of %g is too small for a scale of %g", form->softcap, a.scale);
     a.softcap = form->softcap;
     a.window = form->window;
     a.slopes = form->slopes;

@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       const uint32_t one = elect_one();
       // (values that the compiler knows to be the same in all lanes)
       const int n = __reduce_max_sync(0xffffffffu, steps);
-      const uint32_t cols = ST == 2 ? 0u : __any_sync(0xffffffffu, (tmem & 0xffffu) != 0) ? 256u : 0u;
+      const uint32_t cols = ST == 2 ? 0u : __reduce_max_sync(0xffffffffu, tmem);
       auto wait = [&](uint32_t bar, uint32_t parity) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, a.err));
       };

@@ -334,3 +334,77 @@ def test_pools_that_start_anywhere(dtype, shift, n) -> None:
         flat = torch.empty(t.numel() + shift, dtype=dtype, device=DEV)
         pools.append(flat[shift:].view(t.shape).copy_(t))
     check(paged_attention(x.q.to(DEV), *pools, x.batch(), x.form()), x)
+
+
+def test_a_cap_far_below_the_scale_is_refused() -> None:
+    from microserve_b200._lib import MicroserveError
+
+    for dtype, dh in ((F32, 32), (BF16, 64)):
+        x = make(24, dtype, 2, 2, dh, 16, [30], [4], softcap=1e-38, scale=1.0)
+        with pytest.raises(MicroserveError, match="too small"):
+            run(x)
+        x.softcap = 1e-20  # still a cap: scores of +-1e-20, every key alike
+        check(run(x), x)
+
+
+def test_calls_on_two_streams_at_once() -> None:
+    """Many sequences in order of their length, a long context in ranges, and a model's forward (other
+    tensor-core kernels) side by side."""
+    from microserve_b200.attention import paged_attention
+    from microserve_b200.batching import build_paged_batch
+    from microserve_b200.cache import PagedKVCache
+    from microserve_b200.config import CacheConfig, ModelConfig
+    from microserve_b200.model import Transformer
+
+    rng = np.random.default_rng(0)
+    xs = [make(25, BF16, 8, 4, 64, 16, rng.integers(1, 300, 130).tolist(), rng.integers(17, 33, 130).tolist(), tree=True),
+          make(26, BF16, 16, 2, 128, 16, [3000, 40], [30, 16], tree=True),
+          make(27, BF16, 8, 8, 64, 16, rng.integers(1, 300, 90).tolist(), [1] * 90, softcap=20.0)]
+    wants = [reference(x) for x in xs]
+    held = [(x.q.to(DEV), x.k.to(DEV), x.v.to(DEV), x.batch(), x.form()) for x in xs]
+    model = Transformer(ModelConfig(vocab_size=512, n_layers=2, d_model=512, n_heads=8, n_kv_heads=4, max_seq_len=256,
+                                    dtype="bfloat16"), DEV, seed=1)
+    cache = PagedKVCache(model.cfg, CacheConfig(16, 64, "bfloat16"), DEV)
+    prompts = [rng.integers(0, 512, 200).tolist() for _ in range(3)]
+    batch = build_paged_batch(cache, [0, 1, 2], prompts, [0, 0, 0])
+    logits = model.forward_paged(batch, cache).clone()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(6):
+        for s, h in zip(streams, held):
+            with torch.cuda.stream(s):
+                results.append(paged_attention(*h))
+        with torch.cuda.stream(streams[3]):
+            again = model.forward_paged(batch, cache)
+    torch.cuda.synchronize()
+    # (split sums of the projections are added in no fixed order: two passes alone differ too; each
+    # is within 2e-2 of its scale of the float32 model's, so they are within twice that)
+    assert float((again - logits).abs().max()) <= 4e-2 * max(1.0, float(logits.abs().max()))
+    for i, got in enumerate(results):
+        assert torch.equal(got, results[i % 3])
+    for got, x, want in zip(results, xs, wants):
+        check(got, x, want)
+
+
+@pytest.mark.parametrize("nodes", [1, 20])
+def test_a_captured_batch_takes_other_lengths(nodes) -> None:
+    """A graph of an ordered call, replayed with shorter contexts: nothing of the capture's lengths stays."""
+    from microserve_b200.attention import paged_attention
+
+    rng = np.random.default_rng(1)
+    n = 160
+    x = make(28, BF16, 8, 4, 64, 16, rng.integers(200, 400, n).tolist(), [nodes] * n)
+    q, k, v, batch, form = x.q.to(DEV), x.k.to(DEV), x.v.to(DEV), x.batch(), x.form()
+    out = torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        paged_attention(q, k, v, batch, form, out)
+    g.replay()
+    check(out, x)
+    x.context = [int(c) for c in rng.integers(nodes, 200, n)]
+    x.positions = np.concatenate([np.arange(c - nodes, c) for c in x.context]).astype(np.int32)
+    batch.context_lens.copy_(torch.tensor(x.context, dtype=torch.int32))
+    batch.positions.copy_(torch.from_numpy(x.positions))
+    g.replay()
+    check(out, x)

@@ -372,6 +372,73 @@ def test_no_form_in_a_forward_is_the_plain_forward() -> None:
     torch.testing.assert_close(logits[0], logits[1], rtol=1e-4, atol=1e-5)
 
 
+def test_a_tree_with_adapters() -> None:
+    """Forms and adapters in one pass: a chain as a tree is the plain forward with the same adapters."""
+    from microserve_b200.attention import AttentionForm
+    from microserve_b200.batching import build_paged_batch
+    from microserve_b200.lora import LoraAdapters
+    from microserve_b200.tree import tree_masks
+
+    from .test_gpu_controls_engine import adapter_state
+
+    model = _model()
+    ads = LoraAdapters(model)
+    ads.load("a", adapter_state(model.cfg, 4, 1, ("attn.q_proj", "attn.v_proj", "ffn.down_proj"), 8.0))
+    prompts = [[1, 2, 3, 4, 5, 6, 7], [4, 5], [9] * 40]
+    lens = [len(p) for p in prompts]
+    logits = []
+    for adapter, tree in ((None, False), ("a", False), ("a", True)):
+        cache = _cache(model)
+        batch = build_paged_batch(cache, [0, 1, 2], prompts, [0, 0, 0])
+        parents = _i32(np.concatenate([np.arange(n) - 1 for n in lens]))
+        form = AttentionForm(tree_mask=tree_masks(parents, batch.q_start, batch.max_q)[0]) if tree else None
+        lora = ads.plan([adapter] * 3, lens) if adapter else None
+        logits.append(model.forward_paged(batch, cache, lora=lora, form=form).clone())
+    torch.testing.assert_close(logits[1], logits[2], rtol=1e-4, atol=1e-5)
+    assert float((logits[0] - logits[1]).abs().max()) > 0.01
+
+
+def test_masks_walk_and_moves_in_a_graph() -> None:
+    """A captured round on a side stream, replayed with other target tokens and another tree."""
+    from microserve_b200 import _lib
+    from microserve_b200.cache import move_tokens
+    from microserve_b200.tree import accept_trees, tree_masks
+
+    lens, most, bs, vocab = [9, 40, 1, 17], 6, 16, 65
+    case = _case(31, lens, vocab, bs, 0.9)
+    batch, blocks = case[0], case[-1]
+    pool = torch.randn((2, 2, blocks, 2, bs, 16), device=DEV)
+    parents, target = _i32(case[1]), _i32(case[3])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            masks, depths = tree_masks(parents, batch.q_start, max(lens))
+            got = accept_trees(target, batch, parents, most, bs, blocks)
+            move_tokens(pool, got.src_slots, got.dst_slots)
+    torch.cuda.synchronize()
+    for seed in (31, 32, 33):
+        other = _case(seed, lens, vocab, bs, 0.9)
+        parents.copy_(_i32(other[1]))
+        target.copy_(_i32(other[3]))
+        batch.input_ids.copy_(_i32(other[2]))
+        before = pool.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            g.replay()
+        side.synchronize()
+        want = _walk(lens, other[1], other[2], other[3], case[4], case[5], case[6], bs, most)
+        for name, w in zip(("tokens", "num_accepted", "nodes", "src_slots", "dst_slots"), want):
+            assert np.array_equal(getattr(got, name).cpu().numpy(), w), name
+        for s, d in zip(want[3].ravel(), want[4].ravel()):
+            if s >= 0:
+                assert torch.equal(pool[:, :, d // bs, :, d % bs], before[:, :, s // bs, :, s % bs])
+        plain = tree_masks(parents, batch.q_start, max(lens))
+        assert torch.equal(masks, plain[0]) and torch.equal(depths, plain[1])
+    assert _lib.device_error() == 0
+
+
 def test_verify_trees_refuses_and_leaves_the_cache() -> None:
     from microserve_b200.config import SamplingConfig
     from microserve_b200.tree import verify_trees
