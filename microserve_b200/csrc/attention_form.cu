@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
 // A row a block: the ranges' weights 2^(m - max) first, then their sums, a range
 // a warp at a time with 16 bytes a lane, the warps' sums added in order: the result
 // does not depend on timing.  (A warp a row, range after range, took 24 us for 37
-// ranges of 64 rows x 8 kv heads; this takes 9 with nothing in the caches.)
+// ranges of 64 rows x 8 kv heads; this about 4.  Three ranges a warp are loaded before their weights are known:
+// attention and joining 37.6 -> 35.8 us.)
 template <typename T, bool kBase2>
 __global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows, int dh) {
   pdl_enter();
@@ -191,13 +192,23 @@ __global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows,
   __shared__ float s_red[32];
   const int b = blockIdx.z, g = blockIdx.y, rr = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const FormSeq s = form_seq(a, b);
-  if (rr >= s.qlen * a.group) return;
   const int tile = rr / rows, r = rr - tile * rows;
   const int64_t unit0 = (((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + unit0 * rows + r;
+  const float* po = a.part_o + (unit0 * rows + r) * dh;
+  // (rows that the sequence does not have are part of the workspace too: nothing waits for its length)
+  constexpr int kAhead = 3;
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const int i = warp + u * warps;
+    if (i < a.n_splits && lane * 4 < dh)
+      ahead[u] = *reinterpret_cast<const float4*>(po + (int64_t)i * rows * dh + lane * 4);
+  }
   float mx = -INFINITY;
   for (int i = threadIdx.x; i < a.n_splits; i += blockDim.x) mx = fmaxf(mx, ml[(int64_t)i * rows].x);
+  const FormSeq s = form_seq(a, b);
+  if (rr >= s.qlen * a.group) return;
   mx = warp_max(mx);
   if (lane == 0) s_red[warp] = mx;
   __syncthreads();
@@ -212,19 +223,21 @@ __global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows,
     l = fmaf(w, v.y, l);
   }
   l = block_sum(l, s_red);  // (its barriers cover the weights)
-  const float* po = a.part_o + (unit0 * rows + r) * dh;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float w, const float4& v) {
+    if (w == -1.f) return;
+    acc.x = fmaf(w, v.x, acc.x);
+    acc.y = fmaf(w, v.y, acc.y);
+    acc.z = fmaf(w, v.z, acc.z);
+    acc.w = fmaf(w, v.w, acc.w);
+  };
   if (lane * 4 < dh) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (warp + u * warps < a.n_splits) add(s_comb[warp + u * warps], ahead[u]);
 #pragma unroll 4
-    for (int i = warp; i < a.n_splits; i += warps) {
-      const float w = s_comb[i];
-      if (w == -1.f) continue;
-      const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)i * rows * dh + lane * 4);
-      acc.x = fmaf(w, v.x, acc.x);
-      acc.y = fmaf(w, v.y, acc.y);
-      acc.z = fmaf(w, v.z, acc.z);
-      acc.w = fmaf(w, v.w, acc.w);
-    }
+    for (int i = warp + kAhead * warps; i < a.n_splits; i += warps)
+      add(s_comb[i], *reinterpret_cast<const float4*>(po + (int64_t)i * rows * dh + lane * 4));
   }
   float* sums = s_comb + ((a.n_splits + 3) & ~3);
   if (lane * 4 < dh) *reinterpret_cast<float4*>(sums + warp * dh + lane * 4) = acc;
@@ -240,7 +253,9 @@ __global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows,
 }
 
 // Tiles of `rows` rows; KV ranges where the tiles alone leave SMs without work,
-// of at least `least` keys and in whole chunks of `chunk`, up to `wave` CTAs in all.
+// of at least `least` keys and in whole chunks of `chunk`, up to `wave` CTAs in all.  (Not where a little more
+// than a wave is left: the ranges' sums cost more than the second wave, 123 against 87 us for 40
+// trees of 16 nodes over up to 4 k keys.)
 void plan(FormArgs& a, int max_context, int rows, int chunk, int least, int wave) {
   int64_t span = max_context;
   if (a.window > 0 && !a.prefix) span = min(span, (int64_t)a.window + a.max_q + 2 * a.bs);
@@ -286,7 +301,11 @@ Way choose(FormArgs& a, const ms_kv_cache& c, int max_context) {
   // The least tile that holds a sequence (us; trees of 64 sequences, heads of 128): 64 rows in a tile of
   // 64 and of 128 127 and 137; 128 rows in 128 and 256 145 and 185; 192 rows in two of 128 and one of
   // 256 257 and 221.
-  w.rows = w.kernel == kTma ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  // Sequences of up to 64 rows that fit in one wave take tiles of 128 too, whose second score buffer makes a
+  // step shorter: one tree of 16 nodes, 8 kv heads, 400, 8 k and 32 k keys 13.1, 19.7 and 37.3 us instead
+  // of 14.9, 21.4 and 38.5, 32 of them over 2 k keys 53.3 instead of 55.0.
+  const bool few = (int64_t)a.n_seqs * c.n_kv_heads <= 148 * 2;
+  w.rows = w.kernel == kTma ? 32 : rows <= 64 && !few ? 64 : rows <= 128 ? 128 : 256;
   const int resident = 148 * (w.kernel == kTma ? 3 : w.rows == 256 ? 1 : 2);
   if (w.kernel == kTma)
     plan(a, max_context, w.rows, 64, 512, 148 * 4);

@@ -18,13 +18,13 @@
 //        lies in the page).  With SB score buffers the scores of the next SB steps are
 //        there when p of this one is.
 // Three shapes.  kTwo: 256 rows in two streams, all of TMEM, one CTA an SM.  kOne: 128 rows, two CTAs an
-// SM.  kHalf: up to 64 rows, twice in the tile; each copy takes half of the step's keys, so that no
+// SM.  kHalf: up to 64 rows of many sequences, twice in the tile; each copy takes half of the step's keys, so that no
 // lane of the softmax idles, and the copies meet at the end; two CTAs an SM.
 //
 // What it measured: 64 trees of 33 to 61 nodes, 32 heads over 8 of 128, 1 to 4 k keys (127 GFLOP, 733 MB)
 // 221 us, 0.57 PFLOP/s and 3.3 TB/s; 4 prompts of up to 4096 with cap and prefix (309 GFLOP) 481 us,
 // 0.64 PFLOP/s; 256 trees of 8 nodes, 32 heads over 4 of 64, 1.3 k keys (351 MB) 95 us, 3.7
-// TB/s; one tree of 16 nodes over 32 k keys (134 MB) 42 us with the joining of its 37 ranges.
+// TB/s; one tree of 16 nodes over 32 k keys (134 MB) 36 us with the joining of its 37 ranges (kOne).
 // Every pipe is half idle (tensor 24 to 39%, issue 42 to 56%, SFU 24 to 32%): the bound is the chain of a
 // step, scores -> softmax (about 2400 cycles) -> values (1300 with the hand-offs), which two
 // streams or two CTAs overlap only in part, and what a CTA does before its first and after its

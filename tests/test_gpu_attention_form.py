@@ -408,3 +408,56 @@ def test_a_captured_batch_takes_other_lengths(nodes) -> None:
     batch.positions.copy_(torch.from_numpy(x.positions))
     g.replay()
     check(out, x)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dh,hq,bs", [(64, 32, 16), (128, 32, 64), (64, 48, 8)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_many_sequences_of_few_tokens(tree, dh, hq, bs, form) -> None:
+    """More sequences and kv heads than run at once, of up to 64 rows a sequence and kv head."""
+    rng = np.random.default_rng(2)
+    n = 45
+    q_lens = [int(t) for t in rng.integers(0, 64 // (hq // 8) + 1, n)]
+    q_lens[:3] = [64 // (hq // 8), 1, 64 // (hq // 8)]
+    cached = rng.integers(0, 150, n).tolist()
+    x = make(30, BF16, hq, 8, dh, bs, cached, q_lens, tree=tree, **FORMS[form])
+    check(run(x), x)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan"), 3.3e38])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("tree", [False, True])
+def test_many_sequences_of_which_some_hold_anything(tree, dh, value) -> None:
+    """What a row does not see, or sees, beside many others: as for few sequences."""
+    n = 40
+    x = make(31, BF16, 32, 8, dh, 16, [37, 5] * (n // 2), [9, 14] * (n // 2), tree=tree, prefix=[3, 0] * (n // 2))
+    page, at = x.tables[4, (37 + 2) // 16], (37 + 2) % 16  # the third of the pass's own tokens
+    x.v[page, :, at, 5] = value
+    x.k[page, :, at] = value
+    own = [r for r in range(int(x.q_start[4]), int(x.q_start[5]))
+           if 37 + 2 in visible(x, 4, r - int(x.q_start[4]))[0]]
+    got = run(x).double().cpu()
+    ref, tol = reference(x)
+    keep = torch.ones(len(ref), dtype=torch.bool)
+    keep[own] = False
+    assert own and len(own) < 9 and bool(((got - ref).abs() <= tol)[keep].all())
+    # a key alone is as other sequences' are: only its value is out of the ordinary
+    x.k[page, :, at] = 0.25
+    got, (ref, tol) = run(x).double().cpu(), reference(x)
+    rest = [d for d in range(dh) if d != 5]
+    assert bool(((got - ref).abs() <= tol)[:, :, rest].all())
+    if not np.isfinite(value):
+        assert torch.equal(got[own][:, :, 5].isfinite(), ref[own][:, :, 5].isfinite())
+        assert torch.equal(got[own][:, :, 5].isnan(), ref[own][:, :, 5].isnan())
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+def test_many_sequences_that_see_nothing(dh) -> None:
+    n = 44
+    x = make(32, BF16, 32, 8, dh, 16, [0, 20] * (n // 2), [7, 12] * (n // 2), tree=True)
+    x.masks[:] = False
+    x.window = 5  # of the cached keys only the last few remain
+    x.positions += 100  # (and those are out of the window)
+    got = run(x)
+    assert not bool(got.any())
+    check(got, x)
