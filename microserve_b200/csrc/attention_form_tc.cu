@@ -11,7 +11,8 @@
 //        TMEM, cap, distance, mask (bits, only where some row does not see all keys), p
 //        rounded to bf16 back into TMEM over the scores, and the sum of the rounded values
 //        (the rounding of a dominant p cancels).  m is raised only when a row's maximum has
-//        grown by more than 2^8, so O is rescaled a few times a row at most;
+//        grown by more than 2^8, so O is rescaled a few times a row at most (and values from
+//        2^128 / (256 keys) on may overflow float32 where the formula's result does not);
 //   producer warp  TMA loads of whole pages (or parts of one), a lane a page, into
 //        rings of their own for K and V;
 //   MMA warp  S = Q K^T (both from shared memory) and O += P V (P in TMEM, V MN-major as it
