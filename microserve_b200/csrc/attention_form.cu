@@ -49,8 +49,8 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
   if (r0 >= nrows) return;
   const int nr = min(ROWS, nrows - r0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int minpos, maxpos;
-  position_range(a, s, r0, nr, minpos, maxpos);
+  int minpos = 0, maxpos = 0;
+  if (needs_positions(a)) position_range(a, s, r0, nr, minpos, maxpos);
   const T* q = static_cast<const T*>(a.q);
   for (int idx = threadIdx.x; idx < nr * DH; idx += blockDim.x) {
     const int r = idx / DH, d = idx - r * DH, rr = r0 + r;

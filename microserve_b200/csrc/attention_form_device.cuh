@@ -76,6 +76,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float low_half(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_half(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
+// Whether the keys of a tile depend on its tokens' positions.  A tree without a window takes every key up to its
+// context's end, and a round trip less before its first load (1.1B trees 93.7 -> 91.4 us, 8B 218 -> 214).
+__device__ __forceinline__ bool needs_positions(const FormArgs& a) { return !a.mask || a.window > 0; }
 // Smallest and largest position of the tokens of rows [r0, r0 + nr) (the whole warp calls it).
 __device__ __forceinline__ void position_range(const FormArgs& a, const FormSeq& s, int r0, int nr,
                                                int& lo, int& hi) {

@@ -88,8 +88,8 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
   if (r0 >= s.qlen * a.group) return;
   const int nr = min(kRows, s.qlen * a.group - r0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int minpos, maxpos;
-  position_range(a, s, r0, nr, minpos, maxpos);
+  int minpos = 0, maxpos = 0;
+  if (needs_positions(a)) position_range(a, s, r0, nr, minpos, maxpos);
   const FormKeys keys = form_keys(a, s, minpos, maxpos);
   const int xbeg = min(split * a.split_len, keys.total);
   const int xend = split == a.n_splits - 1 ? keys.total : min(keys.total, xbeg + a.split_len);
