@@ -23,13 +23,15 @@
 // lane of the softmax idles, and the copies meet at the end; two CTAs an SM.
 //
 // What it measured: 64 trees of 33 to 61 nodes, 32 heads over 8 of 128, 1 to 4 k keys (127 GFLOP, 733 MB)
-// 221 us, 0.57 PFLOP/s and 3.3 TB/s; 4 prompts of up to 4096 with cap and prefix (309 GFLOP) 481 us,
-// 0.64 PFLOP/s; 256 trees of 8 nodes, 32 heads over 4 of 64, 1.3 k keys (351 MB) 95 us, 3.7
-// TB/s; one tree of 16 nodes over 32 k keys (134 MB) 36 us with the joining of its 37 ranges (kOne).
-// Every pipe is half idle (tensor 24 to 39%, issue 42 to 56%, SFU 24 to 32%): the bound is the chain of a
-// step, scores -> softmax (about 2400 cycles) -> values (1300 with the hand-offs), which two
-// streams or two CTAs overlap only in part, and what a CTA does before its first and after its
-// last step (8 to 10 thousand cycles of dependent loads, Q and the result).
+// 215 us, 0.59 PFLOP/s and 3.4 TB/s; 4 prompts of up to 4096 with cap and prefix (309 GFLOP) 485 us,
+// 0.64 PFLOP/s; 256 trees of 8 nodes, 32 heads over 4 of 64, 1.3 k keys (351 MB) 92 us, 3.8
+// TB/s; one tree of 16 nodes over 32 k keys (134 MB) 35 us with the joining of its 37 ranges (kOne).
+// Every pipe is half idle (tensor 24 to 39%, issue 42 to 56%, SFU 24 to 32%).  The bound of kTwo is the
+// softmax of a step, about 2200 cycles (2700 with a cap) for 64 keys: TMEM load 160, maxima
+// and vote 400, exponentials 750 to 1100 for the four warps of a scheduler, the store and its hand-off
+// 350; products and copies are done by then.  The bound of kHalf at heads of 64 is the copy unit, 73
+// cycles for a page of 2 KB.  Before its first and after its last step a CTA spends 12 to 16 thousand
+// cycles on loads that depend on one another, Q and the result.
 //
 // Values that no row should meet: where a mask is needed the softmax warps look
 // at the step's values first and put 0 for what is not finite.  If one of those belongs
