@@ -287,7 +287,7 @@ class PagedKVCache:
         # Bumped whenever a sequence gains or loses its table row, so callers
         # may keep ``rows_of`` results while it is unchanged.
         self.generation = 0
-        # Bumped whenever blocks change places (:meth:`compact`).
+        # Bumped whenever blocks of a sequence change (:meth:`compact`, :meth:`unshare_many`).
         self.moves = 0
         self._table = np.zeros((8, self._max_blocks), dtype=np.int32)
         self._freed = np.empty(cache.num_blocks, dtype=np.int32)  # truncate_many's output
@@ -586,6 +586,7 @@ class PagedKVCache:
         for (row, col, old), block in zip(todo, new, strict=True):
             self._table[row, col] = block
             self.allocator.free(old)
+        self.moves += bool(todo)
         self._copy([old for _, _, old in todo], new)
 
     def compact(self) -> int:

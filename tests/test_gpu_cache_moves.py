@@ -220,3 +220,45 @@ def test_pools_beyond_four_gigabytes() -> None:
     move_tokens(pool, _i32([[last + 5, 3 * 16 + 1]]), _i32([[3 * 16 + 1, last + 9]]))
     assert torch.equal(pool[:, :, 3, :, 1], was[:, :, 1, :, 5])
     assert torch.equal(pool[:, :, blocks - 2, :, 9], was[:, :, 0, :, 1])
+
+
+@pytest.mark.parametrize("which", ["target", "draft", "both"])
+def test_compaction_between_chained_rounds(golden, which) -> None:
+    """The caches of a speculative decoder compacted between rounds, with the next round's draft side
+    planned on the device already: the streams stay what they are without."""
+    from microserve_b200.cache import PagedKVCache
+    from microserve_b200.config import CacheConfig, SamplingConfig
+    from microserve_b200.scheduler import Request
+    from microserve_b200.speculative import SpeculativeDecoder
+
+    from .test_gpu_model import device_model
+
+    target, draft = device_model(golden, "target"), device_model(golden, "draft")
+    rng = np.random.default_rng(5)
+    prompts = [rng.integers(0, 32, int(n)).tolist() for n in rng.integers(2, 20, 6)]
+    sc = SamplingConfig(temperature=0.9, top_k=20, max_new_tokens=200)
+
+    def serve(compact: bool):
+        dec = SpeculativeDecoder(target, draft, CacheConfig(8, 128), gamma=3)
+        cache = PagedKVCache(target.cfg, CacheConfig(8, 128), DEV)
+        reqs = [Request(i, list(p), sc) for i, p in enumerate(prompts)]
+        gens = {i: torch.Generator().manual_seed(900 + i) for i in range(6)}
+        live, moved = [0, 1, 2, 3, 4, 5], 0
+        for call in range(9):
+            if call == 3:  # holes in the middle of both pools
+                for i in (1, 4):
+                    cache.free(i)
+                    dec.free(i)
+                live = [0, 2, 3, 5]
+            if compact and call in (4, 5, 7):
+                moved += cache.compact() if which != "draft" else 0
+                moved += dec.draft_cache.compact() if which != "target" else 0
+                cache.allocator.check_invariants()
+            for i, toks in zip(live, dec.step([reqs[i] for i in live], cache, gens), strict=True):
+                reqs[i].output_ids.extend(toks)
+        return [r.output_ids for r in reqs], moved, dec
+
+    want, _, plain = serve(False)
+    got, moved, dec = serve(True)
+    assert got == want and moved > 0
+    assert dec.lookahead_hits > 0 and (which == "target" or plain.lookahead_hits > dec.lookahead_hits)

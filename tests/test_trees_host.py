@@ -208,3 +208,14 @@ def test_a_cache_without_a_device_moves_no_tensors() -> None:
         copy_blocks(pool, i, i)
     with pytest.raises(RuntimeError):
         move_tokens(pool, i.view(1, 1), i.view(1, 1))
+
+
+def test_unsharing_counts_as_a_change_of_blocks() -> None:
+    """A planned round holds its tables on the device: it is dropped when a block of them is replaced."""
+    c = _cache()
+    c.append(0, 5)
+    c.fork(0, 1)
+    c.unshare_many([1])
+    assert c.moves == 1
+    c.unshare_many([0, 1])  # nothing is shared any more
+    assert c.moves == 1
