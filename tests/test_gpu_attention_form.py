@@ -461,3 +461,31 @@ def test_many_sequences_that_see_nothing(dh) -> None:
     got = run(x)
     assert not bool(got.any())
     check(got, x)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,dh,n,cached", [
+    (F32, 4, 2, 32, 3, [40, 900]), (BF16, 8, 2, 64, 1, [40, 2000]), (BF16, 16, 2, 128, 9, [40, 3000]),
+    (BF16, 16, 2, 64, 16, [40, 90]), (BF16, 16, 2, 128, 40, [40, 2500]), (BF16, 16, 8, 64, 17, [30] * 40)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_padded_batches(tree, dtype, hq, hkv, dh, n, cached) -> None:
+    """Rows behind the last sequence keep what they held; sequences without tokens, whose tables hold no
+    block at all, do nothing; nor is any of it read."""
+    from microserve_b200.attention import paged_attention
+
+    x = make(33, dtype, hq, hkv, dh, 16, cached, [n] * len(cached), tree=tree, alibi=True)
+    B, T, extra = len(cached), n * len(cached), 21
+    b, form = x.batch(), x.form()
+    behind = lambda t, count, value: torch.cat([t, torch.full((count, *t.shape[1:]), value, dtype=t.dtype, device=DEV)])  # noqa: E731
+    b.positions = behind(b.positions, extra, -(1 << 31))
+    b.input_ids, b.slot_mapping = behind(b.input_ids, extra, -1), behind(b.slot_mapping, extra, -1)
+    b.q_start = behind(b.q_start, 2, T)
+    b.q_lens, b.context_lens = behind(b.q_lens, 2, 0), behind(b.context_lens, 2, 0)
+    b.block_tables = behind(b.block_tables, 2, -1)
+    b.n_tokens = T + extra
+    if tree:
+        form.tree_mask = behind(form.tree_mask, extra, -1)
+    q = behind(x.q.to(DEV), extra, float("nan"))
+    out = torch.full_like(q, 7.0)
+    paged_attention(q, x.k.to(DEV), x.v.to(DEV), b, form, out)
+    assert bool((out[T:] == 7).all())
+    check(out[:T], x)

@@ -156,6 +156,33 @@ def test_a_walk_without_moves_needs_no_cache() -> None:
     assert torch.equal(nodes.view(3, 5), want.nodes) and _lib.device_error() == 0
 
 
+@pytest.mark.parametrize("vocab", [65, 32000])
+def test_the_walk_of_a_padded_batch(vocab) -> None:
+    """Rows behind the last sequence are not read, and sequences without nodes emit nothing."""
+    from microserve_b200 import _lib
+    from microserve_b200.tree import accept_trees, tree_masks
+
+    lens, most = [7, 0, 12], 4
+    batch, parents, ids, target, cached, tables, q_start, blocks = _case(9, lens, vocab, 16, 0.9)
+    want = _walk(lens, parents, ids, target, cached, tables, q_start, 16, most)
+    plain = tree_masks(_i32(parents), batch.q_start, batch.max_q)
+    T, extra = sum(lens), 5
+    parents, target = np.append(parents, [10 ** 6] * extra), np.append(target, [-7] * extra)
+    batch.input_ids = _i32(np.append(ids, [-1] * extra))
+    batch.positions = batch.slot_mapping = _i32(np.zeros(T + extra))
+    batch.n_tokens = T + extra
+    logits = torch.full((T + extra, vocab), float("nan"), device=DEV)
+    logits[:T] = 0.0
+    logits[torch.arange(T, device=DEV), _i32(target[:T]).long()] = 1.0
+    for t in (_i32(target), logits):
+        got = accept_trees(t, batch, _i32(parents), most, 16, blocks)
+        for name, w in zip(("tokens", "num_accepted", "nodes", "src_slots", "dst_slots"), want):
+            assert np.array_equal(getattr(got, name).cpu().numpy(), w), name
+    masks, depths = tree_masks(_i32(parents), batch.q_start, batch.max_q)
+    assert torch.equal(masks[:T], plain[0]) and torch.equal(depths[:T], plain[1])
+    assert _lib.device_error() == 0
+
+
 def test_rows_of_infinities() -> None:
     """A row of -inf alone, or of NaN alone, gives token 0; +inf is the largest."""
     from microserve_b200.tree import accept_trees
@@ -370,6 +397,37 @@ def test_no_form_in_a_forward_is_the_plain_forward() -> None:
         cache = _cache(model)
         logits.append(model.forward_paged(build_paged_batch(cache, [0, 1], [[1, 2, 3], [4]], [0, 0]), cache, form=form))
     torch.testing.assert_close(logits[0], logits[1], rtol=1e-4, atol=1e-5)
+
+
+def test_forwards_with_a_form_in_two_graphs() -> None:
+    """Each graph has a workspace of its own, whatever runs between, larger passes among it."""
+    from microserve_b200.attention import AttentionForm
+    from microserve_b200.batching import build_paged_batch
+
+    model = _model()
+    rng = np.random.default_rng(3)
+    form = AttentionForm(softcap=2.0, window=9)
+    runs = []
+    for n in (5, 60):
+        prompts = [rng.integers(0, 61, n).tolist() for _ in range(3)]
+        cache = _cache(model)
+        batch = build_paged_batch(cache, [0, 1, 2], prompts, [0, 0, 0])
+        want = model.forward_paged(batch, cache, form=form).clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = model.forward_paged(batch, cache, form=form)
+        runs.append((g, got, want, batch, cache))
+    big = _cache(model, blocks=400)
+    model.forward_paged(build_paged_batch(big, list(range(12)), [[1] * 200] * 12, [0] * 12), big, form=form)
+    junk = [torch.full((1 << 20,), 7.0, device=DEV) for _ in range(8)]  # over whatever was freed
+    for _ in range(2):
+        for g, got, *_ in runs:
+            got.zero_()
+            g.replay()
+        for _, got, want, batch, cache in runs:
+            torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-5)
+            torch.testing.assert_close(model.forward_paged(batch, cache, form=form), want, rtol=1e-4, atol=1e-5)
+    assert all(bool((j == 7).all()) for j in junk)
 
 
 def test_a_tree_with_adapters() -> None:
