@@ -489,3 +489,17 @@ def test_padded_batches(tree, dtype, hq, hkv, dh, n, cached) -> None:
     paged_attention(q, x.k.to(DEV), x.v.to(DEV), b, form, out)
     assert bool((out[T:] == 7).all())
     check(out[:T], x)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,dh", [(F32, 2, 1, 32), (BF16, 4, 1, 64), (BF16, 2, 2, 128)])
+def test_the_largest_tree(dtype, hq, hkv, dh) -> None:
+    x = make(34, dtype, hq, hkv, dh, 16, [33, 500], [1024, 3], tree=True, alibi=True, window=300)
+    check(run(x), x)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [1, 30, 200])
+def test_prefixes_of_any_length(dtype, n) -> None:
+    """Longer than the context, and below zero: as the whole context, and as none."""
+    x = make(35, dtype, 4, 2, 64, 16, [50, 50, 50, 0], [n] * 4, prefix=[10 ** 9, -3, 51, n + 1], window=7)
+    check(run(x), x)
