@@ -46,9 +46,9 @@ def _pack_pool(pool: torch.Tensor, index: int) -> tuple[bytes, np.ndarray]:
     shape = pool.shape
     base = _lib.check_tensor(pool, "pool", pool.dtype, index, shape)
     layers = shape[1]
-    at = np.arange(base, base + 2 * layers * pool.stride(1) * pool.element_size(),
-                   pool.stride(1) * pool.element_size(), dtype=np.uint64) if pool.numel() else \
-        np.zeros(2 * layers, np.uint64)
+    # (a pool of one layer may have any stride there and still be contiguous: the step goes by the sizes)
+    step = shape[2] * shape[3] * shape[4] * shape[5] * pool.element_size()
+    at = base + step * np.arange(2 * layers, dtype=np.uint64)
     where = _addr(at)
     return _PACK_CACHE(layers, shape[2], shape[4], shape[3], shape[5], _CODES[pool.dtype], where,
                        where + 8 * layers), at
