@@ -287,7 +287,8 @@ class PagedKVCache:
         # Bumped whenever a sequence gains or loses its table row, so callers
         # may keep ``rows_of`` results while it is unchanged.
         self.generation = 0
-        # Bumped whenever blocks of a sequence change (:meth:`compact`, :meth:`unshare_many`).
+        # Bumped whenever blocks of a sequence change (:meth:`compact`, :meth:`unshare_many`,
+        # :meth:`unshare_last_block`).
         self.moves = 0
         self._table = np.zeros((8, self._max_blocks), dtype=np.int32)
         self._freed = np.empty(cache.num_blocks, dtype=np.int32)  # truncate_many's output
@@ -536,6 +537,7 @@ class PagedKVCache:
             self.pool[:, :, new].copy_(self.pool[:, :, old])
         self._table[row, n - 1] = new
         self.allocator.free(old)
+        self.moves += 1
 
     def fork_many(self, parent_id: int, child_ids: Sequence[int]) -> None:
         """:meth:`fork` for several children, each with its own copy of a last block that is not
