@@ -26,7 +26,7 @@ import torch
 from . import _lib
 from .attention import AttentionForm, pack_batch
 from .batching import batch_from_host, host_batch_arrays, pack_int32
-from .cache import PagedKVCache, move_tokens
+from .cache import MAX_MOVES, PagedKVCache, move_tokens
 from .config import SamplingConfig
 from .sampling import make_params, params_to_device, validate
 
@@ -196,8 +196,11 @@ def verify_trees(
                            None, None, None, None)
         most = max(max(d) for d in depths)
         got = accept_trees(target, batch, parents_dev, most, cache.block_size, cache.cfg.num_blocks)
-        if most:
-            move_tokens(cache.pool, got.src_slots, got.dst_slots)
+        # (a path's nodes never stand before their new places, so what a later call still has to read
+        # is not written by an earlier one)
+        for at in range(0, most, MAX_MOVES):
+            src, dst = (t[:, at : at + MAX_MOVES].contiguous() for t in (got.src_slots, got.dst_slots))
+            move_tokens(cache.pool, src, dst)
         accepted = got.num_accepted.tolist()
         emitted = [row[: n + 1] for row, n in zip(got.tokens.tolist(), accepted)]
         kept = [n + 1 + k for n, k in zip(before, accepted)]
