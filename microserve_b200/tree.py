@@ -173,7 +173,13 @@ def verify_trees(
         held = cache.tables[s].blocks[n // cache.block_size :] if s in cache.tables else []
         if any(cache.allocator.refcount(block) > 1 for block in held):
             raise ValueError(f"sequence {s} shares its last block with another: unshare it first")
-    parts, width, max_q, n_tokens = host_batch_arrays(cache, seq_ids, [t for t, _ in trees], before)
+    new = [s for s in seq_ids if s not in cache.tables]
+    try:
+        parts, width, max_q, n_tokens = host_batch_arrays(cache, seq_ids, [t for t, _ in trees], before)
+    except BaseException:
+        for s in new:
+            cache.free(s)
+        raise
     emitted, kept = [], list(before)
     try:
         parts[1] = np.array([n + k for n, d in zip(before, depths) for k in d], np.int32)
@@ -204,6 +210,9 @@ def verify_trees(
         accepted = got.num_accepted.tolist()
         emitted = [row[: n + 1] for row, n in zip(got.tokens.tolist(), accepted)]
         kept = [n + 1 + k for n, k in zip(before, accepted)]
+        new = []
     finally:
         cache.truncate_many(seq_ids, kept)
+        for s in new:  # (only an error leaves any)
+            cache.free(s)
     return emitted
