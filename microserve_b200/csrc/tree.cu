@@ -248,7 +248,7 @@ extern "C" int ms_tree_masks(const int32_t* parents, const int32_t* q_start, int
   MS_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && max_nodes >= 0, "ms_tree_masks: bad sizes");
   if (max_nodes > MS_TREE_MAX)
     return fail(MS_ERR_TOO_LARGE, "ms_tree_masks: trees of %d nodes (at most %d)", max_nodes, MS_TREE_MAX);
-  if (n_seqs == 0 || n_tokens == 0 || max_nodes == 0) return MS_OK;
+  if (n_seqs == 0 || n_tokens == 0) return MS_OK;
   MS_REQUIRE(parents && q_start && masks, "ms_tree_masks: null pointer");
   MS_REQUIRE(mask_words >= ceil_div(max_nodes, 32), "ms_tree_masks: %d words for %d nodes", mask_words,
              max_nodes);
