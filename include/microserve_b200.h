@@ -519,7 +519,8 @@ MS_API int ms_forward_form(const ms_model* model, const ms_kv_cache* cache, cons
 
 /* Trees of tokens, one per sequence: sequence b's nodes are tokens [q_start[b],
  * q_start[b+1]), and parents[] gives each node's parent by its number in its tree, an earlier node
- * (-1: none, a root).  Sizes up to max_nodes, at most MS_TREE_MAX.
+ * (-1: none, a root).  Sizes up to max_nodes, at most MS_TREE_MAX; max_nodes * mask_words
+ * below 2^31.
  *
  * masks: (n_tokens, mask_words) rows for ms_attention_form (a node sees its ancestors and
  * itself), depths (n_tokens; nullable): ancestors of each node.  A parent that is no earlier node

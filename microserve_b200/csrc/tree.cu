@@ -252,6 +252,9 @@ extern "C" int ms_tree_masks(const int32_t* parents, const int32_t* q_start, int
   MS_REQUIRE(parents && q_start && masks, "ms_tree_masks: null pointer");
   MS_REQUIRE(mask_words >= ceil_div(max_nodes, 32), "ms_tree_masks: %d words for %d nodes", mask_words,
              max_nodes);
+  // (the kernel's row indices are 32 bits wide)
+  MS_REQUIRE((int64_t)max_nodes * mask_words <= INT_MAX, "ms_tree_masks: %d words for each of %d nodes",
+             mask_words, max_nodes);
   const int64_t bytes = (int64_t)max_nodes * mask_words * 4;
   const bool shared = bytes <= 32 * 1024;  // with the parents and depths within 48 KB
   launch_pdl(tree_masks_kernel, n_seqs, 128, shared ? (size_t)bytes : 0, as_stream(stream), parents,
