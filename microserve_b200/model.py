@@ -390,12 +390,9 @@ class Transformer:
             cl, cp = ref(self.adapters.c_struct()), ref(lora.c_struct(batch.n_tokens, self.device))
         need = int(_lib.load().ms_forward_form_workspace_size(ref(self._c_model), ref(cc), ref(cb), cf,
                                                               cl, n_rows))
-        ws = self._ws
-        capturing = torch.cuda.is_current_stream_capturing()  # a graph keeps a workspace of its own
-        if capturing or ws is None or ws.numel() < need:
-            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
-            if not capturing:
-                self._ws = ws
+        # a workspace of the call's own: passes on two streams, captured ones and those without a form
+        # do not meet in it
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=self.device)
         _lib.call("ms_forward_form", ref(self._c_model), ref(cc), ref(cb), cf, cl, cp, rows_ptr, n_rows,
                   out_ptr, out_row_stride, ws.data_ptr(), ws.numel(), _lib.stream_ptr(self.device))
         return out
