@@ -223,9 +223,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// (a NaN among the three is the result)
 __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
   return d;
 }
 __device__ __forceinline__ float min3(float a, uint32_t b, uint32_t c) {
@@ -234,7 +235,7 @@ __device__ __forceinline__ float min3(float a, uint32_t b, uint32_t c) {
   return d;
 }
 
-// The largest (or smallest) of 32 values.
+// The largest of 32 values, NaN if there is one; or the smallest.
 template <bool kMax>
 __device__ __forceinline__ float reduce(const uint32_t (&x)[32]) {
   float v[4];
@@ -245,7 +246,9 @@ __device__ __forceinline__ float reduce(const uint32_t (&x)[32]) {
     float& to = v[(c >> 1) & 3];
     to = kMax ? max3(to, x[c], x[c + 1]) : min3(to, x[c], x[c + 1]);
   }
-  return kMax ? fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) : fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
+  if constexpr (kMax)
+    return max3(max3(v[0], __float_as_uint(v[1]), __float_as_uint(v[2])), __float_as_uint(v[3]), __float_as_uint(v[3]));
+  return fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
 }
 
 // Adds the two bf16 of a word to two float32 sums.
@@ -274,7 +277,7 @@ struct Cap {
     d2 = d0 * (0.132533633f * kk * kk);
     d3 = d0 * (-0.0498660865f * kk * kk * kk);
     d4 = d0 * (0.0127505842f * kk * kk * kk * kk);
-    limit = k <= 1024.f ? 0.75f / k : -1.f;  // (k^8 stays within float32)
+    limit = k <= 1024.f ? fminf(0.75f / k, FLT_MAX) : -1.f;  // (k^8 stays within float32)
   }
   __device__ __forceinline__ uint64_t series(uint64_t v) const {
     const uint64_t w = mul2(v, v);
@@ -291,7 +294,7 @@ struct Cap {
 // 2^x of two values on the FMA units: x = n + f, |f| <= 1/2 (n by adding and taking off 1.5 2^23), 2^f
 // by a cubic (fitted to the least maximum of the relative error, 1.0e-4, a fortieth of bf16's
 // rounding), n into the exponent.  From -128 down that leaves a negative word, and 0 (an unseen key's p
-// has to be 0: its value may be anything finite).
+// has to be 0: its value may be anything finite).  NaN is taken for -128: the caller sees to such a row.
 __device__ __forceinline__ void exp2_fma(uint64_t v, float& lo, float& hi) {
   float a, b;
   unpair(v, a, b);
@@ -734,7 +737,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
         // `way` says what the exponent still has to do (see exps).  Almost every step of a long context
         // is plain: all keys seen, no maximum grown, the cap's series good for all
         int way = capped ? 1 : 0;
-        if (any_part(!free || sloped || top > plain_top || bottom < plain_bottom)) {
+        if (any_part(!free || sloped || !(top <= plain_top) || bottom < plain_bottom)) {
           // some score is beyond the cap's series
           const bool far = capped && any_part(!(top <= cap.limit && bottom >= -cap.limit));
           if (!free || sloped || far) {
@@ -777,6 +780,8 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           } else {
             top = capped ? cap.exact(top) : top * lin;
           }
+          // a seen score of NaN or +inf: the row is NaN, whatever becomes of the exponentials (see exp2_fma)
+          if (!(top < INFINITY)) l = NAN;
           if constexpr (C::kParts == 2) {
             st32(mine_at, top);
             any_part(false);
@@ -802,7 +807,9 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
             }
           }
           // (tanh(u) <= u for u >= 0: a capped score grows past the limit only if s * lin does)
-          plain_top = !capped ? (m + 8.f) / lin : m + 8.f >= 0.f ? fminf((m + 8.f) / lin, cap.limit) : -INFINITY;
+          // An infinite score is never plain.
+          plain_top = fminf((m + 8.f) / lin, capped ? cap.limit : FLT_MAX);
+          if (capped && m + 8.f < 0.f) plain_top = -INFINITY;
         }
         const float sub = m == -INFINITY ? 0.f : m;
         if (way == 0)
