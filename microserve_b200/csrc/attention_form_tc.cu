@@ -36,7 +36,8 @@
 // Values that no row should meet: where a mask is needed the softmax warps look
 // at the step's values first and put 0 for what is not finite.  If one of those belongs
 // to a key that some row may see, the CTA computes its rows again on the
-// CUDA cores, key by key.
+// CUDA cores, key by key.  kHalf does so too when a copy's sums are not finite: an infinite value in a step
+// without a mask is multiplied by the zeros that stand for the other copy's weights.
 #include <cfloat>
 
 #include "attention_form_device.cuh"
@@ -844,16 +845,26 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     float w0 = 1.f, w1 = 0.f;
     const uint32_t meet = k_s + (t & 63) * 4, meet_o = meet + 512 + dim0 * 256;  // floats [value][row]
     if constexpr (C::kTwin) {
-      if (t >= 64 && warp_live) {
-        st32(meet, m);
-        st32(meet + 256, l);
+      if (warp_live) {
+        if (t >= 64) {
+          st32(meet, m);
+          st32(meet + 256, l);
+        }
+        float zero = 0.f;  // NaN if a sum is not finite
 #pragma unroll
         for (int c = 0; c < kMyDims; c += 32) {
           uint32_t o[32] = {};
           if (steps > 0) tmem_ld(o_col + c, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) st32(meet_o + (c + e) * 256, __uint_as_float(o[e]));
+          for (int e = 0; e < 32; ++e) zero = fmaf(__uint_as_float(o[e]), 0.f, zero);
+          if (t >= 64) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) st32(meet_o + (c + e) * 256, __uint_as_float(o[e]));
+          }
         }
+        // an infinite value times the other copy's weights, which are 0 here (a sum of weights that is not
+        // finite itself makes the row NaN by itself)
+        if (live && zero != 0.f && l < INFINITY) *odd = 1;
       }
       asm volatile("bar.sync 1, %0;" ::"r"(ST * C::kSoft * 32) : "memory");
       if (t < 64 && warp_live) {
