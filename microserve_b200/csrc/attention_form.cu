@@ -125,7 +125,9 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
         }
         int distance = 0;
         const bool sees = kk < n && form_sees(a, s, tok[i], pos[i], keys.key(x0 + min(kk, n - 1)), distance);
-        v = a.softcap > 0.f ? a.softcap * tanhf(v * inv_cap) : v * a.scale;
+        // (tanh(u) = u to 3e-9 up to 1e-4, where u itself may be too small for float32)
+        const float raw = v * a.scale;
+        v = a.softcap > 0.f && !(fabsf(raw) <= 1e-4f * a.softcap) ? a.softcap * tanhf(v * inv_cap) : raw;
         if (a.slopes) v -= slope[i] * fabsf((float)distance);
         x[u] = sees ? v : -INFINITY;
         seen[u] = __ballot_sync(0xffffffffu, sees);

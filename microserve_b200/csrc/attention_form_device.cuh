@@ -4,6 +4,8 @@
 
 #include <cuda.h>
 
+#include <cfloat>
+
 #include "attention_form.cuh"
 
 namespace ms {
@@ -75,6 +77,69 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 __device__ __forceinline__ float low_half(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_half(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// Two floats in a register pair: the packed operations of sm_100 halve the issue slots.
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t twice(float v) { return pair(__float_as_uint(v), __float_as_uint(v)); }
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// cap tanh(u) in base 2, u = k s, k = scale / cap.  For |u| <= 0.75 an odd polynomial (tanh(u) = u (1 + c1 u^2 +
+// .. + c4 u^8), fitted to the least maximum of |error|, 2.7e-7; no SFU), beyond that cap (1 - 2 / (1 + e^2u)),
+// whose error is 2^-22 of the cap and so only good where the score is near it.
+struct Cap {
+  static constexpr float c1 = -0.333280453f, c2 = 0.132533633f, c3 = -0.0498660865f, c4 = 0.0127505842f;
+  float d0, d1, d2, d3, d4;  // of s, s^3, ...
+  float limit;               // of |s| for `series`
+  float cap2, k;
+  __device__ __forceinline__ void set(const FormArgs& a) {
+    cap2 = fminf(a.softcap * kLog2e, FLT_MAX);
+    k = fmaxf(a.scale / a.softcap, 1e-44f);  // (not 0: an infinite score is capped too)
+    const float kk = k * k;
+    d0 = a.scale * kLog2e;
+    d1 = d0 * (c1 * kk);
+    d2 = d0 * (c2 * kk * kk);
+    d3 = d0 * (c3 * kk * kk * kk);
+    d4 = d0 * (c4 * kk * kk * kk * kk);
+    // k^8 has to stay within float32.  Below 1e-4 it does not, but up to |u| = 0.03 the terms that are lost do not
+    // matter (s^2 stays within float32 too).
+    limit = k > 1024.f ? -1.f : k >= 1e-4f ? 0.75f / k : fminf(0.03f / k, 1e19f);
+  }
+  // |s| <= limit: the coefficients take k in.
+  __device__ __forceinline__ uint64_t series(uint64_t v) const {
+    const uint64_t w = mul2(v, v);
+    uint64_t c = fma2(w, twice(d4), twice(d3));
+    c = fma2(w, c, twice(d2));
+    c = fma2(w, c, twice(d1));
+    return mul2(v, fma2(w, c, twice(d0)));
+  }
+  // Any s (NaN stays NaN).
+  __device__ __forceinline__ float any(float s) const {
+    const float u = s * k, w = u * u;
+    const float near = s * d0 * fmaf(w, fmaf(w, fmaf(w, fmaf(w, c4, c3), c2), c1), 1.f);
+    const float far = cap2 * fmaf(-2.f, fast_rcp(1.f + fast_exp2(u * (2.f * kLog2e))), 1.f);
+    return fabsf(u) <= 0.75f ? near : far;
+  }
+};
 
 // Whether the keys of a tile depend on its tokens' positions.  A tree without a window takes every key up to its
 // context's end, and a round trip less before its first load (1.1B trees 93.7 -> 91.4 us, 8B 218 -> 214).

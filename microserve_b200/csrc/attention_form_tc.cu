@@ -199,31 +199,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t v) {
   return __vcmpeq2(v & 0x7f807f80u, 0x7f807f80u);
 }
 
-// Two floats in a register pair: the packed operations of sm_100 halve the issue slots.
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-  return d;
-}
-__device__ __forceinline__ uint64_t twice(float v) { return pair(__float_as_uint(v), __float_as_uint(v)); }
-__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // (a NaN among the three is the result)
 __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
   float d;
@@ -261,36 +236,6 @@ __device__ __forceinline__ void add_bf16(uint32_t v, float& lo, float& hi) {
       : "+f"(lo), "+f"(hi)
       : "r"(v));
 }
-
-// cap tanh(u) in base 2, u = k s.  For |u| <= 0.75 an odd polynomial in s (tanh(u) = u (1 + c1
-// u^2 + .. + c4 u^8), fitted to the least maximum of |error|, 2.7e-7; no SFU), whose
-// coefficients take k in; else cap (1 - 2 / (1 + e^2u)), off by 2^-22 of the cap.
-struct Cap {
-  float d0, d1, d2, d3, d4;  // of s, s^3, ...
-  float limit;               // of |s|
-  float cap2, in;
-  __device__ __forceinline__ void set(const FormArgs& a) {
-    cap2 = a.softcap * kLog2e;
-    const float k = a.scale / a.softcap, kk = k * k;
-    in = 2.f * kLog2e * k;
-    d0 = a.scale * kLog2e;
-    d1 = d0 * (-0.333280453f * kk);
-    d2 = d0 * (0.132533633f * kk * kk);
-    d3 = d0 * (-0.0498660865f * kk * kk * kk);
-    d4 = d0 * (0.0127505842f * kk * kk * kk * kk);
-    limit = k <= 1024.f ? fminf(0.75f / k, FLT_MAX) : -1.f;  // (k^8 stays within float32)
-  }
-  __device__ __forceinline__ uint64_t series(uint64_t v) const {
-    const uint64_t w = mul2(v, v);
-    uint64_t c = fma2(w, twice(d4), twice(d3));
-    c = fma2(w, c, twice(d2));
-    c = fma2(w, c, twice(d1));
-    return mul2(v, fma2(w, c, twice(d0)));
-  }
-  __device__ __forceinline__ float exact(float s) const {
-    return fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(s * in)), cap2);
-  }
-};
 
 // 2^x of two values on the FMA units: x = n + f, |f| <= 1/2 (n by adding and taking off 1.5 2^23), 2^f
 // by a cubic (fitted to the least maximum of the relative error, 1.0e-4, a fortieth of bf16's
@@ -746,7 +691,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
             way = capped || sloped ? 2 : 0;
             if (capped && far) {
 #pragma unroll
-              for (int c = 0; c < W; ++c) x[c] = __float_as_uint(cap.exact(__uint_as_float(x[c])));
+              for (int c = 0; c < W; ++c) x[c] = __float_as_uint(cap.any(__uint_as_float(x[c])));
             } else if (capped) {
 #pragma unroll
               for (int c = 0; c < W; c += 2) {
@@ -779,7 +724,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
             top = reduce<true>(x);
             if (way == 0) top *= lin;
           } else {
-            top = capped ? cap.exact(top) : top * lin;
+            top = capped ? cap.any(top) : top * lin;
           }
           // a seen score of NaN or +inf: the row is NaN, whatever becomes of the exponentials (see exp2_fma)
           if (!(top < INFINITY)) l = NAN;

@@ -59,6 +59,12 @@ template <int DH>
 __device__ __forceinline__ uint32_t tile_addr(uint32_t tile, int k, int c) {
   return tile + (uint32_t)((k >> 3) * (DH * 16) + (c >> 3) * 1024 + (k & 7) * 128 + (((c & 7) ^ (k & 7)) << 4));
 }
+// The largest of |a|, |b| and |c|, NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -177,7 +183,8 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
     slope_b = a.slopes[g * a.group + (r0 + min(rb, nr - 1)) % a.group] * kLog2e;
   }
   const bool cap = a.softcap > 0.f;
-  const float cap2 = a.softcap * kLog2e, cap_in = cap ? 2.f * kLog2e * a.scale / a.softcap : 0.f;
+  Cap capped{};
+  if (cap) capped.set(a);
   // scores as the exponent takes them: x * mul
   const float mul = cap || a.slopes ? 1.f : a.scale * kLog2e;
   const float lin = a.scale * kLog2e;
@@ -214,13 +221,29 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
       const bool free = all_see<kCh>(a, s, keys, x0, xend, minpos, maxpos);
       // ---- scores: cap, distance
       if (cap) {
-        // cap tanh(t) = cap (1 - 2 / (1 + e^2t)): off by 2^-22 cap at most
+        float top[4] = {};  // of |score|, NaN if there is one
 #pragma unroll
-        for (int i = 0; i < kCh / 8; ++i)
+        for (int i = 0; i < kCh / 8; ++i) {
+          top[i & 1] = max3_abs(top[i & 1], sc[i][0], sc[i][1]);
+          if (upper) top[2 + (i & 1)] = max3_abs(top[2 + (i & 1)], sc[i][2], sc[i][3]);
+        }
+        // some score is beyond the cap's series
+        const bool far = !(max3_abs(top[0], top[1], max3_abs(0.f, top[2], top[3])) <= capped.limit);
+        if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < 2 || upper)
-              sc[i][e] = fmaf(-2.f * cap2, fast_rcp(1.f + fast_exp2(sc[i][e] * cap_in)), cap2);
+          for (int i = 0; i < kCh / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < 2 || upper) sc[i][e] = capped.any(sc[i][e]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kCh / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+              if (e < 2 || upper)
+                unpair(capped.series(pair(__float_as_uint(sc[i][e]), __float_as_uint(sc[i][e + 1]))), sc[i][e],
+                       sc[i][e + 1]);
+        }
       }
       if (a.slopes) {
         const float in = cap ? 1.f : lin;
