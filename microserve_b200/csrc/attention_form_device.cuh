@@ -13,6 +13,10 @@ namespace ms {
 constexpr int kErrTimeout = 5;
 constexpr long long kFormWaitCycles = 1ll << 32;
 constexpr float kLog2e = 1.4426950408889634f;
+// Scores (in base 2) up to this size enter the exponent as one fma(product, scale, -maximum): the maximum's own
+// rounding is 2^-4 at most, and cancels.  Larger ones are rounded like their maximum first, so that the
+// largest gives exactly 2^0: at 2^33 a maximum is off by 2^9, and its weight would be 0 or infinite.
+constexpr float kBig = 1048576.f;
 
 __device__ __forceinline__ uint32_t s_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -121,8 +125,8 @@ struct Cap {
     d3 = d0 * (c3 * kk * kk * kk);
     d4 = d0 * (c4 * kk * kk * kk * kk);
     // k^8 has to stay within float32.  Below 1e-4 it does not, but up to |u| = 0.03 the terms that are lost do not
-    // matter (s^2 stays within float32 too).
-    limit = k > 1024.f ? -1.f : k >= 1e-4f ? 0.75f / k : fminf(0.03f / k, 1e19f);
+    // matter (s^2 stays within float32 too).  Scores that pass kBig are all computed alike: equal ones stay equal.
+    limit = k > 1024.f || cap2 > kBig ? -1.f : k >= 1e-4f ? 0.75f / k : fminf(0.03f / k, 1e19f);
   }
   // |s| <= limit: the coefficients take k in.
   __device__ __forceinline__ uint64_t series(uint64_t v) const {

@@ -619,6 +619,8 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           : "memory");
       return any != 0;
     };
+    // whether a score (or a maximum of some) is too large for its product with `lin` to be taken as it is
+    auto beyond = [](float v) { return fabsf(v) > kBig && v > -INFINITY; };
     // a wait that gives up sets `stop`: the later ones return at once, and nothing is written
     auto wait = [&](uint32_t bar, uint32_t parity) {
       mbar_wait(bar, parity, stop, a.err);
@@ -728,10 +730,18 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           }
           // a seen score of NaN or +inf: the row is NaN, whatever becomes of the exponentials (see exp2_fma)
           if (!(top < INFINITY)) l = NAN;
+          bool big = beyond(top) || beyond(m);
           if constexpr (C::kParts == 2) {
             st32(mine_at, top);
-            any_part(false);
+            big = any_part(big);
             top = fmaxf(top, ld32(other_at));
+          } else {
+            big = any_part(big);
+          }
+          if (way == 0 && big) {
+            way = 2;
+#pragma unroll
+            for (int c = 0; c < W; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * lin);
           }
           const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
           // (the same for all threads of a row, and the barrier keeps `share` until all have read it)
@@ -755,7 +765,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           // (tanh(u) <= u for u >= 0: a capped score grows past the limit only if s * lin does)
           // An infinite score is never plain.
           plain_top = fminf((m + 8.f) / lin, capped ? cap.limit : FLT_MAX);
-          if (capped && m + 8.f < 0.f) plain_top = -INFINITY;
+          if ((capped && m + 8.f < 0.f) || fabsf(m) > kBig) plain_top = -INFINITY;
         }
         const float sub = m == -INFINITY ? 0.f : m;
         if (way == 0)

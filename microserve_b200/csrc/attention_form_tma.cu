@@ -283,6 +283,14 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
       const float mn_a = fmaxf(m_a, mx_a * mul), mn_b = fmaxf(m_b, mx_b * mul);
       const bool grow = mn_a > m_a || mn_b > m_b;
       const float sub_a = mn_a == -INFINITY ? 0.f : mn_a, sub_b = mn_b == -INFINITY ? 0.f : mn_b;
+      float by = mul;
+      if (__any_sync(0xffffffffu, fmaxf(fabsf(sub_a), fabsf(sub_b)) > kBig)) {
+        by = 1.f;
+#pragma unroll
+        for (int i = 0; i < kCh / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][e] *= mul;
+      }
       const float al_a = fast_exp2(m_a - sub_a), al_b = fast_exp2(m_b - sub_b);
       m_a = mn_a;
       m_b = mn_b;
@@ -291,10 +299,10 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
       float ps_a = 0.f, ps_b = 0.f;
 #pragma unroll
       for (int i = 0; i < kCh / 8; ++i) {
-        const uint32_t pa = pack2(fast_exp2(fmaf(sc[i][0], mul, -sub_a)), fast_exp2(fmaf(sc[i][1], mul, -sub_a)));
+        const uint32_t pa = pack2(fast_exp2(fmaf(sc[i][0], by, -sub_a)), fast_exp2(fmaf(sc[i][1], by, -sub_a)));
         uint32_t pb = 0;
         if (upper)
-          pb = pack2(fast_exp2(fmaf(sc[i][2], mul, -sub_b)), fast_exp2(fmaf(sc[i][3], mul, -sub_b)));
+          pb = pack2(fast_exp2(fmaf(sc[i][2], by, -sub_b)), fast_exp2(fmaf(sc[i][3], by, -sub_b)));
         ps_a += low_half(pa) + high_half(pa);
         ps_b += low_half(pb) + high_half(pb);
         pf[i / 2][(i & 1) * 2] = pa;
