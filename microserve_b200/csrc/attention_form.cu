@@ -32,7 +32,7 @@ __device__ __forceinline__ float4 load4(const T* p) {
 // e, everything in float32.  The small models that take this kernel are bound by latency:
 // 8 trees of 7 tokens, 4 heads of 32, contexts up to 97: 8.5 us, 14.2 with 32 keys a step.
 template <typename T, int DH>
-__global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
+__global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(const __grid_constant__ FormArgs a) {
   pdl_enter();
   constexpr int PER_LANE = DH >= 32 ? DH / 32 : 1;
   constexpr int RPW = rows_per_warp<DH>();
@@ -162,27 +162,34 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(FormArgs a) {
     const int r = warp + i * kWarps;
     if (r >= nr) continue;
     const int rr = r0 + r;
+    const int64_t part_row = ((((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split) * ROWS + r;
+    float zero = 0.f;  // NaN if a sum is not finite
+#pragma unroll
+    for (int e = 0; e < PER_LANE; ++e) zero = fmaf(acc[i][e], 0.f, zero);
+    if (__any_sync(0xffffffffu, zero != 0.f) && l[i] < INFINITY) {
+      form_row_by_key<T, DH, false>(a, s, keys, table, g, rr, xbeg, xend, 0, DH, part_row);
+      continue;
+    }
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
     if (a.n_splits == 1) {
-      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
       T* o = static_cast<T*>(a.out) + (int64_t)(s.t0 + rr / a.group) * a.out_stride +
              (int64_t)(g * a.group + rr % a.group) * DH;
 #pragma unroll
       for (int e = 0; e < PER_LANE; ++e)
         if (DH >= 32 || lane < DH) o[lane + 32 * e] = from_f<T>(acc[i][e] * inv);
     } else {
-      const int64_t unit = (((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split;
 #pragma unroll
       for (int e = 0; e < PER_LANE; ++e)
-        if (DH >= 32 || lane < DH) a.part_o[(unit * ROWS + r) * DH + lane + 32 * e] = acc[i][e];
+        if (DH >= 32 || lane < DH) a.part_o[part_row * DH + lane + 32 * e] = acc[i][e] * inv;
       if (lane == 0) {
-        a.part_ml[(unit * ROWS + r) * 2] = m[i];
-        a.part_ml[(unit * ROWS + r) * 2 + 1] = l[i];
+        a.part_ml[part_row * 2] = m[i];
+        a.part_ml[part_row * 2 + 1] = l[i];
       }
     }
   }
 }
 
-// A row a block: the ranges' weights 2^(m - max) first, then their sums, a range
+// A row a block: the ranges' weights l 2^(m - max) over their sum first, then the ranges' results, a range
 // a warp at a time with 16 bytes a lane, the warps' sums added in order: the result
 // does not depend on timing.  (A warp a row, range after range, took 24 us for 37
 // ranges of 64 rows x 8 kv heads; this about 4.  Three ranges a warp are loaded before their weights are known:
@@ -221,13 +228,15 @@ __global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows,
     const float2 v = ml[(int64_t)i * rows];
     // (a range without a key for this row has a sum of 0, and its values may be unset)
     const float w = v.y == 0.f ? 0.f : kBase2 ? exp2f(v.x - sub) : expf(v.x - sub);
-    s_comb[i] = v.y == 0.f ? -1.f : w;
+    s_comb[i] = v.y == 0.f ? -1.f : w * v.y;
     l = fmaf(w, v.y, l);
   }
   l = block_sum(l, s_red);  // (its barriers cover the weights)
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float w, const float4& v) {
     if (w == -1.f) return;
+    w *= inv;
     acc.x = fmaf(w, v.x, acc.x);
     acc.y = fmaf(w, v.y, acc.y);
     acc.z = fmaf(w, v.z, acc.z);
@@ -244,13 +253,12 @@ __global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows,
   float* sums = s_comb + ((a.n_splits + 3) & ~3);
   if (lane * 4 < dh) *reinterpret_cast<float4*>(sums + warp * dh + lane * 4) = acc;
   __syncthreads();
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   T* o = static_cast<T*>(a.out) + (int64_t)(s.t0 + rr / a.group) * a.out_stride +
          (int64_t)(g * a.group + rr % a.group) * dh;
   for (int d = threadIdx.x; d < dh; d += blockDim.x) {
     float v = 0.f;
     for (int w = 0; w < warps; ++w) v += sums[w * dh + d];
-    o[d] = from_f<T>(v * inv);
+    o[d] = from_f<T>(v);
   }
 }
 

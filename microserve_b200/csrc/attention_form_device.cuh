@@ -82,6 +82,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float low_half(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_half(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
+// The largest of |a|, |b| and |c|, NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Two floats in a register pair: the packed operations of sm_100 halve the issue slots.
 __device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
   uint64_t d;

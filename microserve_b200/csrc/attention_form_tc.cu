@@ -11,8 +11,7 @@
 //        TMEM, cap, distance, mask (bits, only where some row does not see all keys), p
 //        rounded to bf16 back into TMEM over the scores, and the sum of the rounded values
 //        (the rounding of a dominant p cancels).  m is raised only when a row's maximum has
-//        grown by more than 2^8, so O is rescaled a few times a row at most (and values from
-//        2^128 / (256 keys) on may overflow float32 where the formula's result does not);
+//        grown by more than 2^8, so O is rescaled a few times a row at most;
 //   producer warp  TMA loads of whole pages (or parts of one), a lane a page, into
 //        rings of their own for K and V;
 //   MMA warp  S = Q K^T (both from shared memory) and O += P V (P in TMEM, V MN-major as it
@@ -36,8 +35,9 @@
 // Values that no row should meet: where a mask is needed the softmax warps look
 // at the step's values first and put 0 for what is not finite.  If one of those belongs
 // to a key that some row may see, the CTA computes its rows again on the
-// CUDA cores, key by key.  kHalf does so too when a copy's sums are not finite: an infinite value in a step
-// without a mask is multiplied by the zeros that stand for the other copy's weights.
+// CUDA cores, key by key.  So is a row whose sums are not finite at the end: large values that overflow
+// float32 before the division by l (p reaches 2^8), or an infinite one in a step without a mask, which kHalf
+// multiplies by the zeros that stand for the other copy's weights.
 #include <cfloat>
 
 #include "attention_form_device.cuh"
@@ -310,62 +310,6 @@ __device__ __forceinline__ float exps(const uint32_t (&x)[32], uint32_t* p16, fl
     for (int j = 0; j < 8; ++j) add_bf16(p[j], sum[2 * (j & 1)], sum[2 * (j & 1) + 1]);
   }
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-}
-
-// The rows of a CTA once more, a warp a row: every seen key by itself, a lane a key for the
-// scores and DH / 32 dimensions a lane for the sums.
-template <int DH>
-__device__ __noinline__ void rows_by_key(const FormArgs& a, const FormSeq& s, const FormKeys& keys,
-                                         const int32_t* table, int g, int r0, int nr, int xbeg, int xend,
-                                         int64_t part_row0, int warp, int warps) {
-  const int lane = threadIdx.x & 31;
-  const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16*>(a.k), *vp = static_cast<const __nv_bfloat16*>(a.v);
-  for (int r = warp; r < nr; r += warps) {
-    const int rr = r0 + r, tok = s.t0 + rr / a.group, head = g * a.group + rr % a.group;
-    const int pos = a.positions[tok];
-    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * DH;
-    const float slope = a.slopes ? a.slopes[head] : 0.f;
-    float m = -INFINITY, l = 0.f, acc[DH / 32] = {};
-    for (int x0 = xbeg; x0 < xend; x0 += 32) {
-      const int x = min(x0 + lane, xend - 1), j = keys.key(x);
-      int distance = 0;
-      const bool seen = x0 + lane < xend && form_sees(a, s, tok, pos, j, distance);
-      const int64_t at =
-          (((int64_t)form_block(a, table, j / a.bs) * a.hkv + g) * a.bs + j % a.bs) * DH;
-      float v = 0.f;
-      for (int d = 0; d < DH; ++d) v = fmaf(to_f(q[d]), to_f(kp[at + d]), v);
-      v = a.softcap > 0.f ? a.softcap * tanhf(v * a.scale / a.softcap) : v * a.scale;
-      v = seen ? (v - slope * fabsf((float)distance)) * kLog2e : -INFINITY;
-      const uint32_t all = __ballot_sync(0xffffffffu, seen);
-      const float mn = fmaxf(m, warp_max(v)), sub = mn == -INFINITY ? 0.f : mn;
-      const float alpha = m == -INFINITY ? 0.f : exp2f(m - sub), p = seen ? exp2f(v - sub) : 0.f;
-      l = l * alpha + warp_sum(p);
-      m = mn;
-#pragma unroll
-      for (int e = 0; e < DH / 32; ++e) acc[e] *= alpha;
-      for (int k = 0; k < 32; ++k) {
-        const float pk = __shfl_sync(0xffffffffu, p, k);
-        const int64_t ak = __shfl_sync(0xffffffffu, at, k);
-        if (!((all >> k) & 1)) continue;
-#pragma unroll
-        for (int e = 0; e < DH / 32; ++e) acc[e] = fmaf(pk, to_f(vp[ak + lane + 32 * e]), acc[e]);
-      }
-    }
-    if (a.n_splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      __nv_bfloat16* o =
-          static_cast<__nv_bfloat16*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * DH;
-#pragma unroll
-      for (int e = 0; e < DH / 32; ++e) o[lane + 32 * e] = __float2bfloat16_rn(acc[e] * inv);
-    } else {
-#pragma unroll
-      for (int e = 0; e < DH / 32; ++e) a.part_o[(part_row0 + r) * DH + lane + 32 * e] = acc[e];
-      if (lane == 0) {
-        a.part_ml[(part_row0 + r) * 2] = m;
-        a.part_ml[(part_row0 + r) * 2 + 1] = l;
-      }
-    }
-  }
 }
 
 template <int DH, int SH>
@@ -800,26 +744,16 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     float w0 = 1.f, w1 = 0.f;
     const uint32_t meet = k_s + (t & 63) * 4, meet_o = meet + 512 + dim0 * 256;  // floats [value][row]
     if constexpr (C::kTwin) {
-      if (warp_live) {
-        if (t >= 64) {
-          st32(meet, m);
-          st32(meet + 256, l);
-        }
-        float zero = 0.f;  // NaN if a sum is not finite
+      if (t >= 64 && warp_live) {
+        st32(meet, m);
+        st32(meet + 256, l);
 #pragma unroll
         for (int c = 0; c < kMyDims; c += 32) {
           uint32_t o[32] = {};
           if (steps > 0) tmem_ld(o_col + c, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) zero = fmaf(__uint_as_float(o[e]), 0.f, zero);
-          if (t >= 64) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) st32(meet_o + (c + e) * 256, __uint_as_float(o[e]));
-          }
+          for (int e = 0; e < 32; ++e) st32(meet_o + (c + e) * 256, __uint_as_float(o[e]));
         }
-        // an infinite value times the other copy's weights, which are 0 here (a sum of weights that is not
-        // finite itself makes the row NaN by itself)
-        if (live && zero != 0.f && l < INFINITY) *odd = 1;
       }
       asm volatile("bar.sync 1, %0;" ::"r"(ST * C::kSoft * 32) : "memory");
       if (t < 64 && warp_live) {
@@ -832,7 +766,8 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
     }
     if (*stop) {
     } else if (*odd) {
-      rows_by_key<DH>(a, s, keys, table, g, r0, nr, xbeg, xend, part_row0, warp, C::kSoft * ST);
+      for (int i = warp; i < nr; i += C::kSoft * ST)
+        form_row_by_key<__nv_bfloat16, DH, true>(a, s, keys, table, g, r0 + i, xbeg, xend, 0, DH, part_row0 + i);
     } else if (warp_live && (!C::kTwin || t < 64)) {
       // ---- the warp's rows through its share of the Q tile, so that whole lines are written
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -845,6 +780,7 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
       auto piece = [&](int row, int c) {
         return stage + row * kPitch + ((kPieces >= 8 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4);
       };
+      float far[2] = {};  // the largest sums, NaN if there is one
       // the sums of 16 dimensions
       auto sums = [&](int c, uint32_t (&o)[16]) {
         if (steps > 0)
@@ -856,6 +792,9 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           for (int e = 0; e < 16; ++e)
             o[e] = __float_as_uint(__uint_as_float(o[e]) * w0 + ld32(meet_o + (c + e) * 256) * w1);
         }
+#pragma unroll
+        for (int e = 0; e < 16; e += 2)
+          far[(e >> 1) & 1] = max3_abs(far[(e >> 1) & 1], __uint_as_float(o[e]), __uint_as_float(o[e + 1]));
       };
       // rows that are read back: 32 / kPieces at once
       const int back = lane / kPieces, c_back = lane % kPieces;
@@ -897,6 +836,8 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
             uint32_t o[16];
             sums(half + c, o);
 #pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+#pragma unroll
             for (int e = 0; e < 16; e += 4)
               sts128(piece(lane, (c + e) / 4), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
           }
@@ -909,6 +850,14 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           }
           __syncwarp();
         }
+      }
+      // rows whose weights are finite, and their sums are not
+      uint32_t again = __ballot_sync(0xffffffffu, live && !(max3_abs(far[0], far[1], 0.f) < INFINITY) && l < INFINITY);
+      __syncwarp();
+      for (; again; again &= again - 1) {
+        const int row = r - lane + __ffs(again) - 1;
+        form_row_by_key<__nv_bfloat16, DH, true>(a, s, keys, table, g, r0 + row, xbeg, xend, dim0, dim0 + kMyDims,
+                                                 part_row0 + row);
       }
     }
     fence_before();

@@ -59,12 +59,6 @@ template <int DH>
 __device__ __forceinline__ uint32_t tile_addr(uint32_t tile, int k, int c) {
   return tile + (uint32_t)((k >> 3) * (DH * 16) + (c >> 3) * 1024 + (k & 7) * 128 + (((c & 7) ^ (k & 7)) << 4));
 }
-// The largest of |a|, |b| and |c|, NaN if one of them is.
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {
-  float d;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -74,7 +68,7 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 template <int DH, int MT, int NS, int MINB>
 __global__ void __launch_bounds__((MT + 1) * 32, MINB)
     form_tma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                    const FormArgs a, int log2_bs, int vec) {
+                    const __grid_constant__ FormArgs a, int log2_bs, int vec) {
   pdl_enter();
   using C = Cfg<DH, MT, NS>;
   constexpr int NT = DH / 8;
@@ -371,13 +365,19 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
   }
   if (!live || !ok) return;
   const int col = 2 * (lane & 3);
+  const int64_t part_row0 = ((((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split) * kRows;
+  uint32_t again[2];  // rows whose weights are finite, and their sums are not
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = half ? rb : ra;
-    if (r >= nr) continue;
     const float l = half ? l_b : l_a;
+    float top[2] = {};
+#pragma unroll
+    for (int i = 0; i < NT; ++i) top[i & 1] = max3_abs(top[i & 1], o[i][2 * half], o[i][2 * half + 1]);
+    again[half] = __ballot_sync(0xffffffffu, r < nr && !(max3_abs(top[0], top[1], 0.f) < INFINITY) && l < INFINITY);
+    if (r >= nr) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     if (a.n_splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (int64_t)(half ? tok_b : tok_a) * a.out_stride +
                            (int64_t)(g * a.group + (r0 + r) % a.group) * DH + col;
 #pragma unroll
@@ -391,16 +391,21 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
         }
       }
     } else {
-      const int64_t unit = (((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split;
       if ((lane & 3) == 0)
-        *reinterpret_cast<float2*>(a.part_ml + (unit * kRows + r) * 2) = make_float2(half ? m_b : m_a, l);
+        *reinterpret_cast<float2*>(a.part_ml + (part_row0 + r) * 2) = make_float2(half ? m_b : m_a, l);
       if (l == 0.f) continue;
-      float* po = a.part_o + (unit * kRows + r) * DH + col;
+      float* po = a.part_o + (part_row0 + r) * DH + col;
 #pragma unroll
       for (int i = 0; i < NT; ++i)
-        *reinterpret_cast<float2*>(po + i * 8) = make_float2(o[i][2 * half], o[i][2 * half + 1]);
+        *reinterpret_cast<float2*>(po + i * 8) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
     }
   }
+  if ((again[0] | again[1]) == 0) return;
+  __syncwarp();
+  for (int i = 0; i < 16; ++i)  // (four lanes a row)
+    if ((again[i >> 3] >> (4 * (i & 7))) & 15)
+      form_row_by_key<__nv_bfloat16, DH, true>(a, s, keys, a.tables + (int64_t)b * a.max_blocks, g, r0 + wr + i, xbeg,
+                                               xend, 0, DH, part_row0 + wr + i);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
