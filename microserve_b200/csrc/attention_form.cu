@@ -163,14 +163,10 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(const __grid_con
     if (r >= nr) continue;
     const int rr = r0 + r;
     const int64_t part_row = ((((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split) * ROWS + r;
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
     float zero = 0.f;  // NaN if a sum is not finite
 #pragma unroll
     for (int e = 0; e < PER_LANE; ++e) zero = fmaf(acc[i][e], 0.f, zero);
-    if (__any_sync(0xffffffffu, zero != 0.f) && l[i] < INFINITY) {
-      form_row_by_key<T, DH, false>(a, s, keys, table, g, rr, xbeg, xend, 0, DH, part_row);
-      continue;
-    }
-    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
     if (a.n_splits == 1) {
       T* o = static_cast<T*>(a.out) + (int64_t)(s.t0 + rr / a.group) * a.out_stride +
              (int64_t)(g * a.group + rr % a.group) * DH;
@@ -185,6 +181,11 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(const __grid_con
         a.part_ml[part_row * 2] = m[i];
         a.part_ml[part_row * 2 + 1] = l[i];
       }
+    }
+    if (__any_sync(0xffffffffu, zero != 0.f) && l[i] < INFINITY) {
+      float common[(DH + 31) / 32];
+      form_odd_values<T, DH>(a, s, keys, table, g, xbeg, xend, minpos, maxpos, 0, DH, 0, 1, common);
+      form_row_again<T, DH, false>(a, s, keys, table, g, rr, xbeg, xend, minpos, maxpos, 0, DH, part_row, true, common);
     }
   }
 }

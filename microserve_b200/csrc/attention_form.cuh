@@ -112,73 +112,6 @@ __device__ __forceinline__ bool form_sees(const FormArgs& a, const FormSeq& s, i
   return j < s.pfx || (seen && (a.window <= 0 || distance < a.window));
 }
 
-// One row of a sequence by a warp, key by key: what the kernels give when their sums of p v are not finite, whose
-// terms p reach 1 (2^8 on tcgen05) before the division.  The weights are divided by their sum
-// first, so that a mean of finite values is finite.  A lane a key for the scores, dimensions d0 to d1 over the lanes for
-// the means; maxima in base 2 or e, as the kernel has them.  part_row: the row's place in the workspace.
-template <typename T, int DH, bool kBase2>
-__device__ __noinline__ void form_row_by_key(const FormArgs& a, FormSeq s, FormKeys keys, const int32_t* table, int g,
-                                             int rr, int xbeg, int xend, int d0, int d1, int64_t part_row) {
-  constexpr int kMine = (DH + 31) / 32;
-  const int lane = threadIdx.x & 31;
-  const T *kp = static_cast<const T*>(a.k), *vp = static_cast<const T*>(a.v);
-  const int tok = s.t0 + rr / a.group, head = g * a.group + rr % a.group, pos = a.positions[tok];
-  const T* q = static_cast<const T*>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * DH;
-  const float slope = a.slopes ? a.slopes[head] : 0.f;
-  auto score = [&](int x0, int64_t& at, bool& seen) {
-    const int j = keys.key(min(x0 + lane, xend - 1));
-    int distance = 0;
-    seen = x0 + lane < xend && form_sees(a, s, tok, pos, j, distance);
-    at = (((int64_t)form_block(a, table, j / a.bs) * a.hkv + g) * a.bs + j % a.bs) * DH;
-    float v = 0.f;
-    for (int d = 0; d < DH; ++d) v = fmaf(to_f(q[d]), to_f(kp[at + d]), v);
-    v *= a.scale;
-    if (a.softcap > 0.f && !(fabsf(v) <= 1e-4f * a.softcap)) v = a.softcap * tanhf(v / a.softcap);
-    if (a.slopes) v -= slope * fabsf((float)distance);
-    return !seen ? -INFINITY : kBase2 ? v * 1.4426950408889634f : v;
-  };
-  auto power = [](float v) { return kBase2 ? exp2f(v) : expf(v); };
-  float m = -INFINITY, l = 0.f, mean[kMine] = {};
-  int64_t at;
-  bool seen;
-  for (int x0 = xbeg; x0 < xend; x0 += 32) {
-    const float v = score(x0, at, seen), mn = fmaxf(m, warp_max(v)), sub = mn == -INFINITY ? 0.f : mn;
-    l = l * (m == -INFINITY ? 0.f : power(m - sub)) + warp_sum(seen ? power(v - sub) : 0.f);
-    m = mn;
-  }
-  const float sub = m == -INFINITY ? 0.f : m, inv = l == 0.f ? 0.f : 1.f / l;
-  for (int x0 = xbeg; x0 < xend; x0 += 32) {
-    const float v = score(x0, at, seen), w = seen ? power(v - sub) * inv : 0.f;
-    const uint32_t all = __ballot_sync(0xffffffffu, seen), some = __ballot_sync(0xffffffffu, seen && v > -INFINITY);
-    for (int k = 0; k < 32; ++k) {
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      const int64_t ak = __shfl_sync(0xffffffffu, at, k);
-      if (!((all >> k) & 1)) continue;
-#pragma unroll
-      for (int e = 0; e < kMine; ++e) {
-        if (d0 + lane + 32 * e >= d1) continue;
-        const float vk = to_f(vp[ak + d0 + lane + 32 * e]);
-        // (an infinite value counts however small its weight is)
-        mean[e] = fmaf(wk == 0.f && ((some >> k) & 1) && !(fabsf(vk) < INFINITY) ? 1.f : wk, vk, mean[e]);
-      }
-    }
-  }
-  T* o = static_cast<T*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * DH;
-#pragma unroll
-  for (int e = 0; e < kMine; ++e) {
-    const int d = d0 + lane + 32 * e;
-    if (d >= d1) continue;
-    if (a.n_splits == 1)
-      o[d] = from_f<T>(mean[e]);
-    else
-      a.part_o[part_row * DH + d] = mean[e];
-  }
-  if (a.n_splits > 1 && lane == 0) {
-    a.part_ml[part_row * 2] = m;
-    a.part_ml[part_row * 2 + 1] = l;
-  }
-}
-
 // attention_form.cu: joins the KV ranges' partial results; `rows` per tile, maxima in base 2 or e.
 template <typename T, bool kBase2>
 int form_combine(const FormArgs& a, int rows, int dh, cudaStream_t s);

@@ -184,6 +184,138 @@ __device__ __forceinline__ bool all_see(const FormArgs& a, const FormSeq& s, con
          (a.window <= 0 || maxpos - j0 < a.window);
 }
 
+// The row of key j in a pool, in elements.
+template <int DH>
+__device__ __forceinline__ int64_t form_key_row(const FormArgs& a, const int32_t* table, int g, int j) {
+  return (((int64_t)form_block(a, table, j / a.bs) * a.hkv + g) * a.bs + j % a.bs) * DH;
+}
+// Adds to odd what is not finite of the values of 32 keys (a lane has one's row, `sees` a bit for each), in
+// dimensions d0 + lane, d0 + lane + 32, .. below d1.
+template <typename T, int DH>
+__device__ __forceinline__ void add_odd(const T* v, int64_t at, uint32_t sees, int d0, int d1,
+                                        float (&odd)[(DH + 31) / 32]) {
+  const int lane = threadIdx.x & 31;
+  if (sees == 0) return;
+#pragma unroll 8
+  for (int k = 0; k < 32; ++k) {
+    const T* row = v + __shfl_sync(0xffffffffu, at, k) + d0 + lane;
+#pragma unroll
+    for (int e = 0; e < (DH + 31) / 32; ++e) {
+      const float x = ((sees >> k) & 1) && d0 + lane + 32 * e < d1 ? to_f(row[32 * e]) : 0.f;
+      if (!(fabsf(x) < INFINITY)) odd[e] += x;
+    }
+  }
+}
+
+// The sums of the values that are not finite of the keys that all rows of a tile see, as far as whole groups of 32 places
+// show it: every `warps`th group, by the calling warp.
+template <typename T, int DH>
+__device__ __noinline__ void form_odd_values(const FormArgs& a, FormSeq s, FormKeys keys, const int32_t* table, int g,
+                                             int xbeg, int xend, int minpos, int maxpos, int d0, int d1, int warp,
+                                             int warps, float (&out)[(DH + 31) / 32]) {
+  float odd[(DH + 31) / 32] = {};  // (not `out` itself: a load would wait for each possible store)
+  for (int x0 = xbeg + 32 * warp; x0 < xend; x0 += 32 * warps)
+    if (all_see<32>(a, s, keys, x0, xend, minpos, maxpos))
+      add_odd<T, DH>(static_cast<const T*>(a.v), form_key_row<DH>(a, table, g, keys.key(x0 + (threadIdx.x & 31))),
+                     0xffffffffu, d0, d1, odd);
+#pragma unroll
+  for (int e = 0; e < (DH + 31) / 32; ++e) out[e] = odd[e];
+}
+
+// Dimensions d0 to d1 of one row of a sequence once more, by a warp, after the kernel has written them: for rows whose
+// weights are finite and whose sums of p v are not, or that may see values which the kernel left out because they are
+// not finite.  Where a value that the row sees is infinite or NaN, so is the result, however small its weight.  Elsewhere
+// what is not finite has overflowed: terms p reach 1 (2^8 on tcgen05) before the division.  Then the row is computed
+// key by key, with the weights divided by their sum first, so that a mean of finite values is finite.  A lane a key for
+// visibility and scores, dimensions over the lanes for the values; maxima in base 2 or e, as the kernel has them.
+// part_row: the row's place in the workspace; common: form_odd_values of the same dimensions; masked: among the keys
+// that not all rows see there may be such values too.  (4 prompts of up to 4096 tokens of which all see a NaN 0.55 -> 1.0
+// ms, 256 trees of 8 nodes 0.22 -> 0.30; all values too large 1.3 s and 0.14.)
+template <typename T, int DH, bool kBase2>
+__device__ __noinline__ void form_row_again(const FormArgs& a, FormSeq s, FormKeys keys, const int32_t* table, int g,
+                                            int rr, int xbeg, int xend, int minpos, int maxpos, int d0, int d1,
+                                            int64_t part_row, bool masked,
+                                            const float (&common)[(DH + 31) / 32]) {
+  constexpr int kMine = (DH + 31) / 32;
+  const int lane = threadIdx.x & 31;
+  const T *kp = static_cast<const T*>(a.k), *vp = static_cast<const T*>(a.v);
+  const int tok = s.t0 + rr / a.group, head = g * a.group + rr % a.group, pos = a.positions[tok];
+  const T* q = static_cast<const T*>(a.q) + (int64_t)tok * a.q_stride + (int64_t)head * DH;
+  T* o = static_cast<T*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * DH;
+  float* part = a.part_o + part_row * DH;
+  const float slope = a.slopes ? a.slopes[head] : 0.f;
+  // the key at place x0 + lane: its row in the pools, the distance, and whether the row sees it
+  auto look = [&](int x0, int64_t& at, int& distance) {
+    const int j = keys.key(min(x0 + lane, xend - 1));
+    at = form_key_row<DH>(a, table, g, j);
+    return x0 + lane < xend && form_sees(a, s, tok, pos, j, distance);
+  };
+  int64_t at;
+  int distance = 0;
+  float odd[kMine];  // the sum of the values that are not finite
+#pragma unroll
+  for (int e = 0; e < kMine; ++e) odd[e] = common[e];
+  for (int x0 = xbeg; masked && x0 < xend; x0 += 32) {
+    if (all_see<32>(a, s, keys, x0, xend, minpos, maxpos)) continue;
+    const uint32_t sees = __ballot_sync(0xffffffffu, look(x0, at, distance));
+    add_odd<T, DH>(vp, at, sees, d0, d1, odd);
+  }
+  bool over[kMine], any = false;
+#pragma unroll
+  for (int e = 0; e < kMine; ++e) {
+    const int d = d0 + lane + 32 * e;
+    over[e] = false;
+    if (d >= d1) continue;
+    if (odd[e] == 0.f) {
+      over[e] = !(fabsf(a.n_splits == 1 ? to_f(o[d]) : part[d]) < INFINITY);
+      any |= over[e];
+    } else if (a.n_splits == 1) {
+      o[d] = from_f<T>(odd[e]);
+    } else {
+      part[d] = odd[e];
+    }
+  }
+  if (!__any_sync(0xffffffffu, any)) return;
+  auto score = [&](int x0) {
+    const bool seen = look(x0, at, distance);
+    float v = 0.f;
+    for (int d = 0; d < DH; ++d) v = fmaf(to_f(q[d]), to_f(kp[at + d]), v);
+    v *= a.scale;
+    if (a.softcap > 0.f && !(fabsf(v) <= 1e-4f * a.softcap)) v = a.softcap * tanhf(v / a.softcap);
+    if (a.slopes) v -= slope * fabsf((float)distance);
+    return !seen ? -INFINITY : kBase2 ? v * 1.4426950408889634f : v;
+  };
+  auto power = [](float v) { return v == -INFINITY ? 0.f : kBase2 ? exp2f(v) : expf(v); };
+  float m = -INFINITY, l = 0.f, mean[kMine] = {};
+  for (int x0 = xbeg; x0 < xend; x0 += 32) {
+    const float v = score(x0), mn = fmaxf(m, warp_max(v));
+    if (mn == -INFINITY) continue;
+    l = l * power(m - mn) + warp_sum(power(v - mn));
+    m = mn;
+  }
+  const float inv = 1.f / l;  // (the weights are not all 0: the sums were not)
+  for (int x0 = xbeg; x0 < xend; x0 += 32) {
+    const float w = power(score(x0) - m) * inv;
+    for (int k = 0; k < 32; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      const int64_t ak = __shfl_sync(0xffffffffu, at, k) + d0 + lane;
+      if (wk == 0.f) continue;
+#pragma unroll
+      for (int e = 0; e < kMine; ++e)
+        if (d0 + lane + 32 * e < d1) mean[e] = fmaf(wk, to_f(vp[ak + 32 * e]), mean[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kMine; ++e) {
+    if (!over[e]) continue;
+    const int d = d0 + lane + 32 * e;
+    if (a.n_splits == 1)
+      o[d] = from_f<T>(mean[e]);
+    else
+      part[d] = mean[e];
+  }
+}
+
 __device__ __forceinline__ uint64_t low_bits(int n) {
   return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
 }

@@ -34,8 +34,8 @@
 //
 // Values that no row should meet: where a mask is needed the softmax warps look
 // at the step's values first and put 0 for what is not finite.  If one of those belongs
-// to a key that some row may see, the CTA computes its rows again on the
-// CUDA cores, key by key.  So is a row whose sums are not finite at the end: large values that overflow
+// to a key that some row may see, every row of the CTA looks for such values among those that it sees
+// (form_row_again).  So does a row whose sums are not finite at the end: large values that overflow
 // float32 before the division by l (p reaches 2^8), or an infinite one in a step without a mask, which kHalf
 // multiplies by the zeros that stand for the other copy's weights.
 #include <cfloat>
@@ -764,11 +764,8 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
         m = top;
       }
     }
-    if (*stop) {
-    } else if (*odd) {
-      for (int i = warp; i < nr; i += C::kSoft * ST)
-        form_row_by_key<__nv_bfloat16, DH, true>(a, s, keys, table, g, r0 + i, xbeg, xend, 0, DH, part_row0 + i);
-    } else if (warp_live && (!C::kTwin || t < 64)) {
+    uint32_t again = 0;
+    if (!*stop && warp_live && (!C::kTwin || t < 64)) {
       // ---- the warp's rows through its share of the Q tile, so that whole lines are written
       const float inv = l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst =
@@ -851,13 +848,37 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           __syncwarp();
         }
       }
-      // rows whose weights are finite, and their sums are not
-      uint32_t again = __ballot_sync(0xffffffffu, live && !(max3_abs(far[0], far[1], 0.f) < INFINITY) && l < INFINITY);
-      __syncwarp();
+      // rows whose sums are not finite, or lack values that are not (their weights finite: else they are NaN anyway)
+      again = __ballot_sync(0xffffffffu,
+                            live && (*odd || !(max3_abs(far[0], far[1], 0.f) < INFINITY)) && l < INFINITY);
+    }
+    constexpr int kThreads = ST * C::kSoft * 32;
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(again), "n"(kThreads)
+        : "memory");
+    if (any) {
+      float* sums = reinterpret_cast<float*>(smem_raw + (k_s - raw));  // (the K ring: all products have ended)
+      float common[(DH + 31) / 32];
+      if (threadIdx.x < DH) sums[threadIdx.x] = 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+      form_odd_values<__nv_bfloat16, DH>(a, s, keys, table, g, xbeg, xend, minpos, maxpos, 0, DH, warp, C::kSoft * ST,
+                                         common);
+#pragma unroll
+      for (int e = 0; e < DH / 32; ++e)
+        if (common[e] != 0.f) atomicAdd(sums + lane + 32 * e, common[e]);  // (infinities and NaN: in any order)
+      asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+#pragma unroll
+      for (int e = 0; e < DH / 32; ++e) common[e] = lane + 32 * e < kMyDims ? sums[dim0 + lane + 32 * e] : 0.f;
       for (; again; again &= again - 1) {
         const int row = r - lane + __ffs(again) - 1;
-        form_row_by_key<__nv_bfloat16, DH, true>(a, s, keys, table, g, r0 + row, xbeg, xend, dim0, dim0 + kMyDims,
-                                                 part_row0 + row);
+        form_row_again<__nv_bfloat16, DH, true>(a, s, keys, table, g, r0 + row, xbeg, xend, minpos, maxpos, dim0,
+                                                dim0 + kMyDims, part_row0 + row, *odd != 0, common);
       }
     }
     fence_before();

@@ -402,10 +402,13 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
   }
   if ((again[0] | again[1]) == 0) return;
   __syncwarp();
+  const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
+  float common[DH / 32];
+  form_odd_values<__nv_bfloat16, DH>(a, s, keys, table, g, xbeg, xend, minpos, maxpos, 0, DH, 0, 1, common);
   for (int i = 0; i < 16; ++i)  // (four lanes a row)
     if ((again[i >> 3] >> (4 * (i & 7))) & 15)
-      form_row_by_key<__nv_bfloat16, DH, true>(a, s, keys, a.tables + (int64_t)b * a.max_blocks, g, r0 + wr + i, xbeg,
-                                               xend, 0, DH, part_row0 + wr + i);
+      form_row_again<__nv_bfloat16, DH, true>(a, s, keys, table, g, r0 + wr + i, xbeg, xend, minpos, maxpos, 0, DH,
+                                              part_row0 + wr + i, true, common);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
