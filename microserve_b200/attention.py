@@ -55,6 +55,8 @@ class AttentionForm:
         # (not (a <= x < b): NaN is refused too)
         if not 0.0 <= self.softcap < 3.4e38 or not 0.0 <= self.scale < 3.4e38:
             raise ValueError("softcap and scale must be finite and not negative (0: none, the default)")
+        if 0.0 < self.softcap < 1e-45 or 0.0 < self.scale < 1e-45:  # (would be 0 in float32)
+            raise ValueError("softcap and scale must be 0 or within float32's range")
         if not 0 <= self.window < 1 << 31:
             raise ValueError("window must be 0 (none) or a number of tokens")
         slopes = prefix = mask = words = 0
