@@ -238,6 +238,14 @@ __global__ void __launch_bounds__(256) form_combine_kernel(FormArgs a, int rows,
   auto add = [&](float w, const float4& v) {
     if (w == -1.f) return;
     w *= inv;
+    if (w == 0.f) {  // (an infinite value counts however small its weight is)
+      auto odd = [](float x) { return fabsf(x) < INFINITY ? 0.f : x; };
+      acc.x += odd(v.x);
+      acc.y += odd(v.y);
+      acc.z += odd(v.z);
+      acc.w += odd(v.w);
+      return;
+    }
     acc.x = fmaf(w, v.x, acc.x);
     acc.y = fmaf(w, v.y, acc.y);
     acc.z = fmaf(w, v.z, acc.z);
