@@ -184,6 +184,20 @@ __device__ __forceinline__ bool all_see(const FormArgs& a, const FormSeq& s, con
          (a.window <= 0 || maxpos - j0 < a.window);
 }
 
+// 16 bytes of values as float32; `wide`: they are aligned to it.
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* p, bool wide, float (&f)[N]) {
+  static_assert(N * sizeof(T) == 16, "16 bytes");
+  if (wide) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const T* x = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = to_f(x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = to_f(p[e]);
+  }
+}
 // The row of key j in a pool, in elements.
 template <int DH>
 __device__ __forceinline__ int64_t form_key_row(const FormArgs& a, const int32_t* table, int g, int j) {
@@ -230,7 +244,7 @@ __device__ __noinline__ void form_odd_values(const FormArgs& a, FormSeq s, FormK
 // visibility and scores, dimensions over the lanes for the values; maxima in base 2 or e, as the kernel has them.
 // part_row: the row's place in the workspace; common: form_odd_values of the same dimensions; masked: among the keys
 // that not all rows see there may be such values too.  (4 prompts of up to 4096 tokens of which all see a NaN 0.55 -> 1.0
-// ms, 256 trees of 8 nodes 0.22 -> 0.30; all values too large 1.3 s and 0.14.)
+// ms, 256 trees of 8 nodes 0.22 -> 0.30; all values too large 0.46 s and 0.08.)
 template <typename T, int DH, bool kBase2>
 __device__ __noinline__ void form_row_again(const FormArgs& a, FormSeq s, FormKeys keys, const int32_t* table, int g,
                                             int rr, int xbeg, int xend, int minpos, int maxpos, int d0, int d1,
@@ -276,10 +290,18 @@ __device__ __noinline__ void form_row_again(const FormArgs& a, FormSeq s, FormKe
     }
   }
   if (!__any_sync(0xffffffffu, any)) return;
+  constexpr int kVec = 16 / (int)sizeof(T);
+  const bool q_wide = reinterpret_cast<uintptr_t>(q) % 16 == 0, k_wide = reinterpret_cast<uintptr_t>(kp) % 16 == 0;
   auto score = [&](int x0) {
     const bool seen = look(x0, at, distance);
     float v = 0.f;
-    for (int d = 0; d < DH; ++d) v = fmaf(to_f(q[d]), to_f(kp[at + d]), v);
+    for (int d = 0; d < DH; d += kVec) {
+      float qd[kVec], kd[kVec];
+      load_vec(q + d, q_wide, qd);
+      load_vec(kp + at + d, k_wide, kd);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v = fmaf(qd[e], kd[e], v);
+    }
     v *= a.scale;
     if (a.softcap > 0.f && !(fabsf(v) <= 1e-4f * a.softcap)) v = a.softcap * tanhf(v / a.softcap);
     if (a.slopes) v -= slope * fabsf((float)distance);
