@@ -478,8 +478,12 @@ MS_API int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache, cons
  * p_q - p_k < window (window 0: any): without a tree mask p_k = j <= p_q; with one
  * every key before the pass's own tokens is seen, and of those, which stand at
  * context_lens[b] - q_len onwards, token i if bit i % 32 of word i / 32 of the query's mask
- * row is set (p_k is then that token's position).  A query that sees nothing gives 0; what
- * stands in keys and values that a query does not see never reaches its result.
+ * row is set (p_k is then that token's position).  A query that sees nothing, or whose scores are all -inf, gives 0;
+ * what stands in keys and values that a query does not see never reaches its result.  What it sees does: a
+ * score of NaN or +inf gives NaN, an infinite value an infinite result in its dimension, however small its weight; a
+ * mean of finite values is finite.  Scores, weights' sums and means are float32.  bf16 caches with heads of 64 or 128 round
+ * each weight to bf16 for the product with the values (off by 2^-8 of it at most, and divided by the sum of
+ * the rounded ones) and compute it to 1e-4 of itself; float32 caches, and bf16 ones with other heads, do not.
  * Device arrays, each nullable. */
 typedef struct {
   float scale;

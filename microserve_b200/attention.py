@@ -41,7 +41,11 @@ class AttentionForm:
     ``i`` where bit ``i % 32`` of word ``i / 32`` of the query's row is set (``p_k`` is then
     that token's position: siblings share one).  ``slopes`` (n_heads,) float32, ``prefix_lens``
     (B,) int32, ``tree_mask`` (T, words) int32, from :func:`microserve_b200.tree.tree_masks`
-    or any other bits."""
+    or any other bits.
+
+    A query that sees nothing gives 0.  bfloat16 caches with heads of 64 or 128 round each weight to
+    bfloat16 for the product with the values, and divide by the sum of the rounded ones; all other sums
+    are float32."""
 
     softcap: float = 0.0
     slopes: torch.Tensor | None = None

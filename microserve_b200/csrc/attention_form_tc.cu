@@ -9,7 +9,8 @@
 // at a step; the streams share the keys and values.
 //   softmax warps  two threads (kParts) share a row, 32 scores of a step each: scores out of
 //        TMEM, cap, distance, mask (bits, only where some row does not see all keys), p
-//        rounded to bf16 back into TMEM over the scores, and the sum of the rounded values
+//        rounded to bf16 back into TMEM over the scores (the operand type of the second product:
+//        2^-8 of a p at most), and the sum of the rounded values
 //        (the rounding of a dominant p cancels).  m is raised only when a row's maximum has
 //        grown by more than 2^8, so O is rescaled a few times a row at most;
 //   producer warp  TMA loads of whole pages (or parts of one), a lane a page, into
@@ -21,11 +22,12 @@
 // SM.  kHalf: up to 64 rows of many sequences, twice in the tile; each copy takes half of the step's keys, so that no
 // lane of the softmax idles, and the copies meet at the end; two CTAs an SM.
 //
-// What it measured: 64 trees of 33 to 61 nodes, 32 heads over 8 of 128, 1 to 4 k keys (127 GFLOP, 733 MB)
-// 215 us, 0.59 PFLOP/s and 3.4 TB/s; 4 prompts of up to 4096 with cap and prefix (309 GFLOP) 485 us,
-// 0.64 PFLOP/s; 256 trees of 8 nodes, 32 heads over 4 of 64, 1.3 k keys (351 MB) 92 us, 3.8
-// TB/s; one tree of 16 nodes over 32 k keys (134 MB) 35 us with the joining of its 37 ranges (kOne).
-// Every pipe is half idle (tensor 24 to 39%, issue 42 to 56%, SFU 24 to 32%).  The bound of kTwo is the
+// What it measured, in a burst and under steady load (the 1000 W cap takes the clock to 1.7 GHz): 64 trees of 33 to
+// 61 nodes, 32 heads over 8 of 128, 1 to 4 k keys (127 GFLOP, 733 MB) 208 and 242 us, 0.61 PFLOP/s and 3.5 TB/s in
+// the burst; 4 prompts of up to 4096 with cap and prefix (309 GFLOP) 474 and 488 us, 0.65 PFLOP/s; 256 trees of 8
+// nodes, 32 heads over 4 of 64, 1.3 k keys (351 MB) 92 and 97 us, 3.8 TB/s; one tree of 16 nodes over 32 k keys (134 MB)
+// 36 and 37 us with the joining of its 37 ranges (kOne).
+// Every pipe is half idle (tensor 24 to 42%, issue 31 to 56%, SFU 12 to 33%).  The bound of kTwo is the
 // softmax of a step, about 2200 cycles (2700 with a cap) for 64 keys: TMEM load 160, maxima
 // and vote 400, exponentials 750 to 1100 for the four warps of a scheduler, the store and its hand-off
 // 350; products and copies are done by then.  The bound of kHalf at heads of 64 is the copy unit, 73

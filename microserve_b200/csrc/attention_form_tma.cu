@@ -11,12 +11,13 @@
 //                   that divides it is of the rounded values, so the rounding of a
 //                   dominant p cancels.
 // Bound by HBM, less the start and the end of each CTA: 128 sequences of one token, 32 heads over 8 of 128,
-// cap and a window of 2048 (990 MB) 185 us, 5.3 TB/s; one of 332 keys 14 us, which is latency.
+// cap and a window of 2048 (990 MB) 187 us, 5.3 TB/s; one of 332 keys 14 us, which is latency.
 //
 // Masks cost nothing in chunks that every row sees in full; elsewhere each row
 // has its 64 places as bits.  In those chunks values may be anything (a stale
 // page's tail, a branch that overflowed): what is not finite enters the product
-// as 0 and is added afterwards to the rows that see it.
+// as 0 and is added afterwards to the rows that see it.  Rows whose sums are not finite
+// are looked at again at the end (form_row_again).
 #include <cfloat>
 #include <mutex>
 

@@ -69,9 +69,10 @@ __device__ __forceinline__ bool move_pair(const int32_t* src, const int32_t* dst
 // kRegs elements of `row` a thread, in registers before the first is stored, kPools pools
 // at a time, and go through the pools of their slice (blockIdx.y of gridDim.y).  The
 // places are worked out once a slice: their divisions take longer than the copies of a pool.
-// Rows of 128 to 256 bytes lie anywhere, so what counts is how many are in flight: 192 groups, 32
-// layers, 8 heads of 128 take 20, 27 and 42 us for up to 5, 8 and 24 moves (82, 95 and 113 MB:
-// 4.2, 3.5 and 2.7 TB/s); with 4 elements a thread 23, 26 and 58 us, with 8 pools at a time
+// Bound by latency: with two slices a warp goes through 32 pools in eight rounds of loads, a barrier and stores, none
+// of which begins before the one before has ended (DRAM 31%, warps active 28%).  192 groups, 32
+// layers, 8 heads of 128 take 19, 27 and 42 us for up to 5, 8 and 24 moves (82, 95 and 113 MB:
+// 4.3, 3.5 and 2.7 TB/s); with 4 elements a thread 23, 26 and 58 us, with 8 pools at a time
 // instead of 4 20, 27 and 43.
 template <typename V, int kRegs, int kPools>
 __global__ void __launch_bounds__(kThreads)
