@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("wrong", [0, 1, 7])
 def test_a_round_of_paths_beyond_one_move(wrong) -> None:
     """Trees 299 and 600 deep, `wrong` nodes that are not accepted between any two of a path: the
-    streams are those of ordinary passes, in this round and in the next ones, which read what was moved."""
+    streams are those of ordinary passes, in that call and in the next ones, which read what was moved."""
     from microserve_b200.tree import verify_trees
 
     model = _model(max_seq_len=2048)
