@@ -481,7 +481,7 @@ MS_API int ms_forward_lora(const ms_model* model, const ms_kv_cache* cache, cons
  * row is set (p_k is then that token's position).  A query that sees nothing, or whose scores are all -inf, gives 0;
  * what stands in keys and values that a query does not see never reaches its result.  What it sees does: a
  * score of NaN or +inf gives NaN, an infinite value an infinite result in its dimension, however small its weight; a
- * mean of finite values is finite.  Scores, weights' sums and means are float32.  bf16 caches with heads of 64 or 128 round
+ * mean of finite values is finite (but within its roundings of the largest float32).  Scores, weights' sums and means are float32.  bf16 caches with heads of 64 or 128 round
  * each weight to bf16 for the product with the values (off by 2^-8 of it at most, and divided by the sum of
  * the rounded ones) and compute it to 1e-4 of itself; float32 caches, and bf16 ones with other heads, do not.
  * Device arrays, each nullable. */

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(const __grid_con
              (int64_t)(g * a.group + rr % a.group) * DH;
 #pragma unroll
       for (int e = 0; e < PER_LANE; ++e)
-        if (DH >= 32 || lane < DH) o[lane + 32 * e] = from_f<T>(acc[i][e] * inv);
+        if (DH >= 32 || lane < DH) o[lane + 32 * e] = from_f<T>(l[i] == 0.f ? 0.f : acc[i][e] * inv);
     } else {
 #pragma unroll
       for (int e = 0; e < PER_LANE; ++e)
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kWarps * 32) form_simt_kernel(const __grid_con
         a.part_ml[part_row * 2 + 1] = l[i];
       }
     }
-    if (__any_sync(0xffffffffu, zero != 0.f) && l[i] < INFINITY) {
+    if (__any_sync(0xffffffffu, zero != 0.f) && l[i] > 0.f && l[i] < INFINITY) {
       float common[(DH + 31) / 32];
       form_odd_values<T, DH>(a, s, keys, table, g, xbeg, xend, minpos, maxpos, 0, DH, 0, 1, common);
       form_row_again<T, DH, false>(a, s, keys, table, g, rr, xbeg, xend, minpos, maxpos, 0, DH, part_row, true, common);

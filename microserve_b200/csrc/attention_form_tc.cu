@@ -850,9 +850,9 @@ __global__ void __launch_bounds__(TcCfg<DH, SH>::kThreads, SH == kTwo ? 1 : 2)
           __syncwarp();
         }
       }
-      // rows whose sums are not finite, or lack values that are not (their weights finite: else they are NaN anyway)
-      again = __ballot_sync(0xffffffffu,
-                            live && (*odd || !(max3_abs(far[0], far[1], 0.f) < INFINITY)) && l < INFINITY);
+      // rows whose sums are not finite, or lack values that are not (with weights: else they are 0 or NaN anyway)
+      again = __ballot_sync(0xffffffffu, live && (*odd || !(max3_abs(far[0], far[1], 0.f) < INFINITY)) && l > 0.f &&
+                                             l < INFINITY);
     }
     constexpr int kThreads = ST * C::kSoft * 32;
     uint32_t any;

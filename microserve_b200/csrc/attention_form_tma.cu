@@ -367,7 +367,7 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
   if (!live || !ok) return;
   const int col = 2 * (lane & 3);
   const int64_t part_row0 = ((((int64_t)b * a.hkv + g) * a.row_tiles + tile) * a.n_splits + split) * kRows;
-  uint32_t again[2];  // rows whose weights are finite, and their sums are not
+  uint32_t again[2];  // rows that have weights, all finite, and sums that are not
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = half ? rb : ra;
@@ -375,7 +375,8 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
     float top[2] = {};
 #pragma unroll
     for (int i = 0; i < NT; ++i) top[i & 1] = max3_abs(top[i & 1], o[i][2 * half], o[i][2 * half + 1]);
-    again[half] = __ballot_sync(0xffffffffu, r < nr && !(max3_abs(top[0], top[1], 0.f) < INFINITY) && l < INFINITY);
+    again[half] = __ballot_sync(0xffffffffu, r < nr && !(max3_abs(top[0], top[1], 0.f) < INFINITY) && l > 0.f &&
+                                                 l < INFINITY);
     if (r >= nr) continue;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (a.n_splits == 1) {
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__((MT + 1) * 32, MINB)
                            (int64_t)(g * a.group + (r0 + r) % a.group) * DH + col;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const uint32_t v = pack2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
+        const uint32_t v = l == 0.f ? 0u : pack2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
         if (vec) {
           *reinterpret_cast<uint32_t*>(dst + i * 8) = v;
         } else {
